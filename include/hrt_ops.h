@@ -335,6 +335,35 @@ typedef struct hrt_dq8_args {
   int64_t rows, cols, nblocks;
 } hrt_dq8_args;
 
+/* "mx4_quant_{f32,bf16,f16}" and "mx4_dequant_{f32,bf16,f16}" — microscaled 4-bit floating point (no reference
+ * counterpart).  Blocks of 32 consecutive values of a row share a scale byte s; a value is e2m1(code) * 2^(s - 127), with
+ * e2m1 0, 0.5, 1, 1.5, 2, 3, 4, 6 for codes 0..7 and bit 3 the sign.
+ * codes: [rows, ceil(cols / 2)] bytes, the even element in the low nibble, contiguous (an odd row's last high nibble is 0);
+ * scale: [rows, ceil(cols / 32)] bytes, contiguous.
+ * quant: x [rows, cols] with row stride x_sr (elements, unit column stride).  s = floor(log2(largest magnitude)) - 2 + 127,
+ *   at least 0 (blocks of zeros too); code = x / 2^(s - 127) rounded to nearest, ties to the even code, saturated at 6.  A
+ *   block with an infinity or NaN gets s = 255 and reads back as NaN.
+ * dequant: x [rows, cols] contiguous receives the values, rounded once to its type (exact in fp32 and bf16 up to overflow
+ *   to infinity; s = 255 gives NaN).  x_sr is not read. */
+typedef struct hrt_mx4_args {
+  uint64_t x, codes, scale;
+  int64_t rows, cols, x_sr;
+} hrt_mx4_args;
+
+/* "mx4_mm_{bf16,f16}" — products with 4-bit weights (no reference counterpart):
+ *   y[m, n] = round(sum_k X[m, k] * W[n, k] + bias[n])     (fp32 sums; bias 0: none)
+ * w, w_scale: W as "mx4_quant_*" packs it ([N, K / 2] and [N, K / 32] bytes), read as the values that "mx4_dequant_{dt}"
+ * gives.  x_scale 0: x is [M, K] of the kernel's type with row stride x_sm (elements, a multiple of 8) and unit column
+ * stride.  x_scale not 0: x, x_scale are packed too ([M, K / 2], [M, K / 32], x_sm is not read), and the product runs on
+ * the 4-bit operands (their values exactly).  y: [M, N] contiguous, bias [N], both of the kernel's type.
+ * K % 32 == 0; x and w 16-byte aligned, scales 4-byte aligned.  ws (optional, 0 = none): fp32 workspace of ws_floats,
+ * 16-byte aligned, for partial products over slices of K where hrt_mx4_mm_workspace asks for one; they are added in order. */
+typedef struct hrt_mx4_mm_args {
+  uint64_t x, x_scale, w, w_scale, bias, y, ws;
+  int64_t M, N, K, x_sm, ws_floats;
+} hrt_mx4_mm_args;
+int64_t hrt_mx4_mm_workspace(const hrt_mx4_mm_args* args);
+
 /* "reduce_sum" — out[k] = (sum over the reduced coordinates r of x[k, r]) / div, accumulated in fp32 and
  * rounded once to out_dtype.  x: an ndim-dimensional strided view (ndim <= 8, non-negative strides) of
  * HRT_F32/BF16/F16; bit d of reduce_mask marks dimension d as summed; out: the kept dimensions, in order,

@@ -40,6 +40,8 @@ HRT_SOURCES = [
     "kernels/conv_norm.hip",
     "kernels/conv3x3.hip",
     "kernels/dq8.hip",
+    "kernels/mx4.hip",
+    "kernels/mx4_gemm.hip",
     "kernels/gemm.hip",
     "kernels/gemm_f32.hip",
     "kernels/gemm_mfma.hip",
@@ -61,6 +63,7 @@ SHIM_SOURCES = [
     "shim/op_rows.cpp",
     "shim/op_reduce.cpp",
     "shim/op_quant.cpp",
+    "shim/op_mx4.cpp",
     "shim/op_ew.cpp",
     "shim/op_image.cpp",
 ]

@@ -95,6 +95,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           runtime();
           return dequant_int8_linear_vk(x, q, s, bias);
         });
+  m.def("quantize_mxfp4", [](const at::Tensor& x) {
+    runtime();
+    return quantize_mxfp4_vk(x);
+  });
+  m.def("dequant_mxfp4", [](const at::Tensor& codes, const at::Tensor& scale, at::ScalarType dt, int64_t cols) {
+    runtime();
+    return dequant_mxfp4_vk(codes, scale, dt, cols);
+  });
+  m.def("mxfp4_linear", [](const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
+                           bool quantize_input) {
+    runtime();
+    return mxfp4_linear_vk(x, codes, scale, bias, quantize_input);
+  });
   // accounting and profiling
   m.def("kernel_counts", &gpu_counts);
   m.def("fallback_counts", &cpu_counts);

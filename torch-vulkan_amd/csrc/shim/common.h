@@ -95,4 +95,11 @@ at::Tensor dequant_int8_vk(const at::Tensor& q, const at::Tensor& scale, at::Sca
 at::Tensor dequant_int8_linear_vk(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale,
                                   const std::optional<at::Tensor>& bias);
 
+// Microscaled 4-bit floating point: packing, unpacking, and the linear layer on packed weights (differentiable in x and
+// bias; no reference counterpart).
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_vk(const at::Tensor& x);
+at::Tensor dequant_mxfp4_vk(const at::Tensor& codes, const at::Tensor& scale, at::ScalarType out_dtype, int64_t cols);
+at::Tensor mxfp4_linear_vk(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
+                           bool quantize_input);
+
 }  // namespace vkt

@@ -270,6 +270,66 @@ def dequant_int8_linear(x, q, scale, bias=None):
     return _C.dequant_int8_linear(x, q.contiguous(), scale.contiguous(), bias)
 
 
+_MXFP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)  # e2m1 codes 0..7; bit 3 is the sign
+
+
+def quantize_mxfp4(x):
+    """Pack x [..., cols] (float32, bfloat16 or float16) into microscaled 4-bit floating point: (codes, scale), uint8
+    [..., ceil(cols / 2)] and [..., ceil(cols / 32)].
+
+    Blocks of 32 consecutive values share a scale byte s, and a value reads back as e2m1 * 2**(s - 127) with e2m1 in
+    0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign.  s = floor(log2(largest magnitude)) - 2 + 127, at least 0; each value is
+    rounded to the nearest code, ties to the even one, and saturates at 6.  Two codes a byte, the even element in the low
+    nibble.  A block with an infinity or NaN gets s = 255 and reads back as NaN.  Not differentiable.
+    """
+    if x.device.type == "vk":
+        return _C.quantize_mxfp4(x)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1:
+        raise RuntimeError("quantize_mxfp4: x must be a float32, bfloat16 or float16 tensor of at least one dimension")
+    cols = x.shape[-1]
+    nb = (cols + 31) // 32
+    v = torch.zeros((*x.shape[:-1], nb * 32), dtype=torch.float64)  # exact: quotients by powers of two
+    v[..., :cols] = x.detach()
+    v = v.view(*x.shape[:-1], nb, 32)
+    bits = v.float().abs().view(torch.int32).amax(-1) >> 23  # biased exponents; 255 for infinities and NaN
+    scale = torch.where(bits == 255, 255, (bits - 2).clamp(min=0))
+    m = v * torch.exp2(127.0 - scale.double()).unsqueeze(-1)
+    m = torch.where(scale.unsqueeze(-1) == 255, torch.zeros_like(m), m)
+    a = m.abs()
+    code = sum(((a > t) if i % 2 == 0 else (a >= t)).to(torch.uint8) for i, t in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)))
+    code = (code + 8 * torch.signbit(m).to(torch.uint8)).flatten(-2)
+    packed = (code[..., 0::2] | (code[..., 1::2] << 4))[..., : (cols + 1) // 2]
+    return packed.contiguous(), scale.to(torch.uint8)
+
+
+def dequant_mxfp4(codes, scale, out_dtype=torch.bfloat16, cols=None):
+    """The values that quantize_mxfp4's (codes, scale) stand for, [..., cols] in out_dtype (rounded once: exact in float32
+    and bfloat16 up to overflow).  cols: the rows' length, by default twice the bytes of codes (name it where it is odd)."""
+    cols = 2 * codes.shape[-1] if cols is None else int(cols)
+    if codes.device.type == "vk":
+        return _C.dequant_mxfp4(codes, scale, out_dtype, cols)
+    if codes.dtype != torch.uint8 or scale.dtype != torch.uint8 or codes.shape[:-1] != scale.shape[:-1] or (
+            codes.shape[-1], scale.shape[-1]) != ((cols + 1) // 2, (cols + 31) // 32):
+        raise RuntimeError(f"dequant_mxfp4: codes and scale of rows of {cols} values must be uint8 [..., {(cols + 1) // 2}] and "
+                           f"[..., {(cols + 31) // 32}], got {tuple(codes.shape)} and {tuple(scale.shape)}")
+    code = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)[..., :cols].long()
+    v = torch.tensor(_MXFP4_VALUES, dtype=torch.float64)[code & 7] * torch.where(code >= 8, -1.0, 1.0)
+    s = torch.where(scale == 255, float("nan"), torch.exp2(scale.double() - 127.0))
+    return (v * s.repeat_interleave(32, -1)[..., :cols]).to(out_dtype)
+
+
+def mxfp4_linear(x, codes, scale, bias=None, quantize_input=False):
+    """Linear layer on frozen 4-bit weights: x @ dequant_mxfp4(codes, scale, x.dtype).T (+ bias), x [..., K] bf16/f16 on vk,
+    codes [N, ceil(K / 2)], scale [N, ceil(K / 32)].  The dequantized weights never reach memory where K % 32 == 0.
+
+    quantize_input=True rounds x the same way first (quantize_mxfp4 of its rows) and multiplies 4-bit operands, which the
+    matrix cores do at four times the 16-bit rate.  Differentiable in x and bias; the gradient of a quantized x goes
+    straight through (grad @ W, as if x had gone in unrounded)."""
+    if x.device.type != "vk":
+        raise RuntimeError("mxfp4_linear: x must be a vk tensor")
+    return _C.mxfp4_linear(x, codes, scale, bias, bool(quantize_input))
+
+
 def event_record(slot: int) -> None:
     """Record HIP event `slot` (0..1023) on the runtime's stream (the stream every vk kernel runs on)."""
     _C.event_record(int(slot))

@@ -50,6 +50,15 @@ EW_OPS = {n: i for i, n in enumerate((
     "gelu_tanh_bwd", "addcmul", "addcdiv", "lerp_s", "where"))}
 
 
+class Mx4Args(ctypes.Structure):
+    _fields_ = [("x", u64), ("codes", u64), ("scale", u64), ("rows", i64), ("cols", i64), ("x_sr", i64)]
+
+
+class Mx4MmArgs(ctypes.Structure):
+    _fields_ = [("x", u64), ("x_scale", u64), ("w", u64), ("w_scale", u64), ("bias", u64), ("y", u64), ("ws", u64),
+                ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64), ("ws_floats", i64)]
+
+
 class ReduceArgs(ctypes.Structure):
     _fields_ = [("x", u64), ("out", u64), ("ws", u64), ("ndim", i32), ("x_dtype", i32), ("out_dtype", i32),
                 ("reduce_mask", u32), ("div", f32), ("pad", u32), ("sizes", i64 * MAX_DIMS), ("strides", i64 * MAX_DIMS)]
