@@ -268,6 +268,41 @@ typedef struct hrt_attn_args {
  * added in order (HRT_ATTN_DKDV_WS). */
 int64_t hrt_attn_dkdv_workspace(const hrt_attn_args* args);
 
+/* Attention with a learned relative position bias (no reference counterpart): q [B, H, Sq, D], k, v [B, H, Sk, D] views as for
+ * "attn_fwd_{dt}", table [buckets, H] contiguous of the same type, D <= 128,
+ *   s = scale * q k^T + table[bucket(j - i - q_off), h],  P = softmax of s over the allowed keys,  o = P v.
+ * bucket(r): causal != 0: n = max(-r, 0) over nb = buckets; else n = |r| over nb = buckets / 2, plus nb where r > 0.  With
+ * e = nb / 2: n below e, else the largest e + t <= nb - 1 with (n / e)^(nb - e) >= (max_distance / e)^t, decided in whole
+ * numbers.  Key j is allowed where mask (one byte a key, rows mask_sb apart, 0: no mask) is not 0 and, if causal,
+ * j <= i + q_off.  A row without an allowed key gives o = 0, lse = -inf and no gradient; masked keys and values are not read.
+ *  "attn_rel_fwd_{dt}":  o [B, Sq, H, D]-contiguous, lse fp32 [B, H, Sq].  ws (optional): ws_floats of fp32 workspace, where
+ *     hrt_attn_rel_workspace(&args, dtype, 0) asks for them: few query rows then share their keys out over workgroups.
+ *  "attn_rel_dq_{dt}":   delta[b, h, i] = rowsum(o dout) (fp32, from the o given), dq where it is not 0, and, where dtable != 0, dtable
+ *     [buckets, H] of the type (rounded once), with ws of hrt_attn_rel_workspace(&args, dtype, 1) floats, which it needs then.
+ *  "attn_rel_dkdv_{dt}": dk, dv, from the delta that dq stored.
+ * dq, dk, dv are [B, S, H, D]-contiguous, or with HRT_ATTN_GRAD_LIKE_INPUT in the strides of q, k, v.  All rows (and o, the
+ * gradients) 16-byte aligned, D a multiple of 8 (f32: 4).  16-bit P and dS are rounded to the type before the second
+ * product; the bias, the softmax and the table's gradient are fp32.  buckets: causal 2..256, else even, 4..512;
+ * e < max_distance <= 1024. */
+typedef struct hrt_attn_rel_args {
+  uint64_t q, k, v, table, mask;
+  uint64_t o, lse, dout, delta;
+  uint64_t dq, dk, dv, dtable, ws;
+  int64_t q_sb, q_sh, q_ss;
+  int64_t k_sb, k_sh, k_ss;
+  int64_t v_sb, v_sh, v_ss;
+  int64_t do_sb, do_sh, do_ss;
+  int64_t mask_sb, q_off, ws_floats;
+  int32_t B, H, Sq, Sk, D, buckets, max_distance, causal;
+  float scale;
+  uint32_t flags;
+} hrt_attn_rel_args;
+/* fp32 elements of workspace: backward 0: those that make the forward faster (0: none), 1: those that dtable needs. */
+int64_t hrt_attn_rel_workspace(const hrt_attn_rel_args* args, int32_t dtype, int32_t backward);
+/* The buckets' borders: start[t], t < nb of one direction, is the least distance n in bucket t (a bucket that none falls into
+ * starts where the next one does).  Returns nb, or -1 for values that the kernels refuse.  A pure host function. */
+int hrt_attn_rel_buckets(int32_t buckets, int32_t max_distance, int32_t causal, uint16_t start[256]);
+
 /* Row softmax over R of a contiguous [outer, R, inner] tensor (vkrt/shaders/softmax.comp.in:27-50):
  *  "softmax_fwd_{dt}": y = exp(x - max) / sum(exp(x - max)); with safe != 0 a row whose entries are all
  *                      -inf gives 0 (_safe_softmax).

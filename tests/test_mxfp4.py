@@ -242,7 +242,7 @@ def test_gradients(M, N, K, quantize):
     check(db, g64.sum(0), np.abs(g64).sum(0), M, dtype)
     # only what is asked for; a gradient broadcast from one value; leading dimensions
     X3 = x.view(1, M, K).to(vk).requires_grad_()
-    torch_vulkan.mxfp4_linear(X3, codes.to(vk), scale.to(vk), b.to(vk), quantize).sum().backward()
+    torch_vulkan.mxfp4_linear(X3, codes.to(vk), scale.to(vk), quantize_input=quantize).sum().backward()
     check(X3.grad.view(M, K), np.ones((M, N)) @ w, np.ones((M, N)) @ np.abs(w), N, dtype)
     frozen = torch_vulkan.mxfp4_linear(x.to(vk), codes.to(vk), scale.to(vk), B, quantize)
     frozen.sum().backward()

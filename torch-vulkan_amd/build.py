@@ -52,6 +52,10 @@ HRT_SOURCES = [
     "kernels/attn_bwd.hip",
     "kernels/attn_f32.hip",
     "kernels/attn_f32_mfma.hip",
+    "kernels/attn_rel.hip",
+    "kernels/attn_rel_bf16.hip",
+    "kernels/attn_rel_f16.hip",
+    "kernels/attn_rel_f32.hip",
 ]
 SHIM_SOURCES = [
     "shim/device.cpp",
@@ -64,6 +68,7 @@ SHIM_SOURCES = [
     "shim/op_reduce.cpp",
     "shim/op_quant.cpp",
     "shim/op_mx4.cpp",
+    "shim/op_relbias.cpp",
     "shim/op_ew.cpp",
     "shim/op_image.cpp",
 ]

@@ -1,0 +1,231 @@
+// Attention with a relative position bias: argument checks, the buckets' borders, the plan, and the two small kernels that
+// join partial results.  The attention kernel itself is attn_rel.h.
+#include <cmath>
+#include <cstring>
+#include <vector>
+
+#include "../hrt/registry.h"
+#include "attn_rel_plan.h"
+
+namespace hk {
+
+namespace {
+
+// ---- buckets ---------------------------------------------------------------------------------------------------------------
+// a^x b^y as little-endian 32-bit digits.
+std::vector<uint32_t> power_product(uint32_t a, int x, uint32_t b, int y) {
+  std::vector<uint32_t> v{1};
+  for (int i = 0; i < x + y; ++i) {
+    uint64_t carry = 0;
+    for (uint32_t& d : v) carry += (uint64_t)d * (i < x ? a : b), d = (uint32_t)carry, carry >>= 32;
+    if (carry) v.push_back((uint32_t)carry);
+  }
+  return v;
+}
+
+// (n / e)^L >= (m / e)^t, exactly: by logarithms where they differ clearly, else n^L e^t >= m^t e^L in whole numbers.
+bool reaches(int n, int e, int L, int m, int t) {
+  const double a = L * std::log((double)n / e), b = t * std::log((double)m / e);
+  if (std::fabs(a - b) > 1e-9 * (1.0 + std::fabs(b))) return a > b;
+  const std::vector<uint32_t> x = power_product(n, L, e, t), y = power_product(m, t, e, L);
+  if (x.size() != y.size()) return x.size() > y.size();
+  for (size_t i = x.size(); i-- > 0;)
+    if (x[i] != y[i]) return x[i] > y[i];
+  return true;
+}
+
+bool make_buckets(int buckets, int m, int causal, RelBuckets* out) {
+  const int nb = causal ? buckets : buckets / 2, e = nb / 2;
+  if ((!causal && buckets % 2 != 0) || nb < 2 || nb > 256 || m <= e || m > 1024) return false;
+  out->nb = nb, out->sides = causal ? 1 : 2, out->total = buckets;
+  for (int k = 0; k <= e; ++k) out->start[k] = (uint16_t)k;
+  const int L = nb - e;
+  for (int t = 1, n = e; t < L; ++t) {
+    while (!reaches(n, e, L, m, t)) ++n;  // borders rise with t: m distances in all
+    out->start[e + t] = (uint16_t)n;
+  }
+  out->R = out->start[nb - 1];
+  return true;
+}
+
+// The last one is kept: a model has one kind of bias, and every launch needs it.
+const RelBuckets* buckets_of(const hrt_attn_rel_args& a) {
+  thread_local int key[3] = {-1, -1, -1};
+  thread_local RelBuckets kept;
+  const int want[3] = {a.buckets, a.max_distance, a.causal != 0};
+  if (memcmp(key, want, sizeof(key)) != 0) {
+    key[0] = -1;
+    if (!make_buckets(want[0], want[1], want[2], &kept)) return nullptr;
+    memcpy(key, want, sizeof(key));
+  }
+  return &kept;
+}
+
+// ---- plan ------------------------------------------------------------------------------------------------------------------
+RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R) {
+  const int64_t n = which == 1 ? a.Sk : a.Sq, bh = (int64_t)a.B * a.H;
+  auto blocks = [&](int g) { return cdiv(n, 32 * g); };
+  const int dp = a.D <= 64 ? 64 : 128;
+  RelPlan p{};
+  p.g = blocks(4) * bh >= 512 ? 4 : f32 || blocks(2) * bh >= 256 ? 2 : 1;
+  if (f32 && dp == 128) p.g = 4;  // the other forms' stages fill LDS
+  // four buffers of 128 rows leave 30 KiB for the bands of far-reaching tables
+  if (p.g == 1 && dp == 128 && rel_lds(which, R) > 30 * 1024) p.g = 2;
+  p.nblk = (int)blocks(p.g);
+  p.splits = 1;
+  const int64_t stages = cdiv(a.Sk, rel_stage(f32, dp, p.g)), wgs = p.nblk * bh;
+  p.per = (int)stages;
+  if (which == 0 && ws && wgs < 256 && stages >= 4) {
+    const int64_t want = cdiv(512, wgs), most = stages / 2;
+    p.per = (int)cdiv(stages, want < most ? want : most);
+    p.splits = (int)cdiv(stages, p.per);
+  }
+  return p;
+}
+
+// ---- joins -----------------------------------------------------------------------------------------------------------------
+// Forward partial sums of the key ranges, added in order: a wavefront per row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_rel_join(hrt_attn_rel_args p, int splits, int64_t rows) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const HK_G float* o = gcptr<float>(p.ws);
+  const HK_G float* ms = o + splits * rows * p.D;
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, ms[(s * rows + row) * 2]);
+  float l = 0.f, acc[2] = {0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float mk = ms[(s * rows + row) * 2], f = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - m);
+    l += f * ms[(s * rows + row) * 2 + 1];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 64 * u < p.D) acc[u] += f * o[(s * rows + row) * p.D + lane + 64 * u];
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int64_t q = row % p.Sq, bh = row / p.Sq, b = bh / p.H, h = bh % p.H;
+  if (lane == 0) gptr<float>(p.lse)[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  HK_G typename T::storage* out = gptr<typename T::storage>(p.o) + ((b * p.Sq + q) * p.H + h) * p.D;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 64 * u < p.D) out[lane + 64 * u] = T::from_f32(acc[u] * inv);
+}
+
+// dtable[k, h] = the workgroups' partial sums [H][n][buckets], a wavefront per value: lanes stride the partial sums, then one
+// fixed exchange.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_rel_table(hrt_attn_rel_args p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (int64_t)p.buckets * p.H) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t h = i / p.buckets, k = i % p.buckets;
+  const HK_G float* part = gcptr<float>(p.ws) + h * n * p.buckets + k;
+  float s = 0.f;
+  for (int64_t j = lane; j < n; j += 64) s += part[j * p.buckets];
+  s = wave_sum(s);
+  if (lane == 0) gptr<typename T::storage>(p.dtable)[k * p.H + h] = T::from_f32(s);
+}
+
+// ---- launch ----------------------------------------------------------------------------------------------------------------
+bool check(const hrt_attn_rel_args& a, int which, int esz, hrt::LaunchCtx& ctx) {
+  if (a.B < 1 || a.H < 1 || a.Sq < 1 || a.Sk < 1 || a.D < 1 || a.D > 128) return ctx.fail("attention needs B, H, Sq, Sk >= 1 and 1 <= D <= 128");
+  const int per16 = 16 / esz;
+  if (a.D % per16 != 0) return ctx.fail("D must fill 16-byte pieces");
+  if (!(a.scale >= 1e-20f && a.scale <= 1e20f)) return ctx.fail("scale must lie in 1e-20 .. 1e20");
+  if (a.q_off < -((int64_t)1 << 40) || a.q_off > ((int64_t)1 << 40)) return ctx.fail("query offset out of range");
+  const int64_t strides[] = {a.q_sb, a.q_sh, a.q_ss, a.k_sb, a.k_sh, a.k_ss, a.v_sb, a.v_sh, a.v_ss, a.do_sb, a.do_sh, a.do_ss};
+  const int nstr = which == 0 ? 9 : 12;
+  for (int i = 0; i < nstr; ++i)
+    if (strides[i] < 0 || strides[i] % per16 != 0) return ctx.fail("strides must be non-negative and keep rows on 16 bytes");
+  if (a.mask && a.mask_sb < 0) return ctx.fail("negative mask stride");
+  const int64_t lim = ((int64_t)1 << 31) / (130 * esz);  // a stage's row offsets are 31-bit
+  for (int i : {2, 5, 8, 11})
+    if (i < nstr && strides[i] >= lim) return ctx.fail("rows too far apart");
+  auto view = [&](uint64_t at, int i, int64_t S, const char* what) {
+    const int64_t sz[4] = {a.B, a.H, S, a.D}, st[4] = {strides[i], strides[i + 1], strides[i + 2], 1};
+    if (at % 16 != 0) return ctx.fail(std::string(what) + " must be 16-byte aligned");
+    return ctx.check(at, hrt::span_bytes(4, sz, st, (uint64_t)esz), what);
+  };
+  const uint64_t bh = (uint64_t)a.B * a.H, rows = bh * (uint64_t)a.Sq;
+  if (!view(a.q, 0, a.Sq, "q") || !view(a.k, 3, a.Sk, "k") || !view(a.v, 6, a.Sk, "v") ||
+      !ctx.check(a.table, (uint64_t)a.buckets * a.H * esz, "table") || !ctx.check(a.lse, rows * 4, "lse"))
+    return false;
+  if (a.mask && !ctx.check(a.mask, (uint64_t)((a.B - 1) * a.mask_sb + a.Sk), "mask")) return false;
+  if (which != 1 && a.o % 16 != 0) return ctx.fail("o must be 16-byte aligned");
+  if (which != 1 && !ctx.check(a.o, rows * a.D * esz, "o")) return false;
+  if (which != 0 && (!view(a.dout, 9, a.Sq, "dout") || !ctx.check(a.delta, rows * 4, "delta"))) return false;
+  // gradients: contiguous, or spread like their inputs
+  auto grad = [&](uint64_t at, int i, int64_t S, const char* what) {
+    if (a.flags & HRT_ATTN_GRAD_LIKE_INPUT) return view(at, i, S, what);
+    if (at % 16 != 0) return ctx.fail(std::string(what) + " must be 16-byte aligned");
+    return ctx.check(at, bh * (uint64_t)S * a.D * esz, what);
+  };
+  if (which == 1 && (!grad(a.dk, 3, a.Sk, "dk") || !grad(a.dv, 6, a.Sk, "dv"))) return false;
+  if (which == 2 && a.dq && !grad(a.dq, 0, a.Sq, "dq")) return false;
+  return true;
+}
+
+int64_t fwd_floats(const hrt_attn_rel_args& a, const RelPlan& p) { return p.splits > 1 ? (int64_t)p.splits * a.B * a.H * a.Sq * (a.D + 2) : 0; }
+int64_t table_floats(const hrt_attn_rel_args& a, const RelPlan& p) { return (int64_t)a.B * a.H * p.nblk * a.buckets; }
+
+template <typename T, int WHICH>
+bool launch_rel(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
+  const auto& a = *static_cast<const hrt_attn_rel_args*>(pp);
+  constexpr int esz = sizeof(typename T::storage);
+  const RelBuckets* bk = buckets_of(a);
+  if (bk == nullptr) return ctx.fail("buckets: causal 2..256, else even and 4..512, with max_distance above half of one direction's and at most 1024");
+  if (!check(a, WHICH, esz, ctx)) return false;
+  RelPlan pl = plan_of(a, WHICH, esz == 4, a.ws != 0, bk->R);
+  if (WHICH == 0 && pl.splits > 1) {
+    const int64_t need = fwd_floats(a, pl);
+    if (a.ws % 16 != 0 || a.ws_floats < need) pl = plan_of(a, WHICH, esz == 4, false, bk->R);
+    else if (!ctx.check(a.ws, (uint64_t)need * 4, "ws")) return false;
+  }
+  if (WHICH == 2 && a.dtable) {
+    const int64_t need = table_floats(a, pl);
+    if (a.ws_floats < need || a.ws % 4 != 0) return ctx.fail("the table's gradient needs a workspace of hrt_attn_rel_workspace floats");
+    if (!ctx.check(a.ws, (uint64_t)need * 4, "ws") || !ctx.check(a.dtable, (uint64_t)a.buckets * a.H * esz, "dtable")) return false;
+  }
+  if (!hrt::grid_fits((int64_t)pl.nblk * a.B * a.H * pl.splits, 256) || !hrt::grid_fits(cdiv((int64_t)a.B * a.H * a.Sq, 4), 256))
+    return ctx.fail("too many rows for one launch");
+  attn_rel_queue<T>(a, WHICH, *bk, pl, ctx.stream);
+  if (!hrt::launch_ok(hipGetLastError(), ctx, "attn_rel")) return false;
+  if (WHICH == 0 && pl.splits > 1) {
+    const int64_t rows = (int64_t)a.B * a.H * a.Sq;
+    hipLaunchKernelGGL(attn_rel_join<T>, dim3((uint32_t)cdiv(rows, 4)), dim3(256), 0, ctx.stream, a, pl.splits, rows);
+    return hrt::launch_ok(hipGetLastError(), ctx, "attn_rel_join");
+  }
+  if (WHICH == 2 && a.dtable) {
+    hipLaunchKernelGGL(attn_rel_table<T>, dim3((uint32_t)cdiv((int64_t)a.buckets * a.H, 4)), dim3(256), 0, ctx.stream, a, (int64_t)a.B * pl.nblk);
+    return hrt::launch_ok(hipGetLastError(), ctx, "attn_rel_table");
+  }
+  return true;
+}
+
+HRT_REGISTER("attn_rel_fwd_f32", hrt_attn_rel_args, (launch_rel<F32, 0>));
+HRT_REGISTER("attn_rel_fwd_bf16", hrt_attn_rel_args, (launch_rel<BF16, 0>));
+HRT_REGISTER("attn_rel_fwd_f16", hrt_attn_rel_args, (launch_rel<F16, 0>));
+HRT_REGISTER("attn_rel_dkdv_f32", hrt_attn_rel_args, (launch_rel<F32, 1>));
+HRT_REGISTER("attn_rel_dkdv_bf16", hrt_attn_rel_args, (launch_rel<BF16, 1>));
+HRT_REGISTER("attn_rel_dkdv_f16", hrt_attn_rel_args, (launch_rel<F16, 1>));
+HRT_REGISTER("attn_rel_dq_f32", hrt_attn_rel_args, (launch_rel<F32, 2>));
+HRT_REGISTER("attn_rel_dq_bf16", hrt_attn_rel_args, (launch_rel<BF16, 2>));
+HRT_REGISTER("attn_rel_dq_f16", hrt_attn_rel_args, (launch_rel<F16, 2>));
+
+}  // namespace
+}  // namespace hk
+
+extern "C" int64_t hrt_attn_rel_workspace(const hrt_attn_rel_args* a, int32_t dtype, int32_t backward) {
+  if (a == nullptr || a->B < 1 || a->H < 1 || a->Sq < 1 || a->Sk < 1) return 0;
+  const hk::RelBuckets* bk = hk::buckets_of(*a);
+  if (bk == nullptr) return 0;
+  const bool f32 = dtype == HRT_F32;
+  return backward ? hk::table_floats(*a, hk::plan_of(*a, 2, f32, false, bk->R)) : hk::fwd_floats(*a, hk::plan_of(*a, 0, f32, true, bk->R));
+}
+
+extern "C" int hrt_attn_rel_buckets(int32_t buckets, int32_t max_distance, int32_t causal, uint16_t start[256]) {
+  hk::RelBuckets b;
+  if (start == nullptr || !hk::make_buckets(buckets, max_distance, causal != 0, &b)) return -1;
+  memcpy(start, b.start, sizeof(uint16_t) * b.nb);
+  return b.nb;
+}

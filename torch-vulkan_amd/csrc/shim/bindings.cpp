@@ -108,6 +108,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     runtime();
     return mxfp4_linear_vk(x, codes, scale, bias, quantize_input);
   });
+  m.def("relative_bias_attention",
+        [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const std::optional<at::Tensor>& key_mask,
+           bool causal, std::optional<double> scale, int64_t max_distance, int64_t query_offset) {
+          runtime();
+          return relative_bias_attention_vk(q, k, v, table, key_mask, causal, scale, max_distance, query_offset);
+        });
   // accounting and profiling
   m.def("kernel_counts", &gpu_counts);
   m.def("fallback_counts", &cpu_counts);

@@ -90,6 +90,7 @@ struct Linear : torch::autograd::Function<Linear> {
                             const std::optional<at::Tensor>& bias, bool quantize) {
     ctx->save_for_backward({codes, scale});
     ctx->saved_data["sizes"] = x.sizes().vec();
+    ctx->saved_data["biased"] = present(bias);
     std::vector<int64_t> out = x.sizes().vec();
     out.back() = codes.size(0);
     return linear_rows(as_rows(x), codes, scale, bias, quantize).view(out);
@@ -102,7 +103,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const at::Tensor g = as_rows(grads[0]);
     if (ctx->needs_input_grad(0)) out[0] = at::mm(g, dequant_mxfp4_vk(saved[0], saved[1], g.scalar_type(), sizes.back())).view(sizes);
-    if (ctx->needs_input_grad(3)) out[3] = g.sum(0);
+    if (ctx->saved_data["biased"].toBool() && ctx->needs_input_grad(3)) out[3] = g.sum(0);
     note_gpu("torch_vulkan::mxfp4_linear_backward");
     return out;
   }

@@ -330,6 +330,25 @@ def mxfp4_linear(x, codes, scale, bias=None, quantize_input=False):
     return _C.mxfp4_linear(x, codes, scale, bias, bool(quantize_input))
 
 
+def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=None, max_distance=128, query_offset=0):
+    """Fused attention with a learned relative position bias: softmax(scale * q @ k.T + table[bucket(j - i - query_offset)]) @ v.
+
+    q [B, H, Sq, D], k, v [B, H, Sk, D] on vk (float32, bfloat16 or float16, D <= 128, any strides), table [buckets, H] of the
+    same dtype: one learned bias per bucket and head.  i and j count queries and keys; query_offset is the position of query
+    0 among the keys (new tokens after a cache of n: n).  scale defaults to 1 / sqrt(D).
+
+    Buckets of the distance r = j - i - query_offset: with causal=False half of them serve r <= 0 and half r > 0, with causal=True
+    (which also hides keys j > i + query_offset) all serve r <= 0.  Of a direction's nb buckets the first nb // 2 hold one
+    distance each, the others grow logarithmically up to max_distance, and the last one holds everything beyond.
+
+    key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen; masked keys and values are not read, whatever they
+    hold.  A query without a key to see gets zeros and no gradient.  Returns [B, H, Sq, D]; differentiable once in q, k, v and
+    table.  Nothing of size Sq x Sk is stored."""
+    if q.device.type != "vk":
+        raise RuntimeError("relative_bias_attention: q must be a vk tensor")
+    return _C.relative_bias_attention(q, k, v, table, key_mask, bool(causal), scale, int(max_distance), int(query_offset))
+
+
 def event_record(slot: int) -> None:
     """Record HIP event `slot` (0..1023) on the runtime's stream (the stream every vk kernel runs on)."""
     _C.event_record(int(slot))

@@ -59,6 +59,14 @@ class Mx4MmArgs(ctypes.Structure):
                 ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64), ("ws_floats", i64)]
 
 
+class AttnRelArgs(ctypes.Structure):
+    _fields_ = ([(n, u64) for n in ("q", "k", "v", "table", "mask", "o", "lse", "dout", "delta", "dq", "dk", "dv", "dtable", "ws")]
+                + [(f"{t}_s{d}", i64) for t in ("q", "k", "v", "do") for d in "bhs"]
+                + [("mask_sb", i64), ("q_off", i64), ("ws_floats", i64)]
+                + [(n, i32) for n in ("B", "H", "Sq", "Sk", "D", "buckets", "max_distance", "causal")]
+                + [("scale", f32), ("flags", u32)])
+
+
 class ReduceArgs(ctypes.Structure):
     _fields_ = [("x", u64), ("out", u64), ("ws", u64), ("ndim", i32), ("x_dtype", i32), ("out_dtype", i32),
                 ("reduce_mask", u32), ("div", f32), ("pad", u32), ("sizes", i64 * MAX_DIMS), ("strides", i64 * MAX_DIMS)]
