@@ -284,6 +284,9 @@ int64_t hrt_attn_dkdv_workspace(const hrt_attn_args* args);
  * gradients) 16-byte aligned, D a multiple of 8 (f32: 4).  16-bit P and dS are rounded to the type before the second
  * product; the bias, the softmax and the table's gradient are fp32.  buckets: causal 2..256, else even, 4..512;
  * e < max_distance <= 1024. */
+/* "attn_rel_dq_{dt}" with this flag leaves the table's partial sums in ws, and "attn_rel_dkdv_{dt}" with it (the same dtable,
+ * ws and ws_floats) finishes dtable beside its own work: one launch less. */
+#define HRT_ATTN_REL_TABLE_LATER 16u
 typedef struct hrt_attn_rel_args {
   uint64_t q, k, v, table, mask;
   uint64_t o, lse, dout, delta;

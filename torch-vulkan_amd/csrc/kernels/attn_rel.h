@@ -164,6 +164,7 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   __shared__ __attribute__((aligned(1024))) uint8_t a0_raw[TB], a1_raw[TB], b0_raw[TB], b1_raw[TB];
   __shared__ float stat[2][2][WHICH == 1 ? ST : 1];  // dK/dV: lse (log2 units) and delta of the streamed rows, per buffer
   __shared__ float ml[3][64][2];                     // the merge's maxima and sums; dQ: sums beyond R
+  __shared__ int border[WHICH == 2 ? 256 : 1];       // dQ: the buckets' borders
   extern __shared__ float dyn[];
   auto abuf = [&](auto ic) { return (HK_L uint8_t*)(decltype(ic)::value ? a1_raw : a0_raw); };
   auto bbuf = [&](auto ic) { return (HK_L uint8_t*)(decltype(ic)::value ? b1_raw : b0_raw); };
@@ -171,6 +172,13 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = wave % G, kh = wave / G, l32 = lane & 31, h = lane >> 5;
   uint32_t bh, blk, total = (uint32_t)pl.nblk * p.B * p.H, id = blockIdx.x, split = 0;
+  if constexpr (WHICH == 1) {
+    if (id < (uint32_t)pl.table) {
+      rel_table<T>(p, pl.parts, (int64_t)id * 4 + wave, lane);
+      return;
+    }
+    id -= (uint32_t)pl.table;
+  }
   if (WHICH == 0 && pl.splits > 1) split = id / total, id -= split * total;
   xcd_map32(id, total, pl.nblk, bh, blk);
   bh = __builtin_amdgcn_readfirstlane(bh), blk = __builtin_amdgcn_readfirstlane(blk), split = __builtin_amdgcn_readfirstlane(split);
@@ -271,18 +279,21 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   float* const sums = dyn + NB * (1 + wave);                      // dQ: this wavefront's sums by distance
   float* const patch = dyn + NB * 5 + wave * (32 * 33);           // dQ: its patch
   const float inv_scale = 1.f / p.scale;
-  for (int k = tid; k < bk.total; k += 256) {
-    const bool pos = k >= bk.nb;
-    const int j = pos ? k - bk.nb : k;
-    const float v = T::to_f32(table[(int64_t)k * p.H]) * inv_scale;
-    const int lo = bk.start[j], hi = j + 1 < bk.nb ? bk.start[j + 1] : mid + 1;
-    for (int n = lo; n < hi; ++n)
-      if (!(pos && n == 0)) band[pos ? mid + n : mid - n] = v;
+  for (int t = tid; t < NB; t += 256) {  // the borders are scalars: a distance counts those that it reaches
+    const int r = t - mid, n = r < 0 ? -r : r;
+    int k = 0;
+    for (int i = 1; i < bk.nb; ++i) k += n >= bk.start[i];
+    // one direction: positive distances are masked, and their values not used
+    band[t] = r > 0 && bk.sides == 1 ? 0.f : T::to_f32(table[(int64_t)(r > 0 ? bk.nb + k : k) * p.H]) * inv_scale;
   }
-  if (bk.sides == 1)  // one direction: positive distances are masked, and their values not used
-    for (int n = tid + 1; n <= mid; n += 256) band[mid + n] = 0.f;
-  if constexpr (WHICH == 2)
-    for (int t = lane; t < NB; t += 64) sums[t] = 0.f;
+  if constexpr (WHICH == 2) {
+    if (p.dtable) {
+      for (int t = lane; t < NB; t += 64) sums[t] = 0.f;
+      int from = 0;
+      for (int i = 1; i < bk.nb; ++i) from = tid == i ? bk.start[i] : from;
+      border[tid] = from;
+    }
+  }
   const float far_lo = T::to_f32(table[(int64_t)(bk.nb - 1) * p.H]) * kLog2e;
   const float far_hi = bk.sides == 2 ? T::to_f32(table[(int64_t)(bk.total - 1) * p.H]) * kLog2e : 0.f;
 
@@ -491,26 +502,26 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
     }
   }
 
-  if constexpr (WHICH == 2) {  // this workgroup's sums by bucket, wavefronts in order
+  if constexpr (WHICH == 2) {  // this workgroup's sums by bucket
     if (p.dtable) {
       const float lo = wave_sum(beyond_lo), hi = wave_sum(beyond_hi);
       __syncthreads();
       if (lane == 0) ml[0][wave][0] = lo, ml[0][wave][1] = hi;
+      for (int t = tid; t < NB; t += 256) band[t] = (dyn[NB + t] + dyn[2 * NB + t]) + (dyn[3 * NB + t] + dyn[4 * NB + t]);
       __syncthreads();
-      // partial sums [H][B][nblk][buckets]
+      // partial sums [H][B][nblk][buckets]; eight lanes a bucket
       HK_G float* const out = gptr<float>(p.ws) + ((hh * p.B + b) * pl.nblk + blk) * (int64_t)bk.total;
-      for (int k = tid; k < bk.total; k += 256) {
+      for (int k = tid >> 3; k < bk.total; k += 32) {
         const bool pos = k >= bk.nb;
         const int j = pos ? k - bk.nb : k;
-        const int from = bk.start[j], to = j + 1 < bk.nb ? bk.start[j + 1] : mid + 1;
+        const int from = border[j], to = j + 1 < bk.nb ? border[j + 1] : mid + 1;
         float t = 0.f;
-        for (int wv = 0; wv < 4; ++wv) {
-          const float* const sw = dyn + NB * (1 + wv);
-          for (int n = from; n < to; ++n)
-            if (!(pos && n == 0)) t += sw[pos ? mid + n : mid - n];
-          if (j + 1 == bk.nb) t += ml[0][wv][pos ? 1 : 0];
-        }
-        out[k] = t;
+        for (int n = from + (tid & 7); n < to; n += 8)
+          if (!(pos && n == 0)) t += band[pos ? mid + n : mid - n];
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) t += __shfl_xor(t, x, 64);
+        if (j + 1 == bk.nb) t += (ml[0][0][pos] + ml[0][1][pos]) + (ml[0][2][pos] + ml[0][3][pos]);
+        if ((tid & 7) == 0) out[k] = t;
       }
     }
   }
@@ -559,7 +570,7 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
 
 template <typename T, int WHICH, int DP, int G>
 void attn_rel_go(const hrt_attn_rel_args& a, const RelBuckets& bk, const RelPlan& pl, hipStream_t s) {
-  const uint32_t grid = (uint32_t)((int64_t)pl.nblk * a.B * a.H * pl.splits);
+  const uint32_t grid = (uint32_t)((int64_t)pl.nblk * a.B * a.H * pl.splits + pl.table);
   hipLaunchKernelGGL((attn_rel_k<T, WHICH, DP, G>), dim3(grid), dim3(256), (RelShape<T, WHICH, DP, G>::lds(bk.R)), s, a, bk, pl);
 }
 

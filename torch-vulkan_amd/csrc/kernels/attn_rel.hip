@@ -38,11 +38,11 @@ bool make_buckets(int buckets, int m, int causal, RelBuckets* out) {
   const int nb = causal ? buckets : buckets / 2, e = nb / 2;
   if ((!causal && buckets % 2 != 0) || nb < 2 || nb > 256 || m <= e || m > 1024) return false;
   out->nb = nb, out->sides = causal ? 1 : 2, out->total = buckets;
-  for (int k = 0; k <= e; ++k) out->start[k] = (uint16_t)k;
+  for (int k = 0; k <= e; ++k) out->start[k] = k;
   const int L = nb - e;
   for (int t = 1, n = e; t < L; ++t) {
     while (!reaches(n, e, L, m, t)) ++n;  // borders rise with t: m distances in all
-    out->start[e + t] = (uint16_t)n;
+    out->start[e + t] = n;
   }
   out->R = out->start[nb - 1];
   return true;
@@ -69,8 +69,8 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
   RelPlan p{};
   p.g = blocks(4) * bh >= 512 ? 4 : f32 || blocks(2) * bh >= 256 ? 2 : 1;
   if (f32 && dp == 128) p.g = 4;  // the other forms' stages fill LDS
-  // four buffers of 128 rows leave 30 KiB for the bands of far-reaching tables
-  if (p.g == 1 && dp == 128 && rel_lds(which, R) > 30 * 1024) p.g = 2;
+  // four buffers of 128 rows leave 29 KiB for the bands of far-reaching tables
+  if (p.g == 1 && dp == 128 && rel_lds(which, R) > 29 * 1024) p.g = 2;
   p.nblk = (int)blocks(p.g);
   p.splits = 1;
   const int64_t stages = cdiv(a.Sk, rel_stage(f32, dp, p.g)), wgs = p.nblk * bh;
@@ -111,19 +111,9 @@ __global__ __launch_bounds__(256) void attn_rel_join(hrt_attn_rel_args p, int sp
     if (lane + 64 * u < p.D) out[lane + 64 * u] = T::from_f32(acc[u] * inv);
 }
 
-// dtable[k, h] = the workgroups' partial sums [H][n][buckets], a wavefront per value: lanes stride the partial sums, then one
-// fixed exchange.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rel_table(hrt_attn_rel_args p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= (int64_t)p.buckets * p.H) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t h = i / p.buckets, k = i % p.buckets;
-  const HK_G float* part = gcptr<float>(p.ws) + h * n * p.buckets + k;
-  float s = 0.f;
-  for (int64_t j = lane; j < n; j += 64) s += part[j * p.buckets];
-  s = wave_sum(s);
-  if (lane == 0) gptr<typename T::storage>(p.dtable)[k * p.H + h] = T::from_f32(s);
+  rel_table<T>(p, n, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), threadIdx.x & 63);
 }
 
 // ---- launch ----------------------------------------------------------------------------------------------------------------
@@ -181,12 +171,15 @@ bool launch_rel(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
     if (a.ws % 16 != 0 || a.ws_floats < need) pl = plan_of(a, WHICH, esz == 4, false, bk->R);
     else if (!ctx.check(a.ws, (uint64_t)need * 4, "ws")) return false;
   }
-  if (WHICH == 2 && a.dtable) {
-    const int64_t need = table_floats(a, pl);
+  const bool later = (a.flags & HRT_ATTN_REL_TABLE_LATER) != 0;
+  if (a.dtable && (WHICH == 2 || (WHICH == 1 && later))) {
+    const RelPlan dq = plan_of(a, 2, esz == 4, false, bk->R);
+    const int64_t need = table_floats(a, dq);
     if (a.ws_floats < need || a.ws % 4 != 0) return ctx.fail("the table's gradient needs a workspace of hrt_attn_rel_workspace floats");
     if (!ctx.check(a.ws, (uint64_t)need * 4, "ws") || !ctx.check(a.dtable, (uint64_t)a.buckets * a.H * esz, "dtable")) return false;
+    if (WHICH == 1) pl.table = (int)(cdiv((int64_t)a.buckets * a.H, 32) * 8), pl.parts = (int64_t)a.B * dq.nblk;
   }
-  if (!hrt::grid_fits((int64_t)pl.nblk * a.B * a.H * pl.splits, 256) || !hrt::grid_fits(cdiv((int64_t)a.B * a.H * a.Sq, 4), 256))
+  if (!hrt::grid_fits((int64_t)pl.nblk * a.B * a.H * pl.splits + pl.table, 256) || !hrt::grid_fits(cdiv((int64_t)a.B * a.H * a.Sq, 4), 256))
     return ctx.fail("too many rows for one launch");
   attn_rel_queue<T>(a, WHICH, *bk, pl, ctx.stream);
   if (!hrt::launch_ok(hipGetLastError(), ctx, "attn_rel")) return false;
@@ -195,7 +188,7 @@ bool launch_rel(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
     hipLaunchKernelGGL(attn_rel_join<T>, dim3((uint32_t)cdiv(rows, 4)), dim3(256), 0, ctx.stream, a, pl.splits, rows);
     return hrt::launch_ok(hipGetLastError(), ctx, "attn_rel_join");
   }
-  if (WHICH == 2 && a.dtable) {
+  if (WHICH == 2 && a.dtable && !later) {
     hipLaunchKernelGGL(attn_rel_table<T>, dim3((uint32_t)cdiv((int64_t)a.buckets * a.H, 4)), dim3(256), 0, ctx.stream, a, (int64_t)a.B * pl.nblk);
     return hrt::launch_ok(hipGetLastError(), ctx, "attn_rel_table");
   }
@@ -226,6 +219,6 @@ extern "C" int64_t hrt_attn_rel_workspace(const hrt_attn_rel_args* a, int32_t dt
 extern "C" int hrt_attn_rel_buckets(int32_t buckets, int32_t max_distance, int32_t causal, uint16_t start[256]) {
   hk::RelBuckets b;
   if (start == nullptr || !hk::make_buckets(buckets, max_distance, causal != 0, &b)) return -1;
-  memcpy(start, b.start, sizeof(uint16_t) * b.nb);
+  for (int k = 0; k < b.nb; ++k) start[k] = (uint16_t)b.start[k];
   return b.nb;
 }

@@ -8,13 +8,15 @@ namespace hk {
 // Buckets of one direction: bucket k holds the distances start[k] .. start[k + 1] - 1, the last one all from R = start[nb - 1].
 struct RelBuckets {
   int32_t nb, R, sides, total;  // sides 2: positive distances take buckets nb .. 2 nb - 1
-  uint16_t start[256];
+  int32_t start[256];
 };
 
 struct RelPlan {
   int g;             // query (key) groups per workgroup
   int nblk;          // workgroups per head along the stationary rows
   int splits, per;   // forward: key ranges and stages in each
+  int table;         // dK/dV: workgroups ahead of the others that finish the table's gradient
+  int64_t parts;     // partial sums of it per head
 };
 
 constexpr int kRelMargin = 63;  // distances of a tile that reaches beyond R on one side
@@ -23,6 +25,19 @@ constexpr int kRelMargin = 63;  // distances of a tile that reaches beyond R on 
 constexpr int rel_stage(bool f32, int dp, int g) { return f32 && dp > 64 ? 32 : g == 1 ? 128 : 64; }
 // Dynamic LDS: the band; for dQ also one band of sums and one 32 x 33 patch per wavefront.
 constexpr int rel_lds(int which, int R) { return (2 * R + 1 + 2 * kRelMargin) * 4 * (which == 2 ? 5 : 1) + (which == 2 ? 4 * 32 * 33 * 4 : 0); }
+
+// dtable[k, h] = the workgroups' partial sums [H][n][buckets], value i by one wavefront: lanes stride the partial sums, then
+// one fixed exchange.
+template <typename T>
+__device__ __forceinline__ void rel_table(const hrt_attn_rel_args& p, int64_t n, int64_t i, int lane) {
+  if (i >= (int64_t)p.buckets * p.H) return;
+  const int64_t h = i / p.buckets, k = i % p.buckets;
+  const HK_G float* part = gcptr<float>(p.ws) + h * n * p.buckets + k;
+  float s = 0.f;
+  for (int64_t j = lane; j < n; j += 64) s += part[j * p.buckets];
+  s = wave_sum(s);
+  if (lane == 0) gptr<typename T::storage>(p.dtable)[k * p.H + h] = T::from_f32(s);
+}
 
 // Queues kernel `which` (0 forward, 1 dK/dV, 2 dQ and the table's partial sums) for element type T.
 template <typename T>

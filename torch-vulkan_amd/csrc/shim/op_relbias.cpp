@@ -111,10 +111,13 @@ struct Attention : torch::autograd::Function<Attention> {
     const Options opt{ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["max_distance"].toInt(),
                       ctx->saved_data["offset"].toInt()};
     const at::Tensor dout = rows_of(grads[0].scalar_type() == q.scalar_type() ? grads[0] : grads[0].to(q.scalar_type()), q.size(3));
-    const at::Tensor delta = at::empty_like(lse);
     hrt_attn_rel_args A = base_args(q, k, v, table, mask, opt);
     put(&A.do_sb, &A.dout, dout);
-    A.o = dptr(o), A.lse = dptr(lse), A.delta = dptr(delta);
+    const bool wants_table = ctx->needs_input_grad(3), wants_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    // delta, and the partial sums of the table's gradient behind it
+    const int64_t parts = wants_table ? hrt_attn_rel_workspace(&A, float_code(q.scalar_type()), 1) : 0;
+    const at::Tensor work = at::empty({lse.numel() + parts}, lse.options());
+    A.o = dptr(o), A.lse = dptr(lse), A.delta = dptr(work);
     const bool like = q.is_non_overlapping_and_dense() && k.is_non_overlapping_and_dense() && v.is_non_overlapping_and_dense();
     if (like) A.flags = HRT_ATTN_GRAD_LIKE_INPUT;
     auto grad_for = [&](const at::Tensor& t) {
@@ -122,16 +125,15 @@ struct Attention : torch::autograd::Function<Attention> {
     };
     torch::autograd::variable_list out(9);
     // dQ first: it also leaves delta for dK/dV
-    at::Tensor dq, dtable, part;
+    at::Tensor dq, dtable;
     if (ctx->needs_input_grad(0)) dq = grad_for(q), A.dq = dptr(dq);
-    if (ctx->needs_input_grad(3)) {
+    if (wants_table) {
       dtable = at::empty_like(table);
-      const int64_t n = hrt_attn_rel_workspace(&A, float_code(q.scalar_type()), 1);
-      part = at::empty({n}, lse.options());
-      A.dtable = dptr(dtable), A.ws = dptr(part), A.ws_floats = n;
+      A.dtable = dptr(dtable), A.ws = dptr(work) + 4 * lse.numel(), A.ws_floats = parts;
+      if (wants_kv) A.flags |= HRT_ATTN_REL_TABLE_LATER;
     }
     queue(typed("attn_rel_dq", q.scalar_type()), A);
-    if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+    if (wants_kv) {
       const at::Tensor dk = grad_for(k), dv = grad_for(v);
       A.dk = dptr(dk), A.dv = dptr(dv);
       queue(typed("attn_rel_dkdv", q.scalar_type()), A);
