@@ -394,13 +394,11 @@ typedef struct hrt_mx4_args {
  * gives.  x_scale 0: x is [M, K] of the kernel's type with row stride x_sm (elements, a multiple of 8) and unit column
  * stride.  x_scale not 0: x, x_scale are packed too ([M, K / 2], [M, K / 32], x_sm is not read), and the product runs on
  * the 4-bit operands (their values exactly).  y: [M, N] contiguous, bias [N], both of the kernel's type.
- * K % 32 == 0; x and w 16-byte aligned, scales 4-byte aligned.  ws (optional, 0 = none): fp32 workspace of ws_floats,
- * 16-byte aligned, for partial products over slices of K where hrt_mx4_mm_workspace asks for one; they are added in order. */
+ * K % 32 == 0; x and w 16-byte aligned, scales 4-byte aligned. */
 typedef struct hrt_mx4_mm_args {
-  uint64_t x, x_scale, w, w_scale, bias, y, ws;
-  int64_t M, N, K, x_sm, ws_floats;
+  uint64_t x, x_scale, w, w_scale, bias, y;
+  int64_t M, N, K, x_sm;
 } hrt_mx4_mm_args;
-int64_t hrt_mx4_mm_workspace(const hrt_mx4_mm_args* args);
 
 /* "reduce_sum" — out[k] = (sum over the reduced coordinates r of x[k, r]) / div, accumulated in fp32 and
  * rounded once to out_dtype.  x: an ndim-dimensional strided view (ndim <= 8, non-negative strides) of

@@ -12,7 +12,7 @@
 // Lane layout of the scaled products (checked on the device), l = lane: 32x32x64: operand row l % 32, K block l / 32;
 // 16x16x128: row l % 16, K block l / 16; the scale operand's byte `opsel` belongs to the lane's own block.
 // W is the first operand in both kernels, so an accumulator holds four consecutive columns n of one row m of y.
-#include <cstring>
+#include <utility>
 
 #include "../hrt/registry.h"
 #include "mx4.h"
@@ -28,21 +28,10 @@ __device__ __forceinline__ i32x8 fp4_operand(u32x4 c) {
   return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
 }
 
-// y[m, n .. n + 3] (or the fp32 partial products of a K slice).  Columns past N are not stored; vec: whole groups of four
-// columns, aligned.
+// y[m, n .. n + 3].  Columns past N are not stored; vec: whole groups of four columns, aligned.
 template <typename T>
-__device__ __forceinline__ void store4(const hrt_mx4_mm_args& p, int64_t m, int64_t n, const float* v, float* part, bool vec) {
+__device__ __forceinline__ void store4(const hrt_mx4_mm_args& p, int64_t m, int64_t n, const float* v, bool vec) {
   if (m >= p.M || n >= p.N) return;
-  if (part) {
-    if (vec) {
-      *reinterpret_cast<HK_G f32x4*>((HK_G float*)part + m * p.N + n) = f32x4{v[0], v[1], v[2], v[3]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) ((HK_G float*)part)[m * p.N + n + e] = v[e];
-    }
-    return;
-  }
   HK_G uint16_t* y = gptr<uint16_t>(p.y) + m * p.N + n;
   const HK_G uint16_t* b = gcptr<uint16_t>(p.bias) + n;
   float o[4];
@@ -128,7 +117,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(hrt_mx4_mm_args p, b
 #pragma unroll
     for (int w = 0; w < kRowsWaves - 1; ++w) acc[b] += *reinterpret_cast<const f32x4*>(part[w][b][lane]);
     const float v[4] = {acc[b][0], acc[b][1], acc[b][2], acc[b][3]};
-    store4<T>(p, b * 16 + r16, n0 + 4 * g, v, nullptr, vec);
+    store4<T>(p, b * 16 + r16, n0 + 4 * g, v, vec);
   }
 }
 
@@ -146,50 +135,43 @@ __device__ __forceinline__ int row_off(int row, int c) {
   return row * RB + ((c ^ row_swz<RB>(row)) << 4);
 }
 
-template <typename T, bool A4, int BM, int BN, int WM, int WN>
+// A workgroup's wavefronts are KG groups along K times a grid of WM x WN sub-tiles: a step covers KG pieces of KS values of K,
+// one per group, and the groups' sums are added in order at the end.  KG > 1 gives small grids (few rows) the wavefronts that
+// hide a copy's latency without a second launch.
+template <bool A4, int BM, int BN, int WM, int WN, int KG>
 struct TileShape {
-  static constexpr int KS = A4 ? 128 : 64;               // K values per step
-  static constexpr int NW = (BM / WM) * (BN / WN);       // wavefronts
-  static constexpr int XB = A4 ? 64 : 128, WB = KS / 2;  // bytes of an LDS row of X and of W
-  static constexpr int XT = BM * XB, WT = BN * WB;
-  static constexpr int IPX = XT / 1024 / NW, IPW = WT / 1024 / NW;  // copies per wavefront and step
+  static constexpr int KS = A4 ? 128 : 64;                // K values per piece
+  static constexpr int NWT = (BM / WM) * (BN / WN);       // wavefronts per group
+  static constexpr int NW = NWT * KG;
+  static constexpr int XB = A4 ? 64 : 128, WB = KS / 2;   // bytes of an LDS row of X and of W
+  static constexpr int XT = BM * XB, WT = BN * WB;        // bytes of a piece
+  static constexpr int IPX = KG * XT / 1024 / NW, IPW = KG * WT / 1024 / NW;  // copies per wavefront and step
   static constexpr int FM = WM / 32, FN = WN / 32;
-  static_assert(XT % (1024 * NW) == 0 && WT % (1024 * NW) == 0 && IPX >= 1 && IPW >= 1, "copy split");
+  static_assert(KG * XT % (1024 * NW) == 0 && KG * WT % (1024 * NW) == 0 && IPX >= 1 && IPW >= 1, "copy split");
 };
 
-// STR: a row's scale bytes of one step may straddle two dwords (K / 32 not a multiple of the bytes per step).
-template <typename T, bool A4, int BM, int BN, int WM, int WN, bool STR>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void mx4_tile(hrt_mx4_mm_args p, int tiles_m, int tiles_n, int nk, int kper,
-                                                                       int xbm, bool vec) {
-  using S = TileShape<T, A4, BM, BN, WM, WN>;
-  constexpr int NW = S::NW, XB = S::XB, WB = S::WB, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN, KS = S::KS;
-  constexpr int SD = STR ? 2 : 1;                                      // scale dwords per row and step
-  constexpr int SR = BN + (A4 ? BM : 0), SI = (SR * SD + 63) / 64;     // rows with scales, copies of 64 dwords
-  constexpr int IPS = (SI + NW - 1) / NW;                              // per wavefront (the last ones repeat a copy)
-  constexpr int SB = KS / 32;                                          // scale bytes per row and step
-  static_assert(SR * SD % 64 == 0, "whole scale copies");
+// STR: a row's scale bytes of one piece may straddle two dwords (K / 32 not a multiple of the bytes per piece).
+template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG, bool STR>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_mx4_mm_args p, int tiles_m, int tiles_n, int nk, bool vec) {
+  using S = TileShape<A4, BM, BN, WM, WN, KG>;
+  constexpr int NW = S::NW, NWT = S::NWT, XB = S::XB, WB = S::WB, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN, KS = S::KS;
+  constexpr int SD = STR ? 2 : 1;                                  // scale dwords per row and piece
+  constexpr int SR = BN + (A4 ? BM : 0), SI = KG * SR * SD / 64;   // rows with scales; copies of 64 dwords
+  constexpr int IPS = (SI + NW - 1) / NW;                          // per wavefront (the last ones repeat a copy)
+  constexpr int SB = KS / 32;                                      // scale bytes per row and piece
+  static_assert(SR * SD % 64 == 0 && BN * SD % 64 == 0, "whole scale copies");
   // One LDS object per stage, so that the compiler can tell the reads of one from the copies into another (it tracks only
   // a few objects: with X, W and the scales apart it waited for every copy at the loop's head).
-  constexpr int STAGE = S::XT + S::WT + SI * 256;
+  constexpr int STAGE = KG * (S::XT + S::WT) + SI * 256;
   __shared__ __attribute__((aligned(1024))) uint8_t st0[STAGE], st1[STAGE], st2[STAGE];
   auto buf = [&](auto ic) { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? st0 : I == 1 ? st1 : st2); };
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % (BM / WM), wn = wave / (BM / WM), l32 = lane & 31, h = lane >> 5;
-  // n-fastest tile numbers; xbm > 0: XCD x takes one xbm x (tiles / 8 / xbm) block of the grid
-  uint32_t tile = blockIdx.x, sl = 0, tm, tn;
-  const uint32_t tiles = (uint32_t)tiles_m * (uint32_t)tiles_n;
-  if (xbm > 0) {
-    const uint32_t bnw = tiles / 8 / (uint32_t)xbm, nbn = (uint32_t)tiles_n / bnw, x = tile % 8, loc = tile / 8;
-    tm = (x / nbn) * (uint32_t)xbm + loc / bnw, tn = (x % nbn) * bnw + loc % bnw;
-  } else {
-    sl = tile / tiles, tile -= sl * tiles;
-    tm = tile / (uint32_t)tiles_n, tn = tile % (uint32_t)tiles_n;
-  }
-  // in scalar registers, and with them every buffer resource
-  tm = __builtin_amdgcn_readfirstlane(tm), tn = __builtin_amdgcn_readfirstlane(tn), sl = __builtin_amdgcn_readfirstlane(sl);
+  const int kg = wave / NWT, wt = wave % NWT, wm = wt % (BM / WM), wn = wt / (BM / WM), l32 = lane & 31, h = lane >> 5;
+  // n-fastest tile numbers, in scalar registers, and with them every buffer resource
+  const uint32_t tm = __builtin_amdgcn_readfirstlane(blockIdx.x / (uint32_t)tiles_n);
+  const uint32_t tn = __builtin_amdgcn_readfirstlane(blockIdx.x % (uint32_t)tiles_n);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int ks0 = (int)sl * kper, ks1 = ks0 + kper < nk ? ks0 + kper : nk;  // this slice's steps
   const int64_t nb = p.K / 32;
   const int ml = p.M - m0 < BM ? (int)(p.M - m0) : BM, nl = p.N - n0 < BN ? (int)(p.N - n0) : BN;
 
@@ -198,72 +180,73 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void mx4_tile(hrt_mx4_m
   const HK_G uint8_t* Xb = gcptr<uint8_t>(p.x) + m0 * xss;
   const HK_G uint8_t* Wb = gcptr<uint8_t>(p.w) + n0 * wss;
   uint32_t xo[IPX], wo[IPW];
+  auto xchunk = [&](int i) {  // copy i's chunk within the piece: row and column
+    const int ch = ((wave * IPX + i) * 64 + lane) % (S::XT / 16), row = ch / (XB / 16);
+    return std::pair<int, int>{row, (ch % (XB / 16)) ^ row_swz<XB>(row)};
+  };
+  auto wchunk = [&](int i) {
+    const int ch = ((wave * IPW + i) * 64 + lane) % (S::WT / 16), row = ch / (WB / 16);
+    return std::pair<int, int>{row, (ch % (WB / 16)) ^ row_swz<WB>(row)};
+  };
+  auto xpiece = [&](int i) { return (wave * IPX + i) / (S::XT / 1024); };
+  auto wpiece = [&](int i) { return (wave * IPW + i) / (S::WT / 1024); };
 #pragma unroll
   for (int i = 0; i < IPX; ++i) {
-    const int ch = (wave * IPX + i) * 64 + lane, row = ch / (XB / 16), c = (ch % (XB / 16)) ^ row_swz<XB>(row);
-    xo[i] = row < ml ? (uint32_t)row * xss + (uint32_t)c * 16 : kNoRow;
+    const auto [row, c] = xchunk(i);
+    xo[i] = row < ml ? (uint32_t)row * xss + (uint32_t)(c * 16 + xpiece(i) * XB) : kNoRow;
   }
 #pragma unroll
   for (int i = 0; i < IPW; ++i) {
-    const int ch = (wave * IPW + i) * 64 + lane, row = ch / (WB / 16), c = (ch % (WB / 16)) ^ row_swz<WB>(row);
-    wo[i] = row < nl ? (uint32_t)row * wss + (uint32_t)c * 16 : kNoRow;
+    const auto [row, c] = wchunk(i);
+    wo[i] = row < nl ? (uint32_t)row * wss + (uint32_t)(c * 16 + wpiece(i) * WB) : kNoRow;
   }
-  // scales: dword d of row r (W rows first, then X rows) is LDS dword r * SD + d.  Dwords are aligned down; what a row does
-  // not own is shifted or masked out where it is used.
+  // scales: dword d of row r (W rows first, then X rows) of piece k is LDS dword (k * SR + r) * SD + d.  Dwords are aligned
+  // down; what a row does not own is shifted or masked out where it is used.
   const __amdgpu_buffer_rsrc_t wsr = edge_rsrc(gcptr<uint8_t>(p.w_scale)), xsr = edge_rsrc(gcptr<uint8_t>(A4 ? p.x_scale : p.w_scale));
   uint32_t so[IPS];
   bool sx[IPS];
 #pragma unroll
   for (int i = 0; i < IPS; ++i) {
     const int j = (wave * IPS + i) % SI;  // wavefronts past the last copy repeat an earlier one: the same bytes again
-    const int d = j * 64 + lane, row = d / SD;
-    sx[i] = A4 && j * 64 / SD >= BN;  // uniform: BN * SD is a multiple of 64
+    const int d = (j * 64 + lane) % (SR * SD), row = d / SD, piece = j * 64 / (SR * SD);
+    sx[i] = A4 && j * 64 % (SR * SD) / SD >= BN;  // uniform: BN * SD is a multiple of 64
     const int r = sx[i] ? row - BN : row;
-    const int64_t o = ((sx[i] ? m0 : n0) + r) * nb;  // byte of the row's first scale
+    const int64_t o = ((sx[i] ? m0 : n0) + r) * nb + piece * SB;  // byte of the row's first scale in this piece
+    // (4 (d % SD): the second dword)
     so[i] = r < (sx[i] ? ml : nl) ? (uint32_t)(o + 4 * (d % SD)) : kNoRow;
   }
 
   auto copy = [&](int ks, HK_L uint8_t* xt) {
-    HK_L uint8_t* const wt = xt + S::XT;
-    HK_L uint8_t* const st = wt + S::WT;
-    const __amdgpu_buffer_rsrc_t xr = edge_rsrc(Xb + (int64_t)ks * (A4 ? KS / 2 : KS * 2)), wr = edge_rsrc(Wb + (int64_t)ks * (KS / 2));
-    // the last step may hold fewer than KS values: chunks past K are zeros (a select, not a branch: the compiler counts the
-    // copies in flight along every path)
-    const int64_t left = p.K - (int64_t)ks * KS;
-    const int xc = left >= KS ? XB / 16 : (int)(A4 ? left / 32 : left / 8), wc = left >= KS ? WB / 16 : (int)(left / 32);
+    HK_L uint8_t* const wt = xt + KG * S::XT;
+    HK_L uint8_t* const st = wt + KG * S::WT;
+    const __amdgpu_buffer_rsrc_t xr = edge_rsrc(Xb + (int64_t)ks * (KG * XB)), wr = edge_rsrc(Wb + (int64_t)ks * (KG * WB));
+    // the last step may hold fewer values: chunks past K are zeros (a select, not a branch: the compiler counts the copies
+    // in flight along every path)
+    const int64_t left = p.K - (int64_t)ks * (KG * KS);
+    const int l = left >= KG * KS ? KG * KS : (int)left;
 #pragma unroll
-    for (int i = 0; i < IPX; ++i) {
-      const int ch = (wave * IPX + i) * 64 + lane;
-      edge_copy(xr, xt, wave * IPX + i, ((ch % (XB / 16)) ^ row_swz<XB>(ch / (XB / 16))) < xc ? xo[i] : kNoRow);
-    }
+    for (int i = 0; i < IPX; ++i)
+      edge_copy(xr, xt, wave * IPX + i, xchunk(i).second * (A4 ? 32 : 8) + xpiece(i) * KS < l ? xo[i] : kNoRow);
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) {
-      const int ch = (wave * IPW + i) * 64 + lane;
-      edge_copy(wr, wt, wave * IPW + i, ((ch % (WB / 16)) ^ row_swz<WB>(ch / (WB / 16))) < wc ? wo[i] : kNoRow);
-    }
+    for (int i = 0; i < IPW; ++i) edge_copy(wr, wt, wave * IPW + i, wchunk(i).second * 32 + wpiece(i) * KS < l ? wo[i] : kNoRow);
 #pragma unroll
     for (int i = 0; i < IPS; ++i) {
       const int j = (wave * IPS + i) % SI;
-      const uint32_t o = so[i] == kNoRow ? kNoRow : (so[i] + (uint32_t)(ks * SB)) & ~3u;
+      const uint32_t o = so[i] == kNoRow ? kNoRow : (so[i] + (uint32_t)(ks * KG * SB)) & ~3u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(sx[i] ? xsr : wsr, st + j * 256, 4, (int)o, 0, 0, 0);
     }
   };
 
-  // fragment and scale offsets
-  int xoff[FM], woff[FN], sxo[FM], swo[FN];
+  // This lane's rows: the sub-tile's other 32-row blocks lie a constant further (the swizzle repeats every 16 rows).
+  const int xrow = wm * WM + l32, wrow = wn * WN + l32;
+  const int xbase = kg * S::XT, wbase = KG * S::XT + kg * S::WT, sbase = KG * (S::XT + S::WT) + kg * SR * SD * 4;
+  auto xat = [&](int i, int c) { return xbase + row_off<XB>(xrow, c) + i * 32 * XB; };
+  auto wat = [&](int j, int c) { return wbase + row_off<WB>(wrow, c) + j * 32 * WB; };
   uint32_t wsh[FN], xsh[FM];  // byte of the row's first scale, modulo 4
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int row = wm * WM + i * 32 + l32;
-    xoff[i] = row, sxo[i] = (BN + row) * SD * 4;
-    xsh[i] = (uint32_t)((m0 + row) * nb) & 3u;
-  }
+  for (int i = 0; i < FM; ++i) xsh[i] = (uint32_t)((m0 + xrow + 32 * i) * nb) & 3u;
 #pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int row = wn * WN + j * 32 + l32;
-    woff[j] = row, swo[j] = row * SD * 4;
-    wsh[j] = (uint32_t)((n0 + row) * nb) & 3u;
-  }
+  for (int j = 0; j < FN; ++j) wsh[j] = (uint32_t)((n0 + wrow + 32 * j) * nb) & 3u;
 
   f32x16 acc[FN][FM];
 #pragma unroll
@@ -271,17 +254,18 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void mx4_tile(hrt_mx4_m
 #pragma unroll
     for (int i = 0; i < FM; ++i) acc[j][i] = zero16();
 
-  // the step's scale bytes of one row, its first in byte 0, those past the end of K zero
-  auto scales = [&](const HK_L uint8_t* st, int off, uint32_t sh, int ks) {
-    const int have = (int)(nb - (int64_t)ks * SB);
-    const uint32_t keep = have >= 4 ? ~0u : (1u << (8 * have)) - 1u;
-    const uint32_t by = (sh + (uint32_t)(ks * SB)) & 3u;
+  // the scale bytes of one row in this wavefront's piece, the first in byte 0, those past the end of K zero
+  auto scales = [&](const HK_L uint8_t* st, int row, uint32_t sh, int ks) {
+    const int64_t first = ((int64_t)ks * KG + kg) * SB, have = nb - first;
+    const uint32_t keep = have >= 4 ? ~0u : have <= 0 ? 0u : (1u << (8 * (int)have)) - 1u;
+    const uint32_t by = (sh + (uint32_t)first) & 3u;
+    const HK_L uint8_t* const at = st + sbase + row * SD * 4;
     uint32_t v;
     if constexpr (STR) {
-      const u32x2 d = *reinterpret_cast<const HK_L u32x2*>(st + off);
+      const u32x2 d = *reinterpret_cast<const HK_L u32x2*>(at);
       v = __builtin_amdgcn_alignbyte(d.y, d.x, by);
     } else {
-      v = *reinterpret_cast<const HK_L uint32_t*>(st + off) >> (8 * by);
+      v = *reinterpret_cast<const HK_L uint32_t*>(at) >> (8 * by);
     }
     return v & keep;
   };
@@ -289,51 +273,61 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void mx4_tile(hrt_mx4_m
   constexpr int PER = IPX + IPW + IPS;  // copies per wavefront and step
   auto step = [&](auto bc, int ks, bool more) {
     constexpr int BUF = decltype(bc)::value, NXT = (BUF + 2) % 3;
-    const HK_L uint8_t* const xt = buf(bc);
-    const HK_L uint8_t* const wt = xt + S::XT;
-    const HK_L uint8_t* const st = wt + S::WT;
+    const HK_L uint8_t* const st = buf(bc);
     using N = std::integral_constant<int, NXT>;
+    // fragments of the next slice are read while this one's products run (two register sets, fenced: in the compiler's own
+    // order every slice waited for its reads)
     if constexpr (A4) {
       uint32_t sw[FN], sxv[FM];
+      u32x4 wf[2][FN], xf[2][FM];
+      auto read = [&](int s) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) sw[j] = scales(st, swo[j], wsh[j], ks) >> (8 * h);
+        for (int j = 0; j < FN; ++j) wf[s][j] = *reinterpret_cast<const HK_L u32x4*>(st + wat(j, 2 * s + h));
 #pragma unroll
-      for (int i = 0; i < FM; ++i) sxv[i] = scales(st, sxo[i], xsh[i], ks) >> (8 * h);
+        for (int i = 0; i < FM; ++i) xf[s][i] = *reinterpret_cast<const HK_L u32x4*>(st + xat(i, 2 * s + h));
+      };
+#pragma unroll
+      for (int j = 0; j < FN; ++j) sw[j] = scales(st, wrow + 32 * j, wsh[j], ks) >> (8 * h);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) sxv[i] = scales(st, BN + xrow + 32 * i, xsh[i], ks) >> (8 * h);
+      read(0);
       if (more) copy(ks + 2, buf(N()));
       both([&](auto sc) {
         constexpr int K64 = decltype(sc)::value;
-        if (K64) __builtin_amdgcn_sched_barrier(0);
-        u32x4 wf[FN], xf[FM];
-#pragma unroll
-        for (int j = 0; j < FN; ++j) wf[j] = *reinterpret_cast<const HK_L u32x4*>(wt + row_off<WB>(woff[j], 2 * K64 + h));
-#pragma unroll
-        for (int i = 0; i < FM; ++i) xf[i] = *reinterpret_cast<const HK_L u32x4*>(xt + row_off<XB>(xoff[i], 2 * K64 + h));
+        __builtin_amdgcn_sched_barrier(0);
+        if (K64 == 0) read(1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int i = 0; i < FM; ++i)
-            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(wf[j]), fp4_operand(xf[i]), acc[j][i], 4, 4, 2 * K64,
-                                                                        (int)sw[j], 2 * K64, (int)sxv[i]);
+            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(wf[K64][j]), fp4_operand(xf[K64][i]), acc[j][i], 4, 4,
+                                                                        2 * K64, (int)sw[j], 2 * K64, (int)sxv[i]);
       });
     } else {
-      u32x4 wc[FN];
+      u32x4 wc[FN], xf[2][FM];
       float f[FN];
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        wc[j] = *reinterpret_cast<const HK_L u32x4*>(wt + row_off<WB>(woff[j], h));
-        f[j] = mx_scale((scales(st, swo[j], wsh[j], ks) >> (8 * h)) & 255u);
+        wc[j] = *reinterpret_cast<const HK_L u32x4*>(st + wat(j, h));
+        f[j] = mx_scale((scales(st, wrow + 32 * j, wsh[j], ks) >> (8 * h)) & 255u);
       }
+      auto read = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) xf[t & 1][i] = *reinterpret_cast<const HK_L u32x4*>(st + xat(i, 4 * h + t));
+      };
+      read(0);
       if (more) copy(ks + 2, buf(N()));
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        u32x4 xf[FM];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) xf[i] = *reinterpret_cast<const HK_L u32x4*>(xt + row_off<XB>(xoff[i], 4 * h + t));
+        __builtin_amdgcn_sched_barrier(0);
+        if (t < 3) read(t + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
           const u32x4 wf = mx4_unpack8<T>(wc[j][t], f[j]);
 #pragma unroll
-          for (int i = 0; i < FM; ++i) acc[j][i] = Mfma32<T>::mac(wf, xf[i], acc[j][i]);
+          for (int i = 0; i < FM; ++i) acc[j][i] = Mfma32<T>::mac(wf, xf[t & 1][i], acc[j][i]);
         }
       }
     }
@@ -350,27 +344,49 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void mx4_tile(hrt_mx4_m
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
-  copy(ks0, buf(I0()));
+  copy(0, buf(I0()));
   issue_order_fence();
-  if (ks0 + 1 < ks1) {
-    copy(ks0 + 1, buf(I1()));
-    barrier_keep_vm<PER>();
-  } else {
-    barrier_keep_vm<0>();
-  }
-  int ks = ks0;
-  for (; ks + 5 <= ks1; ks += 3) {  // every step of the body copies: no branch around the copies
+  copy(nk > 1 ? 1 : 0, buf(I1()));  // a single step: a copy that nobody reads, on every path alike
+  barrier_keep_vm<PER>();
+  int ks = 0;
+  for (; ks + 5 <= nk; ks += 3) {  // every step of the body copies: no branch around the copies
     step(I0(), ks, true);
     step(I1(), ks + 1, true);
     step(I2(), ks + 2, true);
   }
   // the last one to four
-  step(I0(), ks, ks + 2 < ks1);
-  if (ks + 1 < ks1) step(I1(), ks + 1, ks + 3 < ks1);
-  if (ks + 2 < ks1) step(I2(), ks + 2, false);
-  if (ks + 3 < ks1) step(I0(), ks + 3, false);
+  step(I0(), ks, ks + 2 < nk);
+  if (ks + 1 < nk) step(I1(), ks + 1, ks + 3 < nk);
+  if (ks + 2 < nk) step(I2(), ks + 2, false);
+  if (ks + 3 < nk) step(I0(), ks + 3, false);
 
-  float* part = p.ws && kper < nk ? reinterpret_cast<float*>(p.ws) + sl * p.M * p.N : nullptr;
+  if constexpr (KG > 1) {  // the groups' sums, in order, through the stages' memory (every copy has landed)
+    constexpr int NB = FN * FM, PB = KG == 2 ? NB / 2 : NB;  // accumulators, and how many of a wavefront's share a stage
+    static_assert((KG == 4 || (KG == 2 && NB % 2 == 0)) && NWT * PB * 4096 <= STAGE, "merge areas");
+    // accumulator b of group k: KG 4: the groups 1, 2, 3 have a stage each; KG 2: group 1 has two
+    auto area = [&](int k, int b) {
+      const int o = KG == 4 ? k - 1 : b / PB;
+      return (float*)(o == 0 ? st0 : o == 1 ? st1 : st2) + (wt * PB + b % PB) * 1024 + lane;
+    };
+    if (kg > 0) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float* const mine = area(kg, b);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[e * 64] = acc[b / FM][b % FM][e];
+      }
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int k = 1; k < KG; ++k)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const float* const part = area(k, b);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b / FM][b % FM][e] += part[e * 64];
+      }
+  }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -378,49 +394,40 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void mx4_tile(hrt_mx4_m
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v[4] = {acc[j][i][4 * e], acc[j][i][4 * e + 1], acc[j][i][4 * e + 2], acc[j][i][4 * e + 3]};
-        store4<T>(p, m0 + wm * WM + i * 32 + l32, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, part, vec);
+        store4<T>(p, m0 + wm * WM + i * 32 + l32, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, vec);
       }
 }
 
 // ---- plan and launch -----------------------------------------------------------------------------------------------------
-struct Plan {
-  int tile = -1;  // index into the tile list, -1: mx4_rows
-  int64_t splits = 1, kper = 0;
-};
-struct Shape2 {
+struct Tile2 {
   int bm, bn;
 };
-constexpr Shape2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
+constexpr Tile2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
 
-Plan plan_of(const hrt_mx4_mm_args& a, bool ws) {
-  Plan p;
-  const int64_t ks = a.x_scale ? 128 : 64, nk = cdiv(a.K, ks);
-  p.kper = nk;
-  if (a.M <= 64) return p;
-  auto grid = [&](int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); };
-  p.tile = grid(0) >= 256 ? 0 : grid(1) >= 192 ? 1 : grid(2) >= 192 ? 2 : 3;
-  (void)ws;
-  return p;
+int64_t tiles_of(const hrt_mx4_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
+// Index of the tile, -1: mx4_rows.
+int plan_of(const hrt_mx4_mm_args& a) {
+  if (a.M <= 64) return -1;
+  return tiles_of(a, 0) >= 256 ? 0 : tiles_of(a, 1) >= 192 ? 1 : tiles_of(a, 2) >= 192 ? 2 : 3;
 }
 
-template <typename T, bool A4, int BM, int BN, int WM, int WN>
-void queue_tile(const hrt_mx4_mm_args& a, const Plan& pl, hipStream_t s, bool vec) {
-  using S = TileShape<T, A4, BM, BN, WM, WN>;
-  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, S::KS);
-  const bool str = (a.K / 32) % (S::KS / 32) != 0;
-  const dim3 grid((uint32_t)(tm * tn * pl.splits)), block(64 * S::NW);
-  if (str) hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, true>), grid, block, 0, s, a, (int)tm, (int)tn, (int)nk, (int)pl.kper, 0, vec);
-  else hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, false>), grid, block, 0, s, a, (int)tm, (int)tn, (int)nk, (int)pl.kper, 0, vec);
+template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG>
+void queue_tile(const hrt_mx4_mm_args& a, hipStream_t s, bool vec) {
+  using S = TileShape<A4, BM, BN, WM, WN, KG>;
+  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, S::KS * KG);
+  const dim3 grid((uint32_t)(tm * tn)), block(64 * S::NW);
+  if ((a.K / 32) % (S::KS / 32) != 0) hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, true>), grid, block, 0, s, a, (int)tm, (int)tn, (int)nk, vec);
+  else hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, false>), grid, block, 0, s, a, (int)tm, (int)tn, (int)nk, vec);
 }
 
 template <typename T, bool A4>
-void queue_mm(const hrt_mx4_mm_args& a, const Plan& pl, hipStream_t s) {
+void queue_mm(const hrt_mx4_mm_args& a, int tile, hipStream_t s) {
   const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0;
-  switch (pl.tile) {
-    case 0: return queue_tile<T, A4, 256, 256, 128, 64>(a, pl, s, vec);
-    case 1: return queue_tile<T, A4, 128, 256, 64, 64>(a, pl, s, vec);
-    case 2: return queue_tile<T, A4, 128, 128, 64, 64>(a, pl, s, vec);
-    case 3: return queue_tile<T, A4, 64, 64, 32, 64>(a, pl, s, vec);
+  switch (tile) {
+    case 0: return queue_tile<T, A4, 256, 256, 128, 64, 1>(a, s, vec);
+    case 1: return queue_tile<T, A4, 128, 256, 64, 64, 1>(a, s, vec);
+    case 2: return queue_tile<T, A4, 128, 128, 64, 64, 2>(a, s, vec);
+    case 3: return queue_tile<T, A4, 64, 64, 32, 64, 4>(a, s, vec);
   }
   const dim3 grid((uint32_t)cdiv(a.N, 16)), block(64 * kRowsWaves);
   switch (cdiv(a.M, 16)) {
@@ -433,13 +440,13 @@ void queue_mm(const hrt_mx4_mm_args& a, const Plan& pl, hipStream_t s) {
 
 template <typename T>
 bool launch_mx4_mm(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
-  hrt_mx4_mm_args a = *static_cast<const hrt_mx4_mm_args*>(pp);
+  const auto& a = *static_cast<const hrt_mx4_mm_args*>(pp);
   if (a.M <= 0 || a.N <= 0 || a.K <= 0) return ctx.fail("empty product");
   if (a.K % kMxBlock != 0) return ctx.fail("K must be a multiple of 32");
   const bool a4 = a.x_scale != 0;
   if (!a4 && (a.x_sm < 0 || a.x_sm % 8 != 0)) return ctx.fail("x's row stride must be a non-negative multiple of 8");
-  if (a.x % 16 != 0 || a.w % 16 != 0 || a.w_scale % 4 != 0 || a.x_scale % 4 != 0 || a.y % 2 != 0 || a.bias % 2 != 0 || a.ws % 16 != 0)
-    return ctx.fail("x, w and ws must be 16-byte aligned, scales 4-byte aligned");
+  if (a.x % 16 != 0 || a.w % 16 != 0 || a.w_scale % 4 != 0 || a.x_scale % 4 != 0 || a.y % 2 != 0 || a.bias % 2 != 0)
+    return ctx.fail("x and w must be 16-byte aligned, scales 4-byte aligned");
   const int64_t nb = a.K / kMxBlock, xs[2] = {a.M, a.K}, xt[2] = {a.x_sm, 1};
   if (!(a4 ? ctx.check(a.x, (uint64_t)(a.M * (a.K / 2)), "x") && ctx.check(a.x_scale, (uint64_t)(a.M * nb), "x_scale")
            : ctx.check(a.x, hrt::span_bytes(2, xs, xt, 2), "x")) ||
@@ -450,26 +457,11 @@ bool launch_mx4_mm(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   const int64_t lim = (int64_t)1 << 31;
   if ((a4 ? a.K / 2 : a.x_sm * 2) * 257 >= lim || a.K / 2 * 257 >= lim || a.N * nb + 8 >= lim || (a4 && a.M * nb + 8 >= lim))
     return ctx.fail("operand rows too long for one launch");
-  const Plan pl = plan_of(a, a.ws != 0);
-  if (pl.splits > 1) {
-    if (a.ws_floats < pl.splits * a.M * a.N) return ctx.fail("workspace too small");
-    if (!ctx.check(a.ws, (uint64_t)(pl.splits * a.M * a.N) * 4, "ws")) return false;
-  } else {
-    a.ws = 0;
-  }
-  const int64_t wgs = pl.tile < 0 ? cdiv(a.N, 16) : cdiv(a.M, kTiles[pl.tile].bm) * cdiv(a.N, kTiles[pl.tile].bn) * pl.splits;
-  if (!hrt::grid_fits(wgs, 512)) return ctx.fail("grid too large");
-  if (a4) queue_mm<T, true>(a, pl, ctx.stream);
-  else queue_mm<T, false>(a, pl, ctx.stream);
-  if (!hrt::launch_ok(hipGetLastError(), ctx, "mx4_mm")) return false;
-  if (pl.splits == 1) return true;
-  hrt_mm_reduce_args r{};
-  r.ws = a.ws, r.c = a.y, r.bias = a.bias, r.M = a.M, r.N = a.N, r.splits = pl.splits;
-  r.c_sm = a.N, r.c_sn = 1, r.bias_sn = 1, r.alpha = 1.f, r.beta = 1.f, r.has_bias = a.bias != 0;
-  const char* name = std::is_same<T, BF16>::value ? "mm_reduce_bf16" : "mm_reduce_f16";
-  for (auto& e : hrt::kernel_table())
-    if (!strcmp(e.name, name)) return e.launch(&r, nullptr, ctx);
-  return ctx.fail("mx4_mm: no reduction kernel");
+  const int tile = plan_of(a);
+  if (!hrt::grid_fits(tile < 0 ? cdiv(a.N, 16) : tiles_of(a, tile), 512)) return ctx.fail("grid too large");
+  if (a4) queue_mm<T, true>(a, tile, ctx.stream);
+  else queue_mm<T, false>(a, tile, ctx.stream);
+  return hrt::launch_ok(hipGetLastError(), ctx, "mx4_mm");
 }
 
 HRT_REGISTER("mx4_mm_bf16", hrt_mx4_mm_args, launch_mx4_mm<BF16>);
@@ -477,9 +469,3 @@ HRT_REGISTER("mx4_mm_f16", hrt_mx4_mm_args, launch_mx4_mm<F16>);
 
 }  // namespace
 }  // namespace hk
-
-extern "C" int64_t hrt_mx4_mm_workspace(const hrt_mx4_mm_args* a) {
-  if (a == nullptr || a->M <= 0 || a->N <= 0 || a->K <= 0 || a->K % hk::kMxBlock != 0) return 0;
-  const hk::Plan p = hk::plan_of(*a, true);
-  return p.splits > 1 ? p.splits * a->M * a->N : 0;
-}

@@ -76,11 +76,6 @@ at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& codes, const at::T
   }
   const at::Tensor y = at::empty({M, N}, x.options());
   A.y = dptr(y);
-  c10::DataPtr part;
-  if (const int64_t n = hrt_mx4_mm_workspace(&A); n > 0) {
-    part = scratch(n * 4);
-    if (part) A.ws = dptr(part), A.ws_floats = n;
-  }
   queue(typed("mx4_mm", x.scalar_type()), A);
   return y;
 }

@@ -55,8 +55,8 @@ class Mx4Args(ctypes.Structure):
 
 
 class Mx4MmArgs(ctypes.Structure):
-    _fields_ = [("x", u64), ("x_scale", u64), ("w", u64), ("w_scale", u64), ("bias", u64), ("y", u64), ("ws", u64),
-                ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64), ("ws_floats", i64)]
+    _fields_ = [("x", u64), ("x_scale", u64), ("w", u64), ("w_scale", u64), ("bias", u64), ("y", u64),
+                ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64)]
 
 
 class AttnRelArgs(ctypes.Structure):
