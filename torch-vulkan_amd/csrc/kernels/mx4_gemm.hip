@@ -152,7 +152,7 @@ struct TileShape {
 
 // STR: a row's scale bytes of one piece may straddle two dwords (K / 32 not a multiple of the bytes per piece).
 template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG, bool STR>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_mx4_mm_args p, int tiles_m, int tiles_n, int nk, bool vec) {
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_mx4_mm_args p, int tiles_n, int nk, bool lines) {
   using S = TileShape<A4, BM, BN, WM, WN, KG>;
   constexpr int NW = S::NW, NWT = S::NWT, XB = S::XB, WB = S::WB, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN, KS = S::KS;
   constexpr int SD = STR ? 2 : 1;                                  // scale dwords per row and piece
@@ -387,15 +387,57 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_
         for (int e = 0; e < 16; ++e) acc[b / FM][b % FM][e] += part[e * 64];
       }
   }
+  if (!lines) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v[4] = {acc[j][i][4 * e], acc[j][i][4 * e + 1], acc[j][i][4 * e + 2], acc[j][i][4 * e + 3]};
+          store4<T>(p, m0 + wm * WM + i * 32 + l32, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, false);
+        }
+    return;
+  }
+  // Whole lines of y: 32 rows at a time go through the wavefront's own LDS area, so that a store writes 16 bytes a lane along
+  // a row (8-byte stores straight from the accumulators touch 32 rows each: 4096 x 8192 x 2048 130 us, so 121).
+  constexpr int RB = WN * 2 + 16;  // bytes of a row in the area, its pad off the banks of the next
+  // KG > 1: in the merge area of group 1's wavefront, which this one has read; else half of the areas in each of two stages
+  constexpr int HALF = (NWT + 1) / 2, MERGED = KG > 1 ? FN * FM / (KG == 2 ? 2 : 1) * 4096 : 0;
+  static_assert(KG > 1 ? 32 * RB <= MERGED : HALF * 32 * RB <= STAGE, "epilogue areas");
+  HK_L uint8_t* const area = KG > 1      ? (HK_L uint8_t*)st0 + wt * MERGED
+                             : wt < HALF ? (HK_L uint8_t*)st0 + wt * (32 * RB)
+                                         : (HK_L uint8_t*)st1 + (wt - HALF) * (32 * RB);
+  const int64_t nw = n0 + wn * WN;
+  u32x2 bias[FN][4];
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bias[j][e] = u32x2{0, 0};
+      const int64_t n = nw + j * 32 + 8 * e + 4 * h;
+      if (p.bias && n < p.N) bias[j][e] = *reinterpret_cast<const HK_G u32x2*>(gcptr<uint16_t>(p.bias) + n);
+    }
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float v[4] = {acc[j][i][4 * e], acc[j][i][4 * e + 1], acc[j][i][4 * e + 2], acc[j][i][4 * e + 3]};
-        store4<T>(p, m0 + wm * WM + i * 32 + l32, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, vec);
+        float o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = acc[j][i][4 * e + r] + (r & 1 ? hi16<T>(bias[j][e][r >> 1]) : lo16<T>(bias[j][e][r >> 1]));
+        *reinterpret_cast<HK_L u32x2*>(area + l32 * RB + (j * 32 + 8 * e + 4 * h) * 2) = pack4<T>(o);
       }
+    constexpr int CPR = WN / 8;  // 16-byte chunks per row
+#pragma unroll
+    for (int u = 0; u < 32 * CPR / 64; ++u) {
+      const int ch = u * 64 + lane, row = ch / CPR, c = ch % CPR;
+      const u32x4 v = *reinterpret_cast<const HK_L u32x4*>(area + row * RB + c * 16);
+      const int64_t m = m0 + wm * WM + i * 32 + row, n = nw + c * 8;
+      if (m < p.M && n < p.N) *reinterpret_cast<HK_G u32x4*>(gptr<uint16_t>(p.y) + m * p.N + n) = v;
+    }
+  }
 }
 
 // ---- plan and launch -----------------------------------------------------------------------------------------------------
@@ -412,22 +454,22 @@ int plan_of(const hrt_mx4_mm_args& a) {
 }
 
 template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG>
-void queue_tile(const hrt_mx4_mm_args& a, hipStream_t s, bool vec) {
+void queue_tile(const hrt_mx4_mm_args& a, hipStream_t s, bool lines) {
   using S = TileShape<A4, BM, BN, WM, WN, KG>;
   const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, S::KS * KG);
   const dim3 grid((uint32_t)(tm * tn)), block(64 * S::NW);
-  if ((a.K / 32) % (S::KS / 32) != 0) hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, true>), grid, block, 0, s, a, (int)tm, (int)tn, (int)nk, vec);
-  else hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, false>), grid, block, 0, s, a, (int)tm, (int)tn, (int)nk, vec);
+  if ((a.K / 32) % (S::KS / 32) != 0) hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, true>), grid, block, 0, s, a, (int)tn, (int)nk, lines);
+  else hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, false>), grid, block, 0, s, a, (int)tn, (int)nk, lines);
 }
 
 template <typename T, bool A4>
 void queue_mm(const hrt_mx4_mm_args& a, int tile, hipStream_t s) {
-  const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0;
+  const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0, lines = vec && a.N % 8 == 0 && a.y % 16 == 0;
   switch (tile) {
-    case 0: return queue_tile<T, A4, 256, 256, 128, 64, 1>(a, s, vec);
-    case 1: return queue_tile<T, A4, 128, 256, 64, 64, 1>(a, s, vec);
-    case 2: return queue_tile<T, A4, 128, 128, 64, 64, 2>(a, s, vec);
-    case 3: return queue_tile<T, A4, 64, 64, 32, 64, 4>(a, s, vec);
+    case 0: return queue_tile<T, A4, 256, 256, 128, 64, 1>(a, s, lines);
+    case 1: return queue_tile<T, A4, 128, 256, 64, 64, 1>(a, s, lines);
+    case 2: return queue_tile<T, A4, 128, 128, 64, 64, 2>(a, s, lines);
+    case 3: return queue_tile<T, A4, 64, 64, 32, 64, 4>(a, s, lines);
   }
   const dim3 grid((uint32_t)cdiv(a.N, 16)), block(64 * kRowsWaves);
   switch (cdiv(a.M, 16)) {
