@@ -1,7 +1,7 @@
 // "mx4_mm_{bf16,f16}": y = X W^T + bias with W in microscaled 4-bit floating point (mx4.h) and X in 16 bits or in 4.
 //
 // Two kernels, each in both forms:
-//   * mx4_rows for few rows (M <= 64): bound by the weights' bytes.  A wavefront takes 16 columns of y and every fourth
+//   * mx4_rows for few rows (M <= 32): bound by the weights' bytes.  A wavefront takes 16 columns of y and every eighth
 //     128-wide piece of K; lane (n, g) loads the 32 codes of its column's block g straight into registers.
 //   * mx4_tile for the rest: bound by the matrix cores and by L2 -> LDS.  Both operands are copied global -> LDS directly
 //     through a ring of three stages (the scheme of gemm_dma_kernel.h), the weights as codes.
@@ -19,6 +19,9 @@
 
 namespace hk {
 namespace {
+
+// Lambdas of a kernel with many copies of its step: the compiler would make them functions.
+#define HK_INLINE __attribute__((always_inline))
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -54,11 +57,23 @@ __device__ __forceinline__ void both(F f) {
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------
-constexpr int kRowsWaves = 4;
+// dword t of lane group g (16 lanes) becomes dword g of group t's: [block g][dword t] -> [block t][dword g].
+__device__ __forceinline__ u32x4 transpose_groups(u32x4 c) {
+  const auto a = __builtin_amdgcn_permlane32_swap(c[0], c[2], false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(c[1], c[3], false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  return u32x4{(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)hi[0], (uint32_t)hi[1]};
+}
 
-template <typename T, bool A4, int MB>
-__global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(hrt_mx4_mm_args p, bool vec) {
-  __shared__ float part[kRowsWaves - 1][MB][64][4];
+// 16 MB rows (MB 1 or 2), NWV wavefronts.  A wavefront's pieces of 128 values of K come in batches of UB whose loads are all
+// issued before the first product: one memory latency a batch.  16-bit rows are read 64 bytes at a time (fragment t: values
+// 32 t + 8 g of a piece; 16 bytes out of each block of a row, as the codes lie in their lanes, touched four times the lines), so
+// the lane groups exchange their codes.
+template <typename T, bool A4, int MB, int NWV, int UB>
+__global__ __launch_bounds__(64 * NWV) void mx4_rows(hrt_mx4_mm_args p, bool vec) {
+  constexpr int XF = A4 ? 1 : 4;  // 16-byte pieces of X per row and piece of K
+  __shared__ float part[NWV - 1][MB][64][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
@@ -74,34 +89,47 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(hrt_mx4_mm_args p, b
 #pragma unroll
   for (int b = 0; b < MB; ++b) {  // rows past M repeat the last one and are not stored
     const int64_t m = b * 16 + r16 < p.M ? b * 16 + r16 : p.M - 1;
-    xr[b] = A4 ? gcptr<uint8_t>(p.x) + m * (p.K / 2) + 16 * g : gcptr<uint8_t>(p.x) + m * p.x_sm * 2 + 64 * g;
+    xr[b] = A4 ? gcptr<uint8_t>(p.x) + m * (p.K / 2) + 16 * g : gcptr<uint8_t>(p.x) + m * p.x_sm * 2 + 16 * g;
     xs[b] = gcptr<uint8_t>(p.x_scale) + m * nb + g;
   }
-  for (int64_t st = wave; st < steps; st += kRowsWaves) {
-    // a block past the end of K (the last step may have fewer than four) contributes zeros with scale 0 (2^-127)
-    const bool in = st * 4 + g < nb;
-    const int64_t at = in ? st : 0;
-    u32x4 c = __builtin_nontemporal_load(reinterpret_cast<const HK_G u32x4*>(wc + at * 64));
-    const uint32_t s = in ? ws[at * 4] : 0u;
-    if (!in) c = u32x4{0, 0, 0, 0};
-    if constexpr (A4) {
+  for (int64_t st = wave; st < steps; st += NWV * UB) {
+    u32x4 c[UB], x[UB][MB][XF];
+    uint32_t s[UB], sx[UB][MB];
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      // a block past the end of K (the last piece may have fewer than four) counts as zeros with scale 0 (2^-127)
+      const int64_t k = st + u * NWV, at = k * 4 + g < nb ? k : 0;
+      c[u] = __builtin_nontemporal_load(reinterpret_cast<const HK_G u32x4*>(wc + at * 64));
+      s[u] = ws[at * 4];
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
-        u32x4 x = *reinterpret_cast<const HK_G u32x4*>(xr[b] + at * 64);
-        const uint32_t xv = in ? xs[b][at * 4] : 0u;
-        if (!in) x = u32x4{0, 0, 0, 0};
-        acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(c), fp4_operand(x), acc[b], 4, 4, 0, (int)s, 0, (int)xv);
-      }
-    } else {
-      const float f = mx_scale(s);
+        if constexpr (A4) {
+          sx[u][b] = xs[b][at * 4];
+          x[u][b][0] = *reinterpret_cast<const HK_G u32x4*>(xr[b] + at * 64);
+        } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const u32x4 wf = mx4_unpack8<T>(c[t], f);
+          for (int t = 0; t < XF; ++t) x[u][b][t] = *reinterpret_cast<const HK_G u32x4*>(xr[b] + (k * 4 + t < nb ? k * 256 + 64 * t : 0));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int64_t k = (st + u * NWV) * 4;
+      if (k + g >= nb) c[u] = u32x4{0, 0, 0, 0}, s[u] = 0;
+      if constexpr (A4) {
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
-          u32x4 x = *reinterpret_cast<const HK_G u32x4*>(xr[b] + at * 256 + 16 * t);
-          if (!in) x = u32x4{0, 0, 0, 0};
-          acc[b] = Mfma<T>::mac(wf, x, acc[b]);
+          if (k + g >= nb) x[u][b][0] = u32x4{0, 0, 0, 0}, sx[u][b] = 0;
+          acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(c[u]), fp4_operand(x[u][b][0]), acc[b], 4, 4, 0, (int)s[u], 0,
+                                                                    (int)sx[u][b]);
+        }
+      } else {
+        const u32x4 w = transpose_groups(c[u]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const u32x4 wf = mx4_unpack8<T>(w[t], mx_scale(__shfl(s[u], r16 + 16 * t, 64)));
+#pragma unroll
+          for (int b = 0; b < MB; ++b) acc[b] = Mfma<T>::mac(wf, k + t < nb ? x[u][b][t] : u32x4{0, 0, 0, 0}, acc[b]);
         }
       }
     }
@@ -115,56 +143,54 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(hrt_mx4_mm_args p, b
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
 #pragma unroll
-    for (int w = 0; w < kRowsWaves - 1; ++w) acc[b] += *reinterpret_cast<const f32x4*>(part[w][b][lane]);
+    for (int w = 0; w < NWV - 1; ++w) acc[b] += *reinterpret_cast<const f32x4*>(part[w][b][lane]);
     const float v[4] = {acc[b][0], acc[b][1], acc[b][2], acc[b][3]};
     store4<T>(p, b * 16 + r16, n0 + 4 * g, v, vec);
   }
 }
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------------
-// Rows of RB bytes in LDS: 32 (64 codes), 64 (128 codes) or 128 (64 16-bit values); a row's 16-byte chunks are XOR-swizzled
-// so that 16 consecutive rows read at one chunk hit distinct banks of a 256-byte line.
-template <int RB>
-__device__ __forceinline__ int row_swz(int row) {
-  if constexpr (RB == 128) return tile_swz<8>(row);
-  else if constexpr (RB == 64) return (row >> 2) & 3;
-  else return (row >> 3) & 1;
-}
-template <int RB>
-__device__ __forceinline__ int row_off(int row, int c) {
-  return row * RB + ((c ^ row_swz<RB>(row)) << 4);
-}
+// Everything in LDS is rows of 128 bytes, whole cache lines of both operands: 64 16-bit values or 256 codes.  (Rows of 32 or 64
+// bytes of codes, one step's worth, fetched each line four or two times over, since X streams through the L1 in between; that
+// traffic from L2 bounded the kernel: 4096 x 2048 x 8192 bf16 157 us, so 132.)  A row's 16-byte chunks are XOR-swizzled
+// (tile_swz<8>).
+constexpr int kLine = 128;
+__device__ __forceinline__ int line_off(int row, int c) { return tile_off<8>(row, c); }
 
-// A workgroup's wavefronts are KG groups along K times a grid of WM x WN sub-tiles: a step covers KG pieces of KS values of K,
-// one per group, and the groups' sums are added in order at the end.  KG > 1 gives small grids (few rows) the wavefronts that
-// hide a copy's latency without a second launch.
-template <bool A4, int BM, int BN, int WM, int WN, int KG>
+// A workgroup's wavefronts are KG groups along K times a grid of WM x WN sub-tiles.  A step takes KG pieces of K, one per group:
+// a piece is a line of X (KX values of K: 64, or 256 codes).  A stage of W holds whole lines of 256 values: 4-bit X uses
+// one per piece, 16-bit X one in four pieces, so that a W stage serves SPW steps.  KG > 1 gives small grids (few rows) the
+// wavefronts that hide a copy's latency without a second launch; the groups' sums are added in order at the end.
+// X has a ring of XR stages, W and the scales two.
+template <bool A4, int BM, int BN, int WM, int WN, int KG, int XR>
 struct TileShape {
-  static constexpr int KS = A4 ? 128 : 64;                // K values per piece
-  static constexpr int NWT = (BM / WM) * (BN / WN);       // wavefronts per group
-  static constexpr int NW = NWT * KG;
-  static constexpr int XB = A4 ? 64 : 128, WB = KS / 2;   // bytes of an LDS row of X and of W
-  static constexpr int XT = BM * XB, WT = BN * WB;        // bytes of a piece
-  static constexpr int IPX = KG * XT / 1024 / NW, IPW = KG * WT / 1024 / NW;  // copies per wavefront and step
+  static constexpr int KX = A4 ? 256 : 64, PPL = A4 ? 1 : 4;          // K values per piece, pieces per line of W
+  static constexpr int SPW = PPL > KG ? PPL / KG : 1, WL = KG > PPL ? KG / PPL : 1;  // steps per W stage, its lines per row
+  static constexpr int NWT = (BM / WM) * (BN / WN), NW = NWT * KG;    // wavefronts per group, in all
+  static constexpr int XT = KG * BM * kLine, WT = WL * BN * kLine;    // bytes of a stage
+  static constexpr int IPX = XT / 1024 / NW, IPW = WT / 1024 / NW;    // copies per wavefront
   static constexpr int FM = WM / 32, FN = WN / 32;
-  static_assert(KG * XT % (1024 * NW) == 0 && KG * WT % (1024 * NW) == 0 && IPX >= 1 && IPW >= 1, "copy split");
+  static constexpr int U = XR % (2 * SPW) == 0 ? XR : 2 * SPW;        // steps after which the buffers repeat
+  static_assert(XT % (1024 * NW) == 0 && WT % (1024 * NW) == 0 && U % XR == 0, "copy split, ring");
 };
 
-// STR: a row's scale bytes of one piece may straddle two dwords (K / 32 not a multiple of the bytes per piece).
-template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG, bool STR>
+// Scale bytes are staged apart, 32 of a row (1024 values of K) at a time: a lane that fetches one step's few bytes of its row
+// still occupies a cache line's turn, and 512 such lanes a step cost as much as the step's products.
+// STR: rows of scales do not start on dwords (K / 32 not a multiple of 4): fetched from the dword before, shifted when used.
+template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG, int XR, bool STR>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_mx4_mm_args p, int tiles_n, int nk, bool lines) {
-  using S = TileShape<A4, BM, BN, WM, WN, KG>;
-  constexpr int NW = S::NW, NWT = S::NWT, XB = S::XB, WB = S::WB, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN, KS = S::KS;
-  constexpr int SD = STR ? 2 : 1;                                  // scale dwords per row and piece
-  constexpr int SR = BN + (A4 ? BM : 0), SI = KG * SR * SD / 64;   // rows with scales; copies of 64 dwords
-  constexpr int IPS = (SI + NW - 1) / NW;                          // per wavefront (the last ones repeat a copy)
-  constexpr int SB = KS / 32;                                      // scale bytes per row and piece
-  static_assert(SR * SD % 64 == 0 && BN * SD % 64 == 0, "whole scale copies");
-  // One LDS object per stage, so that the compiler can tell the reads of one from the copies into another (it tracks only
-  // a few objects: with X, W and the scales apart it waited for every copy at the loop's head).
-  constexpr int STAGE = KG * (S::XT + S::WT) + SI * 256;
-  __shared__ __attribute__((aligned(1024))) uint8_t st0[STAGE], st1[STAGE], st2[STAGE];
-  auto buf = [&](auto ic) { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? st0 : I == 1 ? st1 : st2); };
+  using S = TileShape<A4, BM, BN, WM, WN, KG, XR>;
+  constexpr int NW = S::NW, NWT = S::NWT, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN, KX = S::KX, SPW = S::SPW, U = S::U;
+  constexpr int SB = KX / 32;                                    // scale bytes per row and piece
+  constexpr int SR = BN + (A4 ? BM : 0), SRB = STR ? 48 : 32;    // rows with scales (W's first), bytes of one in LDS
+  constexpr int SPB = 1024 / (KG * KX);                          // steps per block of scales
+  constexpr int SI = SR * SRB / 1024, IPS = (SI + NW - 1) / NW;  // copies per block, per wavefront (the last ones repeat a copy)
+  static_assert(SR * SRB % 1024 == 0 && BN * SRB % 1024 == 0 && SPB >= 1, "whole scale copies");
+  // One LDS object per stage, so that the compiler can tell the reads of one from the copies into another.
+  __shared__ __attribute__((aligned(1024))) uint8_t x0[S::XT], x1[S::XT], x2[XR > 2 ? S::XT : 16], x3[XR > 2 ? S::XT : 16];
+  __shared__ __attribute__((aligned(1024))) uint8_t w0[S::WT], w1[S::WT], sc[2 * SR * SRB];
+  auto xbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? x0 : I == 1 ? x1 : I == 2 ? x2 : x3); };
+  auto wbuf = [&](auto ic) HK_INLINE { return (HK_L uint8_t*)(decltype(ic)::value ? w1 : w0); };
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave / NWT, wt = wave % NWT, wm = wt % (BM / WM), wn = wt / (BM / WM), l32 = lane & 31, h = lane >> 5;
@@ -175,78 +201,87 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_
   const int64_t nb = p.K / 32;
   const int ml = p.M - m0 < BM ? (int)(p.M - m0) : BM, nl = p.N - n0 < BN ? (int)(p.N - n0) : BN;
 
-  // copy sources; lane offsets inside a step, kNoRow where the row does not exist (the buffer's range check gives zeros)
+  // copy sources; lane offsets inside a stage, kNoRow where the row does not exist (the buffer's range check gives zeros)
   const uint32_t xss = (uint32_t)(A4 ? p.K / 2 : p.x_sm * 2), wss = (uint32_t)(p.K / 2);
   const HK_G uint8_t* Xb = gcptr<uint8_t>(p.x) + m0 * xss;
   const HK_G uint8_t* Wb = gcptr<uint8_t>(p.w) + n0 * wss;
+  // copy j of a stage: its line (piece of X, line of W), and this lane's row and chunk in it
+  auto row_of = [&](int j, int rows) HK_INLINE { return (j * 8 + (lane >> 3)) % rows; };
+  auto chunk_of = [&](int j, int rows) HK_INLINE { return (lane & 7) ^ tile_swz<8>(row_of(j, rows)); };
   uint32_t xo[IPX], wo[IPW];
-  auto xchunk = [&](int i) {  // copy i's chunk within the piece: row and column
-    const int ch = ((wave * IPX + i) * 64 + lane) % (S::XT / 16), row = ch / (XB / 16);
-    return std::pair<int, int>{row, (ch % (XB / 16)) ^ row_swz<XB>(row)};
-  };
-  auto wchunk = [&](int i) {
-    const int ch = ((wave * IPW + i) * 64 + lane) % (S::WT / 16), row = ch / (WB / 16);
-    return std::pair<int, int>{row, (ch % (WB / 16)) ^ row_swz<WB>(row)};
-  };
-  auto xpiece = [&](int i) { return (wave * IPX + i) / (S::XT / 1024); };
-  auto wpiece = [&](int i) { return (wave * IPW + i) / (S::WT / 1024); };
 #pragma unroll
   for (int i = 0; i < IPX; ++i) {
-    const auto [row, c] = xchunk(i);
-    xo[i] = row < ml ? (uint32_t)row * xss + (uint32_t)(c * 16 + xpiece(i) * XB) : kNoRow;
+    const int j = wave * IPX + i, row = row_of(j, BM);
+    xo[i] = row < ml ? (uint32_t)row * xss + (uint32_t)(chunk_of(j, BM) * 16 + j / (BM / 8) * kLine) : kNoRow;
   }
 #pragma unroll
   for (int i = 0; i < IPW; ++i) {
-    const auto [row, c] = wchunk(i);
-    wo[i] = row < nl ? (uint32_t)row * wss + (uint32_t)(c * 16 + wpiece(i) * WB) : kNoRow;
+    const int j = wave * IPW + i, row = row_of(j, BN);
+    wo[i] = row < nl ? (uint32_t)row * wss + (uint32_t)(chunk_of(j, BN) * 16 + j / (BN / 8) * kLine) : kNoRow;
   }
-  // scales: dword d of row r (W rows first, then X rows) of piece k is LDS dword (k * SR + r) * SD + d.  Dwords are aligned
-  // down; what a row does not own is shifted or masked out where it is used.
-  const __amdgpu_buffer_rsrc_t wsr = edge_rsrc(gcptr<uint8_t>(p.w_scale)), xsr = edge_rsrc(gcptr<uint8_t>(A4 ? p.x_scale : p.w_scale));
-  uint32_t so[IPS];
-  bool sx[IPS];
+  // The last stage may hold fewer values: chunks past K are zeros (a select, not a branch: the compiler counts the copies in
+  // flight along every path).
+  auto copy_x = [&](int ks, HK_L uint8_t* to) HK_INLINE {
+    const __amdgpu_buffer_rsrc_t rs = edge_rsrc(Xb + (int64_t)ks * (KG * kLine));
+    const int64_t left = p.K - (int64_t)ks * (KG * KX);
+    const int l = left >= KG * KX ? KG * KX : (int)left;
 #pragma unroll
-  for (int i = 0; i < IPS; ++i) {
-    const int j = (wave * IPS + i) % SI;  // wavefronts past the last copy repeat an earlier one: the same bytes again
-    const int d = (j * 64 + lane) % (SR * SD), row = d / SD, piece = j * 64 / (SR * SD);
-    sx[i] = A4 && j * 64 % (SR * SD) / SD >= BN;  // uniform: BN * SD is a multiple of 64
-    const int r = sx[i] ? row - BN : row;
-    const int64_t o = ((sx[i] ? m0 : n0) + r) * nb + piece * SB;  // byte of the row's first scale in this piece
-    // (4 (d % SD): the second dword)
-    so[i] = r < (sx[i] ? ml : nl) ? (uint32_t)(o + 4 * (d % SD)) : kNoRow;
-  }
-
-  auto copy = [&](int ks, HK_L uint8_t* xt) {
-    HK_L uint8_t* const wt = xt + KG * S::XT;
-    HK_L uint8_t* const st = wt + KG * S::WT;
-    const __amdgpu_buffer_rsrc_t xr = edge_rsrc(Xb + (int64_t)ks * (KG * XB)), wr = edge_rsrc(Wb + (int64_t)ks * (KG * WB));
-    // the last step may hold fewer values: chunks past K are zeros (a select, not a branch: the compiler counts the copies
-    // in flight along every path)
-    const int64_t left = p.K - (int64_t)ks * (KG * KS);
-    const int l = left >= KG * KS ? KG * KS : (int)left;
+    for (int i = 0; i < IPX; ++i) {
+      const int j = wave * IPX + i;
+      edge_copy(rs, to, j, chunk_of(j, BM) * (A4 ? 32 : 8) + j / (BM / 8) * KX < l ? xo[i] : kNoRow);
+    }
+  };
+  auto copy_w = [&](int ws, HK_L uint8_t* to) HK_INLINE {
+    const __amdgpu_buffer_rsrc_t rs = edge_rsrc(Wb + (int64_t)ws * (S::WL * kLine));
+    const int64_t left = p.K - (int64_t)ws * (S::WL * 256);
+    const int l = left >= S::WL * 256 ? S::WL * 256 : (int)left;
 #pragma unroll
-    for (int i = 0; i < IPX; ++i)
-      edge_copy(xr, xt, wave * IPX + i, xchunk(i).second * (A4 ? 32 : 8) + xpiece(i) * KS < l ? xo[i] : kNoRow);
-#pragma unroll
-    for (int i = 0; i < IPW; ++i) edge_copy(wr, wt, wave * IPW + i, wchunk(i).second * 32 + wpiece(i) * KS < l ? wo[i] : kNoRow);
+    for (int i = 0; i < IPW; ++i) {
+      const int j = wave * IPW + i;
+      edge_copy(rs, to, j, chunk_of(j, BN) * 32 + j / (BN / 8) * 256 < l ? wo[i] : kNoRow);
+    }
+  };
+  const __amdgpu_buffer_rsrc_t wsr = __builtin_amdgcn_make_buffer_rsrc((void*)p.w_scale, (short)0, (int)((p.N * nb + 3) & ~3), 0x00020000);
+  const __amdgpu_buffer_rsrc_t xsr =
+      __builtin_amdgcn_make_buffer_rsrc((void*)(A4 ? p.x_scale : p.w_scale), (short)0, (int)(((A4 ? p.M : p.N) * nb + 3) & ~3), 0x00020000);
+  // scales of block blk (bytes past a row's end belong to the next one and are masked out where they are used)
+  auto copy_scales = [&](int blk) HK_INLINE {
+    HK_L uint8_t* const to = (HK_L uint8_t*)sc + (blk & 1) * (SR * SRB);
 #pragma unroll
     for (int i = 0; i < IPS; ++i) {
-      const int j = (wave * IPS + i) % SI;
-      const uint32_t o = so[i] == kNoRow ? kNoRow : (so[i] + (uint32_t)(ks * KG * SB)) & ~3u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(sx[i] ? xsr : wsr, st + j * 256, 4, (int)o, 0, 0, 0);
+      const int j = (wave * IPS + i) % SI;  // wavefronts past the last copy repeat an earlier one: the same bytes again
+      const bool isx = j * 1024 / SRB >= BN;
+      const int ch = j * 64 + lane, r = ch / (SRB / 16) - (isx ? BN : 0), c = ch % (SRB / 16);
+      const uint32_t o = ((uint32_t)(((isx ? m0 : n0) + r) * nb) & ~3u) + (uint32_t)(blk * 32 + c * 16);
+      edge_copy(isx ? xsr : wsr, to, j, r < (isx ? ml : nl) ? o : kNoRow);
     }
   };
 
   // This lane's rows: the sub-tile's other 32-row blocks lie a constant further (the swizzle repeats every 16 rows).
   const int xrow = wm * WM + l32, wrow = wn * WN + l32;
-  const int xbase = kg * S::XT, wbase = KG * S::XT + kg * S::WT, sbase = KG * (S::XT + S::WT) + kg * SR * SD * 4;
-  auto xat = [&](int i, int c) { return xbase + row_off<XB>(xrow, c) + i * 32 * XB; };
-  auto wat = [&](int j, int c) { return wbase + row_off<WB>(wrow, c) + j * 32 * WB; };
-  uint32_t wsh[FN], xsh[FM];  // byte of the row's first scale, modulo 4
+  auto xat = [&](int i, int c) HK_INLINE { return kg * BM * kLine + line_off(xrow, c) + i * 32 * kLine; };
+  auto wat = [&](int j, int c) HK_INLINE { return (S::WL > 1 ? kg * BN * kLine : 0) + line_off(wrow, c) + j * 32 * kLine; };
+  // byte of a row's first scale modulo 4 (STR)
+  uint32_t wsh[FN], xsh[FM];
 #pragma unroll
   for (int i = 0; i < FM; ++i) xsh[i] = (uint32_t)((m0 + xrow + 32 * i) * nb) & 3u;
 #pragma unroll
   for (int j = 0; j < FN; ++j) wsh[j] = (uint32_t)((n0 + wrow + 32 * j) * nb) & 3u;
+  // four scale bytes of one row from byte h + 4 d of this wavefront's piece on, those past the end of K zero
+  auto scales = [&](const HK_L uint8_t* cs, int row, uint32_t sh, int ks, int d) HK_INLINE {
+    const int64_t have = nb - ((int64_t)ks * KG + kg) * SB - 4 * d;
+    const uint32_t keep = have >= 4 ? ~0u : have <= 0 ? 0u : (1u << (8 * (int)have)) - 1u;
+    const uint32_t pos = ((uint32_t)((ks * KG + kg) * SB) & 31u) + 4 * d;
+    const HK_L uint8_t* const at = cs + row * SRB;
+    uint32_t v;
+    if constexpr (STR) {
+      const HK_L uint32_t* const q = reinterpret_cast<const HK_L uint32_t*>(at + ((pos + sh) & ~3u));
+      v = __builtin_amdgcn_alignbyte(q[1], q[0], (pos + sh) & 3u);
+    } else {
+      v = *reinterpret_cast<const HK_L uint32_t*>(at + (pos & ~3u)) >> (8 * (pos & 3u));
+    }
+    return (v & keep) >> (8 * h);
+  };
 
   f32x16 acc[FN][FM];
 #pragma unroll
@@ -254,119 +289,106 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_
 #pragma unroll
     for (int i = 0; i < FM; ++i) acc[j][i] = zero16();
 
-  // the scale bytes of one row in this wavefront's piece, the first in byte 0, those past the end of K zero
-  auto scales = [&](const HK_L uint8_t* st, int row, uint32_t sh, int ks) {
-    const int64_t first = ((int64_t)ks * KG + kg) * SB, have = nb - first;
-    const uint32_t keep = have >= 4 ? ~0u : have <= 0 ? 0u : (1u << (8 * (int)have)) - 1u;
-    const uint32_t by = (sh + (uint32_t)first) & 3u;
-    const HK_L uint8_t* const at = st + sbase + row * SD * 4;
-    uint32_t v;
-    if constexpr (STR) {
-      const u32x2 d = *reinterpret_cast<const HK_L u32x2*>(at);
-      v = __builtin_amdgcn_alignbyte(d.y, d.x, by);
-    } else {
-      v = *reinterpret_cast<const HK_L uint32_t*>(at) >> (8 * by);
+  // Step ks, number i of the unrolled U.  GUARD: near the end, where not every copy exists; it waits for all of them.
+  auto step = [&](auto ic, auto guard, int ks) HK_INLINE {
+    constexpr int I = decltype(ic)::value, WI = I % SPW;
+    constexpr bool GUARD = decltype(guard)::value;
+    const HK_L uint8_t* const xs = xbuf(std::integral_constant<int, I % XR>());
+    const HK_L uint8_t* const ws = wbuf(std::integral_constant<int, I / SPW % 2>());
+    const HK_L uint8_t* const cs = (const HK_L uint8_t*)sc + (ks / SPB & 1) * (SR * SRB);
+    u32x4 wf[2][FN], xf[2][FM];  // 16-bit X: wf[0] the piece's codes; 4-bit X: fragments of two slices
+    uint32_t sw[2][FN], sx[2][FM];
+    // a piece is four slices; the fragments of the next one are read while this one's products run (two register sets, fenced:
+    // in the compiler's own order every slice waited for its reads)
+    auto read_w = [&](int s) HK_INLINE {
+      // 16-bit X: piece WI KG + kg of the line
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        wf[s & 1][j] = *reinterpret_cast<const HK_L u32x4*>(ws + wat(j, A4 ? 2 * s + h : S::WL > 1 || KG == 1 ? 2 * WI + h : 2 * (WI * KG + kg) + h));
+    };
+    auto read_x = [&](int s) HK_INLINE {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) xf[s & 1][i] = *reinterpret_cast<const HK_L u32x4*>(xs + xat(i, A4 ? 2 * s + h : 4 * h + s));
+    };
+#pragma unroll
+    for (int d = 0; d < (A4 ? 2 : 1); ++d) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) sw[d][j] = scales(cs, wrow + 32 * j, wsh[j], ks, d);
+      if constexpr (A4)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sx[d][i] = scales(cs, BN + xrow + 32 * i, xsh[i], ks, d);
     }
-    return v & keep;
-  };
-
-  constexpr int PER = IPX + IPW + IPS;  // copies per wavefront and step
-  auto step = [&](auto bc, int ks, bool more) {
-    constexpr int BUF = decltype(bc)::value, NXT = (BUF + 2) % 3;
-    const HK_L uint8_t* const st = buf(bc);
-    using N = std::integral_constant<int, NXT>;
-    // fragments of the next slice are read while this one's products run (two register sets, fenced: in the compiler's own
-    // order every slice waited for its reads)
-    if constexpr (A4) {
-      uint32_t sw[FN], sxv[FM];
-      u32x4 wf[2][FN], xf[2][FM];
-      auto read = [&](int s) {
-#pragma unroll
-        for (int j = 0; j < FN; ++j) wf[s][j] = *reinterpret_cast<const HK_L u32x4*>(st + wat(j, 2 * s + h));
-#pragma unroll
-        for (int i = 0; i < FM; ++i) xf[s][i] = *reinterpret_cast<const HK_L u32x4*>(st + xat(i, 2 * s + h));
-      };
-#pragma unroll
-      for (int j = 0; j < FN; ++j) sw[j] = scales(st, wrow + 32 * j, wsh[j], ks) >> (8 * h);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) sxv[i] = scales(st, BN + xrow + 32 * i, xsh[i], ks) >> (8 * h);
-      read(0);
-      if (more) copy(ks + 2, buf(N()));
-      both([&](auto sc) {
-        constexpr int K64 = decltype(sc)::value;
-        __builtin_amdgcn_sched_barrier(0);
-        if (K64 == 0) read(1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(wf[K64][j]), fp4_operand(xf[K64][i]), acc[j][i], 4, 4,
-                                                                        2 * K64, (int)sw[j], 2 * K64, (int)sxv[i]);
-      });
-    } else {
-      u32x4 wc[FN], xf[2][FM];
-      float f[FN];
+    read_w(0);
+    read_x(0);
+    // copies: the next block of scales, the next stage of W, X of XR - 1 steps on
+    if (ks % SPB == 0 && (ks / SPB + 1) * SPB < nk) copy_scales(ks / SPB + 1);
+    if (WI == 0 && (!GUARD || ks + SPW < nk)) copy_w(ks / SPW + 1, wbuf(std::integral_constant<int, 1 - I / SPW % 2>()));
+    if (!GUARD || ks + XR - 1 < nk) copy_x(ks + XR - 1, xbuf(std::integral_constant<int, (I + XR - 1) % XR>()));
+    auto slice = [&](auto sc) HK_INLINE {
+      constexpr int SL = decltype(sc)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (SL < 3) {
+        if constexpr (A4) read_w(SL + 1);
+        read_x(SL + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        wc[j] = *reinterpret_cast<const HK_L u32x4*>(st + wat(j, h));
-        f[j] = mx_scale((scales(st, wrow + 32 * j, wsh[j], ks) >> (8 * h)) & 255u);
-      }
-      auto read = [&](int t) {
+        if constexpr (A4) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) xf[t & 1][i] = *reinterpret_cast<const HK_L u32x4*>(st + xat(i, 4 * h + t));
-      };
-      read(0);
-      if (more) copy(ks + 2, buf(N()));
+          for (int i = 0; i < FM; ++i)
+            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(wf[SL & 1][j]), fp4_operand(xf[SL & 1][i]), acc[j][i], 4, 4,
+                                                                        2 * (SL & 1), (int)sw[SL >> 1][j], 2 * (SL & 1), (int)sx[SL >> 1][i]);
+        } else {
+          const u32x4 f = mx4_unpack8<T>(wf[0][j][SL], mx_scale(sw[0][j] & 255u));
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (t < 3) read(t + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const u32x4 wf = mx4_unpack8<T>(wc[j][t], f[j]);
-#pragma unroll
-          for (int i = 0; i < FM; ++i) acc[j][i] = Mfma32<T>::mac(wf, xf[t & 1][i], acc[j][i]);
+          for (int i = 0; i < FM; ++i) acc[j][i] = Mfma32<T>::mac(f, xf[SL & 1][i], acc[j][i]);
         }
       }
-    }
-    // The products are pure, and the compiler puts them off to the end of the loop body, all three steps' fragments held
-    // in registers until then, unless their results are used here.
+    };
+    slice(std::integral_constant<int, 0>()), slice(std::integral_constant<int, 1>());
+    slice(std::integral_constant<int, 2>()), slice(std::integral_constant<int, 3>());
+    // The products are pure, and the compiler puts them off to the end of the loop body, the steps' fragments held in registers
+    // until then, unless their results are used here.
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int i = 0; i < FM; ++i) asm volatile("" : "+v"(acc[j][i]));
-    // the next step's copies (issued a step ago) have landed everywhere; this step's stay in flight
-    if (more) barrier_keep_vm_lds<PER>();
-    else barrier_keep_vm_lds<0>();
+    // The next step's X has landed everywhere, and W and scales if it begins a stage of theirs; later X may stay in flight, and
+    // with it W copied in this step or the one before (XR 4: its stage begins two steps on or later).
+    constexpr int KEEP = GUARD || XR == 2 ? 0 : (XR - 2) * IPX + (SPW > 2 && WI < 2 ? IPW : 0);
+    barrier_keep_vm_lds<KEEP>();
   };
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  using I2 = std::integral_constant<int, 2>;
-  copy(0, buf(I0()));
-  issue_order_fence();
-  copy(nk > 1 ? 1 : 0, buf(I1()));  // a single step: a copy that nobody reads, on every path alike
-  barrier_keep_vm<PER>();
-  int ks = 0;
-  for (; ks + 5 <= nk; ks += 3) {  // every step of the body copies: no branch around the copies
-    step(I0(), ks, true);
-    step(I1(), ks + 1, true);
-    step(I2(), ks + 2, true);
+  using Whole = std::integral_constant<bool, false>;
+  using Guard = std::integral_constant<bool, true>;
+  auto steps = [&](auto guard, int ks) HK_INLINE {
+    auto one = [&](auto ic) HK_INLINE {
+      if (!decltype(guard)::value || ks + decltype(ic)::value < nk) step(ic, guard, ks + decltype(ic)::value);
+    };
+    one(std::integral_constant<int, 0>()), one(std::integral_constant<int, 1>());
+    if constexpr (U > 2) one(std::integral_constant<int, 2>()), one(std::integral_constant<int, 3>());
+    if constexpr (U > 4)
+      one(std::integral_constant<int, 4>()), one(std::integral_constant<int, 5>()), one(std::integral_constant<int, 6>()), one(std::integral_constant<int, 7>());
+  };
+  static_assert(U == 2 || U == 4 || U == 8, "unrolled steps");
+  copy_scales(0);
+  copy_w(0, wbuf(std::integral_constant<int, 0>()));
+  copy_x(0, xbuf(std::integral_constant<int, 0>()));
+  if constexpr (XR > 2) {  // X of the steps before the first one's own copies (past the end: zeros that nobody reads)
+    copy_x(1, xbuf(std::integral_constant<int, 1>()));
+    copy_x(2, xbuf(std::integral_constant<int, 2>()));
   }
-  // the last one to four
-  step(I0(), ks, ks + 2 < nk);
-  if (ks + 1 < nk) step(I1(), ks + 1, ks + 3 < nk);
-  if (ks + 2 < nk) step(I2(), ks + 2, false);
-  if (ks + 3 < nk) step(I0(), ks + 3, false);
+  barrier_keep_vm<(XR - 2) * IPX>();
+  int ks = 0;
+  for (; ks + U + (XR - 1 > SPW ? XR - 1 : SPW) <= nk; ks += U) steps(Whole(), ks);
+  for (; ks < nk; ks += U) steps(Guard(), ks);
 
   if constexpr (KG > 1) {  // the groups' sums, in order, through the stages' memory (every copy has landed)
-    constexpr int NB = FN * FM, PB = KG == 2 ? NB / 2 : NB;  // accumulators, and how many of a wavefront's share a stage
-    static_assert((KG == 4 || (KG == 2 && NB % 2 == 0)) && NWT * PB * 4096 <= STAGE, "merge areas");
-    // accumulator b of group k: KG 4: the groups 1, 2, 3 have a stage each; KG 2: group 1 has two
+    constexpr int NB = FN * FM, PER = S::XT / 4096;  // accumulators of a wavefront; how many an X stage holds
+    static_assert((KG - 1) * NWT * NB <= 2 * PER && PER % NB == 0, "merge areas");
     auto area = [&](int k, int b) {
-      const int o = KG == 4 ? k - 1 : b / PB;
-      return (float*)(o == 0 ? st0 : o == 1 ? st1 : st2) + (wt * PB + b % PB) * 1024 + lane;
+      const int q = ((k - 1) * NWT + wt) * NB;
+      return (float*)(q < PER ? x0 + q * 4096 : x1 + (q - PER) * 4096) + b * 1024 + lane;
     };
     if (kg > 0) {
 #pragma unroll
@@ -402,12 +424,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_
   // Whole lines of y: 32 rows at a time go through the wavefront's own LDS area, so that a store writes 16 bytes a lane along
   // a row (8-byte stores straight from the accumulators touch 32 rows each: 4096 x 8192 x 2048 130 us, so 121).
   constexpr int RB = WN * 2 + 16;  // bytes of a row in the area, its pad off the banks of the next
-  // KG > 1: in the merge area of group 1's wavefront, which this one has read; else half of the areas in each of two stages
-  constexpr int HALF = (NWT + 1) / 2, MERGED = KG > 1 ? FN * FM / (KG == 2 ? 2 : 1) * 4096 : 0;
-  static_assert(KG > 1 ? 32 * RB <= MERGED : HALF * 32 * RB <= STAGE, "epilogue areas");
-  HK_L uint8_t* const area = KG > 1      ? (HK_L uint8_t*)st0 + wt * MERGED
-                             : wt < HALF ? (HK_L uint8_t*)st0 + wt * (32 * RB)
-                                         : (HK_L uint8_t*)st1 + (wt - HALF) * (32 * RB);
+  // KG > 1: in the merge area of group 1's wavefront, which this one has read; else in the stages of W
+  constexpr int HALF = (NWT + 1) / 2, AREA = 32 * RB, MERGED = FN * FM * 4096;
+  static_assert(KG > 1 ? AREA <= MERGED : HALF * AREA <= S::WT, "epilogue areas");
+  HK_L uint8_t* const area = KG > 1      ? (HK_L uint8_t*)(wt * MERGED < S::XT ? x0 + wt * MERGED : x1 + (wt * MERGED - S::XT))
+                             : wt < HALF ? (HK_L uint8_t*)w0 + wt * AREA
+                                         : (HK_L uint8_t*)w1 + (wt - HALF) * AREA;
   const int64_t nw = n0 + wn * WN;
   u32x2 bias[FN][4];
 #pragma unroll
@@ -448,36 +470,56 @@ constexpr Tile2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
 
 int64_t tiles_of(const hrt_mx4_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
 // Index of the tile, -1: mx4_rows.
+// Few rows: up to 16, or 32 where K is short (32 rows, 16 bits: 1024 x 1024 5.2 us against 6.4 on 64 x 64 tiles, 8192 x 2048 12.0
+// against 9.7).
+// Tiles: one workgroup fits a CU, so a grid runs in rounds of 256, each a fixed cost (first copies, epilogue) and a time per
+// 256 values of K, both fitted to 512 .. 8192 rows and columns, K 1024 .. 8192 (16-bit rows: 1024 x 8192 x 2048 128 x 256 tiles
+// 37 us, 128 x 128 41, 256 x 256 48; 4096 x 8192 x 2048 134, 158, 119; 640 x 4096 x 4096 51, 31, 83).
 int plan_of(const hrt_mx4_mm_args& a) {
-  if (a.M <= 64) return -1;
-  return tiles_of(a, 0) >= 256 ? 0 : tiles_of(a, 1) >= 192 ? 1 : tiles_of(a, 2) >= 192 ? 2 : 3;
+  if (a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
+  const bool a4 = a.x_scale != 0;
+  static constexpr struct { float fixed, per256; } kCost[2][4] = {{{8.5f, 6.3f}, {6.2f, 3.9f}, {6.1f, 2.1f}, {4.f, 0.75f}},
+                                                                  {{11.f, 1.9f}, {7.4f, 1.4f}, {5.4f, 0.74f}, {4.2f, 0.25f}}};
+  int best = 3;
+  float us = 0.f;
+  for (int t = 3; t >= 0; --t) {
+    // 256 x 256 tiles of 4-bit rows leave no LDS for scale rows that do not start on dwords
+    if (t == 0 && a4 && (a.K / 32) % 4 != 0) continue;
+    const float e = (float)cdiv(tiles_of(a, t), 256) * (kCost[a4][t].fixed + kCost[a4][t].per256 * (float)a.K / 256.f);
+    if (t == 3 || e < us) best = t, us = e;
+  }
+  return best;
 }
 
-template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG>
+template <typename T, bool A4, int BM, int BN, int WM, int WN, int KG, int XR, bool ODD = true>
 void queue_tile(const hrt_mx4_mm_args& a, hipStream_t s, bool lines) {
-  using S = TileShape<A4, BM, BN, WM, WN, KG>;
-  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, S::KS * KG);
+  using S = TileShape<A4, BM, BN, WM, WN, KG, XR>;
+  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, S::KX * KG);
   const dim3 grid((uint32_t)(tm * tn)), block(64 * S::NW);
-  if ((a.K / 32) % (S::KS / 32) != 0) hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, true>), grid, block, 0, s, a, (int)tn, (int)nk, lines);
-  else hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, false>), grid, block, 0, s, a, (int)tn, (int)nk, lines);
+  if constexpr (ODD)
+    if ((a.K / 32) % 4 != 0) {
+      hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, XR, true>), grid, block, 0, s, a, (int)tn, (int)nk, lines);
+      return;
+    }
+  hipLaunchKernelGGL((mx4_tile<T, A4, BM, BN, WM, WN, KG, XR, false>), grid, block, 0, s, a, (int)tn, (int)nk, lines);
 }
 
 template <typename T, bool A4>
 void queue_mm(const hrt_mx4_mm_args& a, int tile, hipStream_t s) {
   const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0, lines = vec && a.N % 8 == 0 && a.y % 16 == 0;
   switch (tile) {
-    case 0: return queue_tile<T, A4, 256, 256, 128, 64, 1>(a, s, lines);
-    case 1: return queue_tile<T, A4, 128, 256, 64, 64, 1>(a, s, lines);
-    case 2: return queue_tile<T, A4, 128, 128, 64, 64, 2>(a, s, lines);
-    case 3: return queue_tile<T, A4, 64, 64, 32, 64, 4>(a, s, lines);
+    case 0: return queue_tile<T, A4, 256, 256, 128, 64, 1, 2, !A4>(a, s, lines);
+    case 1: return queue_tile<T, A4, 128, 256, 64, 64, 1, A4 ? 2 : 4>(a, s, lines);
+    case 2: return queue_tile<T, A4, 128, 128, 64, 64, 2, 2>(a, s, lines);
+    case 3: return queue_tile<T, A4, 64, 64, 32, 64, 4, 2>(a, s, lines);
   }
-  const dim3 grid((uint32_t)cdiv(a.N, 16)), block(64 * kRowsWaves);
-  switch (cdiv(a.M, 16)) {
-    case 1: hipLaunchKernelGGL((mx4_rows<T, A4, 1>), grid, block, 0, s, a, vec); return;
-    case 2: hipLaunchKernelGGL((mx4_rows<T, A4, 2>), grid, block, 0, s, a, vec); return;
-    case 3: hipLaunchKernelGGL((mx4_rows<T, A4, 3>), grid, block, 0, s, a, vec); return;
-    default: hipLaunchKernelGGL((mx4_rows<T, A4, 4>), grid, block, 0, s, a, vec); return;
-  }
+  // wavefronts and batches that cover K once where they can
+  const dim3 grid((uint32_t)cdiv(a.N, 16));
+  const int64_t pieces = cdiv(a.K, 128);
+  if (a.M > 16) hipLaunchKernelGGL((mx4_rows<T, A4, 2, 4, 2>), grid, dim3(256), 0, s, a, vec);
+  else if (pieces <= 8) hipLaunchKernelGGL((mx4_rows<T, A4, 1, 4, 2>), grid, dim3(256), 0, s, a, vec);
+  else if (pieces <= 16) hipLaunchKernelGGL((mx4_rows<T, A4, 1, 8, 2>), grid, dim3(512), 0, s, a, vec);
+  else hipLaunchKernelGGL((mx4_rows<T, A4, 1, 8, 4>), grid, dim3(512), 0, s, a, vec);
 }
 
 template <typename T>
