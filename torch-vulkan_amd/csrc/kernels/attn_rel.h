@@ -181,6 +181,7 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   }
   if (WHICH == 0 && pl.splits > 1) split = id / total, id -= split * total;
   xcd_map32(id, total, pl.nblk, bh, blk);
+  if (WHICH != 1 && p.causal) blk = pl.nblk - 1 - blk;  // the longest rows first
   bh = __builtin_amdgcn_readfirstlane(bh), blk = __builtin_amdgcn_readfirstlane(blk), split = __builtin_amdgcn_readfirstlane(split);
   const int64_t b = bh / (uint32_t)p.H, hh = bh % (uint32_t)p.H;
   const int D = p.D, R = bk.R;
@@ -279,10 +280,9 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   float* const sums = dyn + NB * (1 + wave);                      // dQ: this wavefront's sums by distance
   float* const patch = dyn + NB * 5 + wave * (32 * 33);           // dQ: its patch
   const float inv_scale = 1.f / p.scale;
-  for (int t = tid; t < NB; t += 256) {  // the borders are scalars: a distance counts those that it reaches
+  for (int t = tid; t < NB; t += 256) {
     const int r = t - mid, n = r < 0 ? -r : r;
-    int k = 0;
-    for (int i = 1; i < bk.nb; ++i) k += n >= bk.start[i];
+    const int k = rel_bucket(bk, n);
     // one direction: positive distances are masked, and their values not used
     band[t] = r > 0 && bk.sides == 1 ? 0.f : T::to_f32(table[(int64_t)(r > 0 ? bk.nb + k : k) * p.H]) * inv_scale;
   }
@@ -290,7 +290,9 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
     if (p.dtable) {
       for (int t = lane; t < NB; t += 64) sums[t] = 0.f;
       int from = 0;
-      for (int i = 1; i < bk.nb; ++i) from = tid == i ? bk.start[i] : from;
+      for (int i = 0; i < bk.nb; i += 16)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) from = tid == i + j ? bk.start[i + j] : from;
       border[tid] = from;
     }
   }

@@ -6,6 +6,7 @@
 
 #include "../hrt/registry.h"
 #include "attn_rel_plan.h"
+#include "lds_stage.h"
 
 namespace hk {
 
@@ -45,6 +46,7 @@ bool make_buckets(int buckets, int m, int causal, RelBuckets* out) {
     out->start[e + t] = n;
   }
   out->R = out->start[nb - 1];
+  for (int k = nb; k < 256; ++k) out->start[k] = INT32_MAX;
   return true;
 }
 
@@ -62,29 +64,216 @@ const RelBuckets* buckets_of(const hrt_attn_rel_args& a) {
 }
 
 // ---- plan ------------------------------------------------------------------------------------------------------------------
+// Queries that the forward takes one at a time: their keys are then read once per query, by L2 from the second one on.
+constexpr int kOneMost = 4;
+
 RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R) {
   const int64_t n = which == 1 ? a.Sk : a.Sq, bh = (int64_t)a.B * a.H;
   auto blocks = [&](int g) { return cdiv(n, 32 * g); };
   const int dp = a.D <= 64 ? 64 : 128;
   RelPlan p{};
+  p.splits = 1;
+  if (which == 0 && n <= kOneMost) {  // g 0: one query at a time
+    const int64_t wgs = n * bh, want = cdiv(2048, wgs), most = cdiv(a.Sk, 256);
+    p.nblk = 1;
+    if (ws && want > 1 && most > 1) p.splits = (int)(want < most ? want : most);
+    if (p.splits > 64) p.splits = 64;
+    return p;
+  }
   p.g = blocks(4) * bh >= 512 ? 4 : f32 || blocks(2) * bh >= 256 ? 2 : 1;
   if (f32 && dp == 128) p.g = 4;  // the other forms' stages fill LDS
   // four buffers of 128 rows leave 29 KiB for the bands of far-reaching tables
   if (p.g == 1 && dp == 128 && rel_lds(which, R) > 29 * 1024) p.g = 2;
   p.nblk = (int)blocks(p.g);
-  p.splits = 1;
   const int64_t stages = cdiv(a.Sk, rel_stage(f32, dp, p.g)), wgs = p.nblk * bh;
   p.per = (int)stages;
   if (which == 0 && ws && wgs < 256 && stages >= 4) {
-    const int64_t want = cdiv(512, wgs), most = stages / 2;
+    int64_t want = cdiv(512, wgs), most = stages / 2;
+    if (most > 64) most = 64;  // attn_rel_join
     p.per = (int)cdiv(stages, want < most ? want : most);
     p.splits = (int)cdiv(stages, p.per);
   }
   return p;
 }
 
+// ---- one query at a time ---------------------------------------------------------------------------------------------------
+// Few queries (decoding): bound by the bytes of K and V, which tiles through LDS fetch too few of at a time.  A workgroup takes
+// one query of one head and one range of its keys; LPK lanes hold a key's 16-byte pieces, so a wavefront loads 64 / LPK keys
+// with one instruction, UB such instructions of K and of V in flight before the first is used.  Each lane group keeps its own
+// running maximum, sum and output piece over its keys; the groups are joined at the end, the wavefronts through LDS, the
+// ranges by attn_rel_join, always in one order.  Keys past the range's end or masked get an offset beyond the buffer and
+// are not fetched.
+template <typename T>
+struct Piece {  // 16 bytes of a row
+  static constexpr int N = 16 / sizeof(typename T::storage);
+  __device__ __forceinline__ static void unpack(u32x4 w, float* v) {
+    if constexpr (N == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[2 * i] = lo16<T>(w[i]), v[2 * i + 1] = hi16<T>(w[i]);
+    }
+  }
+};
+
+// The same in every lane of an aligned group of LPK.
+template <int LPK>
+__device__ __forceinline__ float group_sum(float v) {
+  v = dpp_add<0xB1>(v), v = dpp_add<0x4E>(v), v = dpp_add<0x141>(v);  // quads, then their mirror in the half row
+  if constexpr (LPK > 8) v = dpp_add<0x140>(v);
+  if constexpr (LPK > 16) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+template <typename T, int LPK>
+__global__ __launch_bounds__(256) void attn_rel_one(hrt_attn_rel_args p, RelBuckets bk, int64_t rows, int splits, int64_t range) {
+  constexpr int N = Piece<T>::N, KPW = 64 / LPK, UB = 4, ESZ = sizeof(typename T::storage);
+  __shared__ float band[2 * 1024 + 1];
+  __shared__ float part[3][LPK * N + 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), piece = lane % LPK, sub = lane / LPK;
+  const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x % (uint32_t)rows), split = __builtin_amdgcn_readfirstlane(blockIdx.x / (uint32_t)rows);
+  const int64_t q = row % (uint32_t)p.Sq, bh = row / (uint32_t)p.Sq, b = bh / p.H, hh = bh % p.H;
+  const int64_t at = q + p.q_off, R = bk.R;  // the query's position among the keys
+  int64_t k0 = split * range, k1 = k0 + range < p.Sk ? k0 + range : p.Sk;
+  if (p.causal && k1 > at + 1) k1 = at + 1 > 0 ? at + 1 : 0;
+  const uint32_t kss = (uint32_t)(p.k_ss * ESZ), vss = (uint32_t)(p.v_ss * ESZ);
+  const __amdgpu_buffer_rsrc_t kr = edge_rsrc(gcptr<uint8_t>(p.k) + (b * p.k_sb + hh * p.k_sh + k0 * p.k_ss) * ESZ);
+  const __amdgpu_buffer_rsrc_t vr = edge_rsrc(gcptr<uint8_t>(p.v) + (b * p.v_sb + hh * p.v_sh + k0 * p.v_ss) * ESZ);
+  const HK_G uint8_t* mask = gcptr<uint8_t>(p.mask) + b * p.mask_sb;
+  const int len = (int)(k1 > k0 ? k1 - k0 : 0);
+  const bool has = piece * N < p.D;
+  // the wavefronts take batches of UB KPW keys in turn; the next batch's mask is read under this one's arithmetic
+  constexpr int STEP = UB * KPW;
+  bool ok[UB], next[UB];
+  u32x4 kw[UB], vw[UB];
+  auto look = [&](int first, bool (&f)[UB]) {
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int k = first + u * KPW + sub;
+      f[u] = k < len;
+      if (p.mask) f[u] = f[u] && mask[k0 + (f[u] ? k : 0)] != 0;
+    }
+  };
+  auto load = [&](int first) {
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const uint32_t k = first + u * KPW + sub;
+      kw[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, ok[u] && has ? (int)(k * kss + piece * 16) : (int)kNoRow, 0, 0));
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const uint32_t k = first + u * KPW + sub;
+      vw[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, ok[u] && has ? (int)(k * vss + piece * 16) : (int)kNoRow, 0, 0));
+    }
+  };
+  int first = wave * STEP;
+  look(first, ok);
+  load(first);
+  float qv[N], o[N], m = -INFINITY, l = 0.f;
+  {
+    u32x4 w = {0, 0, 0, 0};
+    if (has) w = *reinterpret_cast<const HK_G u32x4*>(gcptr<uint8_t>(p.q) + (b * p.q_sb + hh * p.q_sh + q * p.q_ss) * ESZ + piece * 16);
+    Piece<T>::unpack(w, qv);
+#pragma unroll
+    for (int i = 0; i < N; ++i) qv[i] *= p.scale * 1.4426950408889634f, o[i] = 0.f;
+  }
+  // this query's bias by distance, in log2 units
+  const HK_G typename T::storage* table = gcptr<typename T::storage>(p.table) + hh;
+  for (int t = tid; t <= 2 * R; t += 256) {
+    const int r = t - (int)R, n = r < 0 ? -r : r;
+    const int k = rel_bucket(bk, n);
+    band[t] = r > 0 && bk.sides == 1 ? 0.f : T::to_f32(table[(int64_t)(r > 0 ? bk.nb + k : k) * p.H]) * 1.4426950408889634f;
+  }
+  __syncthreads();
+  for (; first < len; first += 4 * STEP) {
+    const bool more = first + 4 * STEP < len;
+    if (more) look(first + 4 * STEP, next);
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < UB; ++u) any = any || ok[u];
+    if (__any(any)) {
+      float s[UB], mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < UB; ++u) {
+        float kv[N], d = 0.f;
+        Piece<T>::unpack(kw[u], kv);
+#pragma unroll
+        for (int i = 0; i < N; ++i) d = fmaf(qv[i], kv[i], d);
+        const int64_t r = k0 + first + u * KPW + sub - at;
+        s[u] = group_sum<LPK>(d) + band[(r < -R ? -R : r > R ? R : r) + R];
+        if (!ok[u]) s[u] = -INFINITY;
+        mx = fmaxf(mx, s[u]);
+      }
+      const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - base);  // m = -inf: 0
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] *= alpha;
+#pragma unroll
+      for (int u = 0; u < UB; ++u) {
+        float vv[N];
+        const float e = __builtin_amdgcn_exp2f(s[u] - base);
+        Piece<T>::unpack(vw[u], vv);
+        l += e;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(e, vv[i], o[i]);
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < UB; ++u) ok[u] = next[u];
+      load(first + 4 * STEP);
+    }
+  }
+  // the lane groups of a wavefront, then the wavefronts
+#pragma unroll
+  for (int x = LPK; x < 64; x <<= 1) {
+    const float m2 = __shfl_xor(m, x, 64), mt = fmaxf(m, m2), base = mt == -INFINITY ? 0.f : mt;
+    const float a = __builtin_amdgcn_exp2f(m - base), c = __builtin_amdgcn_exp2f(m2 - base);
+    l = a * l + c * __shfl_xor(l, x, 64);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = a * o[i] + c * __shfl_xor(o[i], x, 64);
+    m = mt;
+  }
+  if (wave > 0 && sub == 0) {
+    float* const mine = part[wave - 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine[piece * N + i] = o[i];
+    if (piece == 0) mine[LPK * N] = m, mine[LPK * N + 1] = l;
+  }
+  __syncthreads();
+  if (wave > 0 || sub > 0) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    const float m2 = part[w][LPK * N], mt = fmaxf(m, m2), base = mt == -INFINITY ? 0.f : mt;
+    const float a = __builtin_amdgcn_exp2f(m - base), c = __builtin_amdgcn_exp2f(m2 - base);
+    l = a * l + c * part[w][LPK * N + 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = a * o[i] + c * part[w][piece * N + i];
+    m = mt;
+  }
+  if (splits > 1) {  // as the tile kernel leaves them
+    HK_G float* const to = gptr<float>(p.ws) + ((int64_t)split * rows + row) * p.D + piece * N;
+    if (has)
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<HK_G f32x4*>(to + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+    HK_G float* const st = gptr<float>(p.ws) + splits * rows * p.D + ((int64_t)split * rows + row) * 2;
+    if (piece == 0) st[0] = m, st[1] = l;
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (piece == 0) gptr<float>(p.lse)[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  HK_G typename T::storage* const out = gptr<typename T::storage>(p.o) + ((b * p.Sq + q) * p.H + hh) * p.D + piece * N;
+  if (has)
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = T::from_f32(o[i] * inv);
+}
+
 // ---- joins -----------------------------------------------------------------------------------------------------------------
-// Forward partial sums of the key ranges, added in order: a wavefront per row.
+// Forward partial sums of the key ranges, added in order: a wavefront per row.  The ranges' maxima and sums come in one load
+// per 64 ranges, the outputs four ranges at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rel_join(hrt_attn_rel_args p, int splits, int64_t rows) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -92,15 +281,27 @@ __global__ __launch_bounds__(256) void attn_rel_join(hrt_attn_rel_args p, int sp
   if (row >= rows) return;
   const HK_G float* o = gcptr<float>(p.ws);
   const HK_G float* ms = o + splits * rows * p.D;
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, ms[(s * rows + row) * 2]);
-  float l = 0.f, acc[2] = {0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float mk = ms[(s * rows + row) * 2], f = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - m);
-    l += f * ms[(s * rows + row) * 2 + 1];
+  float mine = -INFINITY, sum = 0.f;  // of range `lane`, splits <= 64
+  if (lane < splits) mine = ms[(lane * rows + row) * 2], sum = ms[(lane * rows + row) * 2 + 1];
+  const float m = wave_max(mine);
+  const float f = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - m);
+  const float l = wave_sum(f * sum);
+  float acc[2] = {0.f, 0.f};
+  for (int s = 0; s < splits; s += 4) {
+    float v[4][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < p.D) acc[u] += f * o[(s * rows + row) * p.D + lane + 64 * u];
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t r = s + x < splits ? s + x : 0;
+        v[x][u] = lane + 64 * u < p.D ? o[(r * rows + row) * p.D + lane + 64 * u] : 0.f;
+      }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float w = s + x < splits ? __shfl(f, s + x, 64) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) acc[u] = fmaf(w, v[x][u], acc[u]);
+    }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int64_t q = row % p.Sq, bh = row / p.Sq, b = bh / p.H, h = bh % p.H;
@@ -114,6 +315,16 @@ __global__ __launch_bounds__(256) void attn_rel_join(hrt_attn_rel_args p, int sp
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rel_table(hrt_attn_rel_args p, int64_t n) {
   rel_table<T>(p, n, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), threadIdx.x & 63);
+}
+
+template <typename T>
+void queue_one(const hrt_attn_rel_args& a, const RelBuckets& bk, const RelPlan& pl, hipStream_t s) {
+  const int64_t rows = (int64_t)a.B * a.H * a.Sq, range = cdiv(a.Sk, pl.splits);
+  const dim3 grid((uint32_t)(rows * pl.splits)), block(256);
+  const int pieces = (int)cdiv(a.D, Piece<T>::N);
+  if (pieces <= 8) hipLaunchKernelGGL((attn_rel_one<T, 8>), grid, block, 0, s, a, bk, rows, pl.splits, range);
+  else if (pieces <= 16) hipLaunchKernelGGL((attn_rel_one<T, 16>), grid, block, 0, s, a, bk, rows, pl.splits, range);
+  else hipLaunchKernelGGL((attn_rel_one<T, 32>), grid, block, 0, s, a, bk, rows, pl.splits, range);
 }
 
 // ---- launch ----------------------------------------------------------------------------------------------------------------
@@ -179,9 +390,15 @@ bool launch_rel(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
     if (!ctx.check(a.ws, (uint64_t)need * 4, "ws") || !ctx.check(a.dtable, (uint64_t)a.buckets * a.H * esz, "dtable")) return false;
     if (WHICH == 1) pl.table = (int)(cdiv((int64_t)a.buckets * a.H, 32) * 8), pl.parts = (int64_t)a.B * dq.nblk;
   }
-  if (!hrt::grid_fits((int64_t)pl.nblk * a.B * a.H * pl.splits + pl.table, 256) || !hrt::grid_fits(cdiv((int64_t)a.B * a.H * a.Sq, 4), 256))
+  if (!hrt::grid_fits((int64_t)(pl.g == 0 ? a.Sq : pl.nblk) * a.B * a.H * pl.splits + pl.table, 256) || !hrt::grid_fits(cdiv((int64_t)a.B * a.H * a.Sq, 4), 256))
     return ctx.fail("too many rows for one launch");
-  attn_rel_queue<T>(a, WHICH, *bk, pl, ctx.stream);
+  if (pl.g == 0) {
+    // a range's offsets are 31-bit
+    if (cdiv(a.Sk, pl.splits) * (a.k_ss > a.v_ss ? a.k_ss : a.v_ss) * esz >= ((int64_t)1 << 31) - 65536) return ctx.fail("keys too far apart");
+    queue_one<T>(a, *bk, pl, ctx.stream);
+  } else {
+    attn_rel_queue<T>(a, WHICH, *bk, pl, ctx.stream);
+  }
   if (!hrt::launch_ok(hipGetLastError(), ctx, "attn_rel")) return false;
   if (WHICH == 0 && pl.splits > 1) {
     const int64_t rows = (int64_t)a.B * a.H * a.Sq;

@@ -5,19 +5,30 @@
 
 namespace hk {
 
-// Buckets of one direction: bucket k holds the distances start[k] .. start[k + 1] - 1, the last one all from R = start[nb - 1].
+// Buckets of one direction: bucket k holds the distances start[k] .. start[k + 1] - 1, the last one all from R = start[nb - 1];
+// from start[nb] on: INT32_MAX.
 struct RelBuckets {
   int32_t nb, R, sides, total;  // sides 2: positive distances take buckets nb .. 2 nb - 1
   int32_t start[256];
 };
 
 struct RelPlan {
-  int g;             // query (key) groups per workgroup
+  int g;             // query (key) groups per workgroup; 0: forward of one query at a time (attn_rel.hip)
   int nblk;          // workgroups per head along the stationary rows
   int splits, per;   // forward: key ranges and stages in each
   int table;         // dK/dV: workgroups ahead of the others that finish the table's gradient
   int64_t parts;     // partial sums of it per head
 };
+
+// The bucket of distance n: how many borders it reaches.  They are scalars, sixteen to a load (one by one, a head's band of
+// distances took two microseconds of waits).
+__device__ __forceinline__ int rel_bucket(const RelBuckets& bk, int n) {
+  int k = -1;
+  for (int i = 0; i < bk.nb; i += 16)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) k += n >= bk.start[i + j];
+  return k;
+}
 
 constexpr int kRelMargin = 63;  // distances of a tile that reaches beyond R on one side
 
