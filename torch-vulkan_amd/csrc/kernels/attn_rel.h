@@ -149,6 +149,7 @@ struct RelShape {
   static constexpr int DCH = DP / 32, NACC = WHICH == 1 ? 2 * DCH : DCH;
   using Tile = RelTile<T, DP, ST>;
   static constexpr int TB = Tile::BYTES;
+  static constexpr int NBUF = std::is_same<T, F32>::value && G == 1 ? 1 : 2;  // 128 fp32 rows: one buffer, two workgroups on a CU
   static int lds(int R) { return rel_lds(WHICH, R); }
 };
 
@@ -159,9 +160,9 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   using S = RelShape<T, WHICH, DP, G>;
   using Tile = typename S::Tile;
   using frag = typename Tile::frag;
-  constexpr int KH = S::KH, ST = S::ST, TPW = S::TPW, DCH = S::DCH, NACC = S::NACC, TB = S::TB, ESZ = Tile::ESZ, NF = Tile::NF;
+  constexpr int KH = S::KH, ST = S::ST, NBUF = S::NBUF, TPW = S::TPW, DCH = S::DCH, NACC = S::NACC, TB = S::TB, ESZ = Tile::ESZ, NF = Tile::NF;
   // one LDS object per buffer: the compiler then knows that reads of one do not wait for the copies into the other
-  __shared__ __attribute__((aligned(1024))) uint8_t a0_raw[TB], a1_raw[TB], b0_raw[TB], b1_raw[TB];
+  __shared__ __attribute__((aligned(1024))) uint8_t a0_raw[TB], a1_raw[NBUF > 1 ? TB : 16], b0_raw[TB], b1_raw[NBUF > 1 ? TB : 16];
   __shared__ float stat[2][2][WHICH == 1 ? ST : 1];  // dK/dV: lse (log2 units) and delta of the streamed rows, per buffer
   __shared__ float ml[3][64][2];                     // the merge's maxima and sums; dQ: sums beyond R
   __shared__ int border[WHICH == 2 ? 256 : 1];       // dQ: the buckets' borders
@@ -427,25 +428,36 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   auto stage = [&](auto ic, int64_t st) {
     // stage st's copies are complete everywhere (and its mask, and the table's band); the other buffer is free
     barrier_keep_vm_lds<0>();
-    if (st + 1 < st1) {
-      stage_rows(st + 1, wn);
-      copy(std::integral_constant<int, 1 - decltype(ic)::value>(), st + 1, wn);
-      mask_load(st + 2);
-    }
+    auto following = [&](auto other) {
+      if (st + 1 < st1) {
+        stage_rows(st + 1, wn);
+        copy(other, st + 1, wn);
+        mask_load(st + 2);
+      }
+    };
+    if constexpr (NBUF > 1) following(std::integral_constant<int, 1 - decltype(ic)::value>());
 #pragma unroll
     for (int u = 0; u < TPW; ++u) {
       const int r0 = 32 * (kh + u * KH);
       const uint32_t bits = (uint32_t)((r0 >= 64 ? w[1] : w[0]) >> (r0 & 63));
       if (bits) tile(ic, st, r0, bits);
     }
+    if constexpr (NBUF == 1) {
+      if (st + 1 < st1) barrier_keep_vm_lds<0>();  // every wavefront is done with the stage
+      following(ic);
+    }
     w[0] = wn[0], w[1] = wn[1];
   };
   int64_t st = st0;
-  for (; st + 2 <= st1; st += 2) {
-    stage(I0(), st);
-    stage(I1(), st + 1);
+  if constexpr (NBUF > 1) {
+    for (; st + 2 <= st1; st += 2) {
+      stage(I0(), st);
+      stage(I1(), st + 1);
+    }
+    if (st < st1) stage(I0(), st);
+  } else {
+    for (; st < st1; ++st) stage(I0(), st);
   }
-  if (st < st1) stage(I0(), st);
 
   // ---- merge the KH partial results of each group into the wavefront kh = 0, in order, through the tiles' memory
   __syncthreads();
@@ -472,8 +484,8 @@ __global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel
   }
   if constexpr (KH > 1) {
     constexpr int CH = TB / 4096 < NACC ? TB / 4096 : NACC;  // accumulators per round: 4 KiB each
-    static_assert(CH >= 1 && NACC % CH == 0, "merge rounds");
-    auto piece = [&](int s) { return (float*)(s == 0 ? a0_raw : s == 1 ? a1_raw : b0_raw); };
+    static_assert(CH >= 1 && NACC % CH == 0 && (NBUF > 1 || 2 * NACC * 4096 <= TB), "merge rounds");
+    auto piece = [&](int s) { return (float*)(s == 0 ? a0_raw : s == 2 ? b0_raw : NBUF > 1 ? a1_raw : a0_raw + NACC * 4096); };
 #pragma unroll
     for (int r = 0; r < NACC; r += CH) {
       if (r > 0) __syncthreads();
@@ -581,7 +593,7 @@ void attn_rel_g(const hrt_attn_rel_args& a, const RelBuckets& bk, const RelPlan&
   if (pl.g == 4) attn_rel_go<T, WHICH, DP, 4>(a, bk, pl, s);
   if constexpr (!std::is_same<T, F32>::value || DP == 64)
     if (pl.g == 2) attn_rel_go<T, WHICH, DP, 2>(a, bk, pl, s);
-  if constexpr (!std::is_same<T, F32>::value)
+  if constexpr (!std::is_same<T, F32>::value || DP == 64)
     if (pl.g == 1) attn_rel_go<T, WHICH, DP, 1>(a, bk, pl, s);
 }
 

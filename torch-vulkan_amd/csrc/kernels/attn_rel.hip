@@ -74,13 +74,27 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
   RelPlan p{};
   p.splits = 1;
   if (which == 0 && n <= kOneMost) {  // g 0: one query at a time
-    const int64_t wgs = n * bh, want = cdiv(2048, wgs), most = cdiv(a.Sk, 256);
+    const int64_t wgs = n * bh, want = cdiv(1024, wgs), most = cdiv(a.Sk, 256);
     p.nblk = 1;
     if (ws && want > 1 && most > 1) p.splits = (int)(want < most ? want : most);
     if (p.splits > 64) p.splits = 64;
     return p;
   }
-  p.g = blocks(4) * bh >= 512 ? 4 : f32 || blocks(2) * bh >= 256 ? 2 : 1;
+  // groups a workgroup: more share a stage, fewer give more workgroups.  bf16, forward and backward, by one / two / four groups:
+  // 48 heads of 512 x 512 x 64 (768 / 384 / 192 workgroups) 90 / 60 / 86 us, 64 heads of 1024 x 1024 x 128 (2048 / 1024 / 512)
+  // 592 / 368 / 303 us
+  p.g = blocks(4) * bh >= 512 ? 4 : blocks(2) * bh >= 256 ? 2 : 1;
+  if (f32) {
+    // fp32 is bound by the matrix cores, so by the CU with the most workgroups: a workgroup of one / two / four groups takes
+    // 50 / 80 / 150 us against 1024 keys.  16 heads of 1040 x 1040 x 64 (528 / 272 / 144): 394 / 411 / 385 us, 12 heads of
+    // 512 x 512 (192 / 96 / 48): 87 / 119 / 187 us
+    const int cost[5] = {0, 10, 16, 0, 30};
+    int64_t least = 0;
+    for (int g : {4, 2, 1}) {
+      const int64_t t = cdiv(blocks(g) * bh, 256) * cost[g];
+      if (g == 4 || t < least) p.g = g, least = t;
+    }
+  }
   if (f32 && dp == 128) p.g = 4;  // the other forms' stages fill LDS
   // four buffers of 128 rows leave 29 KiB for the bands of far-reaching tables
   if (p.g == 1 && dp == 128 && rel_lds(which, R) > 29 * 1024) p.g = 2;
