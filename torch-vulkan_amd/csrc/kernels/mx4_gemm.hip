@@ -79,8 +79,9 @@ __global__ __launch_bounds__(64 * NWV) void mx4_rows(hrt_mx4_mm_args p, bool vec
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;  // columns past N repeat the last one and are not stored
   const int64_t nb = p.K / 32, steps = cdiv(p.K, 128);
-  const HK_G uint8_t* wc = gcptr<uint8_t>(p.w) + n * (p.K / 2) + 16 * g;
-  const HK_G uint8_t* ws = gcptr<uint8_t>(p.w_scale) + n * nb + g;
+  const int gb = g < nb ? g : 0;  // a row of fewer than four blocks: the other lane groups stay inside it
+  const HK_G uint8_t* wc = gcptr<uint8_t>(p.w) + n * (p.K / 2) + 16 * gb;
+  const HK_G uint8_t* ws = gcptr<uint8_t>(p.w_scale) + n * nb + gb;
   f32x4 acc[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -89,8 +90,8 @@ __global__ __launch_bounds__(64 * NWV) void mx4_rows(hrt_mx4_mm_args p, bool vec
 #pragma unroll
   for (int b = 0; b < MB; ++b) {  // rows past M repeat the last one and are not stored
     const int64_t m = b * 16 + r16 < p.M ? b * 16 + r16 : p.M - 1;
-    xr[b] = A4 ? gcptr<uint8_t>(p.x) + m * (p.K / 2) + 16 * g : gcptr<uint8_t>(p.x) + m * p.x_sm * 2 + 16 * g;
-    xs[b] = gcptr<uint8_t>(p.x_scale) + m * nb + g;
+    xr[b] = A4 ? gcptr<uint8_t>(p.x) + m * (p.K / 2) + 16 * gb : gcptr<uint8_t>(p.x) + m * p.x_sm * 2 + 16 * g;
+    xs[b] = gcptr<uint8_t>(p.x_scale) + m * nb + gb;
   }
   for (int64_t st = wave; st < steps; st += NWV * UB) {
     u32x4 c[UB], x[UB][MB][XF];
