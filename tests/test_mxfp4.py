@@ -180,6 +180,22 @@ def test_linear(M, N, K, quantize, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("M,N,K", [(7, 136, 4160), (16, 40, 2112), (1000, 1000, 1280), (2000, 2000, 1280), (2500, 2000, 1280), (2500, 2001, 1184),
+                                   (1000, 8200, 1280), (1000, 8200, 1184)])
+def test_linear_over_several_blocks_of_scales(M, N, K, quantize, dtype):
+    """Every tile over more than 1024 values of K, and few rows over more than 2048; every 37th row is compared, and the last."""
+    x, codes, scale, b = operands(M, N, K, dtype, M + N + K)
+    some = sorted({*range(0, M, 37), M - 1})
+    w, part = values(codes, scale, K), x[some]
+    xr = values(*torch_vulkan.quantize_mxfp4(part), K) if quantize else part.double().numpy()
+    bias = b.double().numpy()
+    y = torch_vulkan.mxfp4_linear(*(t.to(vk) for t in (x, codes, scale, b)), quantize)
+    check(y.cpu()[some], xr @ w.T + bias, np.abs(xr) @ np.abs(w).T + np.abs(bias), K + 1, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("quantize", [False, True])
 @pytest.mark.parametrize("M,N,K", [(5, 40, 33), (70, 64, 100), (3, 8, 1), (4, 8, 0), (0, 8, 64), (4, 0, 64)])
 def test_linear_of_rows_that_end_inside_a_block_and_of_nothing(M, N, K, quantize):

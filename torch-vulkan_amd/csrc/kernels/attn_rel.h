@@ -156,7 +156,7 @@ struct RelShape {
 __device__ __forceinline__ uint64_t low_bits(int64_t n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 template <typename T, int WHICH, int DP, int G>
-__global__ __launch_bounds__(256, DP == 128 && WHICH != 0 ? 1 : 2) void attn_rel_k(hrt_attn_rel_args p, RelBuckets bk, RelPlan pl) {
+__global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) void attn_rel_k(hrt_attn_rel_args p, RelBuckets bk, RelPlan pl) {
   using S = RelShape<T, WHICH, DP, G>;
   using Tile = typename S::Tile;
   using frag = typename Tile::frag;
