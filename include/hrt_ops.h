@@ -275,9 +275,10 @@ int64_t hrt_attn_dkdv_workspace(const hrt_attn_args* args);
  * e = nb / 2: n below e, else the largest e + t <= nb - 1 with (n / e)^(nb - e) >= (max_distance / e)^t, decided in whole
  * numbers.  Key j is allowed where mask (one byte a key, rows mask_sb apart, 0: no mask) is not 0 and, if causal,
  * j <= i + q_off.  A row without an allowed key gives o = 0, lse = -inf and no gradient; masked keys and values are not read.
- *  "attn_rel_fwd_{dt}":  o [B, Sq, H, D]-contiguous, lse fp32 [B, H, Sq].  ws (optional): ws_floats of fp32 workspace, where
+ *  "attn_rel_fwd_{dt}":  o [B, Sq, H, D]-contiguous, lse fp32 [B, H, Sq].  o_lo (optional, 16-bit types): what o's rounding left,
+ *     laid out like o and rounded once more, for dq.  ws (optional): ws_floats of fp32 workspace, where
  *     hrt_attn_rel_workspace(&args, dtype, 0) asks for them: few query rows then share their keys out over workgroups.
- *  "attn_rel_dq_{dt}":   delta[b, h, i] = rowsum(o dout) (fp32, from the o given), dq where it is not 0, and, where dtable != 0, dtable
+ *  "attn_rel_dq_{dt}":   delta[b, h, i] = rowsum(o dout) (fp32, from the o and o_lo given), dq where it is not 0, and, where dtable != 0, dtable
  *     [buckets, H] of the type (rounded once), with ws of hrt_attn_rel_workspace(&args, dtype, 1) floats, which it needs then.
  *  "attn_rel_dkdv_{dt}": dk, dv, from the delta that dq stored.
  * dq, dk, dv are [B, S, H, D]-contiguous, or with HRT_ATTN_GRAD_LIKE_INPUT in the strides of q, k, v.  All rows (and o, the
@@ -290,7 +291,7 @@ int64_t hrt_attn_dkdv_workspace(const hrt_attn_args* args);
 typedef struct hrt_attn_rel_args {
   uint64_t q, k, v, table, mask;
   uint64_t o, lse, dout, delta;
-  uint64_t dq, dk, dv, dtable, ws;
+  uint64_t dq, dk, dv, dtable, ws, o_lo;
   int64_t q_sb, q_sh, q_ss;
   int64_t k_sb, k_sh, k_ss;
   int64_t v_sb, v_sh, v_ss;

@@ -336,6 +336,35 @@ def test_recorded_forward_and_backward():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("B,H,Sq,Sk,D", [(2, 3, 77, 77, 64), (1, 2, 40, 333, 128), (1, 3, 9, 3000, 40), (1, 2, 3, 100, 72), (1, 1, 1, 3000, 64), (16, 32, 70, 50, 16)])
+def test_what_the_outputs_rounding_left(B, H, Sq, Sk, D, dtype):
+    """Queries and a table of zeros: o is the mean of v, P = 1 exactly, so o + o_lo is off by two roundings in a row and the fp32
+    sum's, and so is delta."""
+    g = torch.Generator().manual_seed(Sk)
+    q, v, do = torch.zeros(B, Sq, H, D, dtype=dtype), torch.randn((B, Sk, H, D), generator=g).to(dtype), torch.randn((B, Sq, H, D), generator=g).to(dtype)
+    o, lo, dq = (torch.full((B, Sq, H, D), float("nan"), dtype=dtype, device=vk) for _ in range(3))
+    lse, delta, ws = (torch.empty(n, device=vk) for n in (B * H * Sq, B * H * Sq, 1 << 18))
+    t = {"q": q, "k": v, "v": v, "dout": do, "table": torch.zeros(32, H, dtype=dtype)}
+    t = {n: x.to(vk) for n, x in t.items()}
+    a = abi.AttnRelArgs(B=B, H=H, Sq=Sq, Sk=Sk, D=D, buckets=32, max_distance=128, scale=1.0, ws_floats=1 << 18, **{n: x.data_ptr() for n, x in t.items()},
+                        o=o.data_ptr(), o_lo=lo.data_ptr(), lse=lse.data_ptr(), delta=delta.data_ptr(), dq=dq.data_ptr(), ws=ws.data_ptr())
+    for n, S in (("q", Sq), ("k", Sk), ("v", Sk), ("do", Sq)):
+        setattr(a, f"{n}_sb", S * H * D), setattr(a, f"{n}_sh", D), setattr(a, f"{n}_ss", H * D)
+    tag = {torch.bfloat16: "bf16", torch.float16: "f16"}[dtype]
+    for which in ("fwd", "dq"):
+        abi.Runtime().dispatch(f"attn_rel_{which}_{tag}", a)
+    mean, size = v.double().mean(1, keepdim=True), v.double().abs().mean(1, keepdim=True)  # [B, 1, H, D]
+    u, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    tol = (1.1 * (u * u * mean.abs() + (Sk + 4) * 2.0**-24 * size) + tiny).expand(B, Sq, H, D)
+    got = o.cpu().double() + lo.cpu().double()
+    assert ((got - mean).abs() <= tol).all() and (lo.cpu().double().abs() <= 1.01 * u * o.cpu().double().abs() + tiny).all()
+    ref = (mean * do.double()).sum(-1).transpose(1, 2)
+    tol = (tol * do.double().abs()).sum(-1).transpose(1, 2) + 2 * D * 2.0**-24 * (1.01 * mean * do.double()).abs().sum(-1).transpose(1, 2)
+    assert ((delta.cpu().double().view(B, H, Sq) - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 def test_without_room_for_the_key_ranges():
     """The forward of few rows goes on without its workspace, in the plain order of its sums."""
     c = CASES["split_masked"]

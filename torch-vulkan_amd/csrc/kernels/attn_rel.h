@@ -21,7 +21,9 @@
 // stages and tiles without a single key to see are skipped.  The first product leaves a stationary row per lane, so that the
 // softmax statistics are per lane and P and dS feed the second product from registers (attn_common.h, attn_f32_tile.h).
 // 16-bit P and dS are rounded to the input type before the second product, as in the other fused kernels; sums, statistics
-// and the table's gradient are fp32.
+// and the table's gradient are fp32.  delta = rowsum(o dO) is one error for a whole row of dS, so o comes with what its rounding
+// left (o_lo, a training forward's): f16, one head of 512 x 512 x 128 causal, these roundings alone put dk and dq off by 0.00029 of
+// their norm, 0.00032 without o_lo (the gradients' own rounding 0.00021).  It costs 2 % of forward and backward.
 #pragma once
 
 #include <cmath>
@@ -95,6 +97,23 @@ struct RelTile16 {
       const int d = 32 * n + 8 * j + 4 * h;
       const float o[4] = {v[4 * j] * mul, v[4 * j + 1] * mul, v[4 * j + 2] * mul, v[4 * j + 3] * mul};
       if (d < D) *reinterpret_cast<HK_G u32x2*>(row + 2 * d) = pack4<T>(o);
+    }
+  }
+  // what `store` of the same values leaves, a row like its own
+  __device__ __forceinline__ static void store_left(HK_G uint8_t* row, const f32x16& v, float mul, int n, int D, int h) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = 32 * n + 8 * j + 4 * h;
+      float o[4], left[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = v[4 * j + e] * mul;
+      const u32x2 w = pack4<T>(o);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float r = e & 1 ? hi16<T>(w[e >> 1]) : lo16<T>(w[e >> 1]);
+        left[e] = fabsf(r) < INFINITY ? o[e] - r : 0.f;
+      }
+      if (d < D) *reinterpret_cast<HK_G u32x2*>(row + 2 * d) = pack4<T>(left);
     }
   }
 };
@@ -267,9 +286,15 @@ __global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) v
   if constexpr (WHICH != 0) Tile::load(f1, WHICH == 1 ? V + own * p.v_ss * ESZ : dO + own * p.do_ss * ESZ, own_ok, D, h);
   float lse2 = 0.f, dlt = 0.f;
   if constexpr (WHICH == 2) {
-    frag o[NF];  // delta = rowsum(o dO), from the stored o
-    Tile::load(o, gcptr<uint8_t>(p.o) + ((b * Sq + own) * p.H + hh) * D * ESZ, own_ok, D, h);
-    dlt = halfswap_sum(Tile::dot(o, f1));
+    frag o[NF];  // delta = rowsum(o dO), from the stored o and what its rounding left
+    const int64_t at = ((b * Sq + own) * p.H + hh) * D * ESZ;
+    Tile::load(o, gcptr<uint8_t>(p.o) + at, own_ok, D, h);
+    dlt = Tile::dot(o, f1);
+    if (ESZ == 2 && p.o_lo) {
+      Tile::load(o, gcptr<uint8_t>(p.o_lo) + at, own_ok, D, h);
+      dlt += Tile::dot(o, f1);
+    }
+    dlt = halfswap_sum(dlt);
     lse2 = own_ok ? gcptr<float>(p.lse)[(int64_t)bh * Sq + own] * kLog2e : INFINITY;
     if (lse2 == -INFINITY) lse2 = INFINITY;
     if (own_ok && kh == 0 && h == 0) gptr<float>(p.delta)[(int64_t)bh * Sq + own] = dlt;
@@ -555,9 +580,15 @@ __global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) v
     }
     const float inv = lrow > 0.f ? 1.f / lrow : 0.f;  // no key: zeros
     if (h == 0) gptr<float>(p.lse)[row] = lrow > 0.f ? (m + log2f(lrow)) * kLn2 : -INFINITY;
-    HK_G uint8_t* const o = gptr<uint8_t>(p.o) + ((b * Sq + own) * p.H + hh) * D * ESZ;
+    const int64_t at = ((b * Sq + own) * p.H + hh) * D * ESZ;
 #pragma unroll
-    for (int n = 0; n < DCH; ++n) Tile::store(o, acc[0][n], inv, n, D, h);
+    for (int n = 0; n < DCH; ++n) Tile::store(gptr<uint8_t>(p.o) + at, acc[0][n], inv, n, D, h);
+    if constexpr (ESZ == 2) {
+      if (p.o_lo) {
+#pragma unroll
+        for (int n = 0; n < DCH; ++n) Tile::store_left(gptr<uint8_t>(p.o_lo) + at, acc[0][n], inv, n, D, h);
+      }
+    }
   } else {
     const bool like = (p.flags & HRT_ATTN_GRAD_LIKE_INPUT) != 0;
     auto row_of = [&](uint64_t base, int64_t sb, int64_t sh, int64_t ss, int64_t n) {

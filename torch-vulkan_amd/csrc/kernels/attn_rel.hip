@@ -140,6 +140,17 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// One value of o, and what its rounding left (none of a value that became no number).
+template <typename T>
+__device__ __forceinline__ void put_o(const hrt_attn_rel_args& p, int64_t at, float v) {
+  const typename T::storage o = T::from_f32(v);
+  gptr<typename T::storage>(p.o)[at] = o;
+  if constexpr (!std::is_same<T, F32>::value) {
+    const float r = T::to_f32(o);
+    if (p.o_lo) gptr<typename T::storage>(p.o_lo)[at] = T::from_f32(fabsf(r) < INFINITY ? v - r : 0.f);
+  }
+}
+
 template <typename T, int LPK>
 __global__ __launch_bounds__(256) void attn_rel_one(hrt_attn_rel_args p, RelBuckets bk, int64_t rows, int splits, int64_t range) {
   constexpr int N = Piece<T>::N, KPW = 64 / LPK, UB = 4, ESZ = sizeof(typename T::storage);
@@ -279,10 +290,11 @@ __global__ __launch_bounds__(256) void attn_rel_one(hrt_attn_rel_args p, RelBuck
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   if (piece == 0) gptr<float>(p.lse)[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-  HK_G typename T::storage* const out = gptr<typename T::storage>(p.o) + ((b * p.Sq + q) * p.H + hh) * p.D + piece * N;
-  if (has)
+  if (has) {
+    const int64_t out = ((b * p.Sq + q) * p.H + hh) * p.D + piece * N;
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = T::from_f32(o[i] * inv);
+    for (int i = 0; i < N; ++i) put_o<T>(p, out + i, o[i] * inv);
+  }
 }
 
 // ---- joins -----------------------------------------------------------------------------------------------------------------
@@ -320,10 +332,10 @@ __global__ __launch_bounds__(256) void attn_rel_join(hrt_attn_rel_args p, int sp
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int64_t q = row % p.Sq, bh = row / p.Sq, b = bh / p.H, h = bh % p.H;
   if (lane == 0) gptr<float>(p.lse)[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-  HK_G typename T::storage* out = gptr<typename T::storage>(p.o) + ((b * p.Sq + q) * p.H + h) * p.D;
+  const int64_t out = ((b * p.Sq + q) * p.H + h) * p.D + lane;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
-    if (lane + 64 * u < p.D) out[lane + 64 * u] = T::from_f32(acc[u] * inv);
+    if (lane + 64 * u < p.D) put_o<T>(p, out + 64 * u, acc[u] * inv);
 }
 
 template <typename T>
@@ -368,6 +380,8 @@ bool check(const hrt_attn_rel_args& a, int which, int esz, hrt::LaunchCtx& ctx) 
   if (a.mask && !ctx.check(a.mask, (uint64_t)((a.B - 1) * a.mask_sb + a.Sk), "mask")) return false;
   if (which != 1 && a.o % 16 != 0) return ctx.fail("o must be 16-byte aligned");
   if (which != 1 && !ctx.check(a.o, rows * a.D * esz, "o")) return false;
+  if (which != 1 && esz == 2 && a.o_lo && (a.o_lo % 16 != 0 || !ctx.check(a.o_lo, rows * a.D * esz, "o_lo")))
+    return a.o_lo % 16 != 0 ? ctx.fail("o_lo must be 16-byte aligned") : false;
   if (which != 0 && (!view(a.dout, 9, a.Sq, "dout") || !ctx.check(a.delta, rows * 4, "delta"))) return false;
   // gradients: contiguous, or spread like their inputs
   auto grad = [&](uint64_t at, int i, int64_t S, const char* what) {

@@ -71,7 +71,8 @@ at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& codes, const at::T
     quantize_rows(rows, xc, xs);
     A.x = dptr(xc), A.x_scale = dptr(xs);
   } else {
-    if (rows.stride(0) % 8 != 0 || dptr(rows) % 16 != 0) rows = rows.clone(at::MemoryFormat::Contiguous);
+    // the kernel reads whole 16-byte words and keeps a tile's row offsets in 31 bits
+    if (rows.stride(0) % 8 != 0 || dptr(rows) % 16 != 0 || rows.stride(0) >= 4000000) rows = rows.clone(at::MemoryFormat::Contiguous);
     A.x = dptr(rows), A.x_sm = rows.stride(0);
   }
   const at::Tensor y = at::empty({M, N}, x.options());

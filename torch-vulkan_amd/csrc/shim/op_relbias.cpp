@@ -64,20 +64,29 @@ hrt_attn_rel_args base_args(const at::Tensor& q, const at::Tensor& k, const at::
   return A;
 }
 
-// o [B, H, Sq, D] (in [B, Sq, H, D] memory) and lse, for rows as rows_of gives them.
+int64_t rows_in(const at::Tensor& q) { return q.size(0) * q.size(1) * q.size(2); }
+
+// One block for what the backward needs beside o: lse, and for 16-bit types what o's rounding left, on 16
+// bytes.
+int64_t left_at(const at::Tensor& q) { return (rows_in(q) + 3) / 4 * 4; }
+bool has_left(const at::Tensor& q) { return q.scalar_type() != at::kFloat; }
+
+// o [B, H, Sq, D] (in [B, Sq, H, D] memory) and that block (train: with the second part), for rows as rows_of gives them.
 std::tuple<at::Tensor, at::Tensor> forward_rows(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
-                                                const at::Tensor& mask, const Options& opt) {
+                                                const at::Tensor& mask, const Options& opt, bool train) {
   const at::Tensor o = bshd(q, q.size(2), q.size(3));
-  const at::Tensor lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  const bool left = train && has_left(q);
+  const at::Tensor kept = at::empty({left ? left_at(q) + rows_in(q) * q.size(3) / 2 : rows_in(q)}, q.options().dtype(at::kFloat));
   hrt_attn_rel_args A = base_args(q, k, v, table, mask, opt);
-  A.o = dptr(o), A.lse = dptr(lse);
+  A.o = dptr(o), A.lse = dptr(kept);
+  if (left) A.o_lo = dptr(kept) + 4 * left_at(q);
   c10::DataPtr part;
   if (const int64_t n = hrt_attn_rel_workspace(&A, float_code(q.scalar_type()), 0); n > 0) {
     part = scratch(n * 4);
     if (part) A.ws = dptr(part), A.ws_floats = n;
   }
   queue(typed("attn_rel_fwd", q.scalar_type()), A);
-  return {o, lse};
+  return {o, kept};
 }
 
 struct Attention : torch::autograd::Function<Attention> {
@@ -92,8 +101,8 @@ struct Attention : torch::autograd::Function<Attention> {
       return at::zeros(q.sizes(), q.options());
     }
     const at::Tensor qr = rows_of(q, Dp), kr = rows_of(k, Dp), vr = rows_of(v, Dp), t = dense(table);
-    const auto [o, lse] = forward_rows(qr, kr, vr, t, mask, {causal, scale, max_distance, offset});
-    ctx->save_for_backward({qr, kr, vr, t, mask, o, lse});
+    const auto [o, kept] = forward_rows(qr, kr, vr, t, mask, {causal, scale, max_distance, offset}, true);
+    ctx->save_for_backward({qr, kr, vr, t, mask, o, kept});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["max_distance"] = max_distance;
@@ -107,7 +116,7 @@ struct Attention : torch::autograd::Function<Attention> {
     const auto saved = ctx->get_saved_variables();
     const int64_t D = ctx->saved_data["D"].toInt();
     if (D == 0) return {at::zeros_like(saved[0]), at::zeros_like(saved[1]), at::zeros_like(saved[2]), at::zeros_like(saved[3]), {}, {}, {}, {}, {}};
-    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &mask = saved[4], &o = saved[5], &lse = saved[6];
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &mask = saved[4], &o = saved[5], &kept = saved[6];
     const Options opt{ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["max_distance"].toInt(),
                       ctx->saved_data["offset"].toInt()};
     const at::Tensor dout = rows_of(grads[0].scalar_type() == q.scalar_type() ? grads[0] : grads[0].to(q.scalar_type()), q.size(3));
@@ -116,8 +125,9 @@ struct Attention : torch::autograd::Function<Attention> {
     const bool wants_table = ctx->needs_input_grad(3), wants_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     // delta, and the partial sums of the table's gradient behind it
     const int64_t parts = wants_table ? hrt_attn_rel_workspace(&A, float_code(q.scalar_type()), 1) : 0;
-    const at::Tensor work = at::empty({lse.numel() + parts}, lse.options());
-    A.o = dptr(o), A.lse = dptr(lse), A.delta = dptr(work);
+    const at::Tensor work = at::empty({rows_in(q) + parts}, kept.options());
+    A.o = dptr(o), A.lse = dptr(kept), A.delta = dptr(work);
+    if (has_left(q)) A.o_lo = dptr(kept) + 4 * left_at(q);
     const bool like = q.is_non_overlapping_and_dense() && k.is_non_overlapping_and_dense() && v.is_non_overlapping_and_dense();
     if (like) A.flags = HRT_ATTN_GRAD_LIKE_INPUT;
     auto grad_for = [&](const at::Tensor& t) {
@@ -129,7 +139,7 @@ struct Attention : torch::autograd::Function<Attention> {
     if (ctx->needs_input_grad(0)) dq = grad_for(q), A.dq = dptr(dq);
     if (wants_table) {
       dtable = at::empty_like(table);
-      A.dtable = dptr(dtable), A.ws = dptr(work) + 4 * lse.numel(), A.ws_floats = parts;
+      A.dtable = dptr(dtable), A.ws = dptr(work) + 4 * rows_in(q), A.ws_floats = parts;
       if (wants_kv) A.flags |= HRT_ATTN_REL_TABLE_LATER;
     }
     queue(typed("attn_rel_dq", q.scalar_type()), A);
@@ -188,7 +198,7 @@ at::Tensor relative_bias_attention_vk(const at::Tensor& q, const at::Tensor& k, 
   }
   if (q.numel() == 0 || Sk == 0) return at::zeros(q.sizes(), q.options());
   const int64_t p = per16(q.scalar_type()), Dp = (D + p - 1) / p * p;
-  return std::get<0>(forward_rows(rows_of(q, Dp), rows_of(k, Dp), rows_of(v, Dp), dense(table), mask, {causal, sc, max_distance, query_offset}))
+  return std::get<0>(forward_rows(rows_of(q, Dp), rows_of(k, Dp), rows_of(v, Dp), dense(table), mask, {causal, sc, max_distance, query_offset}, false))
       .narrow(3, 0, D);
 }
 

@@ -60,7 +60,7 @@ class Mx4MmArgs(ctypes.Structure):
 
 
 class AttnRelArgs(ctypes.Structure):
-    _fields_ = ([(n, u64) for n in ("q", "k", "v", "table", "mask", "o", "lse", "dout", "delta", "dq", "dk", "dv", "dtable", "ws")]
+    _fields_ = ([(n, u64) for n in ("q", "k", "v", "table", "mask", "o", "lse", "dout", "delta", "dq", "dk", "dv", "dtable", "ws", "o_lo")]
                 + [(f"{t}_s{d}", i64) for t in ("q", "k", "v", "do") for d in "bhs"]
                 + [("mask_sb", i64), ("q_off", i64), ("ws_floats", i64)]
                 + [(n, i32) for n in ("B", "H", "Sq", "Sk", "D", "buckets", "max_distance", "causal")]
