@@ -395,7 +395,9 @@ typedef struct hrt_mx4_args {
  * gives.  x_scale 0: x is [M, K] of the kernel's type with row stride x_sm (elements, a multiple of 8) and unit column
  * stride.  x_scale not 0: x, x_scale are packed too ([M, K / 2], [M, K / 32], x_sm is not read), and the product runs on
  * the 4-bit operands (their values exactly).  y: [M, N] contiguous, bias [N], both of the kernel's type.
- * K % 32 == 0; x and w 16-byte aligned, scales 4-byte aligned. */
+ * K % 32 == 0; x and w 16-byte aligned, scales 4-byte aligned.
+ * "mx4_mm_back_{bf16,f16}" — the gradient's product: y[m, k] = round(sum_n X[m, n] * W[n, k]), x [M, N] of the kernel's type, y [M, K]
+ *   contiguous; x_scale and bias 0, N % 8 == 0, y 16-byte aligned, the rest as above. */
 typedef struct hrt_mx4_mm_args {
   uint64_t x, x_scale, w, w_scale, bias, y;
   int64_t M, N, K, x_sm;

@@ -299,6 +299,42 @@ def test_refusals():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("M,N,K", [(1, 8, 32), (3, 200, 96), (40, 64, 128), (31, 264, 160), (500, 2048, 4096), (500, 2000, 4128), (1500, 1000, 2080),
+                                   (1010, 456, 8160), (8100, 456, 4064)])
+def test_the_inputs_gradient_on_every_tile(M, N, K, dtype):
+    """Whole and ragged tiles, stages of W's rows and blocks of its columns; every 37th row is compared, and the last."""
+    _, codes, scale, _ = operands(1, N, K, dtype, M + N)
+    g = torch.randn((M, N + 8), generator=torch.Generator().manual_seed(2)).to(dtype)
+    some = sorted({*range(0, M, 37), M - 1})
+    w, rows = values(codes, scale, K), g[some][:, 8:].double().numpy()
+    x = torch.zeros(M, K, dtype=dtype).to(vk).requires_grad_()
+    y = torch_vulkan.mxfp4_linear(x, codes.to(vk), scale.to(vk))
+    for grad in (g.to(vk)[:, 8:], g[:, 8:].contiguous().to(vk)):  # rows further apart than they are long, and dense ones
+        (dx,) = torch.autograd.grad(y, x, grad, retain_graph=True)
+        check(dx.cpu()[some], rows @ w, np.abs(rows) @ np.abs(w), N, dtype)
+
+
+@pytest.mark.gpu
+def test_the_inputs_gradient_of_what_is_no_number():
+    """A block of NaN reaches its 32 columns, an infinite gradient its row, nothing else."""
+    M, N, K = 70, 72, 96
+    _, codes, scale, _ = operands(1, N, K, torch.bfloat16, 4)
+    g = torch.randn((M, N), generator=torch.Generator().manual_seed(3)).bfloat16()
+    x = torch.zeros(M, K, dtype=torch.bfloat16).to(vk).requires_grad_()
+
+    def back():
+        return torch.autograd.grad(torch_vulkan.mxfp4_linear(x, codes.to(vk), scale.to(vk)), x, g.to(vk))[0].cpu()
+
+    want = back()
+    scale[5, 1], g[3, 70] = 255, float("nan")
+    got = back()
+    hit = torch.zeros(M, K, dtype=torch.bool)
+    hit[:, 32:64], hit[3] = True, True
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M,quantize", [(1, False), (200, False), (1, True), (200, True)])
 def test_replayed_graph(M, quantize):
     rt, out = abi.Runtime(), {}

@@ -42,6 +42,7 @@ HRT_SOURCES = [
     "kernels/dq8.hip",
     "kernels/mx4.hip",
     "kernels/mx4_gemm.hip",
+    "kernels/mx4_back.hip",
     "kernels/gemm.hip",
     "kernels/gemm_f32.hip",
     "kernels/gemm_mfma.hip",

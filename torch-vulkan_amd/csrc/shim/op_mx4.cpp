@@ -46,6 +46,11 @@ void quantize_rows(const at::Tensor& x, const at::Tensor& codes, const at::Tenso
 
 at::Tensor unit_rows(const at::Tensor& x) { return x.size(1) <= 1 || x.stride(1) == 1 ? x : x.contiguous(); }
 
+// 16-bit rows with a unit column stride as the products read them: whole 16-byte words, a tile's row offsets in 31 bits.
+at::Tensor whole_words(const at::Tensor& rows) {
+  return rows.stride(0) % 8 != 0 || dptr(rows) % 16 != 0 || rows.stride(0) >= 4000000 ? rows.clone(at::MemoryFormat::Contiguous) : rows;
+}
+
 // y = x W^T + bias for x [M, K] without autograd.
 at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
                        bool quantize) {
@@ -71,13 +76,23 @@ at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& codes, const at::T
     quantize_rows(rows, xc, xs);
     A.x = dptr(xc), A.x_scale = dptr(xs);
   } else {
-    // the kernel reads whole 16-byte words and keeps a tile's row offsets in 31 bits
-    if (rows.stride(0) % 8 != 0 || dptr(rows) % 16 != 0 || rows.stride(0) >= 4000000) rows = rows.clone(at::MemoryFormat::Contiguous);
+    rows = whole_words(rows);
     A.x = dptr(rows), A.x_sm = rows.stride(0);
   }
   const at::Tensor y = at::empty({M, N}, x.options());
   A.y = dptr(y);
   queue(typed("mx4_mm", x.scalar_type()), A);
+  return y;
+}
+
+// g W for g [M, N], of rows of K values.
+at::Tensor linear_back(const at::Tensor& g, const at::Tensor& codes, const at::Tensor& scale, int64_t K) {
+  const int64_t M = g.size(0), N = g.size(1);
+  if (K % kBlock != 0 || N % 8 != 0 || M == 0 || N == 0 || K == 0) return at::mm(g, dequant_mxfp4_vk(codes, scale, g.scalar_type(), K));
+  const at::Tensor rows = whole_words(unit_rows(g)), w = dense_on(codes, 16), ws = dense(scale), y = at::empty({M, K}, g.options());
+  hrt_mx4_mm_args A{};
+  A.x = dptr(rows), A.x_sm = rows.stride(0), A.w = dptr(w), A.w_scale = dptr(ws), A.y = dptr(y), A.M = M, A.N = N, A.K = K;
+  queue(typed("mx4_mm_back", g.scalar_type()), A);
   return y;
 }
 
@@ -98,7 +113,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const auto saved = ctx->get_saved_variables();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const at::Tensor g = as_rows(grads[0]);
-    if (ctx->needs_input_grad(0)) out[0] = at::mm(g, dequant_mxfp4_vk(saved[0], saved[1], g.scalar_type(), sizes.back())).view(sizes);
+    if (ctx->needs_input_grad(0)) out[0] = linear_back(g, saved[0], saved[1], sizes.back()).view(sizes);
     if (ctx->saved_data["biased"].toBool() && ctx->needs_input_grad(3)) out[3] = g.sum(0);
     note_gpu("torch_vulkan::mxfp4_linear_backward");
     return out;
