@@ -365,6 +365,24 @@ def test_what_the_outputs_rounding_left(B, H, Sq, Sk, D, dtype):
 
 
 @pytest.mark.gpu
+def test_one_query_over_rows_past_31_bits():
+    """Keys and values 32 KiB apart, 2.3 GB from first to last, shared by so many heads that their range is not divided."""
+    H, Sk, D = 1024, 70000, 64
+    g = torch.Generator().manual_seed(1)
+    kv, q, table = (torch.randn(s, generator=g).bfloat16() for s in ((Sk, 2 * D), (1, H, 1, D), (32, H)))
+    block = torch.empty(Sk, 16384, dtype=torch.bfloat16, device=vk)
+    block[:, : 2 * D] = kv.to(vk)
+    k, v = (block[:, i * D:(i + 1) * D].view(1, 1, Sk, D).expand(1, H, Sk, D) for i in range(2))
+    y = torch_vulkan.relative_bias_attention(q.to(vk), k, v, table.to(vk), causal=True, query_offset=Sk - 1).cpu()
+    some = [0, 517, 1023]
+    c = case(H=3, Sq=1, Sk=Sk, D=D, causal=True, off=Sk - 1)
+    t = {"q": q[:, some], "table": table[:, some], "g": torch.zeros(1, 3, 1, D).bfloat16()}
+    t |= {n: kv[:, i * D:(i + 1) * D].reshape(1, 1, Sk, D).expand(1, 3, Sk, D) for i, n in enumerate("kv")}
+    ref, tol = oracle(t, c, torch.bfloat16)
+    close(y[:, some], ref["o"], tol["o"], "o")
+
+
+@pytest.mark.gpu
 def test_without_room_for_the_key_ranges():
     """The forward of few rows goes on without its workspace, in the plain order of its sums."""
     c = CASES["split_masked"]

@@ -15,6 +15,12 @@
 //     side.  Other tiles go through a 32 x 33 LDS patch: written by rows, read back along wrapped diagonals (lane t of a
 //     half-wave meets diagonals t and t - 32), so that 16 writes and 16 reads per lane sum 63 diagonals, which are added to a
 //     band array of the wavefront's own.  Every sum has a fixed order: no atomics, the same bits every run.
+// Bound: in 16 bits the matrix cores and the softmax arithmetic between the two products, in fp32 the matrix cores and how the
+// workgroups fall on the CUs.  Measured, forward / dQ and table / dK and dV:
+// bf16, 128 heads of 2048 x 2048 x 64 215 / 309 / 326 us (638, 667, 844 TFLOP/s), 48 heads of 512 x 512 x 64 14 / 26 / 20;
+// 128 heads of 2048 x 2048 x 128 352 / 729 / 934 us; f16, 8 heads of 4020 x 4020 x 128 causal 88 / 125 / 135; fp32, 16 heads of
+// 1040 x 1040 x 64 73 / 144 / 168 (61, 46, 53 TFLOP/s of about 150).  128-wide backward kernels hold 128 to 256 accumulators and
+// operands a lane, so one wavefront runs on a SIMD.
 // Tiling: a workgroup's four wavefronts are G groups of 32 stationary rows (queries; keys for dK/dV) times KH = 4 / G, which
 // share out the 32-row tiles of each streamed stage.  Stages are copied global -> LDS directly, double-buffered; rows that do
 // not exist or whose key is masked are copied as zeros without reading memory (a masked infinity or NaN meets no product),

