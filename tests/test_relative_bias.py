@@ -46,6 +46,7 @@ def pairs(c):
     seen = np.broadcast_to(r <= 0 if c["causal"] else np.ones_like(r, bool), (c["B"], c["Sq"], c["Sk"])).copy()
     if c["mask"] is not None:
         seen &= c["mask"][:, None, :]
+    seen &= ~np.isin(of[r - lo], c.get("hide", []))
     return of[r - lo], seen
 
 
@@ -230,6 +231,39 @@ def test_forward_and_gradients(name, dtype):
     for n, x in got.items():
         assert x.dtype == dtype
         close(x, ref[n], tol[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("low", [float("-inf"), "lowest"])
+@pytest.mark.parametrize("far", [True, False])
+@pytest.mark.parametrize("Sq,Sk,off", [(300, 300, 0), (3, 700, 697), (40, 2500, 2000)])
+def test_a_table_that_hides(Sq, Sk, off, far, low, dtype):
+    """Hidden buckets, the last of each direction (whole tiles) or nearer ones; every query sees others.  The oracle masks their
+    pairs: f16's lowest value is an ordinary bias, but weighs exp(-65504 + 50) = 0 beside any other."""
+    c = case(B=2, H=2, Sq=Sq, Sk=Sk, D=64, off=off, buckets=8, distance=16)
+    hide = [3, 7] if far else [0, 5, 6]
+    c["hide"] = hide
+    t = inputs(c, dtype)
+    ref, tol = oracle({**t, "table": t["table"].index_fill(0, torch.tensor(hide), 0.0)}, c, dtype)
+    t["table"][hide] = torch.finfo(dtype).min if low == "lowest" else low
+    d = tensors(t, c)
+    close(call(d, c), ref["o"], tol["o"], "o")
+    y, got = grads(d, c)
+    close(y, ref["o"], tol["o"], "o")
+    for n, x in got.items():
+        close(x, ref[n], tol[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Sq", [1, 200])
+def test_a_table_that_hides_everything(Sq, dtype):
+    c = case(B=1, H=2, Sq=Sq, Sk=600, D=32, off=200)
+    t = inputs(c, dtype)
+    t["table"].fill_(float("-inf"))
+    y, got = grads(tensors(t, c), c)
+    assert not y.detach().cpu().any() and not any(x.cpu().any() for x in got.values())
 
 
 @pytest.mark.gpu

@@ -385,7 +385,7 @@ __global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) v
           for (int e = 0; e < 16; ++e) acc[0][n][e] *= alpha;
         m = mn;
       }
-      const float nm = m == -INFINITY ? 0.f : c2 - m;
+      const float nm = m == -INFINITY ? c2 : c2 - m;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sl2, nm));

@@ -320,7 +320,8 @@ def dequant_mxfp4(codes, scale, out_dtype=torch.bfloat16, cols=None):
 
 def mxfp4_linear(x, codes, scale, bias=None, quantize_input=False):
     """Linear layer on frozen 4-bit weights: x @ dequant_mxfp4(codes, scale, x.dtype).T (+ bias), x [..., K] bf16/f16 on vk,
-    codes [N, ceil(K / 2)], scale [N, ceil(K / 32)].  The dequantized weights never reach memory where K % 32 == 0.
+    codes [N, ceil(K / 2)], scale [N, ceil(K / 32)].  The dequantized weights never reach memory where K % 32 == 0
+    (and N % 8 == 0, for the gradient).
 
     quantize_input=True rounds x the same way first (quantize_mxfp4 of its rows) and multiplies 4-bit operands, which the
     matrix cores do at four times the 16-bit rate.  Differentiable in x and bias; the gradient of a quantized x goes
@@ -342,7 +343,8 @@ def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=N
     distance each, the others grow logarithmically up to max_distance, and the last one holds everything beyond.
 
     key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen; masked keys and values are not read, whatever they
-    hold.  A query without a key to see gets zeros and no gradient.  Returns [B, H, Sq, D]; differentiable once in q, k, v and
+    hold.  A table entry of -inf, or of bfloat16's or float32's lowest value, hides its pairs.  A query without a key to see gets
+    zeros and no gradient.  Returns [B, H, Sq, D]; differentiable once in q, k, v and
     table.  Nothing of size Sq x Sk is stored."""
     if q.device.type != "vk":
         raise RuntimeError("relative_bias_attention: q must be a vk tensor")
