@@ -18,9 +18,10 @@
 // Bound: in 16 bits the matrix cores and the softmax arithmetic between the two products, in fp32 the matrix cores and how the
 // workgroups fall on the CUs.  Measured, forward / dQ and table / dK and dV:
 // bf16, 128 heads of 2048 x 2048 x 64 215 / 309 / 326 us (638, 667, 844 TFLOP/s), 48 heads of 512 x 512 x 64 14 / 26 / 20;
-// 128 heads of 2048 x 2048 x 128 352 / 729 / 934 us; f16, 8 heads of 4020 x 4020 x 128 causal 88 / 125 / 135; fp32, 16 heads of
-// 1040 x 1040 x 64 73 / 144 / 168 (61, 46, 53 TFLOP/s of about 150).  128-wide backward kernels hold 128 to 256 accumulators and
-// operands a lane, so one wavefront runs on a SIMD.
+// 128 heads of 2048 x 2048 x 128 360 / 574 / 934 us; f16, 8 heads of 4020 x 4020 x 128 causal 88 / 125 / 135; fp32, 16 heads of
+// 1040 x 1040 x 64 73 / 144 / 168 (61, 46, 53 TFLOP/s of about 150).  128-wide dK/dV holds 224 accumulators and
+// operands a lane, so one wavefront runs on a SIMD; 128-wide dQ of 16 bits fits two with one buffer a stage (729 us with two buffers
+// and one workgroup on a CU, so 574; 8 heads of 4020 the same either way).
 // Tiling: a workgroup's four wavefronts are G groups of 32 stationary rows (queries; keys for dK/dV) times KH = 4 / G, which
 // share out the 32-row tiles of each streamed stage.  Stages are copied global -> LDS directly, double-buffered; rows that do
 // not exist or whose key is masked are copied as zeros without reading memory (a masked infinity or NaN meets no product),
@@ -174,14 +175,17 @@ struct RelShape {
   static constexpr int DCH = DP / 32, NACC = WHICH == 1 ? 2 * DCH : DCH;
   using Tile = RelTile<T, DP, ST>;
   static constexpr int TB = Tile::BYTES;
-  static constexpr int NBUF = std::is_same<T, F32>::value && G == 1 ? 1 : 2;  // 128 fp32 rows: one buffer, two workgroups on a CU
+// one buffer a stage where it lets two workgroups share a CU: 128 fp32 rows, 128-wide dQ
+  static constexpr int NBUF = (std::is_same<T, F32>::value ? G == 1 : WHICH == 2 && DP == 128 && G > 1) ? 1 : 2;
+  // registers for two workgroups on a CU
+  static constexpr bool TWO = DP == 64 || (G > 1 && (WHICH == 0 || (WHICH == 2 && !std::is_same<T, F32>::value)));
   static int lds(int R) { return rel_lds(WHICH, R); }
 };
 
 __device__ __forceinline__ uint64_t low_bits(int64_t n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 template <typename T, int WHICH, int DP, int G>
-__global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) void attn_rel_k(hrt_attn_rel_args p, RelBuckets bk, RelPlan pl) {
+__global__ __launch_bounds__(256, (RelShape<T, WHICH, DP, G>::TWO ? 2 : 1)) void attn_rel_k(hrt_attn_rel_args p, RelBuckets bk, RelPlan pl) {
   using S = RelShape<T, WHICH, DP, G>;
   using Tile = typename S::Tile;
   using frag = typename Tile::frag;
@@ -206,6 +210,10 @@ __global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) v
     id -= (uint32_t)pl.table;
   }
   if (WHICH == 0 && pl.splits > 1) split = id / total, id -= split * total;
+  // causal, and all workgroups resident two to a CU: the second ones in the other order, long beside short (2 x 12 heads of 1000 x
+  // 1000 x 64: 86 us forward and backward, so 80)
+  if (S::TWO && p.causal && pl.splits <= 1 && total % 8 == 0 && total > 256 && total <= 512 && id >= 256)
+    id = id % 8 + (total - 8) - (id - 256) / 8 * 8;
   xcd_map32(id, total, pl.nblk, bh, blk);
   if (WHICH != 1 && p.causal) blk = pl.nblk - 1 - blk;  // the longest rows first
   bh = __builtin_amdgcn_readfirstlane(bh), blk = __builtin_amdgcn_readfirstlane(blk), split = __builtin_amdgcn_readfirstlane(split);
@@ -515,8 +523,8 @@ __global__ __launch_bounds__(256, DP == 128 && (WHICH != 0 || G == 1) ? 1 : 2) v
   }
   if constexpr (KH > 1) {
     constexpr int CH = TB / 4096 < NACC ? TB / 4096 : NACC;  // accumulators per round: 4 KiB each
-    static_assert(CH >= 1 && NACC % CH == 0 && (NBUF > 1 || 2 * NACC * 4096 <= TB), "merge rounds");
-    auto piece = [&](int s) { return (float*)(s == 0 ? a0_raw : s == 2 ? b0_raw : NBUF > 1 ? a1_raw : a0_raw + NACC * 4096); };
+    static_assert(CH >= 1 && NACC % CH == 0 && (NBUF > 1 || KH == 2 || 2 * NACC * 4096 <= TB), "merge rounds");
+    auto piece = [&](int s) { return (float*)(s == 0 ? a0_raw : s == 2 ? b0_raw : NBUF > 1 ? a1_raw : KH == 2 ? b0_raw : a0_raw + NACC * 4096); };
 #pragma unroll
     for (int r = 0; r < NACC; r += CH) {
       if (r > 0) __syncthreads();

@@ -83,8 +83,8 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
     p.splits = 1;
   }
   // groups a workgroup: more share a stage, fewer give more workgroups.  bf16, forward and backward, by one / two / four groups:
-  // 48 heads of 512 x 512 x 64 (768 / 384 / 192 workgroups) 90 / 60 / 86 us, 64 heads of 1024 x 1024 x 128 (2048 / 1024 / 512)
-  // 592 / 368 / 303 us
+  // 48 heads of 512 x 512 x 64 (768 / 384 / 192 workgroups) 90 / 60 / 86 us, 128 heads of 2048 x 2048 x 64 (8192 / 4096 / 2048)
+  // 1641 / 963 / 850 us
   p.g = blocks(4) * bh >= 512 ? 4 : blocks(2) * bh >= 256 ? 2 : 1;
   if (f32) {
     // fp32 is bound by the matrix cores, so by the CU with the most workgroups: a workgroup of one / two / four groups takes
