@@ -139,6 +139,7 @@ CASES = {
     "flat": case(Sq=64, Sk=64, scale=1e-3), "groups2": case(B=4, H=64, Sq=50, Sk=70, D=24), "groups4": case(B=8, H=64, Sq=70, Sk=40, D=16),
     "groups4_causal": case(B=8, H=64, Sq=70, Sk=70, D=16, causal=True, mask="tail"), "split": case(B=1, H=1, Sq=1, Sk=5000, off=4999, causal=True),
     "split_masked": case(B=2, H=3, Sq=9, Sk=3000, off=2991, mask="tail"), "split_empty": case(B=2, H=1, Sq=3, Sk=2100, mask="empty"),
+    "wide_d128": case(H=2, Sq=40, Sk=300, D=128, buckets=64, distance=1024, off=200),
     "groups2_d128": case(B=2, H=64, Sq=100, Sk=90, D=80, mask="tail"), "groups4_d128": case(B=8, H=64, Sq=40, Sk=70, D=72),
     "few_d128": case(B=2, H=2, Sq=2, Sk=700, D=128, off=698, causal=True), "split_d112": case(B=2, H=1, Sq=1, Sk=3001, D=112, off=3000, mask="tail"),
 }
