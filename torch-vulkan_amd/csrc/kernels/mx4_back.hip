@@ -11,8 +11,8 @@
 // Bound: the matrix cores and the 32 vector instructions that a slice of 16 rows takes beside its 4 FM products of 36 cycles; half a
 // slice's conversions are issued between the other half's products.  Measured, bf16, M x N x K (in brackets a dequantised copy
 // and its product, which also takes 2 N K bytes of scratch): 16 x 2048 x 2048 13 us (15), 308 x 2048 x 2048 13 (24),
-// 308 x 8192 x 2048 36 (40), 512 x 4096 x 4096 36 (50), 1024 x 2048 x 8192 45 (52), 4096 x 8192 x 2048 145 us, 948 TFLOP/s (147),
-// 4096 x 2048 x 8192 144 (146).
+// 308 x 8192 x 2048 35 (40), 512 x 4096 x 4096 37 (50), 1024 x 2048 x 8192 43 (51), 4096 x 8192 x 2048 140 us, 983 TFLOP/s (149),
+// 4096 x 2048 x 8192 142 (146).
 #include "../hrt/registry.h"
 #include "mx4.h"
 
@@ -87,15 +87,17 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BK / 128) * KG, R > 2 ? 1 : 2) vo
     for (int i = 0; i < IPW; ++i) edge_copy(wr, wbuf(ic), wave * IPW + i, wn[i] < left ? wo[i] : kNoRow);
   };
   // Scales go through registers, as they are turned over: [block of K][row of W], in fp32 (a byte shifted once, not in every lane).
-  // Those past the end are 1.
+  // Those past the end are 1.  Range-checked loads, so that every step issues the same number: a branch around a load of no
+  // lane would let the barrier's count pass a copy that is still in flight.
   uint32_t sb[SPT];
   auto load_scales = [&](int st) HK_INLINE {
     const int64_t n0 = (int64_t)st * (KG * kSlice);
+    const __amdgpu_buffer_rsrc_t rs = edge_rsrc(Sb + n0 * nb);
 #pragma unroll
     for (int u = 0; u < SPT; ++u) {
       const int e = u * 64 * NW + tid, n = e / KB, kb = e % KB;
       const bool ok = n0 + n < p.N && kb * 32 < kl;
-      const uint32_t s = Sb[ok ? (n0 + n) * nb + kb : 0];
+      const uint32_t s = __builtin_amdgcn_raw_buffer_load_b8(rs, ok ? n * (int)nb + kb : (int)kNoRow, 0, 0);
       sb[u] = ok ? s : 127u;
     }
   };
