@@ -371,3 +371,40 @@ def test_argument_blocks_match_the_header(tmp_path):
     got = [l.split() for l in subprocess.run([str(tmp_path / "l")], stdout=subprocess.PIPE, text=True, check=True).stdout.splitlines()]
     for c, f, n in got:
         assert int(n) == (ctypes.sizeof(blocks[c]) if f == "size" else getattr(blocks[c], f).offset), (c, f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("M,N,K", [(37, 136, 320), (3, 64, 96), (37, 130, 320), (5, 40, 50)])
+def test_the_gradients_gradient(M, N, K, quantize, dtype):
+    """dx = g W is linear in g, whichever product makes it: its gradient is h W^T, and that one's k W again."""
+    x, codes, scale, b = operands(M, N, K, dtype, 23)
+    r = torch.Generator().manual_seed(4)
+    g, k = (torch.randn((M, N), generator=r).to(dtype) for _ in range(2))
+    h, hb = torch.randn((M, K), generator=r).to(dtype), torch.randn((N,), generator=r).to(dtype)
+    C, S, w = codes.to(vk), scale.to(vk), values(codes, scale, K)
+    X, B, G, H = (t.to(vk).requires_grad_() for t in (x, b, g, h))
+    f64 = lambda t: t.double().numpy()  # noqa: E731
+    dx, db = torch.autograd.grad(torch_vulkan.mxfp4_linear(X, C, S, B, quantize), (X, B), G, create_graph=True)
+    check(dx, f64(g) @ w, np.abs(f64(g)) @ np.abs(w), N, dtype)
+    (gh,) = torch.autograd.grad(dx, G, H, create_graph=True)
+    check(gh, f64(h) @ w.T, np.abs(f64(h)) @ np.abs(w).T, K, dtype)
+    (gk,) = torch.autograd.grad(gh, H, k.to(vk))
+    check(gk, f64(k) @ w, np.abs(f64(k)) @ np.abs(w), N, dtype)
+    (gb,) = torch.autograd.grad(db, G, hb.to(vk))
+    assert torch.equal(gb.cpu(), hb.expand(M, N))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(37, 136, 320), (37, 130, 320), (5, 40, 50)])
+def test_a_penalty_on_the_inputs_gradient(M, N, K):
+    """d/dx of <(x W^T) W, h> is (h W^T) W: the calls that autograd makes are the ones that a program would make of them."""
+    x, codes, scale, _ = operands(M, N, K, torch.bfloat16, 29)
+    h = torch.randn((M, K), generator=torch.Generator().manual_seed(5)).bfloat16().to(vk)
+    C, S, X = codes.to(vk), scale.to(vk), x.to(vk).requires_grad_()
+    y = torch_vulkan.mxfp4_linear(X, C, S)
+    (dx,) = torch.autograd.grad(y, X, y, create_graph=True)
+    (got,) = torch.autograd.grad((dx * h).sum(), X, retain_graph=True)
+    (want,) = torch.autograd.grad(y, X, torch_vulkan.mxfp4_linear(h, C, S))
+    assert torch.equal(got.cpu(), want.cpu())

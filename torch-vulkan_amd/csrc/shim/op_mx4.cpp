@@ -96,6 +96,20 @@ at::Tensor linear_back(const at::Tensor& g, const at::Tensor& codes, const at::T
   return y;
 }
 
+// The same, differentiable in g: its gradient is the forward product, without bias and on h as it is.
+struct LinearBack : torch::autograd::Function<LinearBack> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& g, const at::Tensor& codes, const at::Tensor& scale,
+                            int64_t K) {
+    ctx->save_for_backward({codes, scale});
+    return linear_back(g, codes, scale, K);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list h) {
+    const auto saved = ctx->get_saved_variables();
+    return {mxfp4_linear_vk(h[0], saved[0], saved[1], std::nullopt, false), {}, {}, {}};
+  }
+};
+
 struct Linear : torch::autograd::Function<Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale,
                             const std::optional<at::Tensor>& bias, bool quantize) {
@@ -107,13 +121,17 @@ struct Linear : torch::autograd::Function<Linear> {
     return linear_rows(as_rows(x), codes, scale, bias, quantize).view(out);
   }
 
-  // dx = g W and db = sum of g over the rows.  quantize: straight through, as if x had gone in unrounded.
+  // dx = g W and db = sum of g over the rows.  quantize: straight through, as if x had gone in unrounded.  Both depend on g, and
+  // stay in the graph that is being made of the backward pass, if one is (create_graph).
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     torch::autograd::variable_list out(5);
     const auto saved = ctx->get_saved_variables();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const at::Tensor g = as_rows(grads[0]);
-    if (ctx->needs_input_grad(0)) out[0] = linear_back(g, saved[0], saved[1], sizes.back()).view(sizes);
+    if (ctx->needs_input_grad(0)) {
+      const bool graph = at::GradMode::is_enabled() && g.requires_grad();
+      out[0] = (graph ? LinearBack::apply(g, saved[0], saved[1], sizes.back()) : linear_back(g, saved[0], saved[1], sizes.back())).view(sizes);
+    }
     if (ctx->saved_data["biased"].toBool() && ctx->needs_input_grad(3)) out[3] = g.sum(0);
     note_gpu("torch_vulkan::mxfp4_linear_backward");
     return out;

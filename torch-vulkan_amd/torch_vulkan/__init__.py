@@ -324,8 +324,8 @@ def mxfp4_linear(x, codes, scale, bias=None, quantize_input=False):
     (and N % 8 == 0, for the gradient).
 
     quantize_input=True rounds x the same way first (quantize_mxfp4 of its rows) and multiplies 4-bit operands, which the
-    matrix cores do at four times the 16-bit rate.  Differentiable in x and bias; the gradient of a quantized x goes
-    straight through (grad @ W, as if x had gone in unrounded)."""
+    matrix cores do at four times the 16-bit rate.  Differentiable in x and bias, any number of times (create_graph); the
+    gradient of a quantized x goes straight through (grad @ W, as if x had gone in unrounded)."""
     if x.device.type != "vk":
         raise RuntimeError("mxfp4_linear: x must be a vk tensor")
     return _C.mxfp4_linear(x, codes, scale, bias, bool(quantize_input))
