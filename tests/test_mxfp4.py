@@ -408,3 +408,23 @@ def test_a_penalty_on_the_inputs_gradient(M, N, K):
     (got,) = torch.autograd.grad((dx * h).sum(), X, retain_graph=True)
     (want,) = torch.autograd.grad(y, X, torch_vulkan.mxfp4_linear(h, C, S))
     assert torch.equal(got.cpu(), want.cpu())
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is never dropped: neither without nor with a gradient wanted."""
+    import torch.autograd.forward_ad as fwd
+
+    x, codes, scale, b = (t.to(vk) for t in operands(4, 64, 96, torch.bfloat16, 1))
+    with fwd.dual_level():
+        for wants in (False, True):
+            for quantize in (False, True):
+                dual = fwd.make_dual(x.detach().requires_grad_(wants), torch.ones_like(x))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch_vulkan.mxfp4_linear(dual, codes, scale, b, quantize)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch_vulkan.mxfp4_linear(x, codes, scale, fwd.make_dual(b.detach().requires_grad_(wants), torch.ones_like(b)), quantize)
+        y = torch_vulkan.mxfp4_linear(x.detach().requires_grad_(), codes, scale, b)  # nor that of an incoming gradient
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            y.backward(fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    assert torch_vulkan.mxfp4_linear(x, codes, scale, b).shape == (4, 64)

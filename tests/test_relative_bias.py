@@ -546,3 +546,21 @@ def test_argument_block_matches_the_header(tmp_path):
     for line in subprocess.run([str(tmp_path / "l")], stdout=subprocess.PIPE, text=True, check=True).stdout.splitlines():
         f, n = line.split()
         assert int(n) == (ctypes.sizeof(abi.AttnRelArgs) if f == "size" else getattr(abi.AttnRelArgs, f).offset), f
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is never dropped: neither without nor with a gradient wanted."""
+    import torch.autograd.forward_ad as fwd
+
+    c = case(B=1, H=2, Sq=8, Sk=8, D=16)
+    t = tensors(inputs(c, torch.bfloat16), c)
+    with fwd.dual_level():
+        for n in ("q", "k", "v", "table"):
+            for wants in (False, True):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call({**t, n: fwd.make_dual(t[n].detach().requires_grad_(wants), torch.ones_like(t[n]))}, c)
+        y = call({**t, "q": t["q"].detach().requires_grad_()}, c)  # nor that of an incoming gradient
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            y.backward(fwd.make_dual(t["g"], t["g"]))
+    assert call(t, c).shape == t["q"].shape

@@ -55,6 +55,10 @@ c10::DataPtr scratch(int64_t bytes, bool reserve = false);
 inline uint64_t dptr(const c10::DataPtr& p) { return reinterpret_cast<uint64_t>(p.get()); }
 uint64_t scratch_left_out();  // how many were empty
 inline bool present(const std::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+// Operators that call their kernels themselves would drop a forward-mode tangent without a word: they refuse one.
+inline void no_tangent(const at::Tensor& t, const char* who) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), who, ": forward-mode differentiation is not supported");
+}
 
 // ---- accounting -------------------------------------------------------------------------------------------
 // Per-operator counts of GPU launches and CPU fallbacks (with the fallback's host time), which the tests

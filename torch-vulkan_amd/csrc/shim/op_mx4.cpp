@@ -124,6 +124,7 @@ struct Linear : torch::autograd::Function<Linear> {
   // dx = g W and db = sum of g over the rows.  quantize: straight through, as if x had gone in unrounded.  Both depend on g, and
   // stay in the graph that is being made of the backward pass, if one is (create_graph).
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    no_tangent(grads[0], "mxfp4_linear");
     torch::autograd::variable_list out(5);
     const auto saved = ctx->get_saved_variables();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
@@ -180,6 +181,8 @@ at::Tensor mxfp4_linear_vk(const at::Tensor& x, const at::Tensor& codes, const a
   if (present(bias))
     TORCH_CHECK(on_vk(*bias) && bias->scalar_type() == x.scalar_type() && bias->dim() == 1 && bias->size(0) == codes.size(0),
                 "mxfp4_linear: bias must be a vk tensor of ", codes.size(0), " elements in x's dtype");
+  no_tangent(x, "mxfp4_linear");
+  if (present(bias)) no_tangent(*bias, "mxfp4_linear");
   note_gpu("torch_vulkan::mxfp4_linear");
   if (at::GradMode::is_enabled() && (x.requires_grad() || (present(bias) && bias->requires_grad())))
     return Linear::apply(x, codes, scale, bias, quantize_input);

@@ -113,6 +113,7 @@ struct Attention : torch::autograd::Function<Attention> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "relative_bias_attention: its gradient is not differentiable (create_graph)");
+    no_tangent(grads[0], "relative_bias_attention");
     const auto saved = ctx->get_saved_variables();
     const int64_t D = ctx->saved_data["D"].toInt();
     if (D == 0) return {at::zeros_like(saved[0]), at::zeros_like(saved[1]), at::zeros_like(saved[2]), at::zeros_like(saved[3]), {}, {}, {}, {}, {}};
@@ -167,6 +168,7 @@ at::Tensor relative_bias_attention_vk(const at::Tensor& q, const at::Tensor& k, 
   for (const at::Tensor* t : {&q, &k, &v, &table})
     TORCH_CHECK(on_vk(*t) && float_code(t->scalar_type()) >= 0 && t->scalar_type() == q.scalar_type(), who,
                 ": q, k, v and table must be vk tensors of one type, float32, bfloat16 or float16");
+  for (const at::Tensor* t : {&q, &k, &v, &table}) no_tangent(*t, who);
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, who, ": q, k and v must be [B, H, S, D], got ", q.sizes(), k.sizes(), v.sizes());
   const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), Sk = k.size(2), D = q.size(3);
   TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == B && k.size(1) == H && k.size(3) == D, who,
