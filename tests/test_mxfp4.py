@@ -428,3 +428,28 @@ def test_forward_mode_is_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             y.backward(fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
     assert torch_vulkan.mxfp4_linear(x, codes, scale, b).shape == (4, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("shape,N", [((6, 96), 64), ((2, 3, 96), 64), ((96,), 64), ((6, 96), 50), ((2, 3, 50), 64), ((0, 96), 64)])
+def test_in_place_operations_on_the_output(shape, N, quantize):
+    """An adapter's output added to the layer's in place, in training and without gradients, as out of place."""
+    K = shape[-1]
+    x, codes, scale, b = operands(6, N, K, torch.bfloat16, 31)
+    n = int(np.prod(shape))
+    C, S, X = codes.to(vk), scale.to(vk), x.flatten()[:n].view(shape).to(vk).requires_grad_()
+    B, A = b.to(vk).requires_grad_(), torch.randn((*shape[:-1], N), generator=torch.Generator().manual_seed(6)).bfloat16().to(vk).requires_grad_()
+
+    def run(add, x, bias):
+        y = add(torch_vulkan.mxfp4_linear(x, C, S, bias, quantize), A)
+        y = add(y, y * 2)
+        return [y, *torch.autograd.grad(y, [t for t in (x, bias, A) if t is not None and t.requires_grad], torch.ones_like(y))]
+
+    for x_, bias in ((X, B), (X, None), (X.detach(), B), (X.detach(), None)):
+        for a, w in zip(run(lambda y, z: y.add_(z), x_, bias), run(lambda y, z: y + z, x_, bias)):
+            assert torch.equal(a.detach().cpu(), w.detach().cpu())
+    y = torch_vulkan.mxfp4_linear(X, C, S, B, quantize)
+    y.view(-1)[: y.numel() // 2].zero_()  # a view of it
+    (dx,) = torch.autograd.grad(y, X, torch.ones_like(y))
+    assert dx.shape == X.shape

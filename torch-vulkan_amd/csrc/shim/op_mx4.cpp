@@ -110,6 +110,10 @@ struct LinearBack : torch::autograd::Function<LinearBack> {
   }
 };
 
+// The rows of a result in the shape of their tensor.  Not a view: nothing else holds the rows, and autograd would forbid in-place
+// operations on a view that was made inside a function of ours.
+at::Tensor in_shape(const at::Tensor& rows, at::IntArrayRef sizes) { return at::_unsafe_view(rows, sizes); }
+
 struct Linear : torch::autograd::Function<Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale,
                             const std::optional<at::Tensor>& bias, bool quantize) {
@@ -118,7 +122,7 @@ struct Linear : torch::autograd::Function<Linear> {
     ctx->saved_data["biased"] = present(bias);
     std::vector<int64_t> out = x.sizes().vec();
     out.back() = codes.size(0);
-    return linear_rows(as_rows(x), codes, scale, bias, quantize).view(out);
+    return in_shape(linear_rows(as_rows(x), codes, scale, bias, quantize), out);
   }
 
   // dx = g W and db = sum of g over the rows.  quantize: straight through, as if x had gone in unrounded.  Both depend on g, and
@@ -188,7 +192,7 @@ at::Tensor mxfp4_linear_vk(const at::Tensor& x, const at::Tensor& codes, const a
     return Linear::apply(x, codes, scale, bias, quantize_input);
   std::vector<int64_t> out = x.sizes().vec();
   out.back() = codes.size(0);
-  return linear_rows(as_rows(x), codes, scale, bias, quantize_input).view(out);
+  return in_shape(linear_rows(as_rows(x), codes, scale, bias, quantize_input), out);
 }
 
 }  // namespace vkt
