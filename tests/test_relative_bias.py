@@ -564,3 +564,26 @@ def test_forward_mode_is_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             y.backward(fwd.make_dual(t["g"], t["g"]))
     assert call(t, c).shape == t["q"].shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 20, 100])
+def test_in_place_operations_on_the_output(D):
+    """The backward pass reads the output, so that one changed in place is refused there, in autograd's own words.  One that no gradient
+    goes through may be changed, and one whose rows are no whole 16-byte pieces, which is a copy."""
+    c = case(B=2, H=2, Sq=40, Sk=40, D=D)
+    t = tensors(inputs(c, torch.bfloat16), c)
+    leaf = t["q"].detach().requires_grad_()
+    out = call({**t, "q": leaf}, c)
+    want = torch.autograd.grad(out * 2, leaf, t["g"])[0].cpu()
+    with torch.no_grad():
+        free = call(t, c)
+        assert torch.equal(free.add_(free).cpu(), (out.detach() * 2).cpu())
+    y = call({**t, "q": leaf}, c).mul_(2)  # not forbidden as a view's
+    assert torch.equal(y.detach().cpu(), (out.detach() * 2).cpu())
+    if D % 8 == 0:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, leaf, t["g"])
+    else:
+        assert torch.equal(torch.autograd.grad(y, leaf, t["g"])[0].cpu(), want)
+    assert y.transpose(1, 2).is_contiguous()  # token-major

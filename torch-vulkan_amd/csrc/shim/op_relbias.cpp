@@ -3,8 +3,8 @@
 // F.scaled_dot_product_attention's fused kernels (op_attention.cpp), which take neither bias nor mask.
 //
 // q, k, v are [B, H, S, D] views read in place through their strides; rows that are not on 16 bytes or do not fill them
-// (D % 8 != 0, f32: D % 4 != 0) cost a padded copy.  The output is [B, S, H, D] memory viewed as [B, H, S, D]; gradients
-// take their inputs' layouts where q, k and v are dense.
+// (D % 8 != 0, f32: D % 4 != 0) cost a padded copy, and in training one of the output.  The output is [B, H, S, D] in
+// [B, S, H, D] memory; gradients take their inputs' layouts where q, k and v are dense.
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "common.h"
@@ -15,9 +15,10 @@ using namespace vkt;
 
 int64_t per16(at::ScalarType t) { return t == at::kFloat ? 4 : 8; }
 
-// [B, S, H, D] memory viewed as [B, H, S, D].
+// [B, H, S, D] in [B, S, H, D] memory.  Not a view: autograd would forbid in-place operations on one that leaves a function of ours.
 at::Tensor bshd(const at::Tensor& like, int64_t S, int64_t D) {
-  return at::empty({like.size(0), S, like.size(1), D}, like.options()).transpose(1, 2);
+  const int64_t H = like.size(1);
+  return at::empty_strided({like.size(0), H, S, D}, {S * H * D, D, H * D, 1}, like.options());
 }
 
 // Whether the kernels read t [B, H, S, D] in place: rows of whole 16-byte pieces on 16-byte lines.
@@ -108,7 +109,7 @@ struct Attention : torch::autograd::Function<Attention> {
     ctx->saved_data["max_distance"] = max_distance;
     ctx->saved_data["offset"] = offset;
     ctx->saved_data["D"] = D;
-    return o.narrow(3, 0, D);
+    return Dp == D ? o : bshd(o, o.size(2), D).copy_(o.narrow(3, 0, D));
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -200,8 +201,9 @@ at::Tensor relative_bias_attention_vk(const at::Tensor& q, const at::Tensor& k, 
   }
   if (q.numel() == 0 || Sk == 0) return at::zeros(q.sizes(), q.options());
   const int64_t p = per16(q.scalar_type()), Dp = (D + p - 1) / p * p;
-  return std::get<0>(forward_rows(rows_of(q, Dp), rows_of(k, Dp), rows_of(v, Dp), dense(table), mask, {causal, sc, max_distance, query_offset}, false))
-      .narrow(3, 0, D);
+  const at::Tensor o =
+      std::get<0>(forward_rows(rows_of(q, Dp), rows_of(k, Dp), rows_of(v, Dp), dense(table), mask, {causal, sc, max_distance, query_offset}, false));
+  return Dp == D ? o : o.narrow(3, 0, D);
 }
 
 }  // namespace vkt

@@ -344,8 +344,8 @@ def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=N
 
     key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen; masked keys and values are not read, whatever they
     hold.  A table entry of -inf, or of bfloat16's or float32's lowest value, hides its pairs.  A query without a key to see gets
-    zeros and no gradient.  Returns [B, H, Sq, D]; differentiable once, in
-    reverse mode, in q, k, v and table.  Nothing of size Sq x Sk is stored."""
+    zeros and no gradient.  Returns [B, H, Sq, D] in token-major memory; differentiable once, in reverse mode, in q, k, v and
+    table.  The backward pass reads the output: one changed in place may be refused there.  Nothing of size Sq x Sk is stored."""
     if q.device.type != "vk":
         raise RuntimeError("relative_bias_attention: q must be a vk tensor")
     return _C.relative_bias_attention(q, k, v, table, key_mask, bool(causal), scale, int(max_distance), int(query_offset))
