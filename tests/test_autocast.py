@@ -70,3 +70,43 @@ def test_autocast_backward_gives_fp32_gradients_of_fp32_leaves():
     loss.backward()
     assert x.grad.dtype == torch.float32 and lin.weight.grad.dtype == torch.float32
     assert torch.isfinite(x.grad.cpu()).all() and torch.isfinite(lin.weight.grad.cpu()).all()
+
+
+def test_four_bit_linear_runs_in_the_autocast_type():
+    """As linear: x and bias are cast, fp32 leaves get fp32 gradients."""
+    x, b = randn((8, 96), torch.float32, 8), randn((64,), torch.float32, 9)
+    codes, scale = (t.to(dev) for t in torch_vulkan.quantize_mxfp4(randn((64, 96), torch.float32, 10)))
+    for dt in (torch.bfloat16, torch.float16):
+        for quantize in (False, True):
+            X, B = x.to(dev).requires_grad_(), b.to(dev).requires_grad_()
+            with torch.autocast(device_type="vk", dtype=dt):
+                y = torch_vulkan.mxfp4_linear(X, codes, scale, B, quantize)
+                other = torch_vulkan.mxfp4_linear(X.detach().half(), codes, scale, B.detach().bfloat16(), quantize)
+            X2, B2 = x.to(dt).to(dev).requires_grad_(), b.to(dt).to(dev).requires_grad_()
+            want = torch_vulkan.mxfp4_linear(X2, codes, scale, B2, quantize)
+            assert y.dtype == dt and other.dtype == dt and torch.equal(y.detach().cpu(), want.detach().cpu())
+            y.float().pow(2).sum().backward()
+            want.float().pow(2).sum().backward()
+            assert X.grad.dtype == torch.float32 and torch.equal(X.grad.cpu(), X2.grad.float().cpu())
+            assert B.grad.dtype == torch.float32 and torch.equal(B.grad.cpu(), B2.grad.float().cpu())
+    with torch.autocast(device_type="vk", dtype=torch.bfloat16, enabled=False), pytest.raises(RuntimeError, match="bfloat16 or float16"):
+        torch_vulkan.mxfp4_linear(x.to(dev), codes, scale)
+
+
+def test_bias_attention_runs_in_the_autocast_type():
+    """As scaled_dot_product_attention: 16-bit q beside an fp32 k and table, fp32 leaves get fp32 gradients."""
+    f = torch_vulkan.relative_bias_attention
+    q, k, v, table = (randn(s, torch.float32, i) for i, s in enumerate(((1, 2, 40, 64), (1, 2, 40, 64), (1, 2, 40, 64), (32, 2))))
+    for dt in (torch.bfloat16, torch.float16):
+        leaves = [t.to(dev).requires_grad_() for t in (q, k, v, table)]
+        with torch.autocast(device_type="vk", dtype=dt):
+            y = f(leaves[0].to(dt), *leaves[1:], causal=True)
+        low = [t.to(dt).to(dev).requires_grad_() for t in (q, k, v, table)]
+        want = f(*low, causal=True)
+        assert y.dtype == dt and torch.equal(y.detach().cpu(), want.detach().cpu())
+        y.float().pow(2).sum().backward()
+        want.float().pow(2).sum().backward()
+        for a, b in zip(leaves, low):
+            assert a.grad.dtype == torch.float32 and torch.equal(a.grad.cpu(), b.grad.float().cpu())
+    with torch.autocast(device_type="vk", dtype=torch.bfloat16, enabled=False):
+        assert f(*(t.to(dev) for t in (q, k, v, table))).dtype == torch.float32

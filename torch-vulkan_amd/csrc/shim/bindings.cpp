@@ -106,13 +106,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mxfp4_linear", [](const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
                            bool quantize_input) {
     runtime();
-    return mxfp4_linear_vk(x, codes, scale, bias, quantize_input);
+    return mxfp4_linear_autocast(x, codes, scale, bias, quantize_input);
   });
   m.def("relative_bias_attention",
         [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const std::optional<at::Tensor>& key_mask,
            bool causal, std::optional<double> scale, int64_t max_distance, int64_t query_offset) {
           runtime();
-          return relative_bias_attention_vk(q, k, v, table, key_mask, causal, scale, max_distance, query_offset);
+          return relative_bias_attention_autocast(q, k, v, table, key_mask, causal, scale, max_distance, query_offset);
         });
   // accounting and profiling
   m.def("kernel_counts", &gpu_counts);

@@ -105,10 +105,15 @@ std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_vk(const at::Tensor& x);
 at::Tensor dequant_mxfp4_vk(const at::Tensor& codes, const at::Tensor& scale, at::ScalarType out_dtype, int64_t cols);
 at::Tensor mxfp4_linear_vk(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
                            bool quantize_input);
+at::Tensor mxfp4_linear_autocast(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
+                                 bool quantize_input);  // x and bias in the autocast dtype where autocast is on
 
 // Fused attention with a learned relative position bias, differentiable (no reference counterpart).
 at::Tensor relative_bias_attention_vk(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
                                       const std::optional<at::Tensor>& key_mask, bool causal, std::optional<double> scale,
                                       int64_t max_distance, int64_t query_offset);
+at::Tensor relative_bias_attention_autocast(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
+                                            const std::optional<at::Tensor>& key_mask, bool causal, std::optional<double> scale,
+                                            int64_t max_distance, int64_t query_offset);  // the same of q, k, v and table
 
 }  // namespace vkt

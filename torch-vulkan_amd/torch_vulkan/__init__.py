@@ -325,7 +325,8 @@ def mxfp4_linear(x, codes, scale, bias=None, quantize_input=False):
 
     quantize_input=True rounds x the same way first (quantize_mxfp4 of its rows) and multiplies 4-bit operands, which the
     matrix cores do at four times the 16-bit rate.  Differentiable in x and bias, any number of times (create_graph), in
-    reverse mode; the gradient of a quantized x goes straight through (grad @ W, as if x had gone in unrounded)."""
+    reverse mode; the gradient of a quantized x goes straight through (grad @ W, as if x had gone in unrounded).  Autocast casts x
+    and bias, as it does for linear."""
     if x.device.type != "vk":
         raise RuntimeError("mxfp4_linear: x must be a vk tensor")
     return _C.mxfp4_linear(x, codes, scale, bias, bool(quantize_input))
@@ -345,7 +346,8 @@ def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=N
     key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen; masked keys and values are not read, whatever they
     hold.  A table entry of -inf, or of bfloat16's or float32's lowest value, hides its pairs.  A query without a key to see gets
     zeros and no gradient.  Returns [B, H, Sq, D] in token-major memory; differentiable once, in reverse mode, in q, k, v and
-    table.  The backward pass reads the output: one changed in place may be refused there.  Nothing of size Sq x Sk is stored."""
+    table.  The backward pass reads the output: one changed in place may be refused there.  Autocast casts q, k, v and
+    table, as it does for scaled_dot_product_attention.  Nothing of size Sq x Sk is stored."""
     if q.device.type != "vk":
         raise RuntimeError("relative_bias_attention: q must be a vk tensor")
     return _C.relative_bias_attention(q, k, v, table, key_mask, bool(causal), scale, int(max_distance), int(query_offset))
