@@ -587,3 +587,23 @@ def test_in_place_operations_on_the_output(D):
     else:
         assert torch.equal(torch.autograd.grad(y, leaf, t["g"])[0].cpu(), want)
     assert y.transpose(1, 2).is_contiguous()  # token-major
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Sq,Sk,D,off,mask", [(1, 2, 40, 200, 64, 60, None), (2, 2, 1, 300, 64, 99, None), (1, 2, 9, 3000, 40, 1000, None), (2, 3, 70, 90, 128, -3, None),
+                                                  (2, 2, 33, 97, 32, 7, "random"), (1, 1, 20, 50, 64, -20, None), (8, 64, 70, 100, 16, 5, None), (2, 64, 100, 150, 80, 0, None)])
+def test_keys_after_the_last_query_are_not_read(B, H, Sq, Sk, D, off, mask, dtype):
+    """A cache longer than what has been written to it: a causal form sees no key behind its last query, whatever stands there."""
+    c = case(B=B, H=H, Sq=Sq, Sk=Sk, D=D, causal=True, off=off, mask=mask)
+    t = inputs(c, dtype)
+    seen = max(Sq + off, 0)
+    ref, tol = oracle(t, c, dtype)
+    for n in "kv":
+        t[n][:, :, seen:] = torch.tensor([float("nan"), float("inf"), -float("inf")], dtype=dtype)[torch.arange(Sk - seen) % 3][:, None]
+    d = tensors(t, c)
+    close(call(d, c), ref["o"], tol["o"], "o")
+    y, got = grads(d, c)
+    close(y, ref["o"], tol["o"], "o")
+    for n, x in got.items():
+        close(x, ref[n], tol[n], n)

@@ -220,7 +220,10 @@ __global__ __launch_bounds__(256, (RelShape<T, WHICH, DP, G>::TWO ? 2 : 1)) void
   const int64_t b = bh / (uint32_t)p.H, hh = bh % (uint32_t)p.H;
   const int D = p.D, R = bk.R;
   const int64_t Sq = p.Sq, Sk = p.Sk, off = p.q_off;
-  const int64_t own_n = WHICH == 1 ? Sk : Sq, str_n = WHICH == 1 ? Sq : Sk;
+  // streamed rows: all queries; the keys, where causal up to the last one that any query sees (one past it would meet a P of zero in a
+  // product, and zero times an infinity or NaN of a cache that nothing was written to is no zero)
+  const int64_t seen = p.causal && off < Sk - Sq ? (Sq + off > 0 ? Sq + off : 0) : Sk;
+  const int64_t own_n = WHICH == 1 ? Sk : Sq, str_n = WHICH == 1 ? Sq : seen;
   const int64_t own0 = (int64_t)blk * (32 * G), grp0 = own0 + 32 * g, own = grp0 + l32;  // this lane's stationary row
   const HK_G uint8_t* Q = gcptr<uint8_t>(p.q) + (b * p.q_sb + hh * p.q_sh) * ESZ;
   const HK_G uint8_t* K = gcptr<uint8_t>(p.k) + (b * p.k_sb + hh * p.k_sh) * ESZ;
@@ -257,8 +260,8 @@ __global__ __launch_bounds__(256, (RelShape<T, WHICH, DP, G>::TWO ? 2 : 1)) void
   auto mask_load = [&](int64_t st) {
     if (KEYS && masked) {
       const int64_t k0 = st * ST + lane, k1 = k0 + 64;
-      mb0 = k0 < Sk ? mask[k0] : 0;
-      if (ST > 64) mb1 = k1 < Sk ? mask[k1] : 0;
+      mb0 = k0 < str_n ? mask[k0] : 0;
+      if (ST > 64) mb1 = k1 < str_n ? mask[k1] : 0;
     }
   };
   auto stage_rows = [&](int64_t st, uint64_t (&w)[2]) {

@@ -343,11 +343,13 @@ def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=N
     (which also hides keys j > i + query_offset) all serve r <= 0.  Of a direction's nb buckets the first nb // 2 hold one
     distance each, the others grow logarithmically up to max_distance, and the last one holds everything beyond.
 
-    key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen; masked keys and values are not read, whatever they
-    hold.  A table entry of -inf, or of bfloat16's or float32's lowest value, hides its pairs.  A query without a key to see gets
-    zeros and no gradient.  Returns [B, H, Sq, D] in token-major memory; differentiable once, in reverse mode, in q, k, v and
-    table.  The backward pass reads the output: one changed in place may be refused there.  Autocast casts q, k, v and
-    table, as it does for scaled_dot_product_attention.  Nothing of size Sq x Sk is stored."""
+    key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen.  Masked keys and values play no part, whatever they hold,
+    nor do those that causal hides from every query (the unwritten end of a cache).  A table entry of -inf, or of bfloat16's or
+    float32's lowest value, hides its pairs.  A query without a key to see gets zeros and no gradient.
+
+    Returns [B, H, Sq, D] in token-major memory; differentiable once, in reverse mode, in q, k, v and table.  The backward pass
+    reads the output: one changed in place may be refused there.  Autocast casts q, k, v and table, as it does for
+    scaled_dot_product_attention.  Nothing of size Sq x Sk is stored."""
     if q.device.type != "vk":
         raise RuntimeError("relative_bias_attention: q must be a vk tensor")
     return _C.relative_bias_attention(q, k, v, table, key_mask, bool(causal), scale, int(max_distance), int(query_offset))
