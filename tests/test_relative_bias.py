@@ -607,3 +607,13 @@ def test_keys_after_the_last_query_are_not_read(B, H, Sq, Sk, D, off, mask, dtyp
     close(y, ref["o"], tol["o"], "o")
     for n, x in got.items():
         close(x, ref[n], tol[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [-(1 << 63), (1 << 63) - 1, (1 << 40) + 1, -(1 << 40) - 1])
+def test_offsets_out_of_range_are_refused(off):
+    """With and without rows: the check is the call's own."""
+    for Sq in (4, 0):
+        t = [torch.zeros(1, 1, n, 8, device=vk) for n in (Sq, 4, 4)]
+        with pytest.raises(RuntimeError, match="relative_bias_attention: query_offset out of range"):
+            torch_vulkan.relative_bias_attention(*t, torch.zeros(32, 1, device=vk), query_offset=off)

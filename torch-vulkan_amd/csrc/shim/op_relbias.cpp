@@ -185,7 +185,8 @@ at::Tensor relative_bias_attention_vk(const at::Tensor& q, const at::Tensor& k, 
               table.size(0), " buckets and max_distance ", max_distance);
   const double sc = scale.value_or(1.0 / std::sqrt(static_cast<double>(D)));
   TORCH_CHECK(sc >= 1e-20 && sc <= 1e20, who, ": scale must lie in 1e-20 .. 1e20, got ", sc);
-  TORCH_CHECK(std::abs(query_offset) <= int64_t(1) << 40, who, ": query_offset out of range");
+  constexpr int64_t far = int64_t(1) << 40;
+  TORCH_CHECK(query_offset >= -far && query_offset <= far, who, ": query_offset out of range, got ", query_offset);
   at::Tensor mask;
   if (present(key_mask)) {
     TORCH_CHECK(on_vk(*key_mask) && key_mask->scalar_type() == at::kBool && key_mask->dim() == 2 && key_mask->size(1) == Sk &&
