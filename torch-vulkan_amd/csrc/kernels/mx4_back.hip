@@ -192,11 +192,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BK / 128) * KG, R > 2 ? 1 : 2) vo
   };
   load_scales(0);
   copy(std::integral_constant<int, 0>(), 0);
-  store_scales(0);
   if (R > 2) {
+    issue_order_fence();  // the first barrier counts on stage 1's copies and scales being the last ones issued
     copy(std::integral_constant<int, 1>(), 1);
-    load_scales(1);
   }
+  store_scales(0);
+  if (R > 2) load_scales(1);
   barrier_keep_vm_lds<KEEP>();
   int st = 0;
   for (; st + R <= steps; st += R) {

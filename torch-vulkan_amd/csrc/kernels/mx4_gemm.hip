@@ -379,6 +379,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void mx4_tile(hrt_
   copy_w(0, wbuf(std::integral_constant<int, 0>()));
   copy_x(0, xbuf(std::integral_constant<int, 0>()));
   if constexpr (XR > 2) {  // X of the steps before the first one's own copies (past the end: zeros that nobody reads)
+    issue_order_fence();     // the first barrier counts on them being the last ones issued
     copy_x(1, xbuf(std::integral_constant<int, 1>()));
     copy_x(2, xbuf(std::integral_constant<int, 2>()));
   }
