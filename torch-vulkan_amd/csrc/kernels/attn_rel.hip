@@ -97,7 +97,10 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
       if (g == 4 || t < least) p.g = g, least = t;
     }
   }
-  if (f32 && dp == 128) p.g = 4;  // the other forms' stages fill LDS
+  // fp32 rows of 128 have a form for four groups only (two or one would need stages of 64 or 128 rows, which fit LDS with one buffer),
+  // so that few heads leave CUs idle: forward and backward, 8 heads of 1000 x 1000 x 128 (64 workgroups) 573 us, elementary operations
+  // 816; one of 4000 x 4000 x 128 (32) 2003, elementary operations 1540
+  if (f32 && dp == 128) p.g = 4;
   // four buffers of 128 rows leave 29 KiB for the bands of far-reaching tables
   if (p.g == 1 && dp == 128 && rel_lds(which, R) > 29 * 1024) p.g = 2;
   p.nblk = (int)blocks(p.g);
@@ -120,7 +123,7 @@ RelPlan plan_of(const hrt_attn_rel_args& a, int which, bool f32, bool ws, int R)
 // ranges by attn_rel_join, always in one order.  Keys past the range's end or masked get an offset beyond the buffer and
 // are not fetched.  As many ranges as give 1024 workgroups (2048: 1 % slower; batches of eight keys, and loads past the
 // caches, were slower too).  Measured: bf16, 128 heads of one query and 4096 x 64 keys, 134 MB of K and V in 25 us and 5 us of
-// join, 4.5 TB/s over both.
+// join, 4.5 TB/s over both; fp32, 268 MB in 44 us with the join, 6.0 TB/s.
 template <typename T>
 struct Piece {  // 16 bytes of a row
   static constexpr int N = 16 / sizeof(typename T::storage);
