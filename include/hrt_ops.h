@@ -275,7 +275,8 @@ int64_t hrt_attn_dkdv_workspace(const hrt_attn_args* args);
  * e = nb / 2: n below e, else the largest e + t <= nb - 1 with (n / e)^(nb - e) >= (max_distance / e)^t, decided in whole
  * numbers.  Key j is allowed where mask (one byte a key, rows mask_sb apart, 0: no mask) is not 0 and, if causal,
  * j <= i + q_off.  A row without an allowed key gives o = 0, lse = -inf and no gradient; forward and dq read no key or value that is
- * masked or, if causal, behind the last query (dk and dv of such a key are 0, whatever it holds).
+ * masked or, if causal, behind the last query (dk and dv of such a key are 0, whatever it holds), and dkdv no query before the
+ * first key.
  *  "attn_rel_fwd_{dt}":  o [B, Sq, H, D]-contiguous, lse fp32 [B, H, Sq].  o_lo (optional, 16-bit types): what o's rounding left,
  *     laid out like o and rounded once more, for dq.  ws (optional): ws_floats of fp32 workspace, where
  *     hrt_attn_rel_workspace(&args, dtype, 0) asks for them: few query rows then share their keys out over workgroups.

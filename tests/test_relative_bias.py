@@ -617,3 +617,21 @@ def test_offsets_out_of_range_are_refused(off):
         t = [torch.zeros(1, 1, n, 8, device=vk) for n in (Sq, 4, 4)]
         with pytest.raises(RuntimeError, match="relative_bias_attention: query_offset out of range"):
             torch_vulkan.relative_bias_attention(*t, torch.zeros(32, 1, device=vk), query_offset=off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Sq,Sk,D,off,mask", [(1, 2, 100, 100, 64, -40, None), (2, 3, 300, 200, 128, -133, "random"), (8, 64, 70, 40, 16, -33, None), (1, 2, 20, 50, 64, -20, None)])
+def test_queries_before_the_first_key_touch_no_gradient(B, H, Sq, Sk, D, off, mask, dtype):
+    """A query that causal leaves no key: whatever stands in it and in its output's gradient, k, v and table get nothing of it."""
+    c = case(B=B, H=H, Sq=Sq, Sk=Sk, D=D, causal=True, off=off, mask=mask)
+    t = inputs(c, dtype)
+    none = min(-off, Sq)
+    t["g"][:, :, :none] = 0
+    ref, tol = oracle(t, c, dtype)
+    for n in "qg":
+        t[n][:, :, :none] = torch.tensor([float("nan"), float("inf"), -float("inf")], dtype=dtype)[torch.arange(none) % 3][:, None]
+    y, got = grads(tensors(t, c), c)
+    close(y, ref["o"], tol["o"], "o")
+    for n, x in got.items():
+        close(x, ref[n], tol[n], n)

@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256, (RelShape<T, WHICH, DP, G>::TWO ? 2 : 1)) void
     st1 = st0 + pl.per < st1 ? st0 + pl.per : st1;
   }
 
-  // a stage's rows: bit set where the row exists and (a key) is not masked
+  // a stage's rows: bit set where the row exists and (a key) is not masked, (a query) has a key by causal
   constexpr bool KEYS = WHICH != 1;
   const bool masked = p.mask != 0;
   uint8_t mb0 = 0, mb1 = 0;
@@ -269,6 +269,10 @@ __global__ __launch_bounds__(256, (RelShape<T, WHICH, DP, G>::TWO ? 2 : 1)) void
       w[0] = __ballot(mb0 != 0), w[1] = ST > 64 ? __ballot(mb1 != 0) : 0;
     } else {
       w[0] = low_bits(str_n - st * ST), w[1] = ST > 64 ? low_bits(str_n - st * ST - 64) : 0;
+      if (!KEYS && p.causal) {  // what stands in Q and dO before the first key may be no number either
+        w[0] &= ~low_bits(-off - st * ST);
+        if (ST > 64) w[1] &= ~low_bits(-off - st * ST - 64);
+      }
     }
   };
   auto copy = [&](auto ic, int64_t st, const uint64_t (&w)[2]) {

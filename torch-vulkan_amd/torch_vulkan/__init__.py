@@ -346,7 +346,7 @@ def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=N
     key_mask: bool [B, Sk] (or [1, Sk]), True where a key may be seen.  Masked keys and values play no part, whatever they hold,
     nor do those that causal hides from every query (the unwritten end of a cache).  A table entry of -inf, or of bfloat16's or
     float32's lowest value, hides its pairs (finite entries beyond 2e38 * min(1, scale) overflow).  A query without a key to
-    see gets zeros and no gradient.
+    see gets zeros and no gradient; one before the first key, by causal, gives none either, whatever it holds.
 
     Returns [B, H, Sq, D] in token-major memory; differentiable once, in reverse mode, in q, k, v and table.  The backward pass
     reads the output: one changed in place may be refused there.  Autocast casts q, k, v and table, as it does for
