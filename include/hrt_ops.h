@@ -405,6 +405,69 @@ typedef struct hrt_mx4_mm_args {
   int64_t M, N, K, x_sm;
 } hrt_mx4_mm_args;
 
+/* 8-bit rows (no reference counterpart): a value is code * scale[row], code in -127..127.
+ * "i8_rows_quant_{f32,bf16,f16}" — x [rows, cols] with row stride x_sr (elements, unit column stride) into q [rows, q_sr] and
+ *   scale [rows] (fp32): scale = top / 127 (at most the largest of which 127 are finite), top the row's largest magnitude, code the whole number nearest to
+ *   127 x / top, ties to even, exactly.  Columns cols .. q_sr - 1 become 0 (q_sr at
+ *   most cols rounded up to 16).  A row of zeros gets scale 0; a row with an
+ *   infinity or NaN gets scale NaN and codes 0.
+ * "i8_rows_dequant_{dt}" — x [rows, cols] (row stride x_sr) = code * scale, the fp32 product rounded once; q's row stride is
+ *   q_sr. */
+typedef struct hrt_i8_rows_args {
+  uint64_t x, q, scale;
+  int64_t rows, cols, x_sr, q_sr;
+} hrt_i8_rows_args;
+
+/* "i8_mm_{bf16,f16}" — product of 8-bit rows (no reference counterpart):
+ *   y[m, n] = round((sum_k x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])      (whole sums; bias 0: none)
+ * x [M, K], w [N, K] int8 with row strides x_sm, w_sn (bytes, multiples of 16), 16-byte aligned; scales fp32; y [M, N]
+ * contiguous and bias [N] of the kernel's type.  K % 16 == 0 and K <= 131056, so that no sum passes 31 bits. */
+typedef struct hrt_i8_mm_args {
+  uint64_t x, x_scale, w, w_scale, bias, y;
+  int64_t M, N, K, x_sm, w_sn;
+} hrt_i8_mm_args;
+
+/* Root-mean-square norm of rows (no reference counterpart).  Row i of a tensor is found through up to three outer dimensions,
+ * i = (i0 * n1 + i1) * n2 + i2, at element i0 * s[0] + i1 * s[1] + i2 * s[2]; D values with unit stride.
+ * "rms_fwd_{f32,bf16,f16}" — h = x + r (r 0: h = x), y = h * rstd * w with rstd = 1 / sqrt(mean(h^2) + eps) in fp32 from the
+ *   unrounded h (w 0: none).  y and, where h_out is not 0, the rounded h are [rows, D] contiguous; rstd [rows] if not 0.
+ *   q not 0: in place of y its rows in 8 bits, q [rows, D] and scale [rows] as "i8_rows_quant_*" makes them from the
+ *   unrounded y (up to the rounding of 127 y / top in fp32).
+ * "rms_bwd_{dt}" — from gy, gh (gradients of y and h, either 0), h (strides hs) and rstd:
+ *   dx = rstd * (gy w - n * mean(gy w n)) + gh with n = h rstd; dw (if not 0) = the sum of gy n over the rows.  dx (if not 0)
+ *   [rows, D] contiguous.  dw needs ws, hrt_rms_workspace(&args, dtype) floats: sums of runs of rows, added in order. */
+typedef struct hrt_rms_args {
+  uint64_t x, r, w, y, h_out, q, scale, rstd;
+  int64_t rows, D, n1, n2;
+  int64_t xs[3], rs[3];
+  float eps;
+  uint32_t pad;
+} hrt_rms_args;
+typedef struct hrt_rms_bwd_args {
+  uint64_t gy, gh, h, rstd, w, dx, dw, ws;
+  int64_t rows, D, n1, n2;
+  int64_t gys[3], ghs[3], hs[3];
+} hrt_rms_bwd_args;
+int64_t hrt_rms_workspace(const hrt_rms_bwd_args* args, int32_t dtype);
+
+/* "rotary_{f32,bf16,f16}" — rotary positions of several axes (no reference counterpart).  Pair j (0 <= j < P) of a head is turned
+ * by pos[axis of j] * freqs[j]: (a, b) -> (a cos - b sin, b cos + a sin), with (a, b) = values (j, j + P), or (2 j, 2 j + 1)
+ * where `interleaved`; the values behind 2 P are copied.  The axis of j is the first one with j < ends[axis] (axes
+ * <= HRT_ROTARY_AXES, the last end is P).  back != 0: by the opposite angle (the gradient).
+ * q [B, Hq, S, D] and k [B, Hk, S, D] (k 0: none) with strides (batch, head, token) and unit last stride; q_out, k_out are in
+ * [B, S, H, D] memory.  pos: strides p_sb, p_ss, p_sa (elements) for batch, token and axis; pos_type 0: int32, 1: int64,
+ * 2: fp32.  freqs: fp64 [P], in radians.  The angle is taken in fp64, its sine and cosine in fp32. */
+#define HRT_ROTARY_AXES 4
+typedef struct hrt_rotary_args {
+  uint64_t q, k, q_out, k_out, pos, freqs;
+  int64_t B, S;
+  int64_t qs[3], ks[3];
+  int64_t p_sb, p_ss, p_sa;
+  int32_t Hq, Hk, D, P;
+  int32_t axes, ends[HRT_ROTARY_AXES];
+  int32_t pos_type, interleaved, back;
+} hrt_rotary_args;
+
 /* "reduce_sum" — out[k] = (sum over the reduced coordinates r of x[k, r]) / div, accumulated in fp32 and
  * rounded once to out_dtype.  x: an ndim-dimensional strided view (ndim <= 8, non-negative strides) of
  * HRT_F32/BF16/F16; bit d of reduce_mask marks dimension d as summed; out: the kept dimensions, in order,

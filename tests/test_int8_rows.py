@@ -1,0 +1,411 @@
+"""8-bit rows and products: packing against its definition in whole numbers, products against float64 products of the values that
+the packed operands stand for.
+
+Tolerances.  Codes are exact; a scale is one fp32 division (correctly rounded: equal to numpy's), a value read back one fp32
+product, rounded once more to its type.  A product's sum of integers is exact; its conversion to fp32, the two scales and the
+bias round four times, 2^-24 each of what they round (scaled sum, or scaled sum plus bias), and the output once (finfo.eps / 2
+relative, half the smallest subnormal of f16).  A gradient's sum over N runs over weights rounded to 16 bits (eps / 2 each; half
+the smallest subnormal of f16) and rounds at most N times in fp32."""
+
+import numpy as np
+import pytest
+import torch
+
+import torch_vulkan
+from torch_vulkan import abi
+
+vk = torch.device("vk")
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+HALF = DTYPES[1:]
+SUB = {torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25, torch.float32: 2.0**-150}  # half the smallest subnormal
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def packed(x):
+    """Codes and fp32 scales from the definition.  127 x and the border (2 n + 1) top / 2 are compared as whole numbers."""
+    x = f64(x)
+    top = np.abs(x).max(-1, keepdims=True)
+    ok = np.isfinite(top) & (top > 0)
+    safe = np.where(ok, top, 1.0)
+    n = np.rint(np.where(ok, x, 0.0) * 127 / safe)
+    # products of a 24-bit by an 8- or 9-bit number: exact, and so is the sign of their difference
+    d = 127 * np.where(ok, x, 0.0) - n * safe
+    n = n + (2 * d > safe) - (2 * d < -safe)
+    n = np.where((2 * np.abs(d) == safe) & (n % 2 == 1), n + np.sign(d), n)
+    with np.errstate(invalid="ignore", over="ignore"):
+        scale = np.where(np.isfinite(top), top.astype(np.float32) / np.float32(127), np.float32(np.nan)).astype(np.float32)
+        # a step of which 127 are finite in fp32: the neighbour below where the nearest is not one
+        scale = np.where(np.isinf(scale * np.float32(127)), np.nextafter(scale, np.float32(0)), scale)
+    return n.astype(np.int8), scale[..., 0]
+
+
+def sample(rows, cols, dtype, seed):
+    """Rows of very different sizes; every third row on rounding borders (multiples of top / 254), one of zeros."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, cols), generator=g) * torch.exp2(torch.randint(-10, 10, (rows, 1), generator=g).float())
+    edge = torch.randint(-254, 255, (rows, cols), generator=g).float() / 128
+    edge[:, 0] = 127 / 64
+    x = torch.where(torch.arange(rows).unsqueeze(1) % 3 == 1, edge, x)
+    x[rows // 2] = 0
+    return x.to(dtype)
+
+
+def same(got, want):
+    codes, scale = (t.cpu().numpy() for t in got)
+    assert codes.dtype == np.int8 and scale.dtype == np.float32
+    assert np.array_equal(codes, want[0]) and np.array_equal(scale, want[1], equal_nan=True)
+
+
+SHAPES = [(1, 1), (3, 7), (5, 16), (4, 33), (7, 127), (6, 128), (2, 130), (9, 256), (5, 500), (9, 1000), (2, 1025), (1030, 2048), (33, 4100), (3, 8192), (2, 8200), (2, 20000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_cpu_form_follows_the_definition(shape, dtype):
+    x = sample(*shape, dtype, sum(shape))
+    got = torch_vulkan.quantize_int8_rows(x)
+    same(got, packed(x))
+    for out in DTYPES:
+        y = torch_vulkan.dequant_int8_rows(*got, out)
+        assert torch.equal(y, (got[0].float() * got[1].unsqueeze(-1)).to(out))
+
+
+def extremes():
+    """Both ends of the exponent range, infinities, NaN, subnormals."""
+    f = torch.finfo(torch.float32)
+    rows = [[f.max, 1.0], [f.tiny, f.tiny * 3], [f.smallest_normal / 4, 1e-40], [2.0**-149, 0.0], [float("inf"), 1.0], [float("nan"), 1.0], [-f.max, f.max / 254],
+            [-0.0, 0.0], [2.0**-100, 2.0**-101], [2.0**100, 2.0**99], [2.0**101, -(2.0**20)], [1e-36, 1e-37], [3e38, -2e38]]
+    x = torch.zeros(len(rows), 40)
+    for i, r in enumerate(rows):
+        x[i, 3:5] = torch.tensor(r)
+    return x
+
+
+def test_cpu_extremes():
+    x = extremes()
+    same(torch_vulkan.quantize_int8_rows(x), packed(x))
+
+
+def test_cpu_refusals():
+    c, s = torch_vulkan.quantize_int8_rows(torch.randn(4, 70))
+    with pytest.raises(RuntimeError, match="without the last dimension"):
+        torch_vulkan.dequant_int8_rows(c, s[:3])
+    with pytest.raises(RuntimeError, match="int8"):
+        torch_vulkan.dequant_int8_rows(c.int(), s)
+    with pytest.raises(RuntimeError, match="float32"):
+        torch_vulkan.quantize_int8_rows(torch.zeros(4, 4, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="vk tensor"):
+        torch_vulkan.int8_linear(torch.zeros(4, 70), c, s)
+
+
+def test_argument_blocks_match_the_header(tmp_path):
+    """abi's blocks of the 8-bit, norm and rotary kernels lay their fields out as include/hrt_ops.h does."""
+    import ctypes
+    import os
+    import subprocess
+
+    blocks = {"hrt_i8_rows_args": abi.I8RowsArgs, "hrt_i8_mm_args": abi.I8MmArgs, "hrt_rms_args": abi.RmsArgs, "hrt_rms_bwd_args": abi.RmsBwdArgs,
+              "hrt_rotary_args": abi.RotaryArgs}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "hrt_ops.h"', "int main(void) {"]
+    for c, py in blocks.items():
+        lines.append(f'  printf("{c} size %zu\\n", sizeof({c}));')
+        lines += [f'  printf("{c} {f} %zu\\n", offsetof({c}, {f}));' for f, _ in py._fields_]
+    (tmp_path / "l.c").write_text("\n".join(lines + ["  return 0; }"]))
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c11", "-I", include, str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    got = [l.split() for l in subprocess.run([str(tmp_path / "l")], stdout=subprocess.PIPE, text=True, check=True).stdout.splitlines()]
+    for c, f, n in got:
+        assert int(n) == (ctypes.sizeof(blocks[c]) if f == "size" else getattr(blocks[c], f).offset), (c, f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_packing_is_exact(shape, dtype):
+    x = sample(*shape, dtype, 1 + sum(shape))
+    got = torch_vulkan.quantize_int8_rows(x.to(vk))
+    want = packed(x)
+    same(got, want)
+    for out in DTYPES:
+        y = torch_vulkan.dequant_int8_rows(*got, out)
+        assert torch.equal(y.cpu(), (torch.from_numpy(want[0]).float() * torch.from_numpy(want[1]).unsqueeze(-1)).to(out))
+
+
+@pytest.mark.gpu
+def test_extremes_on_the_device():
+    x = extremes()
+    got = torch_vulkan.quantize_int8_rows(x.to(vk))
+    same(got, packed(x))
+    y = torch_vulkan.dequant_int8_rows(*got, torch.float32).cpu()
+    bad = ~torch.isfinite(x).all(-1)
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all()
+
+
+@pytest.mark.gpu
+def test_packing_of_views():
+    x = sample(12, 4096, torch.bfloat16, 3)
+    base = x.to(vk)
+    for view, ref in ((base[:, 8:1032], x[:, 8:1032]), (base[:, 3:100], x[:, 3:100]), (base.t(), x.t()), (base[:1].expand(5, 4096), x[:1].expand(5, 4096)),
+                      (base.view(3, 4, 4096), x.view(3, 4, 4096)), (base.view(3, 4, 4096).transpose(0, 1), x.view(3, 4, 4096).transpose(0, 1)), (base[0], x[0]),
+                      (base[:0], x[:0]), (base[:, :0], x[:, :0])):
+        got, want = torch_vulkan.quantize_int8_rows(view), torch_vulkan.quantize_int8_rows(ref)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+        assert torch.equal(torch_vulkan.dequant_int8_rows(*got).cpu(), torch_vulkan.dequant_int8_rows(*want))
+    codes, scale = torch_vulkan.quantize_int8_rows(base)
+    for cv, sv in ((codes[:, 5:77], scale), (codes.t()[:12], scale), (codes[::2], scale[::2])):
+        assert torch.equal(torch_vulkan.dequant_int8_rows(cv, sv).cpu(), torch_vulkan.dequant_int8_rows(cv.cpu(), sv.cpu()))
+
+
+# ---- the linear layer -------------------------------------------------------------------------------------------------
+def operands(M, N, K, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((M, K), generator=g).to(dtype)
+    w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8)
+    s = torch.rand((N,), generator=g) * 2e-3 + 1e-5
+    b = torch.randn((N,), generator=g).to(dtype)
+    return x, w, s, b
+
+
+def product(codes, scale, w, s, b):
+    y = (codes.astype(np.float64) @ f64(w).T) * scale.astype(np.float64)[:, None] * f64(s)
+    return y, (y + f64(b) if b is not None else y)
+
+
+def check_forward(got, y, want, dtype):
+    tol = torch.finfo(dtype).eps / 2 * np.abs(want) + SUB[dtype] + 1.01 * 2.0**-24 * (3 * np.abs(y) + np.abs(want))
+    assert got.dtype == dtype and tuple(got.shape) == want.shape
+    assert (np.abs(f64(got) - want) <= tol).all(), np.max(np.abs(f64(got) - want) / tol)
+
+
+def check_back(got, g, w, s, dtype):
+    v = f64(w) * f64(s)[:, None]
+    want, size = f64(g) @ v, np.abs(f64(g)) @ np.abs(v)
+    e = torch.finfo(dtype).eps / 2
+    tol = e * np.abs(want) + SUB[dtype] + size * (1.01 * e + (len(v) + 1) * 2.0**-24) + np.abs(f64(g)).sum(-1, keepdims=True) * SUB[dtype]
+    assert (np.abs(f64(got) - want) <= tol).all(), np.max(np.abs(f64(got) - want) / tol)
+
+
+# every tile and both sides of its borders, rows, odd widths, ends of K inside a line and inside a piece of 16
+PRODUCTS = [(1, 16, 16), (1, 1, 1), (2, 8, 144), (16, 48, 2064), (16, 100, 128), (17, 64, 1024), (32, 40, 1040), (33, 136, 320), (64, 64, 512), (77, 130, 272),
+            (130, 256, 400), (129, 129, 128), (257, 264, 1000), (300, 512, 77), (5, 33, 50), (200, 2056, 656), (1, 4096, 4096), (20, 512, 9000), (308, 72, 4112),
+            (700, 2048, 512), (1500, 4096, 256), (4100, 2048, 144)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_linear(M, N, K, dtype):
+    x, w, s, b = operands(M, N, K, dtype, M + N + K)
+    codes, scale = packed(x)
+    X, W, S, B = (t.to(vk) for t in (x, w, s, b))
+    y, want = product(codes, scale, w, s, b)
+    check_forward(torch_vulkan.int8_linear(X, W, S, B), y, want, dtype)
+    y, want = product(codes, scale, w, s, None)
+    check_forward(torch_vulkan.int8_linear(X, W, S), y, want, dtype)
+    got = torch_vulkan.int8_linear(torch.from_numpy(codes).to(vk), W, S, x_scale=torch.from_numpy(scale).to(vk), out_dtype=dtype)
+    check_forward(got, y, want, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 16, 40, 300, 1100])
+def test_sums_at_their_largest(M):
+    """All codes at 127 and -127 (-128 among the weights), at the longest K: whole sums of 31 bits."""
+    K = 131056
+    x = torch.ones((M, K), dtype=torch.int8) * 127
+    w = torch.full((24, K), -128, dtype=torch.int8)
+    w[::2] = 127
+    xs, s = torch.linspace(0.5, 2, M), torch.linspace(1e-3, 2e-3, 24)
+    y = (127.0 * K) * torch.where(torch.arange(24) % 2 == 0, 127.0, -128.0).double().numpy() * f64(xs)[:, None] * f64(s)
+    got = torch_vulkan.int8_linear(x.to(vk), w.to(vk), s.to(vk), x_scale=xs.to(vk), out_dtype=torch.bfloat16)
+    check_forward(got, y, y, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (37, 136, 320), (5, 33, 50), (308, 256, 512), (130, 72, 1000), (1030, 512, 264)])
+def test_gradients(M, N, K, dtype):
+    x, w, s, b = operands(M, N, K, dtype, 7)
+    g = torch.randn((M, N), generator=torch.Generator().manual_seed(3)).to(dtype)
+    X, B = x.to(vk).requires_grad_(), b.to(vk).requires_grad_()
+    dx, db = torch.autograd.grad(torch_vulkan.int8_linear(X, w.to(vk), s.to(vk), B), (X, B), g.to(vk))
+    check_back(dx, g, w, s, dtype)
+    want = f64(g).sum(0)
+    assert (np.abs(f64(db) - want) <= torch.finfo(dtype).eps / 2 * np.abs(want) + SUB[dtype] + M * 2.0**-24 * np.abs(f64(g)).sum(0)).all()
+    # one of the two alone, and the bias under an int8 x
+    (dx2,) = torch.autograd.grad(torch_vulkan.int8_linear(X, w.to(vk), s.to(vk)), (X,), g.to(vk))
+    (db2,) = torch.autograd.grad(torch_vulkan.int8_linear(x.to(vk), w.to(vk), s.to(vk), B), (B,), g.to(vk))
+    codes, scale = torch_vulkan.quantize_int8_rows(x.to(vk))
+    (db3,) = torch.autograd.grad(torch_vulkan.int8_linear(codes, w.to(vk), s.to(vk), B, x_scale=scale, out_dtype=dtype), (B,), g.to(vk))
+    assert torch.equal(dx2.cpu(), dx.cpu()) and torch.equal(db2.cpu(), db.cpu()) and torch.equal(db3.cpu(), db.cpu())
+
+
+@pytest.mark.gpu
+def test_the_gradients_gradient():
+    """dx = g W is linear in g: its gradient is h W^T, and that one's k W again."""
+    M, N, K, dtype = 37, 136, 320, torch.bfloat16
+    x, w, s, b = operands(M, N, K, dtype, 23)
+    r = torch.Generator().manual_seed(4)
+    g, k = (torch.randn((M, N), generator=r).to(dtype) for _ in range(2))
+    h = torch.randn((M, K), generator=r).to(dtype)
+    X, G, H = (t.to(vk).requires_grad_() for t in (x, g, h))
+    (dx,) = torch.autograd.grad(torch_vulkan.int8_linear(X, w.to(vk), s.to(vk), b.to(vk)), X, G, create_graph=True)
+    check_back(dx, g, w, s, dtype)
+    (gh,) = torch.autograd.grad(dx, G, H, create_graph=True)
+    v = f64(w) * f64(s)[:, None]
+    e, size = torch.finfo(dtype).eps / 2, np.abs(f64(h)) @ np.abs(v).T
+    assert (np.abs(f64(gh) - f64(h) @ v.T) <= e * np.abs(f64(h) @ v.T) + size * (1.01 * e + (K + 1) * 2.0**-24)).all()
+    (gk,) = torch.autograd.grad(gh, H, k.to(vk))
+    check_back(gk, k, w, s, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+def test_layouts(dtype):
+    x, w, s, b = operands(24, 72, 320, dtype, 11)
+    want = torch_vulkan.int8_linear(x.to(vk), w.to(vk), s.to(vk), b.to(vk)).cpu()
+    wide_x, wide_w = torch.zeros(24, 333, dtype=dtype), torch.zeros(144, 352, dtype=torch.int8)
+    wide_x[:, 5:325], wide_w[::2, 16:336] = x, w
+    off_w = torch.zeros(72, 321, dtype=torch.int8)
+    off_w[:, 1:] = w
+    for X in (x.to(vk), wide_x.to(vk)[:, 5:325], x.t().contiguous().to(vk).t(), x.view(2, 3, 4, 320).to(vk), x.view(4, 6, 320).transpose(0, 1).contiguous().to(vk).transpose(0, 1)):
+        for W in (w.to(vk), wide_w.to(vk)[::2, 16:336], off_w.to(vk)[:, 1:], w.t().contiguous().to(vk).t()):
+            got = torch_vulkan.int8_linear(X, W, torch.stack((s, s), 1).to(vk)[:, 0], b.to(vk))
+            assert got.shape == (*X.shape[:-1], 72) and torch.equal(got.cpu().view(24, 72), want)
+    one = torch_vulkan.int8_linear(x[0].to(vk), w.to(vk), s.to(vk), b.to(vk))
+    assert one.shape == (72,) and torch.equal(one.cpu(), want[0])
+    codes, scale = torch_vulkan.quantize_int8_rows(x[0].to(vk))
+    one = torch_vulkan.int8_linear(codes, w.to(vk), s.to(vk), b.to(vk), x_scale=scale, out_dtype=dtype)
+    assert scale.shape == () and torch.equal(one.cpu(), want[0])
+    codes, scale = torch_vulkan.quantize_int8_rows(x.view(4, 6, 320).to(vk))
+    got = torch_vulkan.int8_linear(codes.transpose(0, 1), w.to(vk), s.to(vk), b.to(vk), x_scale=scale.transpose(0, 1), out_dtype=dtype)
+    assert torch.equal(got.transpose(0, 1).cpu().reshape(24, 72), want)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    x, w, s, b = (t.to(vk) for t in operands(4, 24, 32, torch.bfloat16, 1))
+    assert torch_vulkan.int8_linear(x[:0], w, s, b).shape == (0, 24)
+    assert torch_vulkan.int8_linear(x, w[:0], s[:0], b[:0]).shape == (4, 0)
+    assert torch.equal(torch_vulkan.int8_linear(x[:, :0], w[:, :0], s, b).cpu(), b.cpu().expand(4, 24))
+    assert torch_vulkan.int8_linear(x[:, :0], w[:, :0], s).cpu().abs().sum() == 0
+    X, B = x[:0].detach().requires_grad_(), b.detach().requires_grad_()
+    dx, db = torch.autograd.grad(torch_vulkan.int8_linear(X, w, s, B).sum(), (X, B))
+    assert dx.shape == (0, 32) and db.cpu().abs().sum() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_what_is_not_finite_stays_in_its_row_and_column(M):
+    x, w, s, b = operands(M, 72, 320, torch.bfloat16, 9)
+    want = torch_vulkan.int8_linear(x.to(vk), w.to(vk), s.to(vk), b.to(vk)).cpu()
+    x[1, 5], s[7] = float("inf"), float("nan")
+    x[2] = 0
+    got = torch_vulkan.int8_linear(x.to(vk), w.to(vk), s.to(vk), b.to(vk)).cpu()
+    hit = torch.zeros(M, 72, dtype=torch.bool)
+    hit[1], hit[:, 7] = True, True
+    assert torch.isnan(got[hit]).all() and torch.isfinite(got[~hit]).all()
+    rest = ~hit
+    rest[2] = False
+    assert torch.equal(got[rest], want[rest]) and torch.equal(got[2][~hit[2]], b[~hit[2]])
+
+
+@pytest.mark.gpu
+def test_refusals():
+    x, w, s, b = (t.to(vk) for t in operands(4, 24, 32, torch.bfloat16, 1))
+    c, cs = torch_vulkan.quantize_int8_rows(x)
+    lin = torch_vulkan.int8_linear
+    for match, call in [("vk tensor", lambda: lin(x.float(), w, s)), ("vk device", lambda: lin(x, w.cpu(), s)), ("int8", lambda: lin(x, w.float(), s)),
+                        ("float32", lambda: lin(x, w, s.bfloat16())), ("last dimension", lambda: lin(x, w, s[:3])), (r"\[N, K\]", lambda: lin(x[:, :16], w, s)),
+                        ("bias", lambda: lin(x, w, s, b.half())), ("bias", lambda: lin(x, w, s, b[:3])), ("x_scale", lambda: lin(c, w, s)),
+                        ("x_scale", lambda: lin(x, w, s, x_scale=cs)), ("x's scale", lambda: lin(c, w, s, x_scale=cs[:2])),
+                        ("out_dtype", lambda: lin(c, w, s, x_scale=cs, out_dtype=torch.float32)), ("out_dtype", lambda: lin(x, w, s, out_dtype=torch.float16)),
+                        ("no gradient", lambda: lin(x, w, s.detach().requires_grad_())), ("no gradient", lambda: lin(c, w, s, x_scale=cs.detach().requires_grad_())),
+                        ("131056", lambda: lin(torch.zeros(1, 131072, dtype=torch.bfloat16).to(vk), torch.zeros(1, 131072, dtype=torch.int8).to(vk), s[:1])),
+                        ("last dimension", lambda: torch_vulkan.dequant_int8_rows(c, cs[:2])), ("out_dtype", lambda: torch_vulkan.dequant_int8_rows(c, cs, torch.int32)),
+                        ("float32", lambda: torch_vulkan.quantize_int8_rows(c))]:
+        with pytest.raises(RuntimeError, match=match):
+            call()
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+
+    x, w, s, b = (t.to(vk) for t in operands(4, 64, 96, torch.bfloat16, 1))
+    with fwd.dual_level():
+        for wants in (False, True):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch_vulkan.int8_linear(fwd.make_dual(x.detach().requires_grad_(wants), torch.ones_like(x)), w, s, b)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch_vulkan.int8_linear(x, w, s, fwd.make_dual(b.detach().requires_grad_(wants), torch.ones_like(b)))
+        y = torch_vulkan.int8_linear(x.detach().requires_grad_(), w, s, b)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            y.backward(fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(6, 96), (2, 3, 96), (96,), (0, 96), (6, 50)])
+def test_in_place_operations_on_the_output(shape):
+    x, w, s, b = operands(6, 64, shape[-1], torch.bfloat16, 31)
+    n = int(np.prod(shape))
+    W, S, X, B = w.to(vk), s.to(vk), x.flatten()[:n].view(shape).to(vk).requires_grad_(), b.to(vk).requires_grad_()
+    A = torch.randn((*shape[:-1], 64), generator=torch.Generator().manual_seed(6)).bfloat16().to(vk).requires_grad_()
+
+    def run(add):
+        y = add(torch_vulkan.int8_linear(X, W, S, B), A)
+        y = add(y, y * 2)
+        return [y, *torch.autograd.grad(y, [X, B, A], torch.ones_like(y))]
+
+    for a, c in zip(run(lambda y, z: y.add_(z)), run(lambda y, z: y + z)):
+        assert torch.equal(a.detach().cpu(), c.detach().cpu())
+
+
+@pytest.mark.gpu
+def test_autocast_runs_it_in_its_type():
+    x, w, s, b = operands(6, 64, 96, torch.float32, 2)
+    X, B = x.to(vk).requires_grad_(), b.to(vk).requires_grad_()
+    g = torch.ones(6, 64)
+    for dtype in HALF:
+        with torch.autocast("vk", dtype=dtype):
+            y = torch_vulkan.int8_linear(X, w.to(vk), s.to(vk), B)
+            c, cs = torch_vulkan.quantize_int8_rows(X.detach().to(dtype))
+            z = torch_vulkan.int8_linear(c, w.to(vk), s.to(vk), B.detach(), x_scale=cs)
+            o = torch_vulkan.int8_linear(c, w.to(vk), s.to(vk), B.detach(), x_scale=cs, out_dtype=torch.float16)
+        assert y.dtype == z.dtype == dtype and o.dtype == torch.float16
+        want = torch_vulkan.int8_linear(x.to(dtype).to(vk), w.to(vk), s.to(vk), b.to(dtype).to(vk))
+        assert torch.equal(y.detach().cpu(), want.cpu()) and torch.equal(z.cpu(), want.cpu())
+        dx, db = torch.autograd.grad(y, (X, B), g.to(dtype).to(vk))
+        assert dx.dtype == db.dtype == torch.float32
+        check_back(dx, g, w, s, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20, 200])
+def test_replayed_graph(M):
+    rt, out = abi.Runtime(), {}
+    x, w, s, b = (t.to(vk) for t in operands(M, 512, 2000, torch.bfloat16, 8))
+    g = torch.randn((M, 512), generator=torch.Generator().manual_seed(1)).bfloat16().to(vk)
+    X = x.detach().requires_grad_()
+
+    def run():
+        with torch.autograd.set_multithreading_enabled(False):
+            y = torch_vulkan.int8_linear(X, w, s, b)
+            (dx,) = torch.autograd.grad(y, X, g)
+        return y.detach(), dx
+
+    eager = [t.cpu() for t in run()]
+
+    def record():
+        out["y"] = run()
+
+    gid = rt.graph(record)
+    for _ in range(3):
+        for t in out["y"]:
+            t.zero_()
+        rt.graph_launch(gid)
+        assert all(torch.equal(a.cpu(), b_) for a, b_ in zip(out["y"], eager))
+        assert all(torch.equal(a.cpu(), b_) for a, b_ in zip(run(), eager))
+    rt.graph_destroy(gid)

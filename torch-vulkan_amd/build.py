@@ -43,6 +43,9 @@ HRT_SOURCES = [
     "kernels/mx4.hip",
     "kernels/mx4_gemm.hip",
     "kernels/mx4_back.hip",
+    "kernels/rms.hip",
+    "kernels/i8_gemm.hip",
+    "kernels/rotary.hip",
     "kernels/gemm.hip",
     "kernels/gemm_f32.hip",
     "kernels/gemm_mfma.hip",
@@ -70,6 +73,9 @@ SHIM_SOURCES = [
     "shim/op_quant.cpp",
     "shim/op_mx4.cpp",
     "shim/op_relbias.cpp",
+    "shim/op_int8.cpp",
+    "shim/op_rms.cpp",
+    "shim/op_rotary.cpp",
     "shim/op_ew.cpp",
     "shim/op_image.cpp",
 ]

@@ -1,0 +1,395 @@
+// "i8_mm_{bf16,f16}": y = (X W^T) * x_scale * w_scale + bias on 8-bit rows, whole sums in 32 bits (exact), one rounding at the end.
+//
+// Two kernels:
+//   * i8_rows for few rows: bound by the weights' bytes, in practice by one memory latency.  A wavefront takes 16 columns of y and
+//     every NWVth 128-wide piece of K, its loads all in flight at once; no LDS but for the wavefronts' sums.
+//   * i8_tile for the rest: bound by the matrix cores and by L2 -> LDS.  Both operands are copied global -> LDS directly, in rows
+//     of 128 bytes (whole cache lines), XOR-swizzled by 16-byte chunks (tile_swz<8>).
+// Lane layout of the 8-bit products (checked on the device), l = lane: 32x32x32: operand row l % 32, bytes 16 (l / 32) .. + 15 of K;
+// 16x16x64: row l % 16, bytes 16 (l / 16) .. + 15; accumulators as for the 16-bit products of the same shape.
+// W is the first operand, so an accumulator holds four consecutive columns n of one row m of y.
+#include <utility>
+
+#include "../hrt/registry.h"
+#include "lds_stage.h"
+
+namespace hk {
+namespace {
+
+// Lambdas of a kernel with many copies of its step: the compiler would make them functions.
+#define HK_INLINE __attribute__((always_inline))
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ i32x4 mac16(u32x4 a, u32x4 b, i32x4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ i32x16 mac32(u32x4 a, u32x4 b, i32x16 c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+
+// Values n .. n + 3 of row m from whole sums: sum * x_scale is taken first (the product of two small scales may underflow).
+template <typename T>
+__device__ __forceinline__ void store4(const hrt_i8_mm_args& p, int64_t m, int64_t n, const int* v, bool vec) {
+  if (m >= p.M || n >= p.N) return;
+  const float sx = gcptr<float>(p.x_scale)[m];
+  const HK_G float* sw = gcptr<float>(p.w_scale) + n;
+  HK_G uint16_t* y = gptr<uint16_t>(p.y) + m * p.N + n;
+  const HK_G uint16_t* b = gcptr<uint16_t>(p.bias) + n;
+  float o[4];
+  if (vec) {
+    u32x2 w = {0, 0};
+    if (p.bias) w = *reinterpret_cast<const HK_G u32x2*>(b);
+    const f32x4 s = *reinterpret_cast<const HK_G f32x4*>(sw);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * sx * s[e] + (e & 1 ? hi16<T>(w[e >> 1]) : lo16<T>(w[e >> 1]));
+    *reinterpret_cast<HK_G u32x2*>(y) = pack4<T>(o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < p.N) y[e] = T::from_f32((float)v[e] * sx * sw[e] + (p.bias ? T::to_f32(b[e]) : 0.f));
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------------
+// 16 MB rows (MB 1 or 2), NWV wavefronts.  A wavefront's pieces of 128 bytes of K come in batches of UB whose loads are all issued
+// before the first product: one memory latency a batch.
+template <typename T, int MB, int NWV, int UB>
+__global__ __launch_bounds__(64 * NWV) void i8_rows(hrt_i8_mm_args p, bool vec) {
+  __shared__ int part[NWV - 1][MB][64][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;  // columns past N repeat the last one and are not stored
+  const int64_t chunks = p.K / 16, steps = cdiv(p.K, 128);
+  const HK_G uint8_t* const w = gcptr<uint8_t>(p.w) + n * p.w_sn;
+  const HK_G uint8_t* x[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) x[b] = gcptr<uint8_t>(p.x) + (b * 16 + r16 < p.M ? b * 16 + r16 : p.M - 1) * p.x_sm;  // rows past M: not stored
+  i32x4 acc[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) acc[b] = i32x4{0, 0, 0, 0};
+  for (int64_t st = wave; st < steps; st += NWV * UB) {
+    u32x4 wf[UB][2], xf[UB][2][MB];
+#pragma unroll
+    for (int u = 0; u < UB; ++u)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int64_t c = (st + u * NWV) * 8 + 4 * t + g, at = (c < chunks ? c : 0) * 16;  // chunks past the end of K: zeros
+        wf[u][t] = __builtin_nontemporal_load(reinterpret_cast<const HK_G u32x4*>(w + at));
+#pragma unroll
+        for (int b = 0; b < MB; ++b) xf[u][t][b] = *reinterpret_cast<const HK_G u32x4*>(x[b] + at);
+      }
+#pragma unroll
+    for (int u = 0; u < UB; ++u)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if ((st + u * NWV) * 8 + 4 * t + g >= chunks) wf[u][t] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[b] = mac16(wf[u][t], xf[u][t][b], acc[b]);
+      }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int b = 0; b < MB; ++b) *reinterpret_cast<i32x4*>(part[wave - 1][b][lane]) = acc[b];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+#pragma unroll
+    for (int w2 = 0; w2 < NWV - 1; ++w2) acc[b] += *reinterpret_cast<const i32x4*>(part[w2][b][lane]);
+    const int v[4] = {acc[b][0], acc[b][1], acc[b][2], acc[b][3]};
+    store4<T>(p, b * 16 + r16, n0 + 4 * g, v, vec);
+  }
+}
+
+// ---- tiles ---------------------------------------------------------------------------------------------------------------
+constexpr int kLine = 128;  // bytes and values of K in a row of a stage
+
+// A workgroup's wavefronts are KG groups along K times a grid of WM x WN sub-tiles; a step takes a line per group.  KG > 1 gives
+// small grids the wavefronts that hide a copy's latency without a second launch; the groups' sums are added at the end (whole
+// numbers: the order is free).  Both operands have a ring of R stages.
+template <int BM, int BN, int WM, int WN, int KG, int R>
+struct TileShape {
+  static constexpr int NWT = (BM / WM) * (BN / WN), NW = NWT * KG;    // wavefronts per group, in all
+  static constexpr int XT = KG * BM * kLine, WT = KG * BN * kLine;    // bytes of a stage
+  static constexpr int IPX = XT / 1024 / NW, IPW = WT / 1024 / NW;    // copies per wavefront
+  static constexpr int FM = WM / 32, FN = WN / 32;
+  static_assert(XT % (1024 * NW) == 0 && WT % (1024 * NW) == 0, "copy split");
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int KG, int R>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i8_mm_args p, int tiles_n, int nk, bool lines) {
+  using S = TileShape<BM, BN, WM, WN, KG, R>;
+  constexpr int NWT = S::NWT, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN;
+  // One LDS object per stage, so that the compiler can tell the reads of one from the copies into another.
+  __shared__ __attribute__((aligned(1024))) uint8_t x0[S::XT], x1[S::XT], x2[R > 2 ? S::XT : 16], x3[R > 3 ? S::XT : 16];
+  __shared__ __attribute__((aligned(1024))) uint8_t w0[S::WT], w1[S::WT], w2[R > 2 ? S::WT : 16], w3[R > 3 ? S::WT : 16];
+  auto xbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? x0 : I == 1 ? x1 : I == 2 ? x2 : x3); };
+  auto wbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? w0 : I == 1 ? w1 : I == 2 ? w2 : w3); };
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave / NWT, wt = wave % NWT, wm = wt % (BM / WM), wn = wt / (BM / WM), l32 = lane & 31, h = lane >> 5;
+  // n-fastest tile numbers, in scalar registers, and with them every buffer resource
+  const uint32_t tm = __builtin_amdgcn_readfirstlane(blockIdx.x / (uint32_t)tiles_n);
+  const uint32_t tn = __builtin_amdgcn_readfirstlane(blockIdx.x % (uint32_t)tiles_n);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int ml = p.M - m0 < BM ? (int)(p.M - m0) : BM, nl = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+
+  // copy sources; lane offsets inside a stage, kNoRow where the row does not exist (the buffer's range check gives zeros)
+  const uint32_t xss = (uint32_t)p.x_sm, wss = (uint32_t)p.w_sn;
+  const HK_G uint8_t* Xb = gcptr<uint8_t>(p.x) + m0 * p.x_sm;
+  const HK_G uint8_t* Wb = gcptr<uint8_t>(p.w) + n0 * p.w_sn;
+  // copy j of a stage: this lane's row, and its byte of K in the step
+  auto row_of = [&](int j, int rows) HK_INLINE { return (j * 8 + (lane >> 3)) % rows; };
+  auto byte_of = [&](int j, int rows) HK_INLINE { return ((lane & 7) ^ tile_swz<8>(row_of(j, rows))) * 16 + j / (rows / 8) * kLine; };
+  uint32_t xo[IPX], wo[IPW];
+#pragma unroll
+  for (int i = 0; i < IPX; ++i) {
+    const int j = wave * IPX + i, row = row_of(j, BM);
+    xo[i] = row < ml ? (uint32_t)row * xss + (uint32_t)byte_of(j, BM) : kNoRow;
+  }
+#pragma unroll
+  for (int i = 0; i < IPW; ++i) {
+    const int j = wave * IPW + i, row = row_of(j, BN);
+    wo[i] = row < nl ? (uint32_t)row * wss + (uint32_t)byte_of(j, BN) : kNoRow;
+  }
+  // The last stage may hold fewer values: chunks past K are zeros (a select, not a branch: the compiler counts the copies in
+  // flight along every path).
+  auto copy = [&](auto ic, int ks) HK_INLINE {
+    const __amdgpu_buffer_rsrc_t xr = edge_rsrc(Xb + (int64_t)ks * (KG * kLine)), wr = edge_rsrc(Wb + (int64_t)ks * (KG * kLine));
+    const int64_t left = p.K - (int64_t)ks * (KG * kLine);
+    const int l = left >= KG * kLine ? KG * kLine : (int)left;
+#pragma unroll
+    for (int i = 0; i < IPX; ++i) edge_copy(xr, xbuf(ic), wave * IPX + i, byte_of(wave * IPX + i, BM) < l ? xo[i] : kNoRow);
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) edge_copy(wr, wbuf(ic), wave * IPW + i, byte_of(wave * IPW + i, BN) < l ? wo[i] : kNoRow);
+  };
+  // This lane's rows: the sub-tile's other 32-row blocks lie a constant further (the swizzle repeats every 16 rows).
+  const int xrow = wm * WM + l32, wrow = wn * WN + l32;
+
+  i32x16 acc[FN][FM];
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
+
+  // Step ks from stage I.  GUARD: near the end, where no copy is left to be made; it waits for all of them.
+  auto step = [&](auto ic, auto guard, int ks) HK_INLINE {
+    constexpr int I = decltype(ic)::value;
+    constexpr bool GUARD = decltype(guard)::value;
+    const HK_L uint8_t* const xs = xbuf(ic) + kg * BM * kLine;
+    const HK_L uint8_t* const ws = wbuf(ic) + kg * BN * kLine;
+    u32x4 wf[2][FN], xf[2][FM];
+    // a line is four slices; the fragments of the next one are read while this one's products run (two register sets, fenced)
+    auto read = [&](int s) HK_INLINE {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) wf[s & 1][j] = *reinterpret_cast<const HK_L u32x4*>(ws + tile_off<8>(wrow, 2 * s + h) + j * 32 * kLine);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) xf[s & 1][i] = *reinterpret_cast<const HK_L u32x4*>(xs + tile_off<8>(xrow, 2 * s + h) + i * 32 * kLine);
+    };
+    read(0);
+    if (!GUARD || ks + R - 1 < nk) copy(std::integral_constant<int, (I + R - 1) % R>(), ks + R - 1);
+    auto slice = [&](auto sc) HK_INLINE {
+      constexpr int SL = decltype(sc)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (SL < 3) read(SL + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[j][i] = mac32(wf[SL & 1][j], xf[SL & 1][i], acc[j][i]);
+    };
+    slice(std::integral_constant<int, 0>()), slice(std::integral_constant<int, 1>());
+    slice(std::integral_constant<int, 2>()), slice(std::integral_constant<int, 3>());
+    // The products are pure, and the compiler puts them off to the end of the loop body unless their results are used here.
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) asm volatile("" : "+v"(acc[j][i]));
+    // The next step's stage has landed everywhere; later ones may stay in flight.
+    barrier_keep_vm_lds<GUARD ? 0 : (R - 2) * (IPX + IPW)>();
+  };
+  using Whole = std::integral_constant<bool, false>;
+  using Guard = std::integral_constant<bool, true>;
+  auto steps = [&](auto guard, int ks) HK_INLINE {
+    auto one = [&](auto ic) HK_INLINE {
+      if (!decltype(guard)::value || ks + decltype(ic)::value < nk) step(ic, guard, ks + decltype(ic)::value);
+    };
+    one(std::integral_constant<int, 0>()), one(std::integral_constant<int, 1>());
+    if constexpr (R > 2) one(std::integral_constant<int, 2>());
+    if constexpr (R > 3) one(std::integral_constant<int, 3>());
+  };
+  copy(std::integral_constant<int, 0>(), 0);
+  // stages of the steps before the first one's own copies (past the end of K: zeros that nobody reads)
+  if constexpr (R > 2) {
+    issue_order_fence();  // the first barrier counts on them being the last ones issued
+    copy(std::integral_constant<int, 1>(), 1);
+  }
+  if constexpr (R > 3) copy(std::integral_constant<int, 2>(), 2);
+  barrier_keep_vm<(R - 2) * (IPX + IPW)>();
+  int ks = 0;
+  for (; ks + 2 * R - 1 <= nk; ks += R) steps(Whole(), ks);
+  for (; ks < nk; ks += R) steps(Guard(), ks);
+
+  if constexpr (KG > 1) {  // the groups' sums, through the stages' memory (every copy has landed)
+    constexpr int NB = FN * FM, PER = S::XT / 4096;  // accumulators of a wavefront; how many an X stage holds
+    static_assert((KG - 1) * NWT * NB <= 2 * PER && PER % NB == 0, "merge areas");
+    auto area = [&](int k, int b) {
+      const int q = ((k - 1) * NWT + wt) * NB;
+      return (int*)(q < PER ? x0 + q * 4096 : x1 + (q - PER) * 4096) + b * 1024 + lane;
+    };
+    if (kg > 0) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        int* const mine = area(kg, b);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[e * 64] = acc[b / FM][b % FM][e];
+      }
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int k = 1; k < KG; ++k)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int* const part = area(k, b);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b / FM][b % FM][e] += part[e * 64];
+      }
+  }
+  if (!lines) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v[4] = {acc[j][i][4 * e], acc[j][i][4 * e + 1], acc[j][i][4 * e + 2], acc[j][i][4 * e + 3]};
+          store4<T>(p, m0 + wm * WM + i * 32 + l32, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, false);
+        }
+    return;
+  }
+  // Whole lines of y: 32 rows at a time go through the wavefront's own LDS area, so that a store writes 16 bytes a lane along a row.
+  constexpr int RB = WN * 2 + 16;  // bytes of a row in the area, its pad off the banks of the next
+  // KG > 1: in the merge area of group 1's wavefront, which this one has read; else in the stages
+  constexpr int AREA = 32 * RB, MERGED = FN * FM * 4096, PX = S::XT / AREA, PW = S::WT / AREA;
+  static_assert(KG > 1 ? AREA <= MERGED : 2 * PX + 2 * PW >= NWT, "epilogue areas");
+  HK_L uint8_t* const area = KG > 1           ? (HK_L uint8_t*)(wt * MERGED < S::XT ? x0 + wt * MERGED : x1 + (wt * MERGED - S::XT))
+                             : wt < PW        ? (HK_L uint8_t*)w0 + wt * AREA
+                             : wt < 2 * PW    ? (HK_L uint8_t*)w1 + (wt - PW) * AREA
+                             : wt < 2 * PW + PX ? (HK_L uint8_t*)x0 + (wt - 2 * PW) * AREA
+                                              : (HK_L uint8_t*)x1 + (wt - 2 * PW - PX) * AREA;
+  const int64_t nw = n0 + wn * WN;
+  u32x2 bias[FN][4];
+  f32x4 sw[FN][4];
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t n = nw + j * 32 + 8 * e + 4 * h, at = n < p.N ? n : 0;
+      bias[j][e] = u32x2{0, 0};
+      if (p.bias) bias[j][e] = *reinterpret_cast<const HK_G u32x2*>(gcptr<uint16_t>(p.bias) + at);
+      sw[j][e] = *reinterpret_cast<const HK_G f32x4*>(gcptr<float>(p.w_scale) + at);
+    }
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t mine = m0 + wm * WM + i * 32 + l32;
+    const float sx = gcptr<float>(p.x_scale)[mine < p.M ? mine : p.M - 1];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          o[r] = (float)acc[j][i][4 * e + r] * sx * sw[j][e][r] + (r & 1 ? hi16<T>(bias[j][e][r >> 1]) : lo16<T>(bias[j][e][r >> 1]));
+        *reinterpret_cast<HK_L u32x2*>(area + l32 * RB + (j * 32 + 8 * e + 4 * h) * 2) = pack4<T>(o);
+      }
+    constexpr int CPR = WN / 8;  // 16-byte chunks per row
+#pragma unroll
+    for (int u = 0; u < 32 * CPR / 64; ++u) {
+      const int ch = u * 64 + lane, row = ch / CPR, c = ch % CPR;
+      const u32x4 v = *reinterpret_cast<const HK_L u32x4*>(area + row * RB + c * 16);
+      const int64_t m = m0 + wm * WM + i * 32 + row, n = nw + c * 8;
+      if (m < p.M && n < p.N) *reinterpret_cast<HK_G u32x4*>(gptr<uint16_t>(p.y) + m * p.N + n) = v;
+    }
+  }
+}
+
+// ---- plan and launch -----------------------------------------------------------------------------------------------------
+struct Tile2 {
+  int bm, bn;
+};
+constexpr Tile2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
+
+int64_t tiles_of(const hrt_i8_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
+// Index of the tile, -1: i8_rows.
+int plan_of(const hrt_i8_mm_args& a) {
+  if (a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
+  static constexpr struct { float fixed, per128; } kCost[4] = {{11.f, 1.9f}, {7.4f, 1.4f}, {5.4f, 0.74f}, {4.2f, 0.25f}};
+  int best = 3;
+  float us = 0.f;
+  for (int t = 3; t >= 0; --t) {
+    const float e = (float)cdiv(tiles_of(a, t), 256) * (kCost[t].fixed + kCost[t].per128 * (float)a.K / 128.f);
+    if (t == 3 || e < us) best = t, us = e;
+  }
+  return best;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int KG, int R>
+void queue_tile(const hrt_i8_mm_args& a, hipStream_t s, bool lines) {
+  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, kLine * KG);
+  hipLaunchKernelGGL((i8_tile<T, BM, BN, WM, WN, KG, R>), dim3((uint32_t)(tm * tn)), dim3(64 * TileShape<BM, BN, WM, WN, KG, R>::NW), 0, s, a, (int)tn,
+                     (int)nk, lines);
+}
+
+template <typename T>
+void queue_mm(const hrt_i8_mm_args& a, int tile, hipStream_t s) {
+  const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0 && a.w_scale % 16 == 0, lines = vec && a.N % 8 == 0 && a.y % 16 == 0;
+  switch (tile) {
+    case 0: return queue_tile<T, 256, 256, 128, 64, 1, 2>(a, s, lines);
+    case 1: return queue_tile<T, 128, 256, 64, 64, 1, 2>(a, s, lines);
+    case 2: return queue_tile<T, 128, 128, 64, 64, 2, 2>(a, s, lines);
+    case 3: return queue_tile<T, 64, 64, 32, 64, 4, 2>(a, s, lines);
+  }
+  // wavefronts and batches that cover K once where they can
+  const dim3 grid((uint32_t)cdiv(a.N, 16));
+  const int64_t pieces = cdiv(a.K, 128);
+  if (a.M > 16) hipLaunchKernelGGL((i8_rows<T, 2, 4, 2>), grid, dim3(256), 0, s, a, vec);
+  else if (pieces <= 8) hipLaunchKernelGGL((i8_rows<T, 1, 4, 2>), grid, dim3(256), 0, s, a, vec);
+  else if (pieces <= 16) hipLaunchKernelGGL((i8_rows<T, 1, 8, 2>), grid, dim3(512), 0, s, a, vec);
+  else hipLaunchKernelGGL((i8_rows<T, 1, 8, 4>), grid, dim3(512), 0, s, a, vec);
+}
+
+template <typename T>
+bool launch_i8_mm(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
+  const auto& a = *static_cast<const hrt_i8_mm_args*>(pp);
+  if (a.M <= 0 || a.N <= 0 || a.K <= 0) return ctx.fail("empty product");
+  if (a.K % 16 != 0 || a.K > 131056) return ctx.fail("K must be a multiple of 16 and at most 131056");
+  if (a.x_sm < 0 || a.x_sm % 16 != 0 || a.w_sn < 0 || a.w_sn % 16 != 0) return ctx.fail("row strides must be non-negative multiples of 16");
+  if (a.x % 16 != 0 || a.w % 16 != 0 || a.x_scale % 4 != 0 || a.w_scale % 4 != 0 || a.y % 2 != 0 || a.bias % 2 != 0)
+    return ctx.fail("x and w must be 16-byte aligned, scales 4-byte aligned");
+  const int64_t xs[2] = {a.M, a.K}, xt[2] = {a.x_sm, 1}, wz[2] = {a.N, a.K}, wt[2] = {a.w_sn, 1};
+  if (!ctx.check(a.x, hrt::span_bytes(2, xs, xt, 1), "x") || !ctx.check(a.w, hrt::span_bytes(2, wz, wt, 1), "w") ||
+      !ctx.check(a.x_scale, (uint64_t)a.M * 4, "x_scale") || !ctx.check(a.w_scale, (uint64_t)a.N * 4, "w_scale") ||
+      !ctx.check(a.y, (uint64_t)(a.M * a.N) * 2, "y") || (a.bias && !ctx.check(a.bias, (uint64_t)a.N * 2, "bias")))
+    return false;
+  // offsets of a tile's rows are 31-bit
+  const int64_t lim = (int64_t)1 << 31;
+  if (a.x_sm * 257 >= lim || a.w_sn * 257 >= lim) return ctx.fail("operand rows too long for one launch");
+  const int tile = plan_of(a);
+  if (!hrt::grid_fits(tile < 0 ? cdiv(a.N, 16) : tiles_of(a, tile), 512)) return ctx.fail("grid too large");
+  queue_mm<T>(a, tile, ctx.stream);
+  return hrt::launch_ok(hipGetLastError(), ctx, "i8_mm");
+}
+
+HRT_REGISTER("i8_mm_bf16", hrt_i8_mm_args, launch_i8_mm<BF16>);
+HRT_REGISTER("i8_mm_f16", hrt_i8_mm_args, launch_i8_mm<F16>);
+
+}  // namespace
+}  // namespace hk

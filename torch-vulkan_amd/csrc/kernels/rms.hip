@@ -1,0 +1,583 @@
+// Root-mean-square norm of rows, forward ("rms_fwd_*") and backward ("rms_bwd_*"), and 8-bit rows ("i8_rows_quant_*",
+// "i8_rows_dequant_*").
+//
+// Bound by memory: a row is read once, held in registers as fp32 and written once.  16, 64 or 256 lanes share a row (heads,
+// model widths, wide rows or few of them), which DPP steps and lane swaps add up without LDS, or through four floats of it.
+// Rows longer than a workgroup's registers take several passes.
+#include <initializer_list>
+
+#include "../hrt/registry.h"
+#include "row_vec.h"
+
+namespace hk {
+namespace {
+
+__device__ __forceinline__ int64_t row_at(int64_t row, int64_t n1, int64_t n2, const int64_t* s) {
+  if (n1 * n2 == 1) return row * s[0];
+  const uint32_t r = (uint32_t)row, t = r / (uint32_t)n2, i0 = t / (uint32_t)n1;  // rows < 2^31
+  return (int64_t)i0 * s[0] + (int64_t)(t - i0 * (uint32_t)n1) * s[1] + (int64_t)(r - t * (uint32_t)n2) * s[2];
+}
+
+enum Mode { kNorm, kNorm8, kQuant };
+
+// kQuant reads rows x (stride xs[0]) and writes codes (pitch r, a plain number there) and scales; its arguments come in the same
+// block, so that one kernel serves all three.
+template <typename T, int MODE, int LPR, int NV, bool TAIL>
+__global__ __launch_bounds__(256) void rms_rows(hrt_rms_args p, int64_t q_sr) {
+  using R = RowVec<T>;
+  using S = typename T::storage;
+  constexpr int V = R::V, RPB = 256 / LPR;
+  __shared__ float red[4];
+  __shared__ uint32_t redu[4];
+  const int lane = threadIdx.x % LPR;
+  const int64_t row0 = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
+  const bool live = row0 < p.rows;
+  const int64_t row = live ? row0 : p.rows - 1;  // a row past the end repeats the last one and stores nothing
+  const HK_G S* const x = gcptr<S>(p.x) + (MODE == kQuant ? row * p.xs[0] : row_at(row, p.n1, p.n2, p.xs));
+  u32x4 a[NV], b[NV], w[NV];
+  const bool res = MODE != kQuant && p.r, has_w = MODE != kQuant && p.w;
+#pragma unroll
+  for (int c = 0; c < NV; ++c) a[c] = row_piece<T, TAIL>(x, (int64_t)(c * LPR + lane) * V, p.D);
+  if (res) {
+    const HK_G S* const r = gcptr<S>(p.r) + row_at(row, p.n1, p.n2, p.rs);
+#pragma unroll
+    for (int c = 0; c < NV; ++c) b[c] = row_piece<T, TAIL>(r, (int64_t)(c * LPR + lane) * V, p.D);
+  }
+  if (has_w) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) w[c] = row_piece<T, TAIL>(gcptr<S>(p.w), (int64_t)(c * LPR + lane) * V, p.D);
+  }
+  float v[NV][V];
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int64_t col = (int64_t)(c * LPR + lane) * V;
+    R::unpack(a[c], v[c]);
+    if (res) {
+      float t[V];
+      R::unpack(b[c], t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[c][e] += t[e];
+      if (p.h_out && live) row_put<T, TAIL>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v[c]));
+    }
+    if (!TAIL && col >= p.D) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[c][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) ss = fmaf(v[c][e], v[c][e], ss);
+  }
+  if constexpr (MODE != kQuant) {
+    const float rstd = 1.f / sqrtf(lanes_sum<LPR>(ss, red) / (float)p.D + p.eps);
+    if (p.rstd && live && lane == 0) gptr<float>(p.rstd)[row] = rstd;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      float t[V];
+      if (has_w) R::unpack(w[c], t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[c][e] = has_w ? v[c][e] * rstd * t[e] : v[c][e] * rstd;
+    }
+  }
+  if constexpr (MODE == kNorm) {
+    if (!live) return;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) row_put<T, TAIL>(gptr<S>(p.y) + row * p.D, (int64_t)(c * LPR + lane) * V, p.D, R::pack(v[c]));
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      // lanes past the row hold zeros, but zero times an infinite rstd or weight is no zero
+      const int64_t col = (int64_t)(c * LPR + lane) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint32_t m = __float_as_uint(v[c][e]) & 0x7fffffffu;
+        if ((TAIL ? col + e < p.D : col < p.D) && m > top) top = m;
+      }
+    }
+    const RowCode code(lanes_max<LPR>(top, redu));
+    if (!live) return;
+    if (lane == 0) gptr<float>(p.scale)[row] = code.scale;
+    HK_G uint8_t* const q = gptr<uint8_t>(p.q) + row * q_sr;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int64_t col = (int64_t)(c * LPR + lane) * V;
+      if (col >= q_sr) continue;
+      int k[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        k[e] = MODE == kQuant ? nearest_code<T>(v[c][e], code) : code_of(v[c][e], code);
+        if (TAIL && col + e >= p.D) k[e] = 0;
+      }
+      if (col + V <= q_sr) {
+        typedef uint32_t __attribute__((aligned(1))) u32_any;
+        typedef u32x2 __attribute__((aligned(1))) u32x2_any;
+        if constexpr (V == 8) *reinterpret_cast<HK_G u32x2_any*>(q + col) = u32x2{pack_codes4(k), pack_codes4(k + 4)};
+        else *reinterpret_cast<HK_G u32_any*>(q + col) = pack_codes4(k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (col + e < q_sr) q[col + e] = (uint8_t)k[e];
+      }
+    }
+  }
+}
+
+// Rows longer than a workgroup's registers: a workgroup a row, passes over it (the later ones read it from L2).
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void rms_long(hrt_rms_args p, int64_t q_sr) {
+  using R = RowVec<T>;
+  using S = typename T::storage;
+  constexpr int V = R::V;
+  __shared__ float red[4];
+  __shared__ uint32_t redu[4];
+  const int64_t row = blockIdx.x;
+  const HK_G S* const x = gcptr<S>(p.x) + (MODE == kQuant ? row * p.xs[0] : row_at(row, p.n1, p.n2, p.xs));
+  const HK_G S* const r = MODE != kQuant && p.r ? gcptr<S>(p.r) + row_at(row, p.n1, p.n2, p.rs) : nullptr;
+  auto load = [&](int64_t col, float* v) {
+    R::unpack(row_piece<T, true>(x, col, p.D), v);
+    if (r) {
+      float t[V];
+      R::unpack(row_piece<T, true>(r, col, p.D), t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += t[e];
+    }
+  };
+  float rstd = 1.f;
+  if constexpr (MODE != kQuant) {
+    float ss = 0.f;
+    for (int64_t col = threadIdx.x * V; col < p.D; col += 256 * V) {
+      float v[V];
+      load(col, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss = fmaf(v[e], v[e], ss);
+      if (r && p.h_out) row_put<T, true>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v));
+    }
+    rstd = 1.f / sqrtf(lanes_sum<256>(ss, red) / (float)p.D + p.eps);
+    if (p.rstd && threadIdx.x == 0) gptr<float>(p.rstd)[row] = rstd;
+  }
+  auto norm = [&](int64_t col, float* v) {
+    load(col, v);
+    if constexpr (MODE == kQuant) return;
+    float t[V];
+    if (p.w) R::unpack(row_piece<T, true>(gcptr<S>(p.w), col, p.D), t);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = p.w ? v[e] * rstd * t[e] : v[e] * rstd;
+  };
+  if constexpr (MODE == kNorm) {
+    for (int64_t col = threadIdx.x * V; col < p.D; col += 256 * V) {
+      float v[V];
+      norm(col, v);
+      row_put<T, true>(gptr<S>(p.y) + row * p.D, col, p.D, R::pack(v));
+    }
+  } else {
+    uint32_t top = 0;
+    for (int64_t col = threadIdx.x * V; col < p.D; col += 256 * V) {
+      float v[V];
+      norm(col, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+        if (col + e < p.D && m > top) top = m;
+      }
+    }
+    const RowCode code(lanes_max<256>(top, redu));
+    if (threadIdx.x == 0) gptr<float>(p.scale)[row] = code.scale;
+    HK_G uint8_t* const q = gptr<uint8_t>(p.q) + row * q_sr;
+    for (int64_t col = threadIdx.x * V; col < q_sr; col += 256 * V) {
+      float v[V];
+      norm(col, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (col + e < q_sr) q[col + e] = col + e < p.D ? (uint8_t)(MODE == kQuant ? nearest_code<T>(v[e], code) : code_of(v[e], code)) : 0;
+    }
+  }
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------
+// A workgroup takes `per` consecutive rows, 256 / LPR at a time.  DW: a lane adds gy n of its columns up over its rows, the
+// workgroup's lanes of a column are added in order through LDS, and the sums of all workgroups by rms_dw_sum.
+template <typename T, int LPR, int NV, bool TAIL, bool DW>
+__global__ __launch_bounds__(256) void rms_back(hrt_rms_bwd_args p, int64_t per) {
+  using R = RowVec<T>;
+  using S = typename T::storage;
+  constexpr int V = R::V, RPB = 256 / LPR;
+  __shared__ float red[2][4];
+  __shared__ __attribute__((aligned(16))) float part[DW && RPB > 1 ? RPB * LPR * NV * V : 4];
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  const int64_t first = (int64_t)blockIdx.x * per, end = first + per < p.rows ? first + per : p.rows;
+  float acc[NV][V];
+  u32x4 w[NV];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    w[c] = u32x4{0, 0, 0, 0};
+    if (p.w) w[c] = row_piece<T, TAIL>(gcptr<S>(p.w), (int64_t)(c * LPR + lane) * V, p.D);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[c][e] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t base = first; base < end; base += RPB, turn ^= 1) {
+    const bool live = base + group < end;
+    const int64_t row = live ? base + group : end - 1;
+    const HK_G S* const gy = gcptr<S>(p.gy) + (p.gy ? row_at(row, p.n1, p.n2, p.gys) : 0);
+    const HK_G S* const h = gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs);
+    u32x4 a[NV], b[NV], g[NV];
+    const float rstd = gcptr<float>(p.rstd)[row];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int64_t col = (int64_t)(c * LPR + lane) * V;
+      a[c] = g[c] = u32x4{0, 0, 0, 0};
+      b[c] = row_piece<T, TAIL>(h, col, p.D);
+      if (p.gy) a[c] = row_piece<T, TAIL>(gy, col, p.D);
+    }
+    if (p.gh) {
+      const HK_G S* const gh = gcptr<S>(p.gh) + row_at(row, p.n1, p.n2, p.ghs);
+#pragma unroll
+      for (int c = 0; c < NV; ++c) g[c] = row_piece<T, TAIL>(gh, (int64_t)(c * LPR + lane) * V, p.D);
+    }
+    float d[NV][V], n[NV][V];
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int64_t col = (int64_t)(c * LPR + lane) * V;
+      if (!live || (!TAIL && col >= p.D)) a[c] = u32x4{0, 0, 0, 0}, b[c] = u32x4{0, 0, 0, 0};
+      float t[V];
+      R::unpack(a[c], d[c]);
+      R::unpack(b[c], n[c]);
+      if (p.w) R::unpack(w[c], t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        n[c][e] *= rstd;
+        if constexpr (DW) acc[c][e] += !TAIL || col + e < p.D ? (live && col < p.D ? d[c][e] * n[c][e] : 0.f) : 0.f;
+        if (p.w) d[c][e] *= t[e];
+        if (TAIL ? col + e < p.D : col < p.D) dot = fmaf(d[c][e], n[c][e], dot);
+      }
+    }
+    dot = lanes_sum<LPR>(dot, red[turn]) / (float)p.D;
+    if (!p.dx || !live) continue;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      float t[V];
+      R::unpack(g[c], t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[e] = fmaf(rstd, fmaf(-n[c][e], dot, d[c][e]), t[e]);
+      row_put<T, TAIL>(gptr<S>(p.dx) + row * p.D, (int64_t)(c * LPR + lane) * V, p.D, R::pack(t));
+    }
+  }
+  if constexpr (DW) {
+    HK_G float* const ws = gptr<float>(p.ws) + (int64_t)blockIdx.x * p.D;
+    if constexpr (RPB == 1) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if ((int64_t)(c * LPR + lane) * V + e < p.D) ws[(c * LPR + lane) * V + e] = acc[c][e];
+    } else {
+      constexpr int W = LPR * NV * V;
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+          *reinterpret_cast<f32x4*>(part + group * W + (c * LPR + lane) * V + e) = f32x4{acc[c][e], acc[c][e + 1], acc[c][e + 2], acc[c][e + 3]};
+      __syncthreads();
+      for (int i = threadIdx.x; i < p.D; i += 256) {
+        float t = part[i];
+#pragma unroll
+        for (int k = 1; k < RPB; ++k) t += part[k * W + i];
+        ws[i] = t;
+      }
+    }
+  }
+}
+
+// Rows longer than a workgroup's registers; ws is added to in place, each column by its own thread.
+template <typename T>
+__global__ __launch_bounds__(256) void rms_back_long(hrt_rms_bwd_args p, int64_t per) {
+  using R = RowVec<T>;
+  using S = typename T::storage;
+  constexpr int V = R::V;
+  __shared__ float red[2][4];
+  const int64_t first = (int64_t)blockIdx.x * per, end = first + per < p.rows ? first + per : p.rows;
+  HK_G float* const ws = gptr<float>(p.ws) + (int64_t)blockIdx.x * p.D;
+  for (int64_t row = first; row < end; ++row) {
+    const HK_G S* const gy = gcptr<S>(p.gy) + (p.gy ? row_at(row, p.n1, p.n2, p.gys) : 0);
+    const HK_G S* const h = gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs);
+    const HK_G S* const gh = gcptr<S>(p.gh) + (p.gh ? row_at(row, p.n1, p.n2, p.ghs) : 0);
+    const float rstd = gcptr<float>(p.rstd)[row];
+    auto load = [&](int64_t col, float* d, float* n, float* gyn) {
+      float t[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = 0.f, t[e] = 1.f;
+      if (p.gy) R::unpack(row_piece<T, true>(gy, col, p.D), d);
+      R::unpack(row_piece<T, true>(h, col, p.D), n);
+      if (p.w) R::unpack(row_piece<T, true>(gcptr<S>(p.w), col, p.D), t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) n[e] *= rstd, gyn[e] = d[e] * n[e], d[e] *= t[e];
+    };
+    float dot = 0.f;
+    for (int64_t col = threadIdx.x * V; col < p.D; col += 256 * V) {
+      float d[V], n[V], gyn[V];
+      load(col, d, n, gyn);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (col + e < p.D) {
+          dot = fmaf(d[e], n[e], dot);
+          if (p.dw) ws[col + e] = row == first ? gyn[e] : ws[col + e] + gyn[e];
+        }
+    }
+    dot = lanes_sum<256>(dot, red[row & 1]) / (float)p.D;
+    if (!p.dx) continue;
+    for (int64_t col = threadIdx.x * V; col < p.D; col += 256 * V) {
+      float d[V], n[V], t[V];
+      load(col, d, n, t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[e] = 0.f;
+      if (p.gh) R::unpack(row_piece<T, true>(gh, col, p.D), t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[e] = fmaf(rstd, fmaf(-n[e], dot, d[e]), t[e]);
+      row_put<T, true>(gptr<S>(p.dx) + row * p.D, col, p.D, R::pack(t));
+    }
+  }
+}
+
+// dw: the workgroups' sums of 32 columns, a thread every 32nd of them in order, then the 32 of a column in order.
+template <typename T>
+__global__ __launch_bounds__(256) void rms_dw_sum(const float* ws, typename T::storage* dw, int64_t parts, int64_t D) {
+  __shared__ float red[32][33];
+  const int quad = threadIdx.x & 7, group = threadIdx.x >> 3;
+  const int64_t col = (int64_t)blockIdx.x * 32 + quad * 4;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t c = group; c < parts; c += 32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += col + e < D ? ws[c * D + col + e] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) red[group][quad * 4 + e] = s[e];
+  __syncthreads();
+  const int64_t at = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x >= 32 || at >= D) return;
+  float t = red[0][threadIdx.x];
+#pragma unroll
+  for (int k = 1; k < 32; ++k) t += red[k][threadIdx.x];
+  dw[at] = T::from_f32(t);
+}
+
+// ---- 8-bit rows back to values ----------------------------------------------------------------------------------------------
+// 16 codes a lane; a workgroup takes whole rows, several where they are short.
+template <typename T>
+__global__ __launch_bounds__(256) void i8_dequant(hrt_i8_rows_args p, int lpr) {
+  using R = RowVec<T>;
+  using S = typename T::storage;
+  constexpr int V = R::V;
+  const int per = 256 / lpr;
+  const int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / lpr;
+  if ((int)threadIdx.x >= per * lpr || row >= p.rows) return;
+  const float s = gcptr<float>(p.scale)[row];
+  const HK_G uint8_t* const q = gcptr<uint8_t>(p.q) + row * p.q_sr;
+  HK_G S* const x = gptr<S>(p.x) + row * p.x_sr;
+  for (int64_t col = (int64_t)(threadIdx.x % lpr) * 16; col < p.cols; col += (int64_t)lpr * 16) {
+    if (col + 16 <= p.cols) {
+      typedef u32x4 __attribute__((aligned(1))) any1;
+      const u32x4 c = *reinterpret_cast<const HK_G any1*>(q + col);
+#pragma unroll
+      for (int i = 0; i < 16; i += V) {
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (float)(int8_t)(c[(i + e) >> 2] >> (8 * (e & 3))) * s;
+        R::put(x + col + i, R::pack(v));
+      }
+    } else {
+      for (int64_t e = col; e < p.cols; ++e) x[e] = T::from_f32((float)(int8_t)q[e] * s);
+    }
+  }
+}
+
+// ---- plan and launch --------------------------------------------------------------------------------------------------------
+// Lanes per row and pieces per lane; 0: the passes.  Few rows of model width are shared by a workgroup: its four wavefronts'
+// loads are all in flight at once.
+struct Share {
+  int lpr, nv;
+};
+Share share_of(int64_t rows, int64_t D, int V) {
+  const int64_t n = cdiv(D, V);
+  if (n <= 16) return {16, 1};
+  if (n <= 32) return {16, 2};
+  if (n <= 64) return {64, 1};
+  if (n <= 128) return {64, 2};
+  if (n <= 256) return rows >= 1024 ? Share{64, 4} : Share{256, 1};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {256, 4};
+  return {0, 0};
+}
+
+template <typename F>
+void with_share(Share s, F f) {
+#define HK_SHARE(L, N) \
+  if (s.lpr == L && s.nv == N) return f(std::integral_constant<int, L>(), std::integral_constant<int, N>())
+  HK_SHARE(16, 1);
+  HK_SHARE(16, 2);
+  HK_SHARE(64, 1);
+  HK_SHARE(64, 2);
+  HK_SHARE(64, 4);
+  HK_SHARE(256, 1);
+  HK_SHARE(256, 2);
+  HK_SHARE(256, 4);
+#undef HK_SHARE
+}
+
+template <typename T, int MODE>
+bool queue_rows(const hrt_rms_args& a, int64_t q_sr, hrt::LaunchCtx& ctx) {
+  constexpr int V = RowVec<T>::V;
+  const Share s = share_of(a.rows, a.D, V);
+  if (s.lpr == 0) {
+    if (!hrt::grid_fits(a.rows, 256)) return ctx.fail("grid too large");
+    hipLaunchKernelGGL((rms_long<T, MODE>), dim3((uint32_t)a.rows), dim3(256), 0, ctx.stream, a, q_sr);
+    return true;
+  }
+  const int64_t blocks = cdiv(a.rows, 256 / s.lpr);
+  if (!hrt::grid_fits(blocks, 256)) return ctx.fail("grid too large");
+  with_share(s, [&](auto lc, auto nc) {
+    constexpr int L = decltype(lc)::value, N = decltype(nc)::value;
+    if (a.D % V == 0) hipLaunchKernelGGL((rms_rows<T, MODE, L, N, false>), dim3((uint32_t)blocks), dim3(256), 0, ctx.stream, a, q_sr);
+    else hipLaunchKernelGGL((rms_rows<T, MODE, L, N, true>), dim3((uint32_t)blocks), dim3(256), 0, ctx.stream, a, q_sr);
+  });
+  return true;
+}
+
+// Byte extent of rows reached through three outer dimensions.
+uint64_t rows_span(int64_t rows, int64_t n1, int64_t n2, int64_t D, const int64_t* s, uint64_t elem) {
+  const int64_t n0 = cdiv(rows, n1 * n2);
+  return uint64_t((n0 - 1) * s[0] + (n1 - 1) * s[1] + (n2 - 1) * s[2] + D) * elem;
+}
+bool rows_ok(int64_t rows, int64_t D, int64_t n1, int64_t n2, std::initializer_list<const int64_t*> strides, uint64_t elem,
+             std::initializer_list<uint64_t> addrs, hrt::LaunchCtx& ctx) {
+  if (rows <= 0 || D <= 0 || n1 <= 0 || n2 <= 0 || rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 31) || rows % (n1 * n2) != 0)
+    return ctx.fail("bad shape");
+  for (const int64_t* s : strides)
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0) return ctx.fail("negative stride");
+  for (const uint64_t p : addrs)
+    if (p % elem != 0) return ctx.fail("operands must be aligned to their elements");
+  return true;
+}
+
+template <typename T>
+bool launch_rms_fwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
+  const auto& a = *static_cast<const hrt_rms_args*>(pp);
+  using S = typename T::storage;
+  constexpr uint64_t E = sizeof(S);
+  if (!rows_ok(a.rows, a.D, a.n1, a.n2, {a.xs, a.rs}, E, {a.x, a.r, a.w, a.y, a.h_out}, ctx)) return false;
+  if (a.scale % 4 != 0 || a.rstd % 4 != 0) return ctx.fail("scale and rstd must be 4-byte aligned");
+  if ((a.q != 0) != (a.scale != 0) || (a.q != 0) == (a.y != 0)) return ctx.fail("either y, or q and scale");
+  const uint64_t n = (uint64_t)a.rows * a.D;
+  if (!ctx.check(a.x, rows_span(a.rows, a.n1, a.n2, a.D, a.xs, E), "x") ||
+      (a.r && !ctx.check(a.r, rows_span(a.rows, a.n1, a.n2, a.D, a.rs, E), "r")) || (a.w && !ctx.check(a.w, a.D * E, "w")) ||
+      (a.y && !ctx.check(a.y, n * E, "y")) || (a.h_out && !ctx.check(a.h_out, n * E, "h_out")) || (a.q && !ctx.check(a.q, n, "q")) ||
+      (a.scale && !ctx.check(a.scale, a.rows * 4, "scale")) || (a.rstd && !ctx.check(a.rstd, a.rows * 4, "rstd")))
+    return false;
+  if (!(a.q ? queue_rows<T, kNorm8>(a, a.D, ctx) : queue_rows<T, kNorm>(a, a.D, ctx))) return false;
+  return hrt::launch_ok(hipGetLastError(), ctx, "rms_fwd");
+}
+
+template <typename T>
+bool launch_quant(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
+  const auto& a = *static_cast<const hrt_i8_rows_args*>(pp);
+  constexpr uint64_t E = sizeof(typename T::storage);
+  const int64_t s[3] = {a.x_sr, 0, 0};
+  if (!rows_ok(a.rows, a.cols, 1, 1, {s}, E, {a.x}, ctx)) return false;
+  // the lanes of a row cover a multiple of 16 columns: those that follow the row become 0 without a pass of their own
+  if (a.q_sr < a.cols || a.q_sr > cdiv(a.cols, 16) * 16 || a.scale % 4 != 0) return ctx.fail("bad pitch of q or alignment of scale");
+  const int64_t qt[2] = {a.q_sr, 1}, sz[2] = {a.rows, a.q_sr};
+  if (!ctx.check(a.x, rows_span(a.rows, 1, 1, a.cols, s, E), "x") || !ctx.check(a.q, hrt::span_bytes(2, sz, qt, 1), "q") ||
+      !ctx.check(a.scale, a.rows * 4, "scale"))
+    return false;
+  hrt_rms_args r{};
+  r.x = a.x, r.q = a.q, r.scale = a.scale, r.rows = a.rows, r.D = a.cols, r.n1 = r.n2 = 1, r.xs[0] = a.x_sr;
+  if (!queue_rows<T, kQuant>(r, a.q_sr, ctx)) return false;
+  return hrt::launch_ok(hipGetLastError(), ctx, "i8_rows_quant");
+}
+
+template <typename T>
+bool launch_dequant(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
+  const auto& a = *static_cast<const hrt_i8_rows_args*>(pp);
+  constexpr uint64_t E = sizeof(typename T::storage);
+  const int64_t s[3] = {a.x_sr, 0, 0}, qs[3] = {a.q_sr, 0, 0};
+  if (!rows_ok(a.rows, a.cols, 1, 1, {s, qs}, E, {a.x}, ctx)) return false;
+  if (a.scale % 4 != 0 || a.x_sr < a.cols) return ctx.fail("overlapping rows of x, or scale not 4-byte aligned");
+  if (!ctx.check(a.x, rows_span(a.rows, 1, 1, a.cols, s, E), "x") || !ctx.check(a.q, rows_span(a.rows, 1, 1, a.cols, qs, 1), "q") ||
+      !ctx.check(a.scale, a.rows * 4, "scale"))
+    return false;
+  const int64_t pieces = cdiv(a.cols, 16);
+  const int lpr = pieces < 256 ? (int)pieces : 256;
+  const int64_t blocks = cdiv(a.rows, 256 / lpr);
+  if (!hrt::grid_fits(blocks, 256)) return ctx.fail("grid too large");
+  hipLaunchKernelGGL(i8_dequant<T>, dim3((uint32_t)blocks), dim3(256), 0, ctx.stream, a, lpr);
+  return hrt::launch_ok(hipGetLastError(), ctx, "i8_rows_dequant");
+}
+
+// Rows per workgroup of the backward: with dw as many as leave 512 workgroups.
+int64_t back_rows(const hrt_rms_bwd_args& a, Share s) {
+  const int64_t rpb = s.lpr ? 256 / s.lpr : 1;
+  return a.dw ? cdiv(cdiv(a.rows, 512), rpb) * rpb : rpb;
+}
+template <typename T>
+int64_t back_blocks(const hrt_rms_bwd_args& a) {
+  return cdiv(a.rows, back_rows(a, share_of(a.rows, a.D, RowVec<T>::V)));
+}
+
+template <typename T>
+bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
+  const auto& a = *static_cast<const hrt_rms_bwd_args*>(pp);
+  using S = typename T::storage;
+  constexpr uint64_t E = sizeof(S);
+  constexpr int V = RowVec<T>::V;
+  if (!rows_ok(a.rows, a.D, a.n1, a.n2, {a.gys, a.ghs, a.hs}, E, {a.gy, a.gh, a.h, a.w, a.dx, a.dw}, ctx)) return false;
+  if (a.rstd % 4 != 0 || a.ws % 4 != 0) return ctx.fail("rstd and ws must be 4-byte aligned");
+  if (!a.dx && !a.dw) return true;
+  const uint64_t n = (uint64_t)a.rows * a.D;
+  const int64_t blocks = back_blocks<T>(a);
+  if ((a.gy && !ctx.check(a.gy, rows_span(a.rows, a.n1, a.n2, a.D, a.gys, E), "gy")) ||
+      (a.gh && !ctx.check(a.gh, rows_span(a.rows, a.n1, a.n2, a.D, a.ghs, E), "gh")) ||
+      !ctx.check(a.h, rows_span(a.rows, a.n1, a.n2, a.D, a.hs, E), "h") || !ctx.check(a.rstd, a.rows * 4, "rstd") ||
+      (a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
+      (a.dw && (!ctx.check(a.dw, a.D * E, "dw") || !ctx.check(a.ws, (uint64_t)(blocks * a.D) * 4, "ws"))))
+    return false;
+  if (!hrt::grid_fits(blocks, 256)) return ctx.fail("grid too large");
+  const Share s = share_of(a.rows, a.D, V);
+  const int64_t per = back_rows(a, s);
+  const dim3 grid((uint32_t)blocks);
+  if (s.lpr == 0) {
+    hipLaunchKernelGGL(rms_back_long<T>, grid, dim3(256), 0, ctx.stream, a, per);
+  } else {
+    with_share(s, [&](auto lc, auto nc) {
+      constexpr int L = decltype(lc)::value, N = decltype(nc)::value;
+      const auto go = [&](auto tail, auto dw) {
+        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value>), grid, dim3(256), 0, ctx.stream, a, per);
+      };
+      using Y = std::true_type;
+      using No = std::false_type;
+      if (a.D % V == 0) a.dw ? go(No(), Y()) : go(No(), No());
+      else a.dw ? go(Y(), Y()) : go(Y(), No());
+    });
+  }
+  if (a.dw)
+    hipLaunchKernelGGL(rms_dw_sum<T>, dim3((uint32_t)cdiv(a.D, 32)), dim3(256), 0, ctx.stream, (const float*)a.ws, (S*)a.dw, blocks, a.D);
+  return hrt::launch_ok(hipGetLastError(), ctx, "rms_bwd");
+}
+
+#define HK_ROWS(SUFFIX, T)                                               \
+  HRT_REGISTER("rms_fwd_" SUFFIX, hrt_rms_args, launch_rms_fwd<T>);      \
+  HRT_REGISTER("rms_bwd_" SUFFIX, hrt_rms_bwd_args, launch_rms_bwd<T>);  \
+  HRT_REGISTER("i8_rows_quant_" SUFFIX, hrt_i8_rows_args, launch_quant<T>); \
+  HRT_REGISTER("i8_rows_dequant_" SUFFIX, hrt_i8_rows_args, launch_dequant<T>)
+HK_ROWS("f32", F32);
+HK_ROWS("bf16", BF16);
+HK_ROWS("f16", F16);
+
+}  // namespace
+}  // namespace hk
+
+extern "C" int64_t hrt_rms_workspace(const hrt_rms_bwd_args* a, int32_t dtype) {
+  using namespace hk;
+  if (!a || a->rows <= 0 || a->D <= 0 || !a->dw) return 0;
+  return (dtype == HRT_F32 ? back_blocks<F32>(*a) : back_blocks<BF16>(*a)) * a->D;
+}

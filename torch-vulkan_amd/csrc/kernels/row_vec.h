@@ -1,0 +1,152 @@
+// Rows of any length and alignment in 16-byte pieces, and sums and maxima over the lanes that share a row.
+//
+// gfx950 reads and writes 16 bytes at any address that suits the element type, so rows of odd length need no path of their
+// own: only the piece that a row ends in is touched element by element.
+#pragma once
+
+#include "mfma_common.h"
+
+namespace hk {
+
+typedef u32x4 __attribute__((aligned(2))) u32x4_any2;
+typedef u32x4 __attribute__((aligned(4))) u32x4_any4;
+
+// V values of type T in 16 bytes.
+template <typename T>
+struct RowVec {
+  using S = typename T::storage;
+  static constexpr int V = 16 / (int)sizeof(S);
+  using Any = typename std::conditional<sizeof(S) == 2, u32x4_any2, u32x4_any4>::type;
+
+  __device__ __forceinline__ static void unpack(u32x4 w, float* v) {
+    if constexpr (V == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(w[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[2 * e] = lo16<T>(w[e]), v[2 * e + 1] = hi16<T>(w[e]);
+    }
+  }
+  __device__ __forceinline__ static u32x4 pack(const float* v) {
+    if constexpr (V == 4) return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    else return pack8<T>(v);
+  }
+  __device__ __forceinline__ static u32x4 get(const HK_G S* p) { return *reinterpret_cast<const HK_G Any*>(p); }
+  __device__ __forceinline__ static void put(HK_G S* p, u32x4 w) { *reinterpret_cast<HK_G Any*>(p) = w; }
+  // The first n values (0 < n < V), zeros behind them.
+  __device__ __forceinline__ static u32x4 get_some(const HK_G S* p, int n) {
+    u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < n) {
+        if constexpr (V == 4) w[e] = __float_as_uint(p[e]);
+        else w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+      }
+    return w;
+  }
+  __device__ __forceinline__ static void put_some(HK_G S* p, u32x4 w, int n) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < n) {
+        if constexpr (V == 4) p[e] = __uint_as_float(w[e]);
+        else p[e] = (S)(w[e >> 1] >> (16 * (e & 1)));
+      }
+  }
+};
+
+// Piece `col` of a row of D values; TAIL: rows end inside a piece.  Lanes past the row get zeros; without TAIL they load the row's
+// last piece instead of branching (D >= V then), so that every load of a row is in flight before the first is used.
+template <typename T, bool TAIL>
+__device__ __forceinline__ u32x4 row_piece(const HK_G typename T::storage* row, int64_t col, int64_t D) {
+  constexpr int V = RowVec<T>::V;
+  if constexpr (!TAIL) return RowVec<T>::get(row + (col < D ? col : D - V));
+  if (col + V <= D) return RowVec<T>::get(row + col);
+  if (col < D) return RowVec<T>::get_some(row + col, (int)(D - col));
+  return u32x4{0, 0, 0, 0};
+}
+template <typename T, bool TAIL>
+__device__ __forceinline__ void row_put(HK_G typename T::storage* row, int64_t col, int64_t D, u32x4 w) {
+  constexpr int V = RowVec<T>::V;
+  if (!TAIL ? col < D : col + V <= D) RowVec<T>::put(row + col, w);
+  else if (TAIL && col < D) RowVec<T>::put_some(row + col, w, (int)(D - col));
+}
+
+// Sum over the LPR lanes (16 or 64) that share a row, or over a workgroup of 256 through `red` (four floats, not those of the
+// call before); the same bits in every lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+  return v > o ? v : o;
+}
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v, float* red) {
+  static_assert(LPR == 16 || LPR == 64 || LPR == 256, "lanes per row");
+  if constexpr (LPR == 16) {
+    v = dpp_add<0xB1>(v), v = dpp_add<0x4E>(v), v = dpp_add<0x141>(v), v = dpp_add<0x140>(v);
+    return v;
+  }
+  v = wave_sum_dpp(v);
+  if constexpr (LPR == 256) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (red[0] + red[1]) + (red[2] + red[3]);
+  }
+  return v;
+}
+// Largest magnitude, by the bits without sign: a NaN is larger than an infinity.
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, uint32_t* red) {
+  v = dpp_max_u32<0xB1>(v), v = dpp_max_u32<0x4E>(v), v = dpp_max_u32<0x141>(v), v = dpp_max_u32<0x140>(v);
+  if constexpr (LPR >= 64) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = a[0] > a[1] ? a[0] : a[1];
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = b[0] > b[1] ? b[0] : b[1];
+  }
+  if constexpr (LPR == 256) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const uint32_t a = red[0] > red[1] ? red[0] : red[1], b = red[2] > red[3] ? red[2] : red[3];
+    v = a > b ? a : b;
+  }
+  return v;
+}
+
+// ---- 8-bit rows -----------------------------------------------------------------------------------------------------------
+// A row's values are code * scale with scale = top / 127, top the row's largest magnitude, and code the whole number nearest to
+// 127 v / top (ties to even).  scale is rounded to nearest, but stays where 127 scale is finite.  A row of zeros has scale 0, one with an infinity or NaN scale NaN and codes 0.
+struct RowCode {
+  float mul, top, per, scale;  // v * mul and top are in a range where 127 / top = per is an ordinary number
+  __device__ __forceinline__ explicit RowCode(uint32_t bits) {
+    const float t = __uint_as_float(bits);
+    mul = bits < 0x0d800000u /* 2^-100 */ ? 0x1p64f : bits > 0x71800000u /* 2^100 */ ? 0x1p-64f : 1.f;
+    if (bits >= 0x7f800000u) {
+      mul = top = per = 0.f, scale = __uint_as_float(0x7fc00000u);
+    } else {
+      top = t * mul, per = bits ? 127.f / top : 0.f;
+      scale = fminf(t / 127.f, 0x1.020406p+121f);  // 127 of the largest step that is taken are finite
+    }
+  }
+};
+// Codes of fp32 values that are roundings themselves: the quotient as it comes out.
+__device__ __forceinline__ int code_of(float v, const RowCode& r) {
+  const float q = rintf(v * r.mul * r.per);
+  return r.per == 0.f ? 0 : (int)q;
+}
+// The nearest code exactly: the quotient's error is settled by 127 v - q top, which 16-bit values give exactly in fp32 (127 v has 18
+// bits, q top 18, and the difference of neighbours fits 24), 32-bit ones in fp64.
+template <typename T>
+__device__ __forceinline__ int nearest_code(float v, const RowCode& r) {
+  if (r.per == 0.f) return 0;
+  const float x = v * r.mul;
+  int q = (int)rintf(x * r.per);
+  using F = typename std::conditional<std::is_same<T, F32>::value, double, float>::type;
+  const F d = F(127) * F(x) - F(q) * F(r.top), e = d < 0 ? -d : d, twice = e + e;
+  if (twice > F(r.top) || (twice == F(r.top) && (q & 1))) q += d < 0 ? -1 : 1;
+  return q;
+}
+__device__ __forceinline__ uint32_t pack_codes4(const int* q) {
+  return ((uint32_t)q[0] & 255u) | (((uint32_t)q[1] & 255u) << 8) | (((uint32_t)q[2] & 255u) << 16) | ((uint32_t)q[3] << 24);
+}
+
+}  // namespace hk

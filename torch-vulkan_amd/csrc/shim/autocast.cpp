@@ -1,7 +1,7 @@
 // torch.autocast(device_type="vk"): the policy the reference registers (csrc/shim.cpp:376-394), which is
 // CUDA's: products and attention run in the autocast dtype, layer_norm / softmax / mse_loss in fp32,
-// everything else passes through unchanged.  The 4-bit linear layer and attention with a relative position bias, which have no
-// aten schema, follow linear and scaled_dot_product_attention.
+// everything else passes through unchanged.  The 4-bit and 8-bit linear layers, attention with a relative position bias and the
+// root-mean-square norm, which have no aten schema, follow linear, scaled_dot_product_attention and layer_norm.
 #include <ATen/autocast_mode.h>
 #include <torch/library.h>
 
@@ -31,13 +31,34 @@ namespace vkt {
 
 namespace {
 at::Tensor low(const at::Tensor& t) { return at::autocast::cached_cast(at::autocast::get_autocast_dtype(kDev), t, kDev); }
+std::optional<at::Tensor> low(const std::optional<at::Tensor>& t) { return present(t) ? std::optional<at::Tensor>(low(*t)) : std::nullopt; }
+at::Tensor full(const at::Tensor& t) { return at::autocast::cached_cast(at::kFloat, t, kDev); }
+std::optional<at::Tensor> full(const std::optional<at::Tensor>& t) { return present(t) ? std::optional<at::Tensor>(full(*t)) : std::nullopt; }
 }  // namespace
 
 at::Tensor mxfp4_linear_autocast(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scale, const std::optional<at::Tensor>& bias,
                                  bool quantize_input) {
   if (!at::autocast::is_autocast_enabled(kDev)) return mxfp4_linear_vk(x, codes, scale, bias, quantize_input);
   const c10::impl::ExcludeDispatchKeyGuard done(c10::DispatchKey::AutocastPrivateUse1);
-  return mxfp4_linear_vk(low(x), codes, scale, present(bias) ? std::optional<at::Tensor>(low(*bias)) : std::nullopt, quantize_input);
+  return mxfp4_linear_vk(low(x), codes, scale, low(bias), quantize_input);
+}
+
+at::Tensor int8_linear_autocast(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scale, const std::optional<at::Tensor>& bias,
+                                const std::optional<at::Tensor>& x_scale, std::optional<at::ScalarType> out_dtype) {
+  if (!at::autocast::is_autocast_enabled(kDev)) return int8_linear_vk(x, weight, weight_scale, bias, x_scale, out_dtype);
+  const c10::impl::ExcludeDispatchKeyGuard done(c10::DispatchKey::AutocastPrivateUse1);
+  // an int8 x has its output's type named, if any is
+  const at::ScalarType t = x.scalar_type() == at::kChar && out_dtype ? *out_dtype : at::autocast::get_autocast_dtype(kDev);
+  return int8_linear_vk(low(x), weight, weight_scale, present(bias) ? std::optional<at::Tensor>(at::autocast::cached_cast(t, *bias, kDev)) : std::nullopt,
+                        x_scale, t);
+}
+
+std::vector<at::Tensor> rms_norm_autocast(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& residual, double eps,
+                                          bool int8) {
+  const auto norm = int8 ? &rms_norm_int8_vk : &rms_norm_vk;
+  if (!at::autocast::is_autocast_enabled(kDev)) return norm(x, weight, residual, eps);
+  const c10::impl::ExcludeDispatchKeyGuard done(c10::DispatchKey::AutocastPrivateUse1);
+  return norm(full(x), full(weight), full(residual), eps);
 }
 
 at::Tensor relative_bias_attention_autocast(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,

@@ -114,6 +114,28 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           runtime();
           return relative_bias_attention_autocast(q, k, v, table, key_mask, causal, scale, max_distance, query_offset);
         });
+  m.def("quantize_int8_rows", [](const at::Tensor& x) {
+    runtime();
+    return quantize_int8_rows_vk(x);
+  });
+  m.def("dequant_int8_rows", [](const at::Tensor& q, const at::Tensor& scale, at::ScalarType dt) {
+    runtime();
+    return dequant_int8_rows_vk(q, scale, dt);
+  });
+  m.def("int8_linear", [](const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scale, const std::optional<at::Tensor>& bias,
+                          const std::optional<at::Tensor>& x_scale, std::optional<at::ScalarType> out_dtype) {
+    runtime();
+    return int8_linear_autocast(x, weight, weight_scale, bias, x_scale, out_dtype);
+  });
+  m.def("rms_norm", [](const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& residual, double eps, bool int8) {
+    runtime();
+    return rms_norm_autocast(x, weight, residual, eps, int8);
+  });
+  m.def("rotary_embedding", [](const at::Tensor& q, const std::optional<at::Tensor>& k, const at::Tensor& positions, const at::Tensor& freqs,
+                               const std::vector<int64_t>& sections, bool interleaved) {
+    runtime();
+    return rotary_embedding_vk(q, k, positions, freqs, sections, interleaved);
+  });
   // accounting and profiling
   m.def("kernel_counts", &gpu_counts);
   m.def("fallback_counts", &cpu_counts);

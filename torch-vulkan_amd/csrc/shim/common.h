@@ -116,4 +116,23 @@ at::Tensor relative_bias_attention_autocast(const at::Tensor& q, const at::Tenso
                                             const std::optional<at::Tensor>& key_mask, bool causal, std::optional<double> scale,
                                             int64_t max_distance, int64_t query_offset);  // the same of q, k, v and table
 
+
+// 8-bit rows with one scale each, and the linear layer on them (differentiable in x and bias; no reference counterpart).
+std::tuple<at::Tensor, at::Tensor> quantize_int8_rows_vk(const at::Tensor& x);
+at::Tensor dequant_int8_rows_vk(const at::Tensor& q, const at::Tensor& scale, at::ScalarType out_dtype);
+at::Tensor int8_linear_vk(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scale, const std::optional<at::Tensor>& bias,
+                          const std::optional<at::Tensor>& x_scale, std::optional<at::ScalarType> out_dtype);
+at::Tensor int8_linear_autocast(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scale, const std::optional<at::Tensor>& bias,
+                                const std::optional<at::Tensor>& x_scale, std::optional<at::ScalarType> out_dtype);  // x and bias in the autocast dtype
+
+// Root-mean-square norm, {y} or with a residual {y, h}; in 8 bits {q, scale} or {q, scale, h}.
+std::vector<at::Tensor> rms_norm_vk(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& residual, double eps);
+std::vector<at::Tensor> rms_norm_int8_vk(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& residual, double eps);
+std::vector<at::Tensor> rms_norm_autocast(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& residual, double eps,
+                                          bool int8);  // either of them, in fp32 where autocast is on
+
+// Rotary positions of several axes, {q} or {q, k}.
+std::vector<at::Tensor> rotary_embedding_vk(const at::Tensor& q, const std::optional<at::Tensor>& k, const at::Tensor& positions, const at::Tensor& freqs,
+                                            const std::vector<int64_t>& sections, bool interleaved);
+
 }  // namespace vkt

@@ -356,6 +356,105 @@ def relative_bias_attention(q, k, v, table, key_mask=None, causal=False, scale=N
     return _C.relative_bias_attention(q, k, v, table, key_mask, bool(causal), scale, int(max_distance), int(query_offset))
 
 
+_INT8_MOST = float.fromhex("0x1.020406p+121")  # the largest float32 of which 127 are finite
+
+
+def quantize_int8_rows(x):
+    """Pack x [..., cols] (float32, bfloat16 or float16) into 8-bit rows: (codes, scale), int8 [..., cols] and float32 [...].
+
+    A value reads back as code * scale of its row: scale = largest magnitude / 127 (a finite row reads back finite), and code is the whole number nearest to
+    127 * x / largest magnitude, ties to even.  A row of zeros gets scale 0; one with an infinity or NaN gets scale NaN, codes 0,
+    and reads back as NaN.  Not differentiable."""
+    if x.device.type == "vk":
+        return _C.quantize_int8_rows(x)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1:
+        raise RuntimeError("quantize_int8_rows: x must be a float32, bfloat16 or float16 tensor of at least one dimension")
+    x = x.detach()
+    if x.shape[-1] == 0:
+        return torch.empty(x.shape, dtype=torch.int8), torch.zeros(x.shape[:-1])
+    top = x.float().abs().amax(-1, keepdim=True)
+    ok = top.isfinite() & (top > 0)
+    # in 64 bits 127 x is exact, and a quotient that is no tie is farther from one than its rounding
+    codes = torch.where(ok, torch.round(x.double() * 127.0 / top.double()), 0.0).to(torch.int8)
+    return codes, torch.where(top.isfinite(), (top / 127.0).clamp(max=_INT8_MOST), float("nan")).squeeze(-1)
+
+
+def dequant_int8_rows(q, scale, out_dtype=torch.bfloat16):
+    """The values that quantize_int8_rows's (codes, scale) stand for: the float32 product code * scale rounded to out_dtype."""
+    if q.device.type == "vk":
+        return _C.dequant_int8_rows(q, scale, out_dtype)
+    if q.dtype != torch.int8 or scale.dtype != torch.float32 or q.dim() < 1 or q.shape[:-1] != scale.shape:
+        raise RuntimeError(f"dequant_int8_rows: q must be int8 and its scale float32 of q's shape without the last dimension, got "
+                           f"{q.dtype} {tuple(q.shape)} and {scale.dtype} {tuple(scale.shape)}")
+    return (q.float() * scale.unsqueeze(-1)).to(out_dtype)
+
+
+def int8_linear(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None):
+    """Linear layer on 8-bit integers with one scale for each token and each output channel: (x @ weight.T) * x_scale * weight_scale
+    (+ bias), the sums of integers exact and one rounding at the end.  weight int8 [N, K] and weight_scale float32 [N] as
+    quantize_int8_rows packs a weight's rows, K <= 131056; rows of a multiple of 16 values are read in place.
+
+    x [..., K] bfloat16 or float16 on vk is rounded the same way first; the result has its type.  Or x is int8 with x_scale float32
+    [...] (as rms_norm_int8 gives them), and the result has out_dtype (bfloat16 by default, or float16).
+
+    Differentiable in a 16-bit x and in bias, any number of times (create_graph), in reverse mode.  The gradient of x goes straight
+    through its rounding: grad @ dequant_int8_rows(weight, weight_scale, grad.dtype).  Autocast casts x and bias, as it does
+    for linear."""
+    if x.device.type != "vk":
+        raise RuntimeError("int8_linear: x must be a vk tensor")
+    return _C.int8_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6):
+    """Root-mean-square norm of x's rows, h / sqrt(mean(h**2) + eps) * weight with h = x + residual, in float32, rounded once.
+
+    x [..., D] on vk (float32, bfloat16 or float16, any strides), weight [D] and residual [..., D] of the same dtype.  Returns y, or
+    (y, h) where residual is given: h, the sum rounded to x's dtype, is the next residual; y is taken from the unrounded sum.
+    Differentiable once, in reverse mode, in x, weight and residual.  The backward pass reads h (or x): one changed in place is refused
+    there.  Squares are summed in float32, so magnitudes beyond 1e19 overflow.  Autocast runs it in float32, as it does
+    layer_norm."""
+    if x.device.type != "vk":
+        raise RuntimeError("rms_norm: x must be a vk tensor")
+    out = _C.rms_norm(x, weight, residual, float(eps), False)
+    return out[0] if residual is None else tuple(out)
+
+
+def rms_norm_int8(x, weight=None, residual=None, eps=1e-6):
+    """rms_norm with its result in 8-bit rows for int8_linear: (codes, scale), or (codes, scale, h) where residual is given.  The rows
+    are quantize_int8_rows's of the unrounded float32 result, up to the rounding of the quotient.  It has no gradient, and refuses
+    to run where one is asked for."""
+    if x.device.type != "vk":
+        raise RuntimeError("rms_norm_int8: x must be a vk tensor")
+    return tuple(_C.rms_norm(x, weight, residual, float(eps), True))
+
+
+def rotary_frequencies(sections, theta=10000.0):
+    """Frequencies of rotary_embedding's pairs (float64, on the CPU): theta**(-i / n) for i = 0 .. n - 1 of each section of n pairs.
+    theta: one base, or one for each section (scaled ones for positions beyond the trained size)."""
+    thetas = [float(theta)] * len(sections) if isinstance(theta, (int, float)) else [float(t) for t in theta]
+    if len(thetas) != len(sections) or any(n < 0 for n in sections):
+        raise RuntimeError("rotary_frequencies: one theta, or one for each section, and no negative sections")
+    return torch.cat([t ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n, t in zip(sections, thetas)])
+
+
+def rotary_embedding(q, k, positions, freqs, sections, interleaved=False):
+    """Rotary positions of several axes (frames, rows and columns, for instance): pairs of values of each head are turned by the angle
+    position of the pair's axis * frequency.
+
+    q [B, H, S, D] and k [B, Hk, S, D] (or None) on vk (float32, bfloat16 or float16, D <= 1024, any strides).  sections: how many pairs
+    belong to each axis (1..4 of them), P in all; pair j is the values (j, j + P) of a head, or (2 j, 2 j + 1) where interleaved,
+    and the values behind 2 P stay as they are.  positions [S, axes] or [B, S, axes]: int32, int64 or float32.  freqs [P]: float64,
+    in radians per position (rotary_frequencies gives the usual ones).  Angles are taken in float64, so that far positions keep
+    theirs.
+
+    Returns (q, k), or q alone where k is None, in token-major memory, as the fused attention reads them; differentiable in q and k,
+    any number of times, in reverse mode."""
+    if q.device.type != "vk":
+        raise RuntimeError("rotary_embedding: q must be a vk tensor")
+    out = _C.rotary_embedding(q, k, positions, freqs, [int(n) for n in sections], bool(interleaved))
+    return out[0] if k is None else tuple(out)
+
+
 def event_record(slot: int) -> None:
     """Record HIP event `slot` (0..1023) on the runtime's stream (the stream every vk kernel runs on)."""
     _C.event_record(int(slot))

@@ -50,6 +50,31 @@ EW_OPS = {n: i for i, n in enumerate((
     "gelu_tanh_bwd", "addcmul", "addcdiv", "lerp_s", "where"))}
 
 
+class I8RowsArgs(ctypes.Structure):
+    _fields_ = [("x", u64), ("q", u64), ("scale", u64), ("rows", i64), ("cols", i64), ("x_sr", i64), ("q_sr", i64)]
+
+
+class I8MmArgs(ctypes.Structure):
+    _fields_ = [("x", u64), ("x_scale", u64), ("w", u64), ("w_scale", u64), ("bias", u64), ("y", u64),
+                ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64), ("w_sn", i64)]
+
+
+class RmsArgs(ctypes.Structure):
+    _fields_ = [("x", u64), ("r", u64), ("w", u64), ("y", u64), ("h_out", u64), ("q", u64), ("scale", u64), ("rstd", u64),
+                ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("xs", i64 * 3), ("rs", i64 * 3), ("eps", f32), ("pad", u32)]
+
+
+class RmsBwdArgs(ctypes.Structure):
+    _fields_ = [("gy", u64), ("gh", u64), ("h", u64), ("rstd", u64), ("w", u64), ("dx", u64), ("dw", u64), ("ws", u64),
+                ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("gys", i64 * 3), ("ghs", i64 * 3), ("hs", i64 * 3)]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [("q", u64), ("k", u64), ("q_out", u64), ("k_out", u64), ("pos", u64), ("freqs", u64), ("B", i64), ("S", i64),
+                ("qs", i64 * 3), ("ks", i64 * 3), ("p_sb", i64), ("p_ss", i64), ("p_sa", i64), ("Hq", i32), ("Hk", i32), ("D", i32),
+                ("P", i32), ("axes", i32), ("ends", i32 * 4), ("pos_type", i32), ("interleaved", i32), ("back", i32)]
+
+
 class Mx4Args(ctypes.Structure):
     _fields_ = [("x", u64), ("codes", u64), ("scale", u64), ("rows", i64), ("cols", i64), ("x_sr", i64)]
 
@@ -240,6 +265,7 @@ class Runtime:
             "hrt_graph_launch": (ctypes.c_int, [i64]),
             "hrt_graph_destroy": (ctypes.c_int, [i64]),
             "hrt_reduce_workspace": (i64, [vp]),
+            "hrt_rms_workspace": (i64, [vp, i32]),
             "hrt_ln_bwd_noalloc": (ctypes.c_int, [vp, i32]),
         }
         for name, (res, args) in sig.items():
