@@ -435,7 +435,8 @@ typedef struct hrt_i8_mm_args {
  *   unrounded y (up to the rounding of 127 y / top in fp32).
  * "rms_bwd_{dt}" — from gy, gh (gradients of y and h, either 0), h (strides hs) and rstd:
  *   dx = rstd * (gy w - n * mean(gy w n)) + gh with n = h rstd; dw (if not 0) = the sum of gy n over the rows.  dx (if not 0)
- *   [rows, D] contiguous.  dw needs ws, hrt_rms_workspace(&args, dtype) floats: sums of runs of rows, added in order. */
+ *   [rows, D] contiguous.  dw needs ws, hrt_rms_workspace(&args, dtype) floats (none for few rows): sums of runs of rows, added in
+ *   order. */
 typedef struct hrt_rms_args {
   uint64_t x, r, w, y, h_out, q, scale, rstd;
   int64_t rows, D, n1, n2;

@@ -134,6 +134,32 @@ def test_packing_is_exact(shape, dtype):
         assert torch.equal(y.cpu(), (torch.from_numpy(want[0]).float() * torch.from_numpy(want[1]).unsqueeze(-1)).to(out))
 
 
+def all_quotients(dtype):
+    """Rows whose largest value takes every mantissa (every 31st in f16), with every other mantissa over the nine binades in which
+    codes are not 0; in fp32 the values next to every border of random rows."""
+    if dtype == torch.float32:
+        g = torch.Generator().manual_seed(5)
+        top = (torch.rand(200, 1, generator=g) + 1) * torch.exp2(torch.randint(-60, 60, (200, 1), generator=g).float())
+        edge = (top.double() * torch.arange(1, 254, 2) / 254).float()
+        x = torch.cat([edge, torch.nextafter(edge, torch.zeros(1)), torch.nextafter(edge, torch.full((1,), 2.0**80))], -1)
+    else:
+        n = {torch.bfloat16: 128, torch.float16: 1024}[dtype]
+        man = 1 + torch.arange(n) / n
+        top = man[:: 1 if n == 128 else 31].unsqueeze(-1)
+        x = (man * torch.exp2(-torch.arange(9.0)).unsqueeze(-1)).flatten().expand(len(top), -1)
+        x = torch.where(x <= top, x, torch.zeros(()))
+    x = torch.cat([top, x], -1)
+    return torch.cat([x, -x]).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_quotient(dtype):
+    x = all_quotients(dtype)
+    same(torch_vulkan.quantize_int8_rows(x.to(vk)), packed(x))
+    same(torch_vulkan.quantize_int8_rows(x), packed(x))
+
+
 @pytest.mark.gpu
 def test_extremes_on_the_device():
     x = extremes()

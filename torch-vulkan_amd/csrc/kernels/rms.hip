@@ -102,11 +102,15 @@ __global__ __launch_bounds__(256) void rms_rows(hrt_rms_args p, int64_t q_sr) {
     for (int c = 0; c < NV; ++c) {
       const int64_t col = (int64_t)(c * LPR + lane) * V;
       if (col >= q_sr) continue;
-      int k[V];
+      uint32_t k[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         k[e] = MODE == kQuant ? nearest_code<T>(v[c][e], code) : code_of(v[c][e], code);
         if (TAIL && col + e >= p.D) k[e] = 0;
+      }
+      if (code.per == 0.f) {  // nothing but zeros, or not finite
+#pragma unroll
+        for (int e = 0; e < V; ++e) k[e] = 0;
       }
       if (col + V <= q_sr) {
         typedef uint32_t __attribute__((aligned(1))) u32_any;
@@ -188,19 +192,74 @@ __global__ __launch_bounds__(256) void rms_long(hrt_rms_args p, int64_t q_sr) {
       norm(col, v);
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (col + e < q_sr) q[col + e] = col + e < p.D ? (uint8_t)(MODE == kQuant ? nearest_code<T>(v[e], code) : code_of(v[e], code)) : 0;
+        if (col + e < q_sr) q[col + e] = col + e < p.D && code.per != 0.f ? (uint8_t)(MODE == kQuant ? nearest_code<T>(v[e], code) : code_of(v[e], code)) : 0;
     }
   }
 }
 
+// Four floats of a row of D, zeros behind it.
+__device__ __forceinline__ f32x4 row_piece_f32(const float* row, int64_t col, int64_t D) {
+  const u32x4 w = row_piece<F32, true>(gcptr<float>(reinterpret_cast<uint64_t>(row)), col, D);
+  return __builtin_bit_cast(f32x4, w);
+}
+
 // ---- backward -------------------------------------------------------------------------------------------------------------
+// dw where there are few rows: the workgroups behind those that take rows have strips of 128 bytes of columns each, of all rows
+// (which the others read too: from L2).  A second launch costs more than their reads: 308 x 1001 fp32 both ways 33 us, so 27.
+template <typename T, bool TAIL>
+__device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) {
+  using R = RowVec<T>;
+  using S = typename T::storage;
+  constexpr int V = R::V, G = 32;  // rows at a time
+  __shared__ float red[G][8 * V + 1];
+  const int lane = threadIdx.x & 7, group = threadIdx.x >> 3;
+  const int64_t col = ((int64_t)strip * 8 + lane) * V;
+  float acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  for (int64_t r0 = group; r0 < p.rows; r0 += 4 * G) {
+    u32x4 a[4], b[4];
+    float rstd[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {  // four rows' loads in flight; a row past the end repeats the last one
+      const int64_t row = r0 + u * G < p.rows ? r0 + u * G : p.rows - 1;
+      a[u] = u32x4{0, 0, 0, 0};
+      if (p.gy) a[u] = row_piece<T, TAIL>(gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys), col, p.D);
+      b[u] = row_piece<T, TAIL>(gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs), col, p.D);
+      rstd[u] = gcptr<float>(p.rstd)[row];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float d[V], n[V];
+      R::unpack(a[u], d);
+      R::unpack(b[u], n);
+      if (r0 + u * G < p.rows) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += d[e] * (n[e] * rstd[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) red[group][lane * V + e] = acc[e];
+  __syncthreads();
+  const int64_t at = (int64_t)strip * 8 * V + threadIdx.x;
+  if ((int)threadIdx.x >= 8 * V || at >= p.D) return;
+  float t = red[0][threadIdx.x];
+#pragma unroll
+  for (int k = 1; k < G; ++k) t += red[k][threadIdx.x];
+  gptr<S>(p.dw)[at] = T::from_f32(t);
+}
+
 // A workgroup takes `per` consecutive rows, 256 / LPR at a time.  DW: a lane adds gy n of its columns up over its rows, the
 // workgroup's lanes of a column are added in order through LDS, and the sums of all workgroups by rms_dw_sum.
 template <typename T, int LPR, int NV, bool TAIL, bool DW>
-__global__ __launch_bounds__(256) void rms_back(hrt_rms_bwd_args p, int64_t per) {
+__global__ __launch_bounds__(256) void rms_back(hrt_rms_bwd_args p, int64_t per, int blocks) {
   using R = RowVec<T>;
   using S = typename T::storage;
   constexpr int V = R::V, RPB = 256 / LPR;
+  if constexpr (!DW) {
+    if ((int)blockIdx.x >= blocks) return rms_strip<T, TAIL>(p, (int)blockIdx.x - blocks);
+  }
   __shared__ float red[2][4];
   __shared__ __attribute__((aligned(16))) float part[DW && RPB > 1 ? RPB * LPR * NV * V : 4];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
@@ -339,26 +398,37 @@ __global__ __launch_bounds__(256) void rms_back_long(hrt_rms_bwd_args p, int64_t
   }
 }
 
-// dw: the workgroups' sums of 32 columns, a thread every 32nd of them in order, then the 32 of a column in order.
+// dw: the workgroups' sums of 32 columns, a thread every 128th of them in order (four loads in flight: one round for 512), then
+// the 128 of a column in a fixed tree.
 template <typename T>
-__global__ __launch_bounds__(256) void rms_dw_sum(const float* ws, typename T::storage* dw, int64_t parts, int64_t D) {
-  __shared__ float red[32][33];
+__global__ __launch_bounds__(1024) void rms_dw_sum(const float* ws, typename T::storage* dw, int64_t parts, int64_t D) {
+  constexpr int G = 128;
+  __shared__ float red[G][33];
   const int quad = threadIdx.x & 7, group = threadIdx.x >> 3;
   const int64_t col = (int64_t)blockIdx.x * 32 + quad * 4;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t c = group; c < parts; c += 32) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t c = group; c < parts; c += 4 * G) {
+    f32x4 v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] += col + e < D ? ws[c * D + col + e] : 0.f;
+    for (int u = 0; u < 4; ++u) v[u] = row_piece_f32(ws + (c + u * G < parts ? c + u * G : parts - 1) * D, col, D);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (c + u * G < parts) s += v[u];
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) red[group][quad * 4 + e] = s[e];
   __syncthreads();
+  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;  // four of the 128, then the 32 sums
+  const float t = (red[4 * k][c] + red[4 * k + 1][c]) + (red[4 * k + 2][c] + red[4 * k + 3][c]);
+  __syncthreads();
+  red[k][c] = t;
+  __syncthreads();
   const int64_t at = (int64_t)blockIdx.x * 32 + threadIdx.x;
   if (threadIdx.x >= 32 || at >= D) return;
-  float t = red[0][threadIdx.x];
+  float o = red[0][threadIdx.x];
 #pragma unroll
-  for (int k = 1; k < 32; ++k) t += red[k][threadIdx.x];
-  dw[at] = T::from_f32(t);
+  for (int i = 1; i < 32; ++i) o += red[i][threadIdx.x];
+  dw[at] = T::from_f32(o);
 }
 
 // ---- 8-bit rows back to values ----------------------------------------------------------------------------------------------
@@ -514,10 +584,12 @@ bool launch_dequant(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   return hrt::launch_ok(hipGetLastError(), ctx, "i8_rows_dequant");
 }
 
-// Rows per workgroup of the backward: with dw as many as leave 512 workgroups.
+// Whether dw is summed by strips of columns in the same launch.
+bool strips(const hrt_rms_bwd_args& a, Share s) { return a.dw && s.lpr && a.rows <= 512; }
+// Rows per workgroup of the backward: with sums of dw as many as leave 512 workgroups.
 int64_t back_rows(const hrt_rms_bwd_args& a, Share s) {
   const int64_t rpb = s.lpr ? 256 / s.lpr : 1;
-  return a.dw ? cdiv(cdiv(a.rows, 512), rpb) * rpb : rpb;
+  return a.dw && !strips(a, s) ? cdiv(cdiv(a.rows, 512), rpb) * rpb : rpb;
 }
 template <typename T>
 int64_t back_blocks(const hrt_rms_bwd_args& a) {
@@ -539,28 +611,30 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
       (a.gh && !ctx.check(a.gh, rows_span(a.rows, a.n1, a.n2, a.D, a.ghs, E), "gh")) ||
       !ctx.check(a.h, rows_span(a.rows, a.n1, a.n2, a.D, a.hs, E), "h") || !ctx.check(a.rstd, a.rows * 4, "rstd") ||
       (a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
-      (a.dw && (!ctx.check(a.dw, a.D * E, "dw") || !ctx.check(a.ws, (uint64_t)(blocks * a.D) * 4, "ws"))))
+      (a.dw && !ctx.check(a.dw, a.D * E, "dw")))
     return false;
-  if (!hrt::grid_fits(blocks, 256)) return ctx.fail("grid too large");
   const Share s = share_of(a.rows, a.D, V);
-  const int64_t per = back_rows(a, s);
-  const dim3 grid((uint32_t)blocks);
+  const bool sums = a.dw && !strips(a, s);
+  if (sums && !ctx.check(a.ws, (uint64_t)(blocks * a.D) * 4, "ws")) return false;
+  const int64_t per = back_rows(a, s), all = blocks + (a.dw && !sums ? cdiv(a.D, 8 * V) : 0);
+  if (!hrt::grid_fits(all, 256)) return ctx.fail("grid too large");
+  const dim3 grid((uint32_t)all);
   if (s.lpr == 0) {
     hipLaunchKernelGGL(rms_back_long<T>, grid, dim3(256), 0, ctx.stream, a, per);
   } else {
     with_share(s, [&](auto lc, auto nc) {
       constexpr int L = decltype(lc)::value, N = decltype(nc)::value;
       const auto go = [&](auto tail, auto dw) {
-        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value>), grid, dim3(256), 0, ctx.stream, a, per);
+        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value>), grid, dim3(256), 0, ctx.stream, a, per, (int)blocks);
       };
       using Y = std::true_type;
       using No = std::false_type;
-      if (a.D % V == 0) a.dw ? go(No(), Y()) : go(No(), No());
-      else a.dw ? go(Y(), Y()) : go(Y(), No());
+      if (a.D % V == 0) sums ? go(No(), Y()) : go(No(), No());
+      else sums ? go(Y(), Y()) : go(Y(), No());
     });
   }
-  if (a.dw)
-    hipLaunchKernelGGL(rms_dw_sum<T>, dim3((uint32_t)cdiv(a.D, 32)), dim3(256), 0, ctx.stream, (const float*)a.ws, (S*)a.dw, blocks, a.D);
+  if (sums)
+    hipLaunchKernelGGL(rms_dw_sum<T>, dim3((uint32_t)cdiv(a.D, 32)), dim3(1024), 0, ctx.stream, (const float*)a.ws, (S*)a.dw, blocks, a.D);
   return hrt::launch_ok(hipGetLastError(), ctx, "rms_bwd");
 }
 
@@ -579,5 +653,6 @@ HK_ROWS("f16", F16);
 extern "C" int64_t hrt_rms_workspace(const hrt_rms_bwd_args* a, int32_t dtype) {
   using namespace hk;
   if (!a || a->rows <= 0 || a->D <= 0 || !a->dw) return 0;
+  if (strips(*a, share_of(a->rows, a->D, dtype == HRT_F32 ? 4 : 8))) return 0;
   return (dtype == HRT_F32 ? back_blocks<F32>(*a) : back_blocks<BF16>(*a)) * a->D;
 }

@@ -116,37 +116,41 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v, uint32_t* red) {
 // A row's values are code * scale with scale = top / 127, top the row's largest magnitude, and code the whole number nearest to
 // 127 v / top (ties to even).  scale is rounded to nearest, but stays where 127 scale is finite.  A row of zeros has scale 0, one with an infinity or NaN scale NaN and codes 0.
 struct RowCode {
-  float mul, top, per, scale;  // v * mul and top are in a range where 127 / top = per is an ordinary number
+  float mul, per, scale;  // v * mul is in a range where per = 127 / (top * mul) is an ordinary number
+  double per64;           // the same in fp64, for 32-bit values
   __device__ __forceinline__ explicit RowCode(uint32_t bits) {
     const float t = __uint_as_float(bits);
     mul = bits < 0x0d800000u /* 2^-100 */ ? 0x1p64f : bits > 0x71800000u /* 2^100 */ ? 0x1p-64f : 1.f;
-    if (bits >= 0x7f800000u) {
-      mul = top = per = 0.f, scale = __uint_as_float(0x7fc00000u);
+    if (bits - 1u >= 0x7f7fffffu) {  // zero, infinity, NaN
+      mul = per = 0.f, per64 = 0.0, scale = bits ? __uint_as_float(0x7fc00000u) : 0.f;
     } else {
-      top = t * mul, per = bits ? 127.f / top : 0.f;
+      per = 127.f / (t * mul), per64 = 127.0 / (double)(t * mul);
       scale = fminf(t / 127.f, 0x1.020406p+121f);  // 127 of the largest step that is taken are finite
     }
   }
 };
+// A code is the low byte of the sum of its quotient and 1.5 2^23, whose last place is one: the addition rounds, ties to even.
+constexpr float kRound32 = 12582912.f;
+constexpr double kRound64 = 6755399441055744.0;  // 1.5 2^52
 // Codes of fp32 values that are roundings themselves: the quotient as it comes out.
-__device__ __forceinline__ int code_of(float v, const RowCode& r) {
-  const float q = rintf(v * r.mul * r.per);
-  return r.per == 0.f ? 0 : (int)q;
-}
-// The nearest code exactly: the quotient's error is settled by 127 v - q top, which 16-bit values give exactly in fp32 (127 v has 18
-// bits, q top 18, and the difference of neighbours fits 24), 32-bit ones in fp64.
+__device__ __forceinline__ uint32_t code_of(float v, const RowCode& r) { return __float_as_uint(v * r.mul * r.per + kRound32); }
+// The nearest code exactly.  Relative to its size, a quotient that is no tie is at least 2^-18 away from one (127 times an 11-bit
+// number against an odd multiple of an 11-bit one; 2^-31 for 24-bit ones), and comes out within 2^-22 (2^-51 in fp64).  Rounded to
+// 20 bits (45), ties, which have 8, are ties again, and nothing else becomes one.
 template <typename T>
-__device__ __forceinline__ int nearest_code(float v, const RowCode& r) {
-  if (r.per == 0.f) return 0;
-  const float x = v * r.mul;
-  int q = (int)rintf(x * r.per);
-  using F = typename std::conditional<std::is_same<T, F32>::value, double, float>::type;
-  const F d = F(127) * F(x) - F(q) * F(r.top), e = d < 0 ? -d : d, twice = e + e;
-  if (twice > F(r.top) || (twice == F(r.top) && (q & 1))) q += d < 0 ? -1 : 1;
-  return q;
+__device__ __forceinline__ uint32_t nearest_code(float v, const RowCode& r) {
+  if constexpr (std::is_same<T, F32>::value) {
+    const uint64_t q = (__builtin_bit_cast(uint64_t, (double)(v * r.mul) * r.per64) + 0x80u) & ~(uint64_t)0xff;
+    return (uint32_t)__builtin_bit_cast(uint64_t, __builtin_bit_cast(double, q) + kRound64);
+  } else {
+    const uint32_t q = (__float_as_uint(v * r.mul * r.per) + 8u) & ~15u;
+    return __float_as_uint(__uint_as_float(q) + kRound32);
+  }
 }
-__device__ __forceinline__ uint32_t pack_codes4(const int* q) {
-  return ((uint32_t)q[0] & 255u) | (((uint32_t)q[1] & 255u) << 8) | (((uint32_t)q[2] & 255u) << 16) | ((uint32_t)q[3] << 24);
+// Low bytes of four codes.
+__device__ __forceinline__ uint32_t pack_codes4(const uint32_t* q) {
+  const uint32_t a = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u), b = __builtin_amdgcn_perm(q[3], q[2], 0x0c0c0400u);
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
 
 }  // namespace hk

@@ -137,8 +137,7 @@ struct Norm : torch::autograd::Function<Norm> {
       if (dx.defined()) A.dx = dptr(dx);
       if (wants_w) {
         A.dw = dptr(dw);
-        ws = at::empty({hrt_rms_workspace(&A, float_code(h.scalar_type()))}, rstd.options());
-        A.ws = dptr(ws);
+        if (const int64_t n = hrt_rms_workspace(&A, float_code(h.scalar_type())); n > 0) ws = at::empty({n}, rstd.options()), A.ws = dptr(ws);
       }
       queue(typed("rms_bwd", h.scalar_type()), A);
     }
