@@ -421,11 +421,19 @@ typedef struct hrt_i8_rows_args {
 /* "i8_mm_{bf16,f16}" — product of 8-bit rows (no reference counterpart):
  *   y[m, n] = round((sum_k x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])      (whole sums; bias 0: none)
  * x [M, K], w [N, K] int8 with row strides x_sm, w_sn (bytes, multiples of 16), 16-byte aligned; scales fp32; y [M, N]
- * contiguous and bias [N] of the kernel's type.  K % 16 == 0 and K <= 131056, so that no sum passes 31 bits. */
+ * contiguous and bias [N] of the kernel's type.  K % 16 == 0 and K <= 131056, so that no sum passes 31 bits.
+ * x_scale 0 (where hrt_i8_mm_quantises(M, K)): x is [M, K] of the kernel's type, row stride x_sm elements, and is quantised on the way as
+ * "i8_rows_quant_*" does. */
 typedef struct hrt_i8_mm_args {
   uint64_t x, x_scale, w, w_scale, bias, y;
   int64_t M, N, K, x_sm, w_sn;
 } hrt_i8_mm_args;
+/* Rows are shared out over a workgroup's wavefronts, four of them up to K = 1024 and eight beyond, 2048 values for each at most. */
+static inline int64_t hrt_i8_mm_row_slots(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
+static inline int hrt_i8_mm_quantises(int64_t M, int64_t K) {
+  const int64_t waves = K <= 1024 ? 4 : 8, slots = hrt_i8_mm_row_slots(M);
+  return K % 16 == 0 && M <= 8 && slots <= waves && slots * K <= 2048 * waves;
+}
 
 /* Root-mean-square norm of rows (no reference counterpart).  Row i of a tensor is found through up to three outer dimensions,
  * i = (i0 * n1 + i1) * n2 + i2, at element i0 * s[0] + i1 * s[1] + i2 * s[2]; D values with unit stride.

@@ -217,7 +217,7 @@ def check_back(got, g, w, s, dtype):
 # every tile and both sides of its borders, rows, odd widths, ends of K inside a line and inside a piece of 16
 PRODUCTS = [(1, 16, 16), (1, 1, 1), (2, 8, 144), (16, 48, 2064), (16, 100, 128), (17, 64, 1024), (32, 40, 1040), (33, 136, 320), (64, 64, 512), (77, 130, 272),
             (130, 256, 400), (129, 129, 128), (257, 264, 1000), (300, 512, 77), (5, 33, 50), (200, 2056, 656), (1, 4096, 4096), (20, 512, 9000), (308, 72, 4112),
-            (700, 2048, 512), (1500, 4096, 256), (4100, 2048, 144)]
+            (3, 40, 2720), (3, 24, 4096), (4, 24, 4112), (8, 24, 2048), (7, 24, 1040), (5, 24, 1024), (3, 24, 1008), (4, 8, 512), (8, 24, 2064), (1, 24, 16384), (1, 8, 16400), (2, 8, 8192), (700, 2048, 512), (1500, 4096, 256), (4100, 2048, 144)]
 
 
 @pytest.mark.gpu

@@ -12,6 +12,7 @@
 
 #include "../hrt/registry.h"
 #include "lds_stage.h"
+#include "row_vec.h"
 
 namespace hk {
 namespace {
@@ -31,9 +32,8 @@ __device__ __forceinline__ i32x16 mac32(u32x4 a, u32x4 b, i32x16 c) {
 
 // Values n .. n + 3 of row m from whole sums: sum * x_scale is taken first (the product of two small scales may underflow).
 template <typename T>
-__device__ __forceinline__ void store4(const hrt_i8_mm_args& p, int64_t m, int64_t n, const int* v, bool vec) {
+__device__ __forceinline__ void store4(const hrt_i8_mm_args& p, int64_t m, int64_t n, const int* v, float sx, bool vec) {
   if (m >= p.M || n >= p.N) return;
-  const float sx = gcptr<float>(p.x_scale)[m];
   const HK_G float* sw = gcptr<float>(p.w_scale) + n;
   HK_G uint16_t* y = gptr<uint16_t>(p.y) + m * p.N + n;
   const HK_G uint16_t* b = gcptr<uint16_t>(p.bias) + n;
@@ -55,31 +55,90 @@ __device__ __forceinline__ void store4(const hrt_i8_mm_args& p, int64_t m, int64
 // ---- few rows ------------------------------------------------------------------------------------------------------------
 // 16 MB rows (MB 1 or 2), NWV wavefronts.  A wavefront's pieces of 128 bytes of K come in batches of UB whose loads are all issued
 // before the first product: one memory latency a batch.
-template <typename T, int MB, int NWV, int UB>
+// PX > 0 (hrt_i8_mm_quantises): X is one to eight rows in 16 bits, and every workgroup quantises them for itself while its first
+// weights are on the way: each row by its share of the wavefronts, PX 16-byte pieces a lane, into LDS.  GPU time against a
+// launch of its own, M x N x K: 1 x 2048 x 512 3.0 us against 4.8, 1 x 8192 x 2048 4.3 against 6.6, 8 x 8192 x 2048 5.6 against 7.4,
+// 1 x 8192 x 16384 26 against 36.
+template <typename T, int MB, int NWV, int UB, int PX>
 __global__ __launch_bounds__(64 * NWV) void i8_rows(hrt_i8_mm_args p, bool vec) {
+  constexpr bool Q = PX > 0;
+  static_assert(!Q || MB == 1, "few rows");
+  constexpr int kCodes = Q ? 512 * PX * NWV : 16;
   __shared__ int part[NWV - 1][MB][64][4];
+  __shared__ __attribute__((aligned(16))) uint8_t xq[kCodes];
+  __shared__ uint32_t tops[NWV];
+  __shared__ float scales[NWV];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + r16 < p.N ? n0 + r16 : p.N - 1;  // columns past N repeat the last one and are not stored
   const int64_t chunks = p.K / 16, steps = cdiv(p.K, 128);
   const HK_G uint8_t* const w = gcptr<uint8_t>(p.w) + n * p.w_sn;
+  // this lane's chunk t of piece k; chunks past the end of K: any, and zeros for W
+  auto place = [&](int64_t k, int t) HK_INLINE { return (k * 8 + 4 * t + g < chunks ? k * 8 + 4 * t + g : 0) * 16; };
+  u32x4 wf[UB][2];
+  auto load_w = [&](int64_t st) HK_INLINE {
+#pragma unroll
+    for (int u = 0; u < UB; ++u)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) wf[u][t] = __builtin_nontemporal_load(reinterpret_cast<const HK_G u32x4*>(w + place(st + u * NWV, t)));
+  };
+  if constexpr (Q) {
+    const int rows = p.M == 1 ? 1 : p.M == 2 ? 2 : p.M <= 4 ? 4 : 8, wpr = NWV / rows, row = wave / wpr;  // wavefronts per row
+    const int m = row < p.M ? row : (int)p.M - 1, first = (wave % wpr * 64 + lane) * 8, stride = wpr * 512;
+    const HK_G uint16_t* const x = gcptr<uint16_t>(p.x) + m * p.x_sm;
+    u32x4 raw[PX];
+#pragma unroll
+    for (int i = 0; i < PX; ++i) raw[i] = first + i * stride < p.K ? RowVec<T>::get(x + first + i * stride) : u32x4{0, 0, 0, 0};
+    issue_order_fence();
+    load_w(wave);
+    float v[PX][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < PX; ++i) {
+      RowVec<T>::unpack(raw[i], v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b = __float_as_uint(v[i][e]) & 0x7fffffffu;
+        top = b > top ? b : top;
+      }
+    }
+    top = lanes_max<64>(top, nullptr);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    for (int k = 0; k < wpr; ++k) top = tops[row * wpr + k] > top ? tops[row * wpr + k] : top;
+    const RowCode code(top);
+    if (lane == 0) scales[row] = code.scale;
+#pragma unroll
+    for (int i = 0; i < PX; ++i) {
+      uint32_t k[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[e] = nearest_code<T>(v[i][e], code);
+      const u32x2 q = code.per == 0.f ? u32x2{0, 0} : u32x2{pack_codes4(k), pack_codes4(k + 4)};
+      if (row < p.M && first + i * stride < p.K) *reinterpret_cast<u32x2*>(xq + m * p.K + first + i * stride) = q;
+    }
+    __syncthreads();
+  }
   const HK_G uint8_t* x[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) x[b] = gcptr<uint8_t>(p.x) + (b * 16 + r16 < p.M ? b * 16 + r16 : p.M - 1) * p.x_sm;  // rows past M: not stored
+  const HK_L uint8_t* const xl = (const HK_L uint8_t*)xq + (Q ? (r16 < p.M ? r16 : (int)p.M - 1) * (int)p.K : 0);
   i32x4 acc[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) acc[b] = i32x4{0, 0, 0, 0};
   for (int64_t st = wave; st < steps; st += NWV * UB) {
-    u32x4 wf[UB][2], xf[UB][2][MB];
+    u32x4 xf[UB][2][MB];
+    if (!Q || st != wave) load_w(st);
 #pragma unroll
     for (int u = 0; u < UB; ++u)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int64_t c = (st + u * NWV) * 8 + 4 * t + g, at = (c < chunks ? c : 0) * 16;  // chunks past the end of K: zeros
-        wf[u][t] = __builtin_nontemporal_load(reinterpret_cast<const HK_G u32x4*>(w + at));
+        const int64_t at = place(st + u * NWV, t);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) xf[u][t][b] = *reinterpret_cast<const HK_G u32x4*>(x[b] + at);
+        for (int b = 0; b < MB; ++b) {
+          if constexpr (Q) xf[u][t][b] = *reinterpret_cast<const HK_L u32x4*>(xl + at);
+          else xf[u][t][b] = *reinterpret_cast<const HK_G u32x4*>(x[b] + at);
+        }
       }
 #pragma unroll
     for (int u = 0; u < UB; ++u)
@@ -101,7 +160,8 @@ __global__ __launch_bounds__(64 * NWV) void i8_rows(hrt_i8_mm_args p, bool vec) 
 #pragma unroll
     for (int w2 = 0; w2 < NWV - 1; ++w2) acc[b] += *reinterpret_cast<const i32x4*>(part[w2][b][lane]);
     const int v[4] = {acc[b][0], acc[b][1], acc[b][2], acc[b][3]};
-    store4<T>(p, b * 16 + r16, n0 + 4 * g, v, vec);
+    const int64_t m = b * 16 + r16;
+    store4<T>(p, m, n0 + 4 * g, v, Q ? scales[m < p.M ? m : 0] : gcptr<float>(p.x_scale)[m < p.M ? m : 0], vec);
   }
 }
 
@@ -264,14 +324,17 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
   }
   if (!lines) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < FM; ++i) {
+      const int64_t m = m0 + wm * WM + i * 32 + l32;
+      const float sx = gcptr<float>(p.x_scale)[m < p.M ? m : 0];
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int v[4] = {acc[j][i][4 * e], acc[j][i][4 * e + 1], acc[j][i][4 * e + 2], acc[j][i][4 * e + 3]};
-          store4<T>(p, m0 + wm * WM + i * 32 + l32, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, false);
+          store4<T>(p, m, n0 + wn * WN + j * 32 + 8 * e + 4 * h, v, sx, false);
         }
+    }
     return;
   }
   // Whole lines of y: 32 rows at a time go through the wavefront's own LDS area, so that a store writes 16 bytes a lane along a row.
@@ -330,7 +393,7 @@ constexpr Tile2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
 int64_t tiles_of(const hrt_i8_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
 // Index of the tile, -1: i8_rows.
 int plan_of(const hrt_i8_mm_args& a) {
-  if (a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
+  if (a.x_scale == 0 || a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
   static constexpr struct { float fixed, per128; } kCost[4] = {{11.f, 1.9f}, {7.4f, 1.4f}, {5.4f, 0.74f}, {4.2f, 0.25f}};
   int best = 3;
   float us = 0.f;
@@ -360,10 +423,16 @@ void queue_mm(const hrt_i8_mm_args& a, int tile, hipStream_t s) {
   // wavefronts and batches that cover K once where they can
   const dim3 grid((uint32_t)cdiv(a.N, 16));
   const int64_t pieces = cdiv(a.K, 128);
-  if (a.M > 16) hipLaunchKernelGGL((i8_rows<T, 2, 4, 2>), grid, dim3(256), 0, s, a, vec);
-  else if (pieces <= 8) hipLaunchKernelGGL((i8_rows<T, 1, 4, 2>), grid, dim3(256), 0, s, a, vec);
-  else if (pieces <= 16) hipLaunchKernelGGL((i8_rows<T, 1, 8, 2>), grid, dim3(512), 0, s, a, vec);
-  else hipLaunchKernelGGL((i8_rows<T, 1, 8, 4>), grid, dim3(512), 0, s, a, vec);
+  const auto go = [&](auto px) {
+    constexpr int Q = decltype(px)::value;
+    if (pieces <= 8) hipLaunchKernelGGL((i8_rows<T, 1, 4, 2, Q>), grid, dim3(256), 0, s, a, vec);
+    else if (pieces <= 16) hipLaunchKernelGGL((i8_rows<T, 1, 8, 2, Q>), grid, dim3(512), 0, s, a, vec);
+    else hipLaunchKernelGGL((i8_rows<T, 1, 8, 4, Q>), grid, dim3(512), 0, s, a, vec);
+  };
+  if (a.M > 16) hipLaunchKernelGGL((i8_rows<T, 2, 4, 2, 0>), grid, dim3(256), 0, s, a, vec);
+  else if (a.x_scale != 0) go(std::integral_constant<int, 0>());
+  else if (hrt_i8_mm_row_slots(a.M) * a.K <= (pieces <= 8 ? 4096 : 8192)) go(std::integral_constant<int, 2>());
+  else go(std::integral_constant<int, 4>());
 }
 
 template <typename T>
@@ -371,12 +440,14 @@ bool launch_i8_mm(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   const auto& a = *static_cast<const hrt_i8_mm_args*>(pp);
   if (a.M <= 0 || a.N <= 0 || a.K <= 0) return ctx.fail("empty product");
   if (a.K % 16 != 0 || a.K > 131056) return ctx.fail("K must be a multiple of 16 and at most 131056");
-  if (a.x_sm < 0 || a.x_sm % 16 != 0 || a.w_sn < 0 || a.w_sn % 16 != 0) return ctx.fail("row strides must be non-negative multiples of 16");
-  if (a.x % 16 != 0 || a.w % 16 != 0 || a.x_scale % 4 != 0 || a.w_scale % 4 != 0 || a.y % 2 != 0 || a.bias % 2 != 0)
+  const bool q = a.x_scale == 0;
+  if (q && !hrt_i8_mm_quantises(a.M, a.K)) return ctx.fail("too many values to quantise on the way");
+  if (a.x_sm < 0 || (!q && a.x_sm % 16 != 0) || a.w_sn < 0 || a.w_sn % 16 != 0) return ctx.fail("row strides must be non-negative multiples of 16");
+  if (a.x % (q ? 2 : 16) != 0 || a.w % 16 != 0 || a.x_scale % 4 != 0 || a.w_scale % 4 != 0 || a.y % 2 != 0 || a.bias % 2 != 0)
     return ctx.fail("x and w must be 16-byte aligned, scales 4-byte aligned");
   const int64_t xs[2] = {a.M, a.K}, xt[2] = {a.x_sm, 1}, wz[2] = {a.N, a.K}, wt[2] = {a.w_sn, 1};
-  if (!ctx.check(a.x, hrt::span_bytes(2, xs, xt, 1), "x") || !ctx.check(a.w, hrt::span_bytes(2, wz, wt, 1), "w") ||
-      !ctx.check(a.x_scale, (uint64_t)a.M * 4, "x_scale") || !ctx.check(a.w_scale, (uint64_t)a.N * 4, "w_scale") ||
+  if (!ctx.check(a.x, hrt::span_bytes(2, xs, xt, q ? 2 : 1), "x") || !ctx.check(a.w, hrt::span_bytes(2, wz, wt, 1), "w") ||
+      (!q && !ctx.check(a.x_scale, (uint64_t)a.M * 4, "x_scale")) || !ctx.check(a.w_scale, (uint64_t)a.N * 4, "w_scale") ||
       !ctx.check(a.y, (uint64_t)(a.M * a.N) * 2, "y") || (a.bias && !ctx.check(a.bias, (uint64_t)a.N * 2, "bias")))
     return false;
   // offsets of a tile's rows are 31-bit

@@ -67,13 +67,15 @@ at::Tensor linear_rows(const Operands& o) {
   at::Tensor xq, xs, b;
   if (o.x_scale.defined()) {
     xq = product_rows(o.x), xs = dense(o.x_scale);
+  } else if (hrt_i8_mm_quantises(M, K)) {  // quantised by the product itself
+    xq = unit_rows(o.x);
   } else {
     xq = at::empty({M, round16(K)}, o.w.options()), xs = at::empty({M}, o.w_scale.options());
     quantize_rows(o.x, xq, xs);
   }
   const at::Tensor w = product_rows(o.w), ws = dense(o.w_scale);
   hrt_i8_mm_args A{};
-  A.x = dptr(xq), A.x_scale = dptr(xs), A.w = dptr(w), A.w_scale = dptr(ws), A.y = dptr(y);
+  A.x = dptr(xq), A.x_scale = xs.defined() ? dptr(xs) : 0, A.w = dptr(w), A.w_scale = dptr(ws), A.y = dptr(y);
   if (present(o.bias)) b = dense(*o.bias), A.bias = dptr(b);
   A.M = M, A.N = N, A.K = w.size(1), A.x_sm = pitch(xq), A.w_sn = pitch(w);
   queue(typed("i8_mm", o.out), A);
