@@ -418,6 +418,14 @@ typedef struct hrt_i8_rows_args {
   int64_t rows, cols, x_sr, q_sr;
 } hrt_i8_rows_args;
 
+/* "i8_linear_back_{bf16,f16}" — what the gradients of y = X W^T + bias (8-bit rows W) take beside a product: v [N, K] = the values
+ *   of w's rows (row stride w_sn bytes) in the kernel's type, as "i8_rows_dequant_*" gives them, and db [N] = the sums of g's [M, N]
+ *   columns (row stride g_sm, unit column stride) in fp32, rounded once.  Either of v and db may be 0. */
+typedef struct hrt_i8_linear_back_args {
+  uint64_t w, w_scale, v, g, db;
+  int64_t M, N, K, w_sn, g_sm;
+} hrt_i8_linear_back_args;
+
 /* "i8_mm_{bf16,f16}" — product of 8-bit rows (no reference counterpart):
  *   y[m, n] = round((sum_k x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])      (whole sums; bias 0: none)
  * x [M, K], w [N, K] int8 with row strides x_sm, w_sn (bytes, multiples of 16), 16-byte aligned; scales fp32; y [M, N]

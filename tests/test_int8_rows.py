@@ -107,7 +107,7 @@ def test_argument_blocks_match_the_header(tmp_path):
     import os
     import subprocess
 
-    blocks = {"hrt_i8_rows_args": abi.I8RowsArgs, "hrt_i8_mm_args": abi.I8MmArgs, "hrt_rms_args": abi.RmsArgs, "hrt_rms_bwd_args": abi.RmsBwdArgs,
+    blocks = {"hrt_i8_rows_args": abi.I8RowsArgs, "hrt_i8_mm_args": abi.I8MmArgs, "hrt_i8_linear_back_args": abi.I8LinearBackArgs, "hrt_rms_args": abi.RmsArgs, "hrt_rms_bwd_args": abi.RmsBwdArgs,
               "hrt_rotary_args": abi.RotaryArgs}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "hrt_ops.h"', "int main(void) {"]
     for c, py in blocks.items():

@@ -44,6 +44,7 @@ HRT_SOURCES = [
     "kernels/mx4_gemm.hip",
     "kernels/mx4_back.hip",
     "kernels/rms.hip",
+    "kernels/i8_rows.hip",
     "kernels/i8_gemm.hip",
     "kernels/rotary.hip",
     "kernels/gemm.hip",

@@ -1,5 +1,4 @@
-// Root-mean-square norm of rows, forward ("rms_fwd_*") and backward ("rms_bwd_*"), and 8-bit rows ("i8_rows_quant_*",
-// "i8_rows_dequant_*").
+// Root-mean-square norm of rows, forward ("rms_fwd_*") and backward ("rms_bwd_*"), and rows into 8 bits ("i8_rows_quant_*").
 //
 // Bound by memory: a row is read once, held in registers as fp32 and written once.  16, 64 or 256 lanes share a row (heads,
 // model widths, wide rows or few of them), which DPP steps and lane swaps add up without LDS, or through four floats of it.
@@ -431,36 +430,6 @@ __global__ __launch_bounds__(1024) void rms_dw_sum(const float* ws, typename T::
   dw[at] = T::from_f32(o);
 }
 
-// ---- 8-bit rows back to values ----------------------------------------------------------------------------------------------
-// 16 codes a lane; a workgroup takes whole rows, several where they are short.
-template <typename T>
-__global__ __launch_bounds__(256) void i8_dequant(hrt_i8_rows_args p, int lpr) {
-  using R = RowVec<T>;
-  using S = typename T::storage;
-  constexpr int V = R::V;
-  const int per = 256 / lpr;
-  const int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / lpr;
-  if ((int)threadIdx.x >= per * lpr || row >= p.rows) return;
-  const float s = gcptr<float>(p.scale)[row];
-  const HK_G uint8_t* const q = gcptr<uint8_t>(p.q) + row * p.q_sr;
-  HK_G S* const x = gptr<S>(p.x) + row * p.x_sr;
-  for (int64_t col = (int64_t)(threadIdx.x % lpr) * 16; col < p.cols; col += (int64_t)lpr * 16) {
-    if (col + 16 <= p.cols) {
-      typedef u32x4 __attribute__((aligned(1))) any1;
-      const u32x4 c = *reinterpret_cast<const HK_G any1*>(q + col);
-#pragma unroll
-      for (int i = 0; i < 16; i += V) {
-        float v[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (float)(int8_t)(c[(i + e) >> 2] >> (8 * (e & 3))) * s;
-        R::put(x + col + i, R::pack(v));
-      }
-    } else {
-      for (int64_t e = col; e < p.cols; ++e) x[e] = T::from_f32((float)(int8_t)q[e] * s);
-    }
-  }
-}
-
 // ---- plan and launch --------------------------------------------------------------------------------------------------------
 // Lanes per row and pieces per lane; 0: the passes.  Few rows of model width are shared by a workgroup: its four wavefronts'
 // loads are all in flight at once.
@@ -566,24 +535,6 @@ bool launch_quant(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   return hrt::launch_ok(hipGetLastError(), ctx, "i8_rows_quant");
 }
 
-template <typename T>
-bool launch_dequant(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
-  const auto& a = *static_cast<const hrt_i8_rows_args*>(pp);
-  constexpr uint64_t E = sizeof(typename T::storage);
-  const int64_t s[3] = {a.x_sr, 0, 0}, qs[3] = {a.q_sr, 0, 0};
-  if (!rows_ok(a.rows, a.cols, 1, 1, {s, qs}, E, {a.x}, ctx)) return false;
-  if (a.scale % 4 != 0 || a.x_sr < a.cols) return ctx.fail("overlapping rows of x, or scale not 4-byte aligned");
-  if (!ctx.check(a.x, rows_span(a.rows, 1, 1, a.cols, s, E), "x") || !ctx.check(a.q, rows_span(a.rows, 1, 1, a.cols, qs, 1), "q") ||
-      !ctx.check(a.scale, a.rows * 4, "scale"))
-    return false;
-  const int64_t pieces = cdiv(a.cols, 16);
-  const int lpr = pieces < 256 ? (int)pieces : 256;
-  const int64_t blocks = cdiv(a.rows, 256 / lpr);
-  if (!hrt::grid_fits(blocks, 256)) return ctx.fail("grid too large");
-  hipLaunchKernelGGL(i8_dequant<T>, dim3((uint32_t)blocks), dim3(256), 0, ctx.stream, a, lpr);
-  return hrt::launch_ok(hipGetLastError(), ctx, "i8_rows_dequant");
-}
-
 // Whether dw is summed by strips of columns in the same launch.
 bool strips(const hrt_rms_bwd_args& a, Share s) { return a.dw && s.lpr && a.rows <= 512; }
 // Rows per workgroup of the backward: with sums of dw as many as leave 512 workgroups.
@@ -638,11 +589,10 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   return hrt::launch_ok(hipGetLastError(), ctx, "rms_bwd");
 }
 
-#define HK_ROWS(SUFFIX, T)                                               \
-  HRT_REGISTER("rms_fwd_" SUFFIX, hrt_rms_args, launch_rms_fwd<T>);      \
-  HRT_REGISTER("rms_bwd_" SUFFIX, hrt_rms_bwd_args, launch_rms_bwd<T>);  \
-  HRT_REGISTER("i8_rows_quant_" SUFFIX, hrt_i8_rows_args, launch_quant<T>); \
-  HRT_REGISTER("i8_rows_dequant_" SUFFIX, hrt_i8_rows_args, launch_dequant<T>)
+#define HK_ROWS(SUFFIX, T)                                              \
+  HRT_REGISTER("rms_fwd_" SUFFIX, hrt_rms_args, launch_rms_fwd<T>);     \
+  HRT_REGISTER("rms_bwd_" SUFFIX, hrt_rms_bwd_args, launch_rms_bwd<T>); \
+  HRT_REGISTER("i8_rows_quant_" SUFFIX, hrt_i8_rows_args, launch_quant<T>)
 HK_ROWS("f32", F32);
 HK_ROWS("bf16", BF16);
 HK_ROWS("f16", F16);

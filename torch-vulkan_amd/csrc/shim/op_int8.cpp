@@ -82,9 +82,6 @@ at::Tensor linear_rows(const Operands& o) {
   return y;
 }
 
-// The weights' values in g's type.
-at::Tensor weights_in(const at::Tensor& w, const at::Tensor& scale, at::ScalarType t) { return dequant_int8_rows_vk(w, scale, t); }
-
 // The rows of a result in the shape of their tensor.  Not a view: nothing else holds the rows, and autograd would forbid in-place
 // operations on a view that was made inside a function of ours.
 at::Tensor in_shape(const at::Tensor& rows, at::IntArrayRef sizes) { return at::_unsafe_view(rows, sizes); }
@@ -108,10 +105,29 @@ struct Linear : torch::autograd::Function<Linear> {
     torch::autograd::variable_list out(6);
     const auto saved = ctx->get_saved_variables();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
-    const at::Tensor g = as_rows(grads[0]);
-    if (ctx->needs_input_grad(0)) out[0] = at::mm(g, weights_in(saved[0], saved[1], g.scalar_type())).view(sizes);
-    if (ctx->saved_data["biased"].toBool() && ctx->needs_input_grad(3)) out[3] = g.sum(0);
+    const at::Tensor g = as_rows(grads[0]), &w = saved[0], &scale = saved[1];
+    const bool wants_x = ctx->needs_input_grad(0), wants_b = ctx->saved_data["biased"].toBool() && ctx->needs_input_grad(3);
     note_gpu("torch_vulkan::int8_linear_backward");
+    if (at::GradMode::is_enabled() && g.requires_grad()) {
+      if (wants_x) out[0] = at::mm(g, dequant_int8_rows_vk(w, scale, g.scalar_type())).view(sizes);
+      if (wants_b) out[3] = g.sum(0);
+      return out;
+    }
+    // the weights' values in g's type and the bias's sums in one launch, then the product
+    const int64_t N = w.size(0), K = w.size(1);
+    const bool product = wants_x && N > 0 && K > 0, sums = wants_b && N > 0 && g.size(0) > 0;
+    const at::Tensor rows = unit_rows(g);
+    at::Tensor v, codes, s;
+    hrt_i8_linear_back_args A{};
+    A.M = g.size(0), A.N = N, A.K = K;
+    if (product) {
+      v = at::empty({N, K}, g.options()), codes = unit_rows(w), s = dense(scale);
+      A.w = dptr(codes), A.w_scale = dptr(s), A.v = dptr(v), A.w_sn = codes.stride(0);
+    }
+    if (wants_b) out[3] = sums ? at::empty({N}, g.options()) : at::zeros({N}, g.options());
+    if (sums) A.g = dptr(rows), A.db = dptr(out[3]), A.g_sm = pitch(rows);
+    if (product || sums) queue(typed("i8_linear_back", g.scalar_type()), A);
+    if (wants_x) out[0] = (product ? at::mm(rows, v) : at::zeros({g.size(0), K}, g.options())).view(sizes);
     return out;
   }
 };

@@ -59,6 +59,11 @@ class I8MmArgs(ctypes.Structure):
                 ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64), ("w_sn", i64)]
 
 
+class I8LinearBackArgs(ctypes.Structure):
+    _fields_ = [("w", u64), ("w_scale", u64), ("v", u64), ("g", u64), ("db", u64), ("M", i64), ("N", i64), ("K", i64),
+                ("w_sn", i64), ("g_sm", i64)]
+
+
 class RmsArgs(ctypes.Structure):
     _fields_ = [("x", u64), ("r", u64), ("w", u64), ("y", u64), ("h_out", u64), ("q", u64), ("scale", u64), ("rstd", u64),
                 ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("xs", i64 * 3), ("rs", i64 * 3), ("eps", f32), ("pad", u32)]
