@@ -8,6 +8,10 @@
 // Lane layout of the 8-bit products (checked on the device), l = lane: 32x32x32: operand row l % 32, bytes 16 (l / 32) .. + 15 of K;
 // 16x16x64: row l % 16, bytes 16 (l / 16) .. + 15; accumulators as for the 16-bit products of the same shape.
 // W is the first operand, so an accumulator holds four consecutive columns n of one row m of y.
+// Measured, M x N x K: 1 x 8192 x 2048 4.6 us, 16 x 8192 x 2048 5.7, 308 x 2048 x 2048 7.6, 1024 x 2048 x 8192 36, 4096 x 8192 x 2048 71 us
+// (1.94 POP/s), 4096 x 2048 x 8192 65 (2.1), 8192 cubed 436 us, 2.52 POP/s (a library's 8-bit product of that size: 526).
+// Bound on the large tiles: the matrix cores' 2048 cycles a step, LDS's 2048 (192 KiB of fragments, 64 KiB of copies) and the copies'
+// own 2200 overlap to 4000; prefetching into L2, a third stage and 128 x 128 sub-tiles on four wavefronts did not change that.
 #include <utility>
 
 #include "../hrt/registry.h"
@@ -170,7 +174,9 @@ constexpr int kLine = 128;  // bytes and values of K in a row of a stage
 
 // A workgroup's wavefronts are KG groups along K times a grid of WM x WN sub-tiles; a step takes a line per group.  KG > 1 gives
 // small grids the wavefronts that hide a copy's latency without a second launch; the groups' sums are added at the end (whole
-// numbers: the order is free).  Both operands have a ring of R stages.
+// numbers: the order is free).  Both operands have a ring of R stages.  A step's copies are issued between the products of its
+// first SP slices (0: all at its start, where every wavefront of the workgroup then waits at issue for the others' to be taken:
+// 8192 cubed on 256 x 256 tiles 454 us, so 436; on 128 x 256 ones 504, so 485; the smaller tiles do not gain).
 template <int BM, int BN, int WM, int WN, int KG, int R>
 struct TileShape {
   static constexpr int NWT = (BM / WM) * (BN / WN), NW = NWT * KG;    // wavefronts per group, in all
@@ -180,7 +186,7 @@ struct TileShape {
   static_assert(XT % (1024 * NW) == 0 && WT % (1024 * NW) == 0, "copy split");
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int KG, int R>
+template <typename T, int BM, int BN, int WM, int WN, int KG, int R, int SP>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i8_mm_args p, int tiles_n, int nk, bool lines) {
   using S = TileShape<BM, BN, WM, WN, KG, R>;
   constexpr int NWT = S::NWT, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN;
@@ -218,15 +224,17 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
   }
   // The last stage may hold fewer values: chunks past K are zeros (a select, not a branch: the compiler counts the copies in
   // flight along every path).
-  auto copy = [&](auto ic, int ks) HK_INLINE {
+  auto copies = [&](auto ic, int ks, int from, int to) HK_INLINE {
     const __amdgpu_buffer_rsrc_t xr = edge_rsrc(Xb + (int64_t)ks * (KG * kLine)), wr = edge_rsrc(Wb + (int64_t)ks * (KG * kLine));
     const int64_t left = p.K - (int64_t)ks * (KG * kLine);
     const int l = left >= KG * kLine ? KG * kLine : (int)left;
 #pragma unroll
-    for (int i = 0; i < IPX; ++i) edge_copy(xr, xbuf(ic), wave * IPX + i, byte_of(wave * IPX + i, BM) < l ? xo[i] : kNoRow);
-#pragma unroll
-    for (int i = 0; i < IPW; ++i) edge_copy(wr, wbuf(ic), wave * IPW + i, byte_of(wave * IPW + i, BN) < l ? wo[i] : kNoRow);
+    for (int i = from; i < to; ++i) {
+      if (i < IPX) edge_copy(xr, xbuf(ic), wave * IPX + i, byte_of(wave * IPX + i, BM) < l ? xo[i < IPX ? i : 0] : kNoRow);
+      else edge_copy(wr, wbuf(ic), wave * IPW + i - IPX, byte_of(wave * IPW + i - IPX, BN) < l ? wo[i < IPX ? 0 : i - IPX] : kNoRow);
+    }
   };
+  auto copy = [&](auto ic, int ks) HK_INLINE { copies(ic, ks, 0, IPX + IPW); };
   // This lane's rows: the sub-tile's other 32-row blocks lie a constant further (the swizzle repeats every 16 rows).
   const int xrow = wm * WM + l32, wrow = wn * WN + l32;
 
@@ -253,7 +261,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
       for (int i = 0; i < FM; ++i) xf[s & 1][i] = *reinterpret_cast<const HK_L u32x4*>(xs + tile_off<8>(xrow, 2 * s + h) + i * 32 * kLine);
     };
     read(0);
-    if (!GUARD || ks + R - 1 < nk) copy(std::integral_constant<int, (I + R - 1) % R>(), ks + R - 1);
+    const bool more = !GUARD || ks + R - 1 < nk;
+    if (SP == 0 && more) copy(std::integral_constant<int, (I + R - 1) % R>(), ks + R - 1);
     auto slice = [&](auto sc) HK_INLINE {
       constexpr int SL = decltype(sc)::value;
       __builtin_amdgcn_sched_barrier(0);
@@ -262,7 +271,19 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int i = 0; i < FM; ++i) acc[j][i] = mac32(wf[SL & 1][j], xf[SL & 1][i], acc[j][i]);
+        for (int i = 0; i < FM; ++i) {
+          acc[j][i] = mac32(wf[SL & 1][j], xf[SL & 1][i], acc[j][i]);
+          if constexpr (SL < SP) {  // PER copies a slice, one behind every EV products
+            constexpr int SLICES = SP > 0 ? SP : 1, PER = (IPX + IPW + SLICES - 1) / SLICES, EV = FM * FN / PER;
+            static_assert(SP == 0 || EV >= 1, "a product for each copy");
+            const int q = j * FM + i, c = SL * PER + q / EV;
+            if (q % EV == EV - 1 && q / EV < PER && c < IPX + IPW) {
+              __builtin_amdgcn_sched_barrier(0);
+              if (more) copies(std::integral_constant<int, (I + R - 1) % R>(), ks + R - 1, c, c + 1);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        }
     };
     slice(std::integral_constant<int, 0>()), slice(std::integral_constant<int, 1>());
     slice(std::integral_constant<int, 2>()), slice(std::integral_constant<int, 3>());
@@ -391,23 +412,28 @@ struct Tile2 {
 constexpr Tile2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
 
 int64_t tiles_of(const hrt_i8_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
-// Index of the tile, -1: i8_rows.
+// Index of the tile, -1: i8_rows (up to 16 rows, or 32 where K is short).
+// Tiles: one workgroup fits a CU, so a grid runs in rounds of 256, each a fixed cost (first copies, epilogue) and a time per 128 values
+// of K, both fitted to full rounds of K 2048 and 8192; a grid that does not fill its rounds runs up to a fifth faster.  Measured, us
+// (tiles in this order): 4096 x 8192 x 2048 71, 83, 105, 229; 4096 x 2048 x 8192 85, 65, 80, 148; 2048 cubed 28, 17.5, 16.4, 30;
+// 308 x 2048 x 2048 24, 14.8, 11.6, 7.5; over 26 drawn sizes the choice is 1% behind the best.
 int plan_of(const hrt_i8_mm_args& a) {
   if (a.x_scale == 0 || a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
-  static constexpr struct { float fixed, per128; } kCost[4] = {{11.f, 1.9f}, {7.4f, 1.4f}, {5.4f, 0.74f}, {4.2f, 0.25f}};
+  static constexpr struct { float fixed, per128; } kCost[4] = {{11.f, 1.5f}, {9.f, 0.82f}, {6.7f, 0.525f}, {3.6f, 0.235f}};
   int best = 3;
   float us = 0.f;
   for (int t = 3; t >= 0; --t) {
-    const float e = (float)cdiv(tiles_of(a, t), 256) * (kCost[t].fixed + kCost[t].per128 * (float)a.K / 128.f);
+    const float rounds = (float)cdiv(tiles_of(a, t), 256), fill = (float)tiles_of(a, t) / (256.f * rounds);
+    const float e = rounds * (kCost[t].fixed + kCost[t].per128 * (float)a.K / 128.f) * (fill > 0.5f ? 0.6f + 0.4f * fill : 0.8f);
     if (t == 3 || e < us) best = t, us = e;
   }
   return best;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int KG, int R>
+template <typename T, int BM, int BN, int WM, int WN, int KG, int R, int SP>
 void queue_tile(const hrt_i8_mm_args& a, hipStream_t s, bool lines) {
   const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, kLine * KG);
-  hipLaunchKernelGGL((i8_tile<T, BM, BN, WM, WN, KG, R>), dim3((uint32_t)(tm * tn)), dim3(64 * TileShape<BM, BN, WM, WN, KG, R>::NW), 0, s, a, (int)tn,
+  hipLaunchKernelGGL((i8_tile<T, BM, BN, WM, WN, KG, R, SP>), dim3((uint32_t)(tm * tn)), dim3(64 * TileShape<BM, BN, WM, WN, KG, R>::NW), 0, s, a, (int)tn,
                      (int)nk, lines);
 }
 
@@ -415,10 +441,10 @@ template <typename T>
 void queue_mm(const hrt_i8_mm_args& a, int tile, hipStream_t s) {
   const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0 && a.w_scale % 16 == 0, lines = vec && a.N % 8 == 0 && a.y % 16 == 0;
   switch (tile) {
-    case 0: return queue_tile<T, 256, 256, 128, 64, 1, 2>(a, s, lines);
-    case 1: return queue_tile<T, 128, 256, 64, 64, 1, 2>(a, s, lines);
-    case 2: return queue_tile<T, 128, 128, 64, 64, 2, 2>(a, s, lines);
-    case 3: return queue_tile<T, 64, 64, 32, 64, 4, 2>(a, s, lines);
+    case 0: return queue_tile<T, 256, 256, 128, 64, 1, 2, 2>(a, s, lines);
+    case 1: return queue_tile<T, 128, 256, 64, 64, 1, 3, 3>(a, s, lines);
+    case 2: return queue_tile<T, 128, 128, 64, 64, 2, 2, 0>(a, s, lines);
+    case 3: return queue_tile<T, 64, 64, 32, 64, 4, 2, 0>(a, s, lines);
   }
   // wavefronts and batches that cover K once where they can
   const dim3 grid((uint32_t)cdiv(a.N, 16));
