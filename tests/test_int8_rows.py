@@ -435,3 +435,51 @@ def test_replayed_graph(M):
         assert all(torch.equal(a.cpu(), b_) for a, b_ in zip(out["y"], eager))
         assert all(torch.equal(a.cpu(), b_) for a, b_ in zip(run(), eager))
     rt.graph_destroy(gid)
+
+
+@pytest.mark.gpu
+def test_rows_far_apart():
+    """8-bit rows 2^30 bytes apart are copied together first, 16-bit ones are quantised where they lie."""
+    x, w, s, b = operands(3, 24, 64, torch.bfloat16, 3)
+    far = torch.zeros((1 << 31) + 4096, dtype=torch.int8, device=vk)
+    wide = far.as_strided((3, 64), (1 << 30, 1))
+    wide.copy_(w[:3].to(vk))
+    got = torch_vulkan.int8_linear(x.to(vk), wide, s[:3].to(vk), b[:3].to(vk))
+    assert torch.equal(got.cpu(), torch_vulkan.int8_linear(x.to(vk), w[:3].to(vk), s[:3].to(vk), b[:3].to(vk)).cpu())
+    assert torch.equal(torch_vulkan.dequant_int8_rows(wide, s[:3].to(vk)).cpu(), torch_vulkan.dequant_int8_rows(w[:3], s[:3]))
+    G = torch.randn((3, 3), generator=torch.Generator().manual_seed(1)).bfloat16().to(vk)
+    X = x.to(vk).requires_grad_()
+    (dx,) = torch.autograd.grad(torch_vulkan.int8_linear(X, wide, s[:3].to(vk)), X, G)
+    (want,) = torch.autograd.grad(torch_vulkan.int8_linear(X, w[:3].to(vk), s[:3].to(vk)), X, G)
+    assert torch.equal(dx.cpu(), want.cpu())
+    del far, wide
+    far = torch.zeros((1 << 31) + 4096, dtype=torch.bfloat16, device=vk)
+    wide = far.as_strided((3, 64), (1 << 30, 1))
+    wide.copy_(x.to(vk))
+    got = torch_vulkan.int8_linear(wide, w.to(vk), s.to(vk), b.to(vk))
+    assert torch.equal(got.cpu(), torch_vulkan.int8_linear(x.to(vk), w.to(vk), s.to(vk), b.to(vk)).cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(20000, 72, 48), (3, 50000, 32), (700, 20011, 16)])
+def test_long_and_thin(M, N, K):
+    x, w, s, b = operands(M, N, K, torch.bfloat16, 5)
+    codes, scale = packed(x)
+    y, want = product(codes, scale, w, s, b)
+    X, B = x.to(vk).requires_grad_(), b.to(vk).requires_grad_()
+    out = torch_vulkan.int8_linear(X, w.to(vk), s.to(vk), B)
+    check_forward(out, y, want, torch.bfloat16)
+    g = torch.randn((M, N), generator=torch.Generator().manual_seed(3)).bfloat16()
+    dx, db = torch.autograd.grad(out, (X, B), g.to(vk))
+    check_back(dx, g, w, s, torch.bfloat16)
+    want = f64(g).sum(0)
+    assert (np.abs(f64(db) - want) <= 2.0**-8 * np.abs(want) + M * 2.0**-24 * np.abs(f64(g)).sum(0)).all()
+
+
+@pytest.mark.gpu
+def test_an_expanded_gradient():
+    x, w, s, b = operands(6, 24, 64, torch.bfloat16, 3)
+    X, B = x.to(vk).requires_grad_(), b.to(vk).requires_grad_()
+    dx, db = torch.autograd.grad(torch_vulkan.int8_linear(X, w.to(vk), s.to(vk), B).sum(), (X, B))
+    check_back(dx, torch.ones(6, 24).bfloat16(), w, s, torch.bfloat16)
+    assert (db.cpu() == 6).all()

@@ -341,3 +341,61 @@ def test_two_threads():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows, heads and outputs that begin more than 2^31 elements into their tensors."""
+    far = torch.zeros((1 << 31) + 8192, dtype=torch.bfloat16, device=vk)
+    x, w, r, gy, gh = data((3, 2, 136), torch.bfloat16, 12)
+    view = far.as_strided((3, 2, 136), (1 << 30, 1 << 12, 1))  # the last row lies 2^31 + 2^12 in
+    view.copy_(x.to(vk))
+    X, C, W, R = view.detach().requires_grad_(), x.to(vk).requires_grad_(), w.to(vk).requires_grad_(), r.to(vk)
+    for a in (torch_vulkan.rms_norm_int8(view, W.detach(), residual=R), torch_vulkan.rms_norm_int8(R, W.detach(), residual=view)):
+        b = torch_vulkan.rms_norm_int8(C.detach(), W.detach(), residual=R)
+        assert all(torch.equal(p.cpu(), q.cpu()) for p, q in zip(a, b))
+    a, b = torch_vulkan.rms_norm(X, W), torch_vulkan.rms_norm(C, W)
+    assert torch.equal(a.detach().cpu(), b.detach().cpu())
+    for p, q in zip(torch.autograd.grad(a, (X, W), gy.to(vk)), torch.autograd.grad(b, (C, W), gy.to(vk))):
+        assert torch.equal(p.cpu(), q.cpu())
+    assert all(torch.equal(p.cpu(), q.cpu()) for p, q in zip(torch_vulkan.quantize_int8_rows(view), torch_vulkan.quantize_int8_rows(x.to(vk))))
+    del far, view, X, a
+    n = (1 << 31) // 4096 + 3  # outputs past 2^31 elements
+    y = torch_vulkan.rms_norm(torch.ones(1, 4096, dtype=torch.bfloat16, device=vk).expand(n, 4096), None, eps=0.0)
+    q, s = torch_vulkan.rms_norm_int8(torch.ones(1, 4096, dtype=torch.bfloat16, device=vk).expand(n, 4096), None, eps=0.0)
+    assert (y[-4:].cpu() == 1).all() and (q[-4:].cpu() == 127).all() and (s[-4:].cpu() == torch.tensor(1.0) / 127).all()
+    z = torch_vulkan.dequant_int8_rows(q, s)
+    assert (z[-4:].cpu() == 1).all()
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_a_live_eager_one():
+    """Two recordings of the same leaves, replayed in turn, with gradients that accumulate, while an eager graph of them lives."""
+    rt = abi.Runtime()
+    x, w, r, gy, gh = (t.to(vk) for t in data((1500, 264), torch.float32, 8))
+    X, W = x.detach().requires_grad_(), w.detach().requires_grad_()
+    live = torch_vulkan.rms_norm(X, W)
+
+    def step(g):
+        with torch.autograd.set_multithreading_enabled(False):
+            torch_vulkan.rms_norm(X, W, residual=r)[0].backward(g)
+
+    want = []
+    for g in (gy, gh):
+        X.grad = W.grad = None
+        step(g)
+        want.append((X.grad.cpu(), W.grad.cpu()))
+    step(gy)  # gradients exist: what is recorded adds to them
+    held = X.grad, W.grad
+    ids = [rt.graph(lambda g=g: step(g)) for g in (gy, gh)]
+    assert X.grad is held[0] and W.grad is held[1]
+    for i in (0, 1, 1, 0):
+        X.grad.zero_(), W.grad.zero_()
+        rt.graph_launch(ids[i])
+        assert torch.equal(X.grad.cpu(), want[i][0]) and torch.equal(W.grad.cpu(), want[i][1])
+    X.grad = W.grad = None
+    live.backward(gy)
+    (dx, dw) = torch.autograd.grad(torch_vulkan.rms_norm(X, W), (X, W), gy)
+    assert torch.equal(X.grad.cpu(), dx.cpu()) and torch.equal(W.grad.cpu(), dw.cpu())
+    for i in ids:
+        rt.graph_destroy(i)

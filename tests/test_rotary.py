@@ -239,6 +239,24 @@ def test_replayed_graph():
     rt.graph_destroy(gid)
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    far = torch.zeros((1 << 31) + 8192, dtype=torch.bfloat16, device=vk)
+    sections, pos, freqs = (5, 3), grid((2, 3)).to(vk), torch_vulkan.rotary_frequencies((5, 3)).to(vk)
+    q, k, _, _ = data(3, 2, 2, 6, 24, torch.bfloat16, 12)
+    view = far.as_strided((3, 2, 6, 24), (1 << 30, 1 << 11, 24, 1))
+    view.copy_(q.to(vk))
+    for a, b in ((view, k.to(vk)), (k.to(vk), view)):
+        got = torch_vulkan.rotary_embedding(a, b, pos, freqs, sections)
+        want = torch_vulkan.rotary_embedding(a.contiguous(), b.contiguous(), pos, freqs, sections)
+        assert all(torch.equal(x.cpu(), y.cpu()) for x, y in zip(got, want))
+    del far, view
+    S = (1 << 31) // (128 * 64) + 5  # outputs past 2^31 elements
+    one = torch.ones(1, 1, 1, 64, dtype=torch.bfloat16, device=vk).expand(1, 128, S, 64)
+    y = torch_vulkan.rotary_embedding(one, None, torch.zeros(S, 1, dtype=torch.int32, device=vk), freqs, (8,))
+    assert (y[:, :, -3:].cpu() == 1).all()
+
+
 # ---- the operators of a block on an 8-bit base together -----------------------------------------------------------------
 class Block(torch.nn.Module):
     """Self-attention and MLP of a transformer block on frozen 8-bit weights with trained adapters: residual norms, 8-bit products,

@@ -476,10 +476,9 @@ bool launch_i8_mm(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
       (!q && !ctx.check(a.x_scale, (uint64_t)a.M * 4, "x_scale")) || !ctx.check(a.w_scale, (uint64_t)a.N * 4, "w_scale") ||
       !ctx.check(a.y, (uint64_t)(a.M * a.N) * 2, "y") || (a.bias && !ctx.check(a.bias, (uint64_t)a.N * 2, "bias")))
     return false;
-  // offsets of a tile's rows are 31-bit
-  const int64_t lim = (int64_t)1 << 31;
-  if (a.x_sm * 257 >= lim || a.w_sn * 257 >= lim) return ctx.fail("operand rows too long for one launch");
   const int tile = plan_of(a);
+  const int64_t lim = (int64_t)1 << 31;  // offsets of a tile's rows are 31-bit
+  if (tile >= 0 && (a.x_sm * 257 >= lim || a.w_sn * 257 >= lim)) return ctx.fail("operand rows too long for one launch");
   if (!hrt::grid_fits(tile < 0 ? cdiv(a.N, 16) : tiles_of(a, tile), 512)) return ctx.fail("grid too large");
   queue_mm<T>(a, tile, ctx.stream);
   return hrt::launch_ok(hipGetLastError(), ctx, "i8_mm");
