@@ -1,8 +1,10 @@
 // Root-mean-square norm of rows, forward ("rms_fwd_*") and backward ("rms_bwd_*"), and rows into 8 bits ("i8_rows_quant_*").
 //
-// Bound by memory: a row is read once, held in registers as fp32 and written once.  16, 64 or 256 lanes share a row (heads,
-// model widths, wide rows or few of them), which DPP steps and lane swaps add up without LDS, or through four floats of it.
-// Rows longer than a workgroup's registers take several passes.
+// Bound by memory: a row is read once, held in registers as fp32 and written once.  16, 64, 256 or 1024 lanes share a row (heads,
+// model widths, wide rows or few of them), which DPP steps and lane swaps add up without LDS, or through a few floats of it.
+// Rows longer than a workgroup's registers take several passes.  Measured, GPU us (bf16, forward with a residual, backward with dw, without):
+// 1 x 2048 3.1, 3.3, 3.0; 4020 x 2048 12.3, 15.7, 10.4 (66 and 82 MB: 5.4 and 5.2 TB/s); 65536 x 128 14.0, 15.6, 10.3; 16384 x 2048 43, 38,
+// 32.  Into 8 bits without the norm: 4020 x 2048 5.6, 8192 x 2048 9.5.
 #include <initializer_list>
 
 #include "../hrt/registry.h"
@@ -17,17 +19,20 @@ __device__ __forceinline__ int64_t row_at(int64_t row, int64_t n1, int64_t n2, c
   return (int64_t)i0 * s[0] + (int64_t)(t - i0 * (uint32_t)n1) * s[1] + (int64_t)(r - t * (uint32_t)n2) * s[2];
 }
 
+// Threads of a workgroup whose rows are shared by LPR lanes each.
+constexpr int threads_of(int lpr) { return lpr > 256 ? lpr : 256; }
+
 enum Mode { kNorm, kNorm8, kQuant };
 
 // kQuant reads rows x (stride xs[0]) and writes codes (pitch r, a plain number there) and scales; its arguments come in the same
 // block, so that one kernel serves all three.
 template <typename T, int MODE, int LPR, int NV, bool TAIL>
-__global__ __launch_bounds__(256) void rms_rows(hrt_rms_args p, int64_t q_sr) {
+__global__ __launch_bounds__(threads_of(LPR)) void rms_rows(hrt_rms_args p, int64_t q_sr) {
   using R = RowVec<T>;
   using S = typename T::storage;
-  constexpr int V = R::V, RPB = 256 / LPR;
-  __shared__ float red[4];
-  __shared__ uint32_t redu[4];
+  constexpr int V = R::V, RPB = threads_of(LPR) / LPR;
+  __shared__ float red[threads_of(LPR) / 64];
+  __shared__ uint32_t redu[threads_of(LPR) / 64];
   const int lane = threadIdx.x % LPR;
   const int64_t row0 = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
   const bool live = row0 < p.rows;
@@ -36,25 +41,25 @@ __global__ __launch_bounds__(256) void rms_rows(hrt_rms_args p, int64_t q_sr) {
   u32x4 a[NV], b[NV], w[NV];
   const bool res = MODE != kQuant && p.r, has_w = MODE != kQuant && p.w;
 #pragma unroll
-  for (int c = 0; c < NV; ++c) a[c] = row_piece<T, TAIL>(x, (int64_t)(c * LPR + lane) * V, p.D);
+  for (int c = 0; c < NV; ++c) a[c] = row_load<T, TAIL>(x, (int64_t)(c * LPR + lane) * V, p.D);
   if (res) {
     const HK_G S* const r = gcptr<S>(p.r) + row_at(row, p.n1, p.n2, p.rs);
 #pragma unroll
-    for (int c = 0; c < NV; ++c) b[c] = row_piece<T, TAIL>(r, (int64_t)(c * LPR + lane) * V, p.D);
+    for (int c = 0; c < NV; ++c) b[c] = row_load<T, TAIL>(r, (int64_t)(c * LPR + lane) * V, p.D);
   }
   if (has_w) {
 #pragma unroll
-    for (int c = 0; c < NV; ++c) w[c] = row_piece<T, TAIL>(gcptr<S>(p.w), (int64_t)(c * LPR + lane) * V, p.D);
+    for (int c = 0; c < NV; ++c) w[c] = row_load<T, TAIL>(gcptr<S>(p.w), (int64_t)(c * LPR + lane) * V, p.D);
   }
   float v[NV][V];
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < NV; ++c) {
     const int64_t col = (int64_t)(c * LPR + lane) * V;
-    R::unpack(a[c], v[c]);
+    R::unpack(row_fix<T, TAIL>(a[c], col, p.D), v[c]);
     if (res) {
       float t[V];
-      R::unpack(b[c], t);
+      R::unpack(row_fix<T, TAIL>(b[c], col, p.D), t);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[c][e] += t[e];
       if (p.h_out && live) row_put<T, TAIL>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v[c]));
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(256) void rms_rows(hrt_rms_args p, int64_t q_sr) {
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       float t[V];
-      if (has_w) R::unpack(w[c], t);
+      if (has_w) R::unpack(row_fix<T, TAIL>(w[c], (int64_t)(c * LPR + lane) * V, p.D), t);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[c][e] = has_w ? v[c][e] * rstd * t[e] : v[c][e] * rstd;
     }
@@ -196,20 +201,14 @@ __global__ __launch_bounds__(256) void rms_long(hrt_rms_args p, int64_t q_sr) {
   }
 }
 
-// Four floats of a row of D, zeros behind it.
-__device__ __forceinline__ f32x4 row_piece_f32(const float* row, int64_t col, int64_t D) {
-  const u32x4 w = row_piece<F32, true>(gcptr<float>(reinterpret_cast<uint64_t>(row)), col, D);
-  return __builtin_bit_cast(f32x4, w);
-}
-
 // ---- backward -------------------------------------------------------------------------------------------------------------
 // dw where there are few rows: the workgroups behind those that take rows have strips of 128 bytes of columns each, of all rows
-// (which the others read too: from L2).  A second launch costs more than their reads: 308 x 1001 fp32 both ways 33 us, so 27.
-template <typename T, bool TAIL>
+// (which the others read too: from L2).
+template <typename T, bool TAIL, int TPB>
 __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) {
   using R = RowVec<T>;
   using S = typename T::storage;
-  constexpr int V = R::V, G = 32;  // rows at a time
+  constexpr int V = R::V, G = TPB / 8;  // rows at a time
   __shared__ float red[G][8 * V + 1];
   const int lane = threadIdx.x & 7, group = threadIdx.x >> 3;
   const int64_t col = ((int64_t)strip * 8 + lane) * V;
@@ -223,15 +222,15 @@ __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) 
     for (int u = 0; u < 4; ++u) {  // four rows' loads in flight; a row past the end repeats the last one
       const int64_t row = r0 + u * G < p.rows ? r0 + u * G : p.rows - 1;
       a[u] = u32x4{0, 0, 0, 0};
-      if (p.gy) a[u] = row_piece<T, TAIL>(gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys), col, p.D);
-      b[u] = row_piece<T, TAIL>(gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs), col, p.D);
+      if (p.gy) a[u] = row_load<T, TAIL>(gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys), col, p.D);
+      b[u] = row_load<T, TAIL>(gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs), col, p.D);
       rstd[u] = gcptr<float>(p.rstd)[row];
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float d[V], n[V];
-      R::unpack(a[u], d);
-      R::unpack(b[u], n);
+      R::unpack(row_fix<T, TAIL>(a[u], col, p.D), d);
+      R::unpack(row_fix<T, TAIL>(b[u], col, p.D), n);
       if (r0 + u * G < p.rows) {
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] += d[e] * (n[e] * rstd[u]);
@@ -244,22 +243,22 @@ __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) 
   const int64_t at = (int64_t)strip * 8 * V + threadIdx.x;
   if ((int)threadIdx.x >= 8 * V || at >= p.D) return;
   float t = red[0][threadIdx.x];
-#pragma unroll
+#pragma unroll 8
   for (int k = 1; k < G; ++k) t += red[k][threadIdx.x];
   gptr<S>(p.dw)[at] = T::from_f32(t);
 }
 
-// A workgroup takes `per` consecutive rows, 256 / LPR at a time.  DW: a lane adds gy n of its columns up over its rows, the
+// A workgroup takes `per` consecutive rows, one for every LPR threads at a time.  DW: a lane adds gy n of its columns up over its rows, the
 // workgroup's lanes of a column are added in order through LDS, and the sums of all workgroups by rms_dw_sum.
 template <typename T, int LPR, int NV, bool TAIL, bool DW>
-__global__ __launch_bounds__(256) void rms_back(hrt_rms_bwd_args p, int64_t per, int blocks) {
+__global__ __launch_bounds__(threads_of(LPR)) void rms_back(hrt_rms_bwd_args p, int64_t per, int blocks) {
   using R = RowVec<T>;
   using S = typename T::storage;
-  constexpr int V = R::V, RPB = 256 / LPR;
+  constexpr int V = R::V, RPB = threads_of(LPR) / LPR;
   if constexpr (!DW) {
-    if ((int)blockIdx.x >= blocks) return rms_strip<T, TAIL>(p, (int)blockIdx.x - blocks);
+    if ((int)blockIdx.x >= blocks) return rms_strip<T, TAIL, threads_of(LPR)>(p, (int)blockIdx.x - blocks);
   }
-  __shared__ float red[2][4];
+  __shared__ float red[2][threads_of(LPR) / 64];
   __shared__ __attribute__((aligned(16))) float part[DW && RPB > 1 ? RPB * LPR * NV * V : 4];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const int64_t first = (int64_t)blockIdx.x * per, end = first + per < p.rows ? first + per : p.rows;
@@ -284,19 +283,20 @@ __global__ __launch_bounds__(256) void rms_back(hrt_rms_bwd_args p, int64_t per,
     for (int c = 0; c < NV; ++c) {
       const int64_t col = (int64_t)(c * LPR + lane) * V;
       a[c] = g[c] = u32x4{0, 0, 0, 0};
-      b[c] = row_piece<T, TAIL>(h, col, p.D);
-      if (p.gy) a[c] = row_piece<T, TAIL>(gy, col, p.D);
+      b[c] = row_load<T, TAIL>(h, col, p.D);
+      if (p.gy) a[c] = row_load<T, TAIL>(gy, col, p.D);
     }
     if (p.gh) {
       const HK_G S* const gh = gcptr<S>(p.gh) + row_at(row, p.n1, p.n2, p.ghs);
 #pragma unroll
-      for (int c = 0; c < NV; ++c) g[c] = row_piece<T, TAIL>(gh, (int64_t)(c * LPR + lane) * V, p.D);
+      for (int c = 0; c < NV; ++c) g[c] = row_load<T, TAIL>(gh, (int64_t)(c * LPR + lane) * V, p.D);
     }
     float d[NV][V], n[NV][V];
     float dot = 0.f;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int64_t col = (int64_t)(c * LPR + lane) * V;
+      a[c] = row_fix<T, TAIL>(a[c], col, p.D), b[c] = row_fix<T, TAIL>(b[c], col, p.D);
       if (!live || (!TAIL && col >= p.D)) a[c] = u32x4{0, 0, 0, 0}, b[c] = u32x4{0, 0, 0, 0};
       float t[V];
       R::unpack(a[c], d[c]);
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void rms_back(hrt_rms_bwd_args p, int64_t per,
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       float t[V];
-      R::unpack(g[c], t);
+      R::unpack(row_fix<T, TAIL>(g[c], (int64_t)(c * LPR + lane) * V, p.D), t);
 #pragma unroll
       for (int e = 0; e < V; ++e) t[e] = fmaf(rstd, fmaf(-n[c][e], dot, d[c][e]), t[e]);
       row_put<T, TAIL>(gptr<S>(p.dx) + row * p.D, (int64_t)(c * LPR + lane) * V, p.D, R::pack(t));
@@ -397,36 +397,28 @@ __global__ __launch_bounds__(256) void rms_back_long(hrt_rms_bwd_args p, int64_t
   }
 }
 
-// dw: the workgroups' sums of 32 columns, a thread every 128th of them in order (four loads in flight: one round for 512), then
-// the 128 of a column in a fixed tree.
+// dw: the workgroups' sums of 32 columns, a thread every 32nd of one column in order (16 loads in flight: one round for 512), then the
+// 32 of a column in order.
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_dw_sum(const float* ws, typename T::storage* dw, int64_t parts, int64_t D) {
-  constexpr int G = 128;
-  __shared__ float red[G][33];
-  const int quad = threadIdx.x & 7, group = threadIdx.x >> 3;
-  const int64_t col = (int64_t)blockIdx.x * 32 + quad * 4;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t c = group; c < parts; c += 4 * G) {
-    f32x4 v[4];
+  constexpr int U = 16;
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+  const int64_t at = (int64_t)blockIdx.x * 32 + lane, col = at < D ? at : D - 1;
+  float s = 0.f;
+  for (int64_t c = group; c < parts; c += 32 * U) {
+    float v[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = row_piece_f32(ws + (c + u * G < parts ? c + u * G : parts - 1) * D, col, D);
+    for (int u = 0; u < U; ++u) v[u] = ws[(c + u * 32 < parts ? c + u * 32 : parts - 1) * D + col];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (c + u * G < parts) s += v[u];
+    for (int u = 0; u < U; ++u) s += c + u * 32 < parts ? v[u] : 0.f;
   }
+  red[group][lane] = s;
+  __syncthreads();
+  if (group > 0 || at >= D) return;
+  float o = red[0][lane];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) red[group][quad * 4 + e] = s[e];
-  __syncthreads();
-  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;  // four of the 128, then the 32 sums
-  const float t = (red[4 * k][c] + red[4 * k + 1][c]) + (red[4 * k + 2][c] + red[4 * k + 3][c]);
-  __syncthreads();
-  red[k][c] = t;
-  __syncthreads();
-  const int64_t at = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  if (threadIdx.x >= 32 || at >= D) return;
-  float o = red[0][threadIdx.x];
-#pragma unroll
-  for (int i = 1; i < 32; ++i) o += red[i][threadIdx.x];
+  for (int i = 1; i < 32; ++i) o += red[i][lane];
   dw[at] = T::from_f32(o);
 }
 
@@ -445,6 +437,7 @@ Share share_of(int64_t rows, int64_t D, int V) {
   if (n <= 256) return rows >= 1024 ? Share{64, 4} : Share{256, 1};
   if (n <= 512) return {256, 2};
   if (n <= 1024) return {256, 4};
+  if (n <= 2048) return {1024, 2};
   return {0, 0};
 }
 
@@ -460,6 +453,7 @@ void with_share(Share s, F f) {
   HK_SHARE(256, 1);
   HK_SHARE(256, 2);
   HK_SHARE(256, 4);
+  HK_SHARE(1024, 2);
 #undef HK_SHARE
 }
 
@@ -472,12 +466,12 @@ bool queue_rows(const hrt_rms_args& a, int64_t q_sr, hrt::LaunchCtx& ctx) {
     hipLaunchKernelGGL((rms_long<T, MODE>), dim3((uint32_t)a.rows), dim3(256), 0, ctx.stream, a, q_sr);
     return true;
   }
-  const int64_t blocks = cdiv(a.rows, 256 / s.lpr);
-  if (!hrt::grid_fits(blocks, 256)) return ctx.fail("grid too large");
+  const int64_t blocks = cdiv(a.rows, threads_of(s.lpr) / s.lpr);
+  if (!hrt::grid_fits(blocks, threads_of(s.lpr))) return ctx.fail("grid too large");
   with_share(s, [&](auto lc, auto nc) {
     constexpr int L = decltype(lc)::value, N = decltype(nc)::value;
-    if (a.D % V == 0) hipLaunchKernelGGL((rms_rows<T, MODE, L, N, false>), dim3((uint32_t)blocks), dim3(256), 0, ctx.stream, a, q_sr);
-    else hipLaunchKernelGGL((rms_rows<T, MODE, L, N, true>), dim3((uint32_t)blocks), dim3(256), 0, ctx.stream, a, q_sr);
+    if (a.D % V == 0) hipLaunchKernelGGL((rms_rows<T, MODE, L, N, false>), dim3((uint32_t)blocks), dim3(threads_of(L)), 0, ctx.stream, a, q_sr);
+    else hipLaunchKernelGGL((rms_rows<T, MODE, L, N, true>), dim3((uint32_t)blocks), dim3(threads_of(L)), 0, ctx.stream, a, q_sr);
   });
   return true;
 }
@@ -535,12 +529,14 @@ bool launch_quant(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   return hrt::launch_ok(hipGetLastError(), ctx, "i8_rows_quant");
 }
 
-// Whether dw is summed by strips of columns in the same launch.
-bool strips(const hrt_rms_bwd_args& a, Share s) { return a.dw && s.lpr && a.rows <= 512; }
-// Rows per workgroup of the backward: with sums of dw as many as leave 512 workgroups.
+// Whether dw is summed by strips of columns in the same launch: the GPU's time then meets that of the two launches at 800 x 800 and
+// 1024 x 2048 (7.6, 9.5 us both ways; 308 x 1000 fp32 4.5 against 7.5, 512 x 8192 bf16 8.8 against 25), the host's is 5 us less.
+bool strips(const hrt_rms_bwd_args& a, Share s) { return a.dw && s.lpr && a.rows <= 1024; }
+// Rows per workgroup of the backward: with sums of dw as many as leave 512 workgroups, or 256 of 1024 threads (4096 x 8192 bf16 47 us
+// with 512 workgroups, 52 with 256; 2000 x 5001 fp32 36 and 32).
 int64_t back_rows(const hrt_rms_bwd_args& a, Share s) {
-  const int64_t rpb = s.lpr ? 256 / s.lpr : 1;
-  return a.dw && !strips(a, s) ? cdiv(cdiv(a.rows, 512), rpb) * rpb : rpb;
+  const int64_t rpb = s.lpr ? threads_of(s.lpr) / s.lpr : 1;
+  return a.dw && !strips(a, s) ? cdiv(cdiv(a.rows, s.lpr > 256 ? 256 : 512), rpb) * rpb : rpb;
 }
 template <typename T>
 int64_t back_blocks(const hrt_rms_bwd_args& a) {
@@ -568,7 +564,7 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   const bool sums = a.dw && !strips(a, s);
   if (sums && !ctx.check(a.ws, (uint64_t)(blocks * a.D) * 4, "ws")) return false;
   const int64_t per = back_rows(a, s), all = blocks + (a.dw && !sums ? cdiv(a.D, 8 * V) : 0);
-  if (!hrt::grid_fits(all, 256)) return ctx.fail("grid too large");
+  if (!hrt::grid_fits(all, threads_of(s.lpr))) return ctx.fail("grid too large");
   const dim3 grid((uint32_t)all);
   if (s.lpr == 0) {
     hipLaunchKernelGGL(rms_back_long<T>, grid, dim3(256), 0, ctx.stream, a, per);
@@ -576,7 +572,7 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
     with_share(s, [&](auto lc, auto nc) {
       constexpr int L = decltype(lc)::value, N = decltype(nc)::value;
       const auto go = [&](auto tail, auto dw) {
-        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value>), grid, dim3(256), 0, ctx.stream, a, per, (int)blocks);
+        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value>), grid, dim3(threads_of(L)), 0, ctx.stream, a, per, (int)blocks);
       };
       using Y = std::true_type;
       using No = std::false_type;

@@ -115,7 +115,8 @@ struct Linear : torch::autograd::Function<Linear> {
     }
     // the weights' values in g's type and the bias's sums in one launch, then the product
     const int64_t N = w.size(0), K = w.size(1);
-    const bool product = wants_x && N > 0 && K > 0, sums = wants_b && N > 0 && g.size(0) > 0;
+    // so many rows that the sums' workgroups (64 columns each) would outlast the rest are summed by themselves: 16384 x 1024 34 us, so 16
+    const bool product = wants_x && N > 0 && K > 0, sums = wants_b && N > 0 && g.size(0) > 0 && g.size(0) <= 8192;
     const at::Tensor rows = unit_rows(g);
     at::Tensor v, codes, s;
     hrt_i8_linear_back_args A{};
@@ -124,7 +125,7 @@ struct Linear : torch::autograd::Function<Linear> {
       v = at::empty({N, K}, g.options()), codes = unit_rows(w), s = dense(scale);
       A.w = dptr(codes), A.w_scale = dptr(s), A.v = dptr(v), A.w_sn = codes.stride(0);
     }
-    if (wants_b) out[3] = sums ? at::empty({N}, g.options()) : at::zeros({N}, g.options());
+    if (wants_b) out[3] = sums ? at::empty({N}, g.options()) : g.sum(0);
     if (sums) A.g = dptr(rows), A.db = dptr(out[3]), A.g_sm = pitch(rows);
     if (product || sums) queue(typed("i8_linear_back", g.scalar_type()), A);
     if (wants_x) out[0] = (product ? at::mm(rows, v) : at::zeros({g.size(0), K}, g.options())).view(sizes);
