@@ -311,6 +311,22 @@ def test_layouts(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 5, 20, 100, 300])
+def test_scales_and_bias_off_their_lines(M):
+    """Slices of longer vectors, which do not begin on 16 bytes; rows given with scales of their own."""
+    x, w, s, b = operands(M, 64, 320, torch.float16, 17)
+    X, W = x.to(vk), w.to(vk)
+    want = torch_vulkan.int8_linear(X, W, s.to(vk), b.to(vk)).cpu()
+    codes, scale = torch_vulkan.quantize_int8_rows(X)
+    for k in (1, 2, 3):
+        S, B = torch.cat([torch.ones(k), s]).to(vk)[k:], torch.cat([torch.ones(k).half(), b]).to(vk)[k:]
+        xs = torch.cat([torch.ones(k), scale.cpu()]).to(vk)[k:]
+        assert torch.equal(torch_vulkan.int8_linear(X, W, S, B).cpu(), want)
+        assert torch.equal(torch_vulkan.int8_linear(codes, W, S, B, x_scale=xs, out_dtype=torch.float16).cpu(), want)
+        assert torch.equal(torch_vulkan.dequant_int8_rows(W, S).cpu(), torch_vulkan.dequant_int8_rows(w, s))
+
+
+@pytest.mark.gpu
 def test_nothing_to_do():
     x, w, s, b = (t.to(vk) for t in operands(4, 24, 32, torch.bfloat16, 1))
     assert torch_vulkan.int8_linear(x[:0], w, s, b).shape == (0, 24)

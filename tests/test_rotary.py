@@ -208,6 +208,8 @@ def test_frequencies_and_cpu_refusals():
     assert torch.allclose(f[:22], 10000.0 ** (-2 * torch.arange(22, dtype=torch.float64) / 44), rtol=1e-14, atol=0)
     with pytest.raises(RuntimeError, match="theta"):
         torch_vulkan.rotary_frequencies((4, 4), (1e4,))
+    with pytest.raises(RuntimeError, match="section"):
+        torch_vulkan.rotary_frequencies(())
     with pytest.raises(RuntimeError, match="vk tensor"):
         torch_vulkan.rotary_embedding(torch.zeros(1, 1, 2, 4), None, torch.zeros(2, 1), f, (2,))
 

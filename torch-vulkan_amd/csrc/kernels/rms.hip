@@ -483,7 +483,8 @@ uint64_t rows_span(int64_t rows, int64_t n1, int64_t n2, int64_t D, const int64_
 }
 bool rows_ok(int64_t rows, int64_t D, int64_t n1, int64_t n2, std::initializer_list<const int64_t*> strides, uint64_t elem,
              std::initializer_list<uint64_t> addrs, hrt::LaunchCtx& ctx) {
-  if (rows <= 0 || D <= 0 || n1 <= 0 || n2 <= 0 || rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 31) || rows % (n1 * n2) != 0)
+  constexpr int64_t lim = int64_t(1) << 31;
+  if (rows <= 0 || D <= 0 || n1 <= 0 || n2 <= 0 || rows >= lim || D >= lim || n1 > rows || n2 > rows || rows % (n1 * n2) != 0)
     return ctx.fail("bad shape");
   for (const int64_t* s : strides)
     for (int i = 0; i < 3; ++i)

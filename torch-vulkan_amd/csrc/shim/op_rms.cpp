@@ -98,6 +98,8 @@ Out forward_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& r, 
   return o;
 }
 
+// With a residual the backward pass reads h as it was rounded: n is then off by half a step of its type in each value, as is a norm's
+// of a stored stream, instead of both of its terms being kept (a tensor of x's size more, read again).
 struct Norm : torch::autograd::Function<Norm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& w,
                                                 const std::optional<at::Tensor>& r, double eps) {

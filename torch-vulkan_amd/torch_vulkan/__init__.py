@@ -432,8 +432,8 @@ def rotary_frequencies(sections, theta=10000.0):
     """Frequencies of rotary_embedding's pairs (float64, on the CPU): theta**(-i / n) for i = 0 .. n - 1 of each section of n pairs.
     theta: one base, or one for each section (scaled ones for positions beyond the trained size)."""
     thetas = [float(theta)] * len(sections) if isinstance(theta, (int, float)) else [float(t) for t in theta]
-    if len(thetas) != len(sections) or any(n < 0 for n in sections):
-        raise RuntimeError("rotary_frequencies: one theta, or one for each section, and no negative sections")
+    if not len(sections) or len(thetas) != len(sections) or any(n < 0 for n in sections):
+        raise RuntimeError("rotary_frequencies: at least one section, none of them negative, and one theta, or one for each section")
     return torch.cat([t ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n, t in zip(sections, thetas)])
 
 
