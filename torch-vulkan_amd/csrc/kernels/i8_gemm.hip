@@ -8,10 +8,10 @@
 // Lane layout of the 8-bit products (checked on the device), l = lane: 32x32x32: operand row l % 32, bytes 16 (l / 32) .. + 15 of K;
 // 16x16x64: row l % 16, bytes 16 (l / 16) .. + 15; accumulators as for the 16-bit products of the same shape.
 // W is the first operand, so an accumulator holds four consecutive columns n of one row m of y.
-// Measured, M x N x K: 1 x 8192 x 2048 4.6 us, 16 x 8192 x 2048 5.7, 308 x 2048 x 2048 7.6, 1024 x 2048 x 8192 36, 4096 x 8192 x 2048 71 us
-// (1.94 POP/s), 4096 x 2048 x 8192 65 (2.1), 8192 cubed 436 us, 2.52 POP/s (a library's 8-bit product of that size: 526).
-// Bound on the large tiles: the matrix cores' 2048 cycles a step, LDS's 2048 (192 KiB of fragments, 64 KiB of copies) and the copies'
-// own 2200 overlap to 4000; prefetching into L2, a third stage and 128 x 128 sub-tiles on four wavefronts did not change that.
+// Measured, M x N x K: 1 x 8192 x 2048 4.6 us, 16 x 8192 x 2048 5.7, 308 x 2048 x 2048 6.4, 1024 x 2048 x 8192 27, 4096 x 8192 x 2048 71 us
+// (1.93 POP/s), 4096 x 2048 x 8192 65 (2.1), 8192 cubed 422 us, 2.6 POP/s (a library's 8-bit product of that size: 526).
+// The largest tiles' step has 2048 cycles of products, 2048 of LDS (192 KiB of fragments, 64 KiB of copies) and 2200 of L2 -> LDS; it takes
+// 2900 on half of the CUs and 4000 on all of them (matrix cores busy 55%).
 #include <utility>
 
 #include "../hrt/registry.h"
@@ -174,27 +174,29 @@ constexpr int kLine = 128;  // bytes and values of K in a row of a stage
 
 // A workgroup's wavefronts are KG groups along K times a grid of WM x WN sub-tiles; a step takes a line per group.  KG > 1 gives
 // small grids the wavefronts that hide a copy's latency without a second launch; the groups' sums are added at the end (whole
-// numbers: the order is free).  Both operands have a ring of R stages.  A step's copies are issued between the products of its
-// first SP slices (0: all at its start, where every wavefront of the workgroup then waits at issue for the others' to be taken:
-// 8192 cubed on 256 x 256 tiles 454 us, so 436; on 128 x 256 ones 504, so 485; the smaller tiles do not gain).
-template <int BM, int BN, int WM, int WN, int KG, int R>
+// numbers: the order is free).  X has a ring of XR stages, W of WR: X may be a step further ahead, which the largest tiles' 160 KiB
+// just hold (4096 x 2048 x 8192 on 128 CUs 84 us, so 78; 8192 cubed 430, so 422).  A step's copies are issued between the products
+// of its first SP slices, W's first (0: all at its start, where every wavefront of the workgroup then waits at issue for the
+// others' to be taken: 8192 cubed on 256 x 256 tiles 454 us, so 436, on 128 x 256 ones 504, so 485; smaller tiles do not gain).
+template <int BM, int BN, int WM, int WN, int KG, int XR, int WR>
 struct TileShape {
   static constexpr int NWT = (BM / WM) * (BN / WN), NW = NWT * KG;    // wavefronts per group, in all
   static constexpr int XT = KG * BM * kLine, WT = KG * BN * kLine;    // bytes of a stage
   static constexpr int IPX = XT / 1024 / NW, IPW = WT / 1024 / NW;    // copies per wavefront
   static constexpr int FM = WM / 32, FN = WN / 32;
+  static constexpr int U = XR == WR ? XR : XR * WR;                   // steps after which the buffers repeat
   static_assert(XT % (1024 * NW) == 0 && WT % (1024 * NW) == 0, "copy split");
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int KG, int R, int SP>
+template <typename T, int BM, int BN, int WM, int WN, int KG, int XR, int WR, int SP>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i8_mm_args p, int tiles_n, int nk, bool lines) {
-  using S = TileShape<BM, BN, WM, WN, KG, R>;
+  using S = TileShape<BM, BN, WM, WN, KG, XR, WR>;
   constexpr int NWT = S::NWT, IPX = S::IPX, IPW = S::IPW, FM = S::FM, FN = S::FN;
   // One LDS object per stage, so that the compiler can tell the reads of one from the copies into another.
-  __shared__ __attribute__((aligned(1024))) uint8_t x0[S::XT], x1[S::XT], x2[R > 2 ? S::XT : 16], x3[R > 3 ? S::XT : 16];
-  __shared__ __attribute__((aligned(1024))) uint8_t w0[S::WT], w1[S::WT], w2[R > 2 ? S::WT : 16], w3[R > 3 ? S::WT : 16];
-  auto xbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? x0 : I == 1 ? x1 : I == 2 ? x2 : x3); };
-  auto wbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? w0 : I == 1 ? w1 : I == 2 ? w2 : w3); };
+  __shared__ __attribute__((aligned(1024))) uint8_t x0[S::XT], x1[S::XT], x2[XR > 2 ? S::XT : 16];
+  __shared__ __attribute__((aligned(1024))) uint8_t w0[S::WT], w1[S::WT], w2[WR > 2 ? S::WT : 16];
+  auto xbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? x0 : I == 1 ? x1 : x2); };
+  auto wbuf = [&](auto ic) HK_INLINE { constexpr int I = decltype(ic)::value; return (HK_L uint8_t*)(I == 0 ? w0 : I == 1 ? w1 : w2); };
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave / NWT, wt = wave % NWT, wm = wt % (BM / WM), wn = wt / (BM / WM), l32 = lane & 31, h = lane >> 5;
@@ -224,17 +226,24 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
   }
   // The last stage may hold fewer values: chunks past K are zeros (a select, not a branch: the compiler counts the copies in
   // flight along every path).
-  auto copies = [&](auto ic, int ks, int from, int to) HK_INLINE {
-    const __amdgpu_buffer_rsrc_t xr = edge_rsrc(Xb + (int64_t)ks * (KG * kLine)), wr = edge_rsrc(Wb + (int64_t)ks * (KG * kLine));
+  auto left_of = [&](int ks) HK_INLINE {
     const int64_t left = p.K - (int64_t)ks * (KG * kLine);
-    const int l = left >= KG * kLine ? KG * kLine : (int)left;
-#pragma unroll
-    for (int i = from; i < to; ++i) {
-      if (i < IPX) edge_copy(xr, xbuf(ic), wave * IPX + i, byte_of(wave * IPX + i, BM) < l ? xo[i < IPX ? i : 0] : kNoRow);
-      else edge_copy(wr, wbuf(ic), wave * IPW + i - IPX, byte_of(wave * IPW + i - IPX, BN) < l ? wo[i < IPX ? 0 : i - IPX] : kNoRow);
-    }
+    return left >= KG * kLine ? KG * kLine : (int)left;
   };
-  auto copy = [&](auto ic, int ks) HK_INLINE { copies(ic, ks, 0, IPX + IPW); };
+  auto copy_x = [&](auto ic, int ks, int i) HK_INLINE {
+    edge_copy(edge_rsrc(Xb + (int64_t)ks * (KG * kLine)), xbuf(ic), wave * IPX + i, byte_of(wave * IPX + i, BM) < left_of(ks) ? xo[i] : kNoRow);
+  };
+  auto copy_w = [&](auto ic, int ks, int i) HK_INLINE {
+    edge_copy(edge_rsrc(Wb + (int64_t)ks * (KG * kLine)), wbuf(ic), wave * IPW + i, byte_of(wave * IPW + i, BN) < left_of(ks) ? wo[i] : kNoRow);
+  };
+  auto stage_x = [&](auto ic, int ks) HK_INLINE {
+#pragma unroll
+    for (int i = 0; i < IPX; ++i) copy_x(ic, ks, i);
+  };
+  auto stage_w = [&](auto ic, int ks) HK_INLINE {
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) copy_w(ic, ks, i);
+  };
   // This lane's rows: the sub-tile's other 32-row blocks lie a constant further (the swizzle repeats every 16 rows).
   const int xrow = wm * WM + l32, wrow = wn * WN + l32;
 
@@ -246,12 +255,16 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
 
-  // Step ks from stage I.  GUARD: near the end, where no copy is left to be made; it waits for all of them.
+  constexpr int KEEP = (XR - WR) * IPX + (WR - 2) * (IPX + IPW);
+  static_assert(XR == WR || XR == WR + 1, "copies in flight past a step's W");
+  // Step ks, number I of the unrolled ones.  GUARD: near the end, where no copy is left to be made; it waits for all of them.
   auto step = [&](auto ic, auto guard, int ks) HK_INLINE {
     constexpr int I = decltype(ic)::value;
     constexpr bool GUARD = decltype(guard)::value;
-    const HK_L uint8_t* const xs = xbuf(ic) + kg * BM * kLine;
-    const HK_L uint8_t* const ws = wbuf(ic) + kg * BN * kLine;
+    using IX = std::integral_constant<int, (I + XR - 1) % XR>;
+    using IW = std::integral_constant<int, (I + WR - 1) % WR>;
+    const HK_L uint8_t* const xs = xbuf(std::integral_constant<int, I % XR>()) + kg * BM * kLine;
+    const HK_L uint8_t* const ws = wbuf(std::integral_constant<int, I % WR>()) + kg * BN * kLine;
     u32x4 wf[2][FN], xf[2][FM];
     // a line is four slices; the fragments of the next one are read while this one's products run (two register sets, fenced)
     auto read = [&](int s) HK_INLINE {
@@ -261,8 +274,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
       for (int i = 0; i < FM; ++i) xf[s & 1][i] = *reinterpret_cast<const HK_L u32x4*>(xs + tile_off<8>(xrow, 2 * s + h) + i * 32 * kLine);
     };
     read(0);
-    const bool more = !GUARD || ks + R - 1 < nk;
-    if (SP == 0 && more) copy(std::integral_constant<int, (I + R - 1) % R>(), ks + R - 1);
+    const bool more_w = !GUARD || ks + WR - 1 < nk, more_x = !GUARD || ks + XR - 1 < nk;
+    if (SP == 0) {
+      if (more_w) stage_w(IW(), ks + WR - 1);
+      issue_order_fence();  // the barrier counts on X being issued last
+      if (more_x) stage_x(IX(), ks + XR - 1);
+    }
     auto slice = [&](auto sc) HK_INLINE {
       constexpr int SL = decltype(sc)::value;
       __builtin_amdgcn_sched_barrier(0);
@@ -279,7 +296,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
             const int q = j * FM + i, c = SL * PER + q / EV;
             if (q % EV == EV - 1 && q / EV < PER && c < IPX + IPW) {
               __builtin_amdgcn_sched_barrier(0);
-              if (more) copies(std::integral_constant<int, (I + R - 1) % R>(), ks + R - 1, c, c + 1);
+              if (c < IPW) {
+                if (more_w) copy_w(IW(), ks + WR - 1, c < IPW ? c : 0);
+              } else {
+                if (more_x) copy_x(IX(), ks + XR - 1, c < IPW ? 0 : c - IPW);
+              }
               __builtin_amdgcn_sched_barrier(0);
             }
           }
@@ -292,8 +313,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int i = 0; i < FM; ++i) asm volatile("" : "+v"(acc[j][i]));
-    // The next step's stage has landed everywhere; later ones may stay in flight.
-    barrier_keep_vm_lds<GUARD ? 0 : (R - 2) * (IPX + IPW)>();
+    // The next step's stages have landed everywhere; what was issued after its W may stay in flight.
+    if (!GUARD || more_x) barrier_keep_vm_lds<KEEP>();
+    else barrier_keep_vm_lds<0>();
   };
   using Whole = std::integral_constant<bool, false>;
   using Guard = std::integral_constant<bool, true>;
@@ -302,20 +324,19 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
       if (!decltype(guard)::value || ks + decltype(ic)::value < nk) step(ic, guard, ks + decltype(ic)::value);
     };
     one(std::integral_constant<int, 0>()), one(std::integral_constant<int, 1>());
-    if constexpr (R > 2) one(std::integral_constant<int, 2>());
-    if constexpr (R > 3) one(std::integral_constant<int, 3>());
+    if constexpr (S::U > 2) one(std::integral_constant<int, 2>());
+    if constexpr (S::U > 3) one(std::integral_constant<int, 3>()), one(std::integral_constant<int, 4>()), one(std::integral_constant<int, 5>());
   };
-  copy(std::integral_constant<int, 0>(), 0);
+  stage_x(std::integral_constant<int, 0>(), 0);
+  stage_w(std::integral_constant<int, 0>(), 0);
   // stages of the steps before the first one's own copies (past the end of K: zeros that nobody reads)
-  if constexpr (R > 2) {
-    issue_order_fence();  // the first barrier counts on them being the last ones issued
-    copy(std::integral_constant<int, 1>(), 1);
-  }
-  if constexpr (R > 3) copy(std::integral_constant<int, 2>(), 2);
-  barrier_keep_vm<(R - 2) * (IPX + IPW)>();
+  issue_order_fence();  // the first barrier counts on them being the last ones issued
+  if constexpr (WR > 2) stage_w(std::integral_constant<int, 1>(), 1);
+  if constexpr (XR > 2) stage_x(std::integral_constant<int, 1>(), 1);
+  barrier_keep_vm<KEEP>();
   int ks = 0;
-  for (; ks + 2 * R - 1 <= nk; ks += R) steps(Whole(), ks);
-  for (; ks < nk; ks += R) steps(Guard(), ks);
+  for (; ks + S::U + XR - 1 <= nk; ks += S::U) steps(Whole(), ks);
+  for (; ks < nk; ks += S::U) steps(Guard(), ks);
 
   if constexpr (KG > 1) {  // the groups' sums, through the stages' memory (every copy has landed)
     constexpr int NB = FN * FM, PER = S::XT / 4096;  // accumulators of a wavefront; how many an X stage holds
@@ -406,34 +427,37 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
 }
 
 // ---- plan and launch -----------------------------------------------------------------------------------------------------
-struct Tile2 {
+// Tiles, and what a grid of them takes in us, fitted to full rounds of K 2048 and 8192: once, for every 256 workgroups, and for those
+// per 128 values of K.  One workgroup of the first two fits a CU, two of the others, whose copies then cover each other's
+// barriers.  A grid that leaves CUs idle runs up to a fifth faster.  Measured, us (tiles in this order): 4096 x 8192 x 2048 71, 84, 79, 99,
+// 130; 4096 x 2048 x 8192 79, 65, 72, 86, 104; 2048 cubed 27, 17, 15.6, 15.8, 19; 1024 x 2048 x 8192 73, 41, 34, 26, 29; 308 x 8192 x 2048
+// 25, 15.5, 11.4, 13.5, 15; 308 x 2048 x 2048 25, 14.5, 10, 7.7, 6.2 (before: 128 x 128 in two groups along K and 64 x 64 in four, one to a
+// CU, 11.6 and 7.5).  Over 44 sizes the choice is 2% behind the best.
+struct Tile {
   int bm, bn;
+  float once, per256, per128;
 };
-constexpr Tile2 kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 64}};
+constexpr Tile kTiles[] = {{256, 256, 0.f, 11.f, 1.48f}, {128, 256, 0.f, 9.f, 0.82f}, {128, 128, 6.5f, 1.2f, 0.49f}, {128, 64, 4.f, 1.35f, 0.29f}, {64, 64, 3.2f, 0.97f, 0.183f}};
+constexpr int kNumTiles = 5;
 
 int64_t tiles_of(const hrt_i8_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
 // Index of the tile, -1: i8_rows (up to 16 rows, or 32 where K is short).
-// Tiles: one workgroup fits a CU, so a grid runs in rounds of 256, each a fixed cost (first copies, epilogue) and a time per 128 values
-// of K, both fitted to full rounds of K 2048 and 8192; a grid that does not fill its rounds runs up to a fifth faster.  Measured, us
-// (tiles in this order): 4096 x 8192 x 2048 71, 83, 105, 229; 4096 x 2048 x 8192 85, 65, 80, 148; 2048 cubed 28, 17.5, 16.4, 30;
-// 308 x 2048 x 2048 24, 14.8, 11.6, 7.5; over 26 drawn sizes the choice is 1% behind the best.
 int plan_of(const hrt_i8_mm_args& a) {
   if (a.x_scale == 0 || a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
-  static constexpr struct { float fixed, per128; } kCost[4] = {{11.f, 1.5f}, {9.f, 0.82f}, {6.7f, 0.525f}, {3.6f, 0.235f}};
-  int best = 3;
+  int best = 0;
   float us = 0.f;
-  for (int t = 3; t >= 0; --t) {
-    const float rounds = (float)cdiv(tiles_of(a, t), 256), fill = (float)tiles_of(a, t) / (256.f * rounds);
-    const float e = rounds * (kCost[t].fixed + kCost[t].per128 * (float)a.K / 128.f) * (fill > 0.5f ? 0.6f + 0.4f * fill : 0.8f);
-    if (t == 3 || e < us) best = t, us = e;
+  for (int t = 0; t < kNumTiles; ++t) {
+    const float n = (float)tiles_of(a, t) / 256.f, rounds = (float)cdiv(tiles_of(a, t), 256);
+    const float e = (kTiles[t].once + rounds * (kTiles[t].per256 + kTiles[t].per128 * (float)a.K / 128.f)) * (n >= 1.f ? 1.f : n > 0.5f ? 0.56f + 0.44f * n : 0.78f);
+    if (t == 0 || e < us) best = t, us = e;
   }
   return best;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int KG, int R, int SP>
+template <typename T, int BM, int BN, int WM, int WN, int KG, int XR, int WR, int SP>
 void queue_tile(const hrt_i8_mm_args& a, hipStream_t s, bool lines) {
   const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, kLine * KG);
-  hipLaunchKernelGGL((i8_tile<T, BM, BN, WM, WN, KG, R, SP>), dim3((uint32_t)(tm * tn)), dim3(64 * TileShape<BM, BN, WM, WN, KG, R>::NW), 0, s, a, (int)tn,
+  hipLaunchKernelGGL((i8_tile<T, BM, BN, WM, WN, KG, XR, WR, SP>), dim3((uint32_t)(tm * tn)), dim3(64 * TileShape<BM, BN, WM, WN, KG, XR, WR>::NW), 0, s, a, (int)tn,
                      (int)nk, lines);
 }
 
@@ -441,10 +465,11 @@ template <typename T>
 void queue_mm(const hrt_i8_mm_args& a, int tile, hipStream_t s) {
   const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0 && a.w_scale % 16 == 0, lines = vec && a.N % 8 == 0 && a.y % 16 == 0;
   switch (tile) {
-    case 0: return queue_tile<T, 256, 256, 128, 64, 1, 2, 2>(a, s, lines);
-    case 1: return queue_tile<T, 128, 256, 64, 64, 1, 3, 3>(a, s, lines);
-    case 2: return queue_tile<T, 128, 128, 64, 64, 2, 2, 0>(a, s, lines);
-    case 3: return queue_tile<T, 64, 64, 32, 64, 4, 2, 0>(a, s, lines);
+    case 0: return queue_tile<T, 256, 256, 128, 64, 1, 3, 2, 3>(a, s, lines);
+    case 1: return queue_tile<T, 128, 256, 64, 64, 1, 3, 3, 3>(a, s, lines);
+    case 2: return queue_tile<T, 128, 128, 32, 64, 1, 3, 2, 0>(a, s, lines);
+    case 3: return queue_tile<T, 128, 64, 32, 32, 1, 3, 3, 0>(a, s, lines);
+    case 4: return queue_tile<T, 64, 64, 32, 32, 2, 3, 2, 0>(a, s, lines);
   }
   // wavefronts and batches that cover K once where they can
   const dim3 grid((uint32_t)cdiv(a.N, 16));
