@@ -121,6 +121,21 @@ def test_argument_blocks_match_the_header(tmp_path):
         assert int(n) == (ctypes.sizeof(blocks[c]) if f == "size" else getattr(blocks[c], f).offset), (c, f)
 
 
+def test_the_order_that_the_products_barriers_count_on():
+    """Stage 0 is issued before a fence and later stages behind it, and in a step X behind a fence behind W, at its start or spread."""
+    import os
+    import re
+
+    kernels = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "torch-vulkan_amd", "csrc", "kernels")
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(kernels, "i8_gemm.hip")).read())
+    zero, one = "(std::integral_constant<int, 0>(), 0);", "(std::integral_constant<int, 1>(), 1);"
+    for first, later in ((f"stage_x{zero}", f"stage_w{one}"), (f"stage_w{zero}", f"stage_x{one}"), (f"stage_w{zero}", f"stage_w{one}"),
+                         ("stage_w(IW(), ks + WR - 1);", "stage_x(IX(), ks + XR - 1);")):
+        between = text[text.index(first) : text.index(later)]
+        assert text.count(first) == text.count(later) == 1 and "issue_order_fence();" in between
+    assert re.search(r"if \(c == IPW\) issue_order_fence\(\);\s*if \(c < IPW\) \{\s*if \(more_w\) copy_w\(.*?\} else \{\s*if \(more_x\) copy_x\(", text, re.S)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", SHAPES)

@@ -9,7 +9,8 @@
 // 16x16x64: row l % 16, bytes 16 (l / 16) .. + 15; accumulators as for the 16-bit products of the same shape.
 // W is the first operand, so an accumulator holds four consecutive columns n of one row m of y.
 // Measured, M x N x K: 1 x 8192 x 2048 4.6 us, 16 x 8192 x 2048 5.7, 308 x 2048 x 2048 6.4, 1024 x 2048 x 8192 27, 4096 x 8192 x 2048 71 us
-// (1.93 POP/s), 4096 x 2048 x 8192 65 (2.1), 8192 cubed 422 us, 2.6 POP/s (a library's 8-bit product of that size: 526).
+// (1.93 POP/s), 4096 x 2048 x 8192 65 (2.1), 8192 cubed 422 to 445 us by box, 2.5 to 2.6 POP/s (a library's 8-bit
+// product of that size: 526).
 // The largest tiles' step has 2048 cycles of products, 2048 of LDS (192 KiB of fragments, 64 KiB of copies) and 2200 of L2 -> LDS; it takes
 // 2900 on half of the CUs and 4000 on all of them (matrix cores busy 55%).
 #include <utility>
@@ -296,6 +297,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
             const int q = j * FM + i, c = SL * PER + q / EV;
             if (q % EV == EV - 1 && q / EV < PER && c < IPX + IPW) {
               __builtin_amdgcn_sched_barrier(0);
+              if (c == IPW) issue_order_fence();  // as above: X behind W
               if (c < IPW) {
                 if (more_w) copy_w(IW(), ks + WR - 1, c < IPW ? c : 0);
               } else {

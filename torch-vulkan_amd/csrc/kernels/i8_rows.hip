@@ -12,7 +12,8 @@ namespace {
 
 constexpr int kThreads = 512;
 
-// 16 codes a lane, lpr lanes a row; a workgroup takes whole rows, several where they are short.
+// 16 codes a lane, lpr lanes a row; a workgroup takes whole rows, several where they are short.  A row's last piece is its last 16
+// codes, some of them its neighbour's too, which writes the same values (one by one the last codes cost a load's latency each).
 template <typename T>
 __device__ __forceinline__ void dequant_rows(const hrt_i8_rows_args& p, int64_t block, int lpr) {
   using R = RowVec<T>;
@@ -24,8 +25,9 @@ __device__ __forceinline__ void dequant_rows(const hrt_i8_rows_args& p, int64_t 
   const float s = gcptr<float>(p.scale)[row];
   const HK_G uint8_t* const q = gcptr<uint8_t>(p.q) + row * p.q_sr;
   HK_G S* const x = gptr<S>(p.x) + row * p.x_sr;
-  for (int64_t col = (int64_t)(threadIdx.x % lpr) * 16; col < p.cols; col += (int64_t)lpr * 16) {
-    if (col + 16 <= p.cols) {
+  for (int64_t piece = (int64_t)(threadIdx.x % lpr) * 16; piece < p.cols; piece += (int64_t)lpr * 16) {
+    const int64_t col = piece + 16 <= p.cols ? piece : p.cols - 16;
+    if (col >= 0) {
       typedef u32x4 __attribute__((aligned(1))) any1;
       const u32x4 c = *reinterpret_cast<const HK_G any1*>(q + col);
 #pragma unroll
@@ -36,7 +38,7 @@ __device__ __forceinline__ void dequant_rows(const hrt_i8_rows_args& p, int64_t 
         R::put(x + col + i, R::pack(v));
       }
     } else {
-      for (int64_t e = col; e < p.cols; ++e) x[e] = T::from_f32((float)(int8_t)q[e] * s);
+      for (int64_t e = 0; e < p.cols; ++e) x[e] = T::from_f32((float)(int8_t)q[e] * s);
     }
   }
 }
