@@ -137,7 +137,7 @@ bool launch_rotary(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   using S = typename T::storage;
   constexpr uint64_t E = sizeof(S);
   constexpr int V = RowVec<T>::V;
-  if (a.B <= 0 || a.S <= 0 || a.Hq <= 0 || a.Hk < 0 || (a.Hk > 0) != (a.k != 0) || a.Hq > (1 << 24) || a.Hk > (1 << 24)) return ctx.fail("bad shape");
+  if (a.B <= 0 || a.S <= 0 || a.Hq <= 0 || a.Hk < 0 || (a.Hk > 0) != (a.k != 0) || a.Hq > 65536 || a.Hk > 65536) return ctx.fail("bad shape");
   if (a.D <= 0 || a.D > 1024 || a.P <= 0 || 2 * a.P > a.D) return ctx.fail("D must be 1..1024 and pairs must fit it");
   if (a.axes < 1 || a.axes > HRT_ROTARY_AXES || a.ends[a.axes - 1] != a.P) return ctx.fail("bad axes");
   for (int i = 0; i < a.axes; ++i)

@@ -119,7 +119,7 @@ std::vector<at::Tensor> rotary_embedding_vk(const at::Tensor& q, const std::opti
                   positions.size(-1) == axes,
               who, ": positions must be [", S, ", ", axes, "] or [", B, ", ", S, ", ", axes, "], got ", positions.sizes());
   constexpr int64_t lim = int64_t(1) << 31;
-  TORCH_CHECK(B * S < lim && q.size(1) < (1 << 24) && (!present(k) || k->size(1) < (1 << 24)), who, ": too many tokens or heads");
+  TORCH_CHECK(B * S < lim && q.size(1) <= 65536 && (!present(k) || k->size(1) <= 65536), who, ": too many tokens or heads");
   const bool grad = at::GradMode::is_enabled();
   TORCH_CHECK(!grad || !(positions.requires_grad() || freqs.requires_grad()), who, ": positions and freqs take no gradient");
   no_tangent(q, who), no_tangent(positions, who), no_tangent(freqs, who);

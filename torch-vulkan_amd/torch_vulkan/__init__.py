@@ -380,7 +380,8 @@ def quantize_int8_rows(x):
 
 
 def dequant_int8_rows(q, scale, out_dtype=torch.bfloat16):
-    """The values that quantize_int8_rows's (codes, scale) stand for: the float32 product code * scale rounded to out_dtype."""
+    """The values that quantize_int8_rows's (codes, scale) stand for: the float32 product code * scale rounded to out_dtype.
+    Not differentiable."""
     if q.device.type == "vk":
         return _C.dequant_int8_rows(q, scale, out_dtype)
     if q.dtype != torch.int8 or scale.dtype != torch.float32 or q.dim() < 1 or q.shape[:-1] != scale.shape:
