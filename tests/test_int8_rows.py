@@ -469,6 +469,27 @@ def test_replayed_graph(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K", [64, 1040, 2048])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 7, 8])
+def test_few_rows_where_they_lie(M, K):
+    """Rows that the product quantises itself: off their lines, apart, repeated, of zeros, not finite; the codes of the packed rows."""
+    x, w, s, b = operands(M, 40, K, torch.bfloat16, K)
+    x[M // 2, 5:] = 0
+    if M > 2:
+        x[1], x[2, 7] = 0, float("nan")
+    codes, scale = torch_vulkan.quantize_int8_rows(x)
+    W, S, B = w.to(vk), s.to(vk), b.to(vk)
+    want = torch_vulkan.int8_linear(codes.to(vk), W, S, B, x_scale=scale.to(vk)).cpu()
+    wide = torch.full((2 * M, K + 13), 1e4, dtype=torch.bfloat16)
+    wide[::2, 3 : K + 3] = x
+    for X in (x.to(vk), wide.to(vk)[::2, 3 : K + 3]):
+        got = torch_vulkan.int8_linear(X, W, S, B).cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+    one = torch_vulkan.int8_linear(x[:1].to(vk).expand(M, K), W, S, B).cpu()
+    assert torch.equal(torch.nan_to_num(one), torch.nan_to_num(want[:1].expand(M, 40)))
+
+
+@pytest.mark.gpu
 def test_rows_far_apart():
     """8-bit rows 2^30 bytes apart are copied together first, 16-bit ones are quantised where they lie."""
     x, w, s, b = operands(3, 24, 64, torch.bfloat16, 3)

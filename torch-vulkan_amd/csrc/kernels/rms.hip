@@ -24,8 +24,8 @@ constexpr int threads_of(int lpr) { return lpr > 256 ? lpr : 256; }
 
 enum Mode { kNorm, kNorm8, kQuant };
 
-// kQuant reads rows x (stride xs[0]) and writes codes (pitch r, a plain number there) and scales; its arguments come in the same
-// block, so that one kernel serves all three.
+// kQuant reads rows x (stride xs[0]) and writes codes (pitch q_sr) and scales; its arguments come in the same block, so that one
+// kernel serves all three.
 template <typename T, int MODE, int LPR, int NV, bool TAIL>
 __global__ __launch_bounds__(threads_of(LPR)) void rms_rows(hrt_rms_args p, int64_t q_sr) {
   using R = RowVec<T>;
