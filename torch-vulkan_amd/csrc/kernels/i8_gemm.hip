@@ -443,7 +443,10 @@ constexpr Tile kTiles[] = {{256, 256, 0.f, 11.f, 1.48f}, {128, 256, 0.f, 9.f, 0.
 constexpr int kNumTiles = 5;
 
 int64_t tiles_of(const hrt_i8_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
-// Index of the tile, -1: i8_rows (up to 16 rows, or 32 where K is short).
+// Index of the tile, -1: i8_rows (up to 16 rows, or 32 where K is short).  us of i8_rows and of the tile chosen otherwise, at 16, 17 and 32
+// rows, N x K: 2048 x 1024 3.7, 4.0, 4.3 against 4.9, 4.9, 5.0; 2048 x 2048 4.5, 5.0, 5.5 against 5.9, 5.9, 6.0; 8192 x 1024 4.8, 5.3, 5.9
+// against 5.1; 8192 x 2048 6.9, 7.4, 8.5 against 6.1; 2048 x 8192 11.4, 11.7, 14.2 against 11.8.  The rule is on M and K alone: it is up
+// to 0.8 us off the better one on either side.
 int plan_of(const hrt_i8_mm_args& a) {
   if (a.x_scale == 0 || a.M <= 16 || (a.M <= 32 && a.K <= 1024)) return -1;
   int best = 0;

@@ -424,7 +424,8 @@ __global__ __launch_bounds__(1024) void rms_dw_sum(const float* ws, typename T::
 
 // ---- plan and launch --------------------------------------------------------------------------------------------------------
 // Lanes per row and pieces per lane; 0: the passes.  Few rows of model width are shared by a workgroup: its four wavefronts'
-// loads are all in flight at once.
+// loads are all in flight at once (D 2048 in bf16, us with a wavefront and with a workgroup a row: 64 rows 3.5, 3.1; 308 3.7, 3.3; 1024
+// 4.1, 4.3; 2048 5.0, 5.9; 8192 12.0, 15.7).
 struct Share {
   int lpr, nv;
 };

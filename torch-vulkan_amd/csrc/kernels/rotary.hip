@@ -3,15 +3,13 @@
 // Bound by memory: every value is read once and written once.  The sines and cosines depend on the token and the pair alone, so a
 // workgroup takes all heads of a few tokens, computes each of them once into LDS and its lanes keep theirs in registers over
 // the heads.  Far positions: the angle is reduced to an eighth of a turn in fp64 (position times frequency in 53 bits) before its
-// sine and cosine are taken in fp32, which leaves them within 2^-23.  Measured, bf16, 16 + 16 heads of 128: 2 x 4096 tokens 26.6 us (5.05
-// TB/s), 23.5 us where the operands stay in the last cache; 8 tokens 3.7 us.
+// sine and cosine are taken in fp32, which leaves them within 2^-23.  Measured, bf16, 16 + 16 heads of 128: 2 x 4096 tokens 24.9 us
+// by the kernel trace (5.4 TB/s, part of it from the last cache; 26.6 with four tokens to a workgroup), 22.5 replayed on the same operands; 8 tokens 3.7 us.
 #include "../hrt/registry.h"
 #include "row_vec.h"
 
 namespace hk {
 namespace {
-
-constexpr int kTokens = 4;  // of a workgroup at most
 
 // cos and sin of `turns` full turns.
 __device__ __forceinline__ void turn_of(double turns, float& c, float& s) {
@@ -156,9 +154,10 @@ bool launch_rotary(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
       !ctx.check(a.k, hrt::span_bytes(4, kz, kt, E), "k") || !ctx.check(a.k_out, row * a.Hk, "k_out") ||
       !ctx.check(a.pos, hrt::span_bytes(3, pz, pt, pe), "pos") || !ctx.check(a.freqs, (uint64_t)a.P * 8, "freqs"))
     return false;
-  // a workgroup for every token until the chip is full, then several tokens for each
+  // A workgroup for every token until the chip is full, then one for two.  bf16, 16 + 16 heads of 128, replayed on the same operands, us
+  // with 1, 2, 4 tokens each: 2048 tokens 7.6, 7.7, 8.4; 4096 13.5, 12.8, 13.6; 8192 23.7, 22.5, 23.6; 16384 46.5, 44.0, 46.6.
   const int64_t all = a.B * a.S;
-  const int tokens = all >= 8192 ? kTokens : all >= 4096 ? 2 : 1;
+  const int tokens = all >= 4096 ? 2 : 1;
   if (all >= (int64_t(1) << 31) || !hrt::grid_fits(cdiv(all, tokens), 256)) return ctx.fail("grid too large");
   // whole pieces: pairs by W, and what is copied by W
   const auto fits = [&](int w) { return a.P % w == 0 && (a.D - 2 * a.P) % w == 0; };
