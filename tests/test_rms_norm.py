@@ -399,3 +399,24 @@ def test_two_graphs_and_a_live_eager_one():
     assert torch.equal(X.grad.cpu(), dx.cpu()) and torch.equal(W.grad.cpu(), dw.cpu())
     for i in ids:
         rt.graph_destroy(i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(5, 64), (3, 7), (5, 1000), (9, 2048), (3, 8192), (2, 20001)])
+def test_the_block_writes_h_without_a_residual(shape, dtype):
+    """r 0 in the argument block: h = x, written where h_out asks for it, beside y and beside 8-bit rows."""
+    rt, (rows, D) = abi.Runtime(), shape
+    x, w, _, _, _ = data(shape, dtype, 4)
+    suffix = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}[dtype]
+    X, W, Y, H = x.to(vk), w.to(vk), torch.zeros(shape, dtype=dtype, device=vk), torch.full(shape, 7.0, dtype=dtype, device=vk)
+    Q, S = torch.zeros(shape, dtype=torch.int8, device=vk), torch.zeros(rows, device=vk)
+    xs = (abi.i64 * 3)(D, 0, 0)
+    for out in (dict(y=Y.data_ptr()), dict(q=Q.data_ptr(), scale=S.data_ptr())):
+        for h in (H.data_ptr(), 0):
+            H.fill_(7.0)
+            rt.dispatch("rms_fwd_" + suffix, abi.RmsArgs(x=X.data_ptr(), w=W.data_ptr(), h_out=h, rows=rows, D=D, n1=1, n2=1, xs=xs, eps=1e-6, **out))
+            assert torch.equal(H.cpu(), x if h else torch.full(shape, 7.0, dtype=dtype))
+    assert torch.equal(Y.cpu(), torch_vulkan.rms_norm(X, W).cpu())
+    q, s = torch_vulkan.rms_norm_int8(X, W)
+    assert torch.equal(Q.cpu(), q.cpu()) and torch.equal(S.cpu(), s.cpu())

@@ -62,8 +62,8 @@ __global__ __launch_bounds__(threads_of(LPR)) void rms_rows(hrt_rms_args p, int6
       R::unpack(row_fix<T, TAIL>(b[c], col, p.D), t);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[c][e] += t[e];
-      if (p.h_out && live) row_put<T, TAIL>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v[c]));
     }
+    if (MODE != kQuant && p.h_out && live) row_put<T, TAIL>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v[c]));
     if (!TAIL && col >= p.D) {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[c][e] = 0.f;
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void rms_long(hrt_rms_args p, int64_t q_sr) {
       load(col, v);
 #pragma unroll
       for (int e = 0; e < V; ++e) ss = fmaf(v[e], v[e], ss);
-      if (r && p.h_out) row_put<T, true>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v));
+      if (p.h_out) row_put<T, true>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v));
     }
     rstd = 1.f / sqrtf(lanes_sum<256>(ss, red) / (float)p.D + p.eps);
     if (p.rstd && threadIdx.x == 0) gptr<float>(p.rstd)[row] = rstd;
