@@ -535,3 +535,27 @@ def test_an_expanded_gradient():
     dx, db = torch.autograd.grad(torch_vulkan.int8_linear(X, w.to(vk), s.to(vk), B).sum(), (X, B))
     check_back(dx, torch.ones(6, 24).bfloat16(), w, s, torch.bfloat16)
     assert (db.cpu() == 6).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [72, 70])
+@pytest.mark.parametrize("M", [1, 5, 12, 20, 40, 140, 300])
+def test_far_scales_whose_product_is_near(M, N):
+    """Sums of which one scale's share alone passes fp32's range, beside rows of ordinary size."""
+    K = 320
+    x, w, s, b = operands(M, N, K, torch.bfloat16, M)
+    x[::2] *= 2.0**120
+    x[::4] = x[::4].abs()  # codes of one sign: the largest sums
+    w[:8] = w[:8].abs()
+    x[0, :K] = 1e36
+    codes, scale = packed(x)
+    y, want = product(codes, scale, w, s, b)
+    assert (np.abs(y).max() < 2.0**127) and (np.abs(codes.astype(np.float64) @ f64(w).T) * scale[:, None]).max() > 2.0**128
+    X, W, S, B, C, XS = (t.to(vk) for t in (x, w, s, b, torch.from_numpy(codes), torch.from_numpy(scale)))
+    check_forward(torch_vulkan.int8_linear(X, W, S, B), y, want, torch.bfloat16)
+    check_forward(torch_vulkan.int8_linear(C, W, S, B, x_scale=XS), y, want, torch.bfloat16)
+    near = (s * 2.0**-118).float()  # and an fp16 result under scales that all but cancel
+    y, _ = product(codes, scale, w, near, None)
+    y[1::2], want = 0, None
+    got = torch_vulkan.int8_linear(C, W, near.to(vk), x_scale=XS, out_dtype=torch.float16)
+    check_forward(got[::2], y[::2], y[::2], torch.float16)

@@ -35,7 +35,9 @@ __device__ __forceinline__ i32x16 mac32(u32x4 a, u32x4 b, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
-// Values n .. n + 3 of row m from whole sums: sum * x_scale is taken first (the product of two small scales may underflow).
+// Values n .. n + 3 of row m from whole sums: sum * x_scale is taken first (the product of two small scales may underflow), or
+// sum * w_scale where x_scale is so large that the sum times it might overflow under a small w_scale: a sum is at most 2^31.
+constexpr float kFarScale = 0x1p64f;
 template <typename T>
 __device__ __forceinline__ void store4(const hrt_i8_mm_args& p, int64_t m, int64_t n, const int* v, float sx, bool vec) {
   if (m >= p.M || n >= p.N) return;
@@ -43,17 +45,19 @@ __device__ __forceinline__ void store4(const hrt_i8_mm_args& p, int64_t m, int64
   HK_G uint16_t* y = gptr<uint16_t>(p.y) + m * p.N + n;
   const HK_G uint16_t* b = gcptr<uint16_t>(p.bias) + n;
   float o[4];
+  const bool far = sx > kFarScale;
+  auto value = [&](int sum, float s, float add) HK_INLINE { return (float)sum * (far ? s : sx) * (far ? sx : s) + add; };
   if (vec) {
     u32x2 w = {0, 0};
     if (p.bias) w = *reinterpret_cast<const HK_G u32x2*>(b);
     const f32x4 s = *reinterpret_cast<const HK_G f32x4*>(sw);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * sx * s[e] + (e & 1 ? hi16<T>(w[e >> 1]) : lo16<T>(w[e >> 1]));
+    for (int e = 0; e < 4; ++e) o[e] = value(v[e], s[e], e & 1 ? hi16<T>(w[e >> 1]) : lo16<T>(w[e >> 1]));
     *reinterpret_cast<HK_G u32x2*>(y) = pack4<T>(o);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e < p.N) y[e] = T::from_f32((float)v[e] * sx * sw[e] + (p.bias ? T::to_f32(b[e]) : 0.f));
+      if (n + e < p.N) y[e] = T::from_f32(value(v[e], sw[e], p.bias ? T::to_f32(b[e]) : 0.f));
   }
 }
 
@@ -366,11 +370,19 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
         for (int e = 0; e < 16; ++e) acc[b / FM][b % FM][e] += part[e * 64];
       }
   }
-  if (!lines) {
+  float sxs[FM];
+  bool far = false;  // rows that store4 takes the other way round, which the lines below do not
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t m = m0 + wm * WM + i * 32 + l32;
+    sxs[i] = gcptr<float>(p.x_scale)[m < p.M ? m : p.M - 1];
+    far |= sxs[i] > kFarScale;
+  }
+  if (!lines || __any(far)) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int64_t m = m0 + wm * WM + i * 32 + l32;
-      const float sx = gcptr<float>(p.x_scale)[m < p.M ? m : 0];
+      const float sx = sxs[i];
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -405,8 +417,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
     }
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int64_t mine = m0 + wm * WM + i * 32 + l32;
-    const float sx = gcptr<float>(p.x_scale)[mine < p.M ? mine : p.M - 1];
+    const float sx = sxs[i];
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
