@@ -559,3 +559,33 @@ def test_far_scales_whose_product_is_near(M, N):
     y[1::2], want = 0, None
     got = torch_vulkan.int8_linear(C, W, near.to(vk), x_scale=XS, out_dtype=torch.float16)
     check_forward(got[::2], y[::2], y[::2], torch.float16)
+
+
+def test_tangents_and_gradients_are_not_dropped_on_the_cpu():
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.randn(4, 70)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch_vulkan.quantize_int8_rows(fwd.make_dual(x, x))
+        assert torch_vulkan.quantize_int8_rows(x)[0].shape == (4, 70)
+
+
+@pytest.mark.gpu
+def test_tangents_and_gradients_are_not_dropped():
+    """Packing and unpacking refuse a tangent, and unpacking a scale whose gradient would be lost."""
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.randn(4, 70).to(vk)
+    c, s = torch_vulkan.quantize_int8_rows(x)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch_vulkan.quantize_int8_rows(fwd.make_dual(x, x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch_vulkan.dequant_int8_rows(c, fwd.make_dual(s, s))
+    wants = s.detach().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch_vulkan.dequant_int8_rows(c, wants)
+    with torch.no_grad():
+        assert torch.equal(torch_vulkan.dequant_int8_rows(c, wants).cpu(), torch_vulkan.dequant_int8_rows(c, s).cpu())
+    assert torch.equal(torch_vulkan.quantize_int8_rows(x.detach().requires_grad_())[0].cpu(), c.cpu())  # a weight at rest

@@ -140,6 +140,7 @@ namespace vkt {
 std::tuple<at::Tensor, at::Tensor> quantize_int8_rows_vk(const at::Tensor& x) {
   TORCH_CHECK(on_vk(x) && float_code(x.scalar_type()) >= 0, "quantize_int8_rows: x must be a float32, bfloat16 or float16 vk tensor");
   TORCH_CHECK(x.dim() >= 1, "quantize_int8_rows: x must have at least one dimension");
+  no_tangent(x, "quantize_int8_rows");
   const at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
   const at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
   if (x.numel() == 0) {
@@ -154,6 +155,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8_rows_vk(const at::Tensor& x) {
 at::Tensor dequant_int8_rows_vk(const at::Tensor& q, const at::Tensor& scale, at::ScalarType out_dtype) {
   check_rows(q, scale, "dequant_int8_rows", "q");
   TORCH_CHECK(float_code(out_dtype) >= 0, "dequant_int8_rows: out_dtype must be float32, bfloat16 or float16, got ", out_dtype);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !scale.requires_grad(), "dequant_int8_rows: scale takes no gradient");
+  no_tangent(scale, "dequant_int8_rows");
   const at::Tensor out = at::empty(q.sizes(), q.options().dtype(out_dtype));
   if (out.numel() == 0) return out;
   dequant_rows(unit_rows(as_rows(q)), dense(scale), as_rows(out));

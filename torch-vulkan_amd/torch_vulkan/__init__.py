@@ -364,11 +364,13 @@ def quantize_int8_rows(x):
 
     A value reads back as code * scale of its row: scale = largest magnitude / 127 (a finite row reads back finite), and code is the whole number nearest to
     127 * x / largest magnitude, ties to even.  A row of zeros gets scale 0; one with an infinity or NaN gets scale NaN, codes 0,
-    and reads back as NaN.  Not differentiable."""
+    and reads back as NaN.  Not differentiable: an x that requires a gradient is taken by its values, a forward-mode tangent refused."""
     if x.device.type == "vk":
         return _C.quantize_int8_rows(x)
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1:
         raise RuntimeError("quantize_int8_rows: x must be a float32, bfloat16 or float16 tensor of at least one dimension")
+    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError("quantize_int8_rows: forward-mode differentiation is not supported")
     x = x.detach()
     if x.shape[-1] == 0:
         return torch.empty(x.shape, dtype=torch.int8), torch.zeros(x.shape[:-1])
@@ -381,7 +383,7 @@ def quantize_int8_rows(x):
 
 def dequant_int8_rows(q, scale, out_dtype=torch.bfloat16):
     """The values that quantize_int8_rows's (codes, scale) stand for: the float32 product code * scale rounded to out_dtype.
-    Not differentiable."""
+    Not differentiable on vk: a scale that requires a gradient or carries a forward-mode tangent is refused."""
     if q.device.type == "vk":
         return _C.dequant_int8_rows(q, scale, out_dtype)
     if q.dtype != torch.int8 or scale.dtype != torch.float32 or q.dim() < 1 or q.shape[:-1] != scale.shape:
