@@ -453,3 +453,21 @@ def test_in_place_operations_on_the_output(shape, N, quantize):
     y.view(-1)[: y.numel() // 2].zero_()  # a view of it
     (dx,) = torch.autograd.grad(y, X, torch.ones_like(y))
     assert dx.shape == X.shape
+
+
+def refuses_a_tangent(x):
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch_vulkan.quantize_mxfp4(fwd.make_dual(x, x))
+        assert torch_vulkan.quantize_mxfp4(x)[0].shape == (4, 35)
+
+
+def test_packing_refuses_a_tangent_on_the_cpu():
+    refuses_a_tangent(torch.randn(4, 70))
+
+
+@pytest.mark.gpu
+def test_packing_refuses_a_tangent():
+    refuses_a_tangent(torch.randn(4, 70).to(vk))

@@ -150,6 +150,7 @@ namespace vkt {
 std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_vk(const at::Tensor& x) {
   TORCH_CHECK(on_vk(x) && float_code(x.scalar_type()) >= 0, "quantize_mxfp4: x must be a float32, bfloat16 or float16 vk tensor");
   TORCH_CHECK(x.dim() >= 1, "quantize_mxfp4: x must have at least one dimension");
+  no_tangent(x, "quantize_mxfp4");
   const int64_t cols = x.size(-1);
   std::vector<int64_t> sizes = x.sizes().vec();
   const auto bytes = x.options().dtype(at::kByte);

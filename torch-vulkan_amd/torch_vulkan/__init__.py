@@ -280,12 +280,15 @@ def quantize_mxfp4(x):
     Blocks of 32 consecutive values share a scale byte s, and a value reads back as e2m1 * 2**(s - 127) with e2m1 in
     0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign.  s = floor(log2(largest magnitude)) - 2 + 127, at least 0; each value is
     rounded to the nearest code, ties to the even one, and saturates at 6.  Two codes a byte, the even element in the low
-    nibble.  A block with an infinity or NaN gets s = 255 and reads back as NaN.  Not differentiable.
+    nibble.  A block with an infinity or NaN gets s = 255 and reads back as NaN.  Not differentiable: an x that
+    requires a gradient is taken by its values, a forward-mode tangent refused.
     """
     if x.device.type == "vk":
         return _C.quantize_mxfp4(x)
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1:
         raise RuntimeError("quantize_mxfp4: x must be a float32, bfloat16 or float16 tensor of at least one dimension")
+    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError("quantize_mxfp4: forward-mode differentiation is not supported")
     cols = x.shape[-1]
     nb = (cols + 31) // 32
     v = torch.zeros((*x.shape[:-1], nb * 32), dtype=torch.float64)  # exact: quotients by powers of two
