@@ -420,3 +420,23 @@ def test_the_block_writes_h_without_a_residual(shape, dtype):
     assert torch.equal(Y.cpu(), torch_vulkan.rms_norm(X, W).cpu())
     q, s = torch_vulkan.rms_norm_int8(X, W)
     assert torch.equal(Q.cpu(), q.cpu()) and torch.equal(S.cpu(), s.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(7, 130), (1030, 264), (7, 4100), (7, 20001), (70000, 7)])
+def test_the_residuals_way_is_its_own(shape, dtype):
+    """Where h alone is used its gradient goes through as it is, rows that have no norm among them, and the weight's is zero."""
+    x, w, r, _, gh = data(shape, dtype, 9)
+    x[1, 3], x[2, 5], x[4], r[4], w[6] = float("nan"), float("inf"), 0, 0, float("inf")
+    for weight in (w.to(vk).requires_grad_(), None):
+        X, R = x.to(vk).requires_grad_(), r.to(vk).requires_grad_()
+        for g in (gh.to(vk), gh.t().contiguous().to(vk).t(), gh[:, :1].to(vk).expand(shape)):
+            h = torch_vulkan.rms_norm(X, weight, residual=R, eps=0.0)[1]
+            grads = torch.autograd.grad(h, [t for t in (X, R, weight) if t is not None], g)
+            assert torch.equal(grads[0].cpu(), g.cpu()) and torch.equal(grads[1].cpu(), g.cpu())
+            assert weight is None or (grads[2].shape == w.shape and (grads[2].cpu() == 0).all())
+    X, R = x.to(vk).requires_grad_(), r.to(vk).requires_grad_()
+    torch_vulkan.rms_norm(X, None, residual=R, eps=0.0)[1].backward(gh.to(vk))
+    X.grad.add_(1)  # two gradients, not one tensor
+    assert torch.equal(R.grad.cpu(), gh)

@@ -221,8 +221,7 @@ __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) 
 #pragma unroll
     for (int u = 0; u < 4; ++u) {  // four rows' loads in flight; a row past the end repeats the last one
       const int64_t row = r0 + u * G < p.rows ? r0 + u * G : p.rows - 1;
-      a[u] = u32x4{0, 0, 0, 0};
-      if (p.gy) a[u] = row_load<T, TAIL>(gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys), col, p.D);
+      a[u] = row_load<T, TAIL>(gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys), col, p.D);
       b[u] = row_load<T, TAIL>(gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs), col, p.D);
       rstd[u] = gcptr<float>(p.rstd)[row];
     }
@@ -275,16 +274,16 @@ __global__ __launch_bounds__(threads_of(LPR)) void rms_back(hrt_rms_bwd_args p, 
   for (int64_t base = first; base < end; base += RPB, turn ^= 1) {
     const bool live = base + group < end;
     const int64_t row = live ? base + group : end - 1;
-    const HK_G S* const gy = gcptr<S>(p.gy) + (p.gy ? row_at(row, p.n1, p.n2, p.gys) : 0);
+    const HK_G S* const gy = gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys);
     const HK_G S* const h = gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs);
     u32x4 a[NV], b[NV], g[NV];
     const float rstd = gcptr<float>(p.rstd)[row];
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int64_t col = (int64_t)(c * LPR + lane) * V;
-      a[c] = g[c] = u32x4{0, 0, 0, 0};
+      g[c] = u32x4{0, 0, 0, 0};
       b[c] = row_load<T, TAIL>(h, col, p.D);
-      if (p.gy) a[c] = row_load<T, TAIL>(gy, col, p.D);
+      a[c] = row_load<T, TAIL>(gy, col, p.D);
     }
     if (p.gh) {
       const HK_G S* const gh = gcptr<S>(p.gh) + row_at(row, p.n1, p.n2, p.ghs);
@@ -357,15 +356,15 @@ __global__ __launch_bounds__(256) void rms_back_long(hrt_rms_bwd_args p, int64_t
   const int64_t first = (int64_t)blockIdx.x * per, end = first + per < p.rows ? first + per : p.rows;
   HK_G float* const ws = gptr<float>(p.ws) + (int64_t)blockIdx.x * p.D;
   for (int64_t row = first; row < end; ++row) {
-    const HK_G S* const gy = gcptr<S>(p.gy) + (p.gy ? row_at(row, p.n1, p.n2, p.gys) : 0);
+    const HK_G S* const gy = gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys);
     const HK_G S* const h = gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs);
     const HK_G S* const gh = gcptr<S>(p.gh) + (p.gh ? row_at(row, p.n1, p.n2, p.ghs) : 0);
     const float rstd = gcptr<float>(p.rstd)[row];
     auto load = [&](int64_t col, float* d, float* n, float* gyn) {
       float t[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = 0.f, t[e] = 1.f;
-      if (p.gy) R::unpack(row_piece<T, true>(gy, col, p.D), d);
+      for (int e = 0; e < V; ++e) t[e] = 1.f;
+      R::unpack(row_piece<T, true>(gy, col, p.D), d);
       R::unpack(row_piece<T, true>(h, col, p.D), n);
       if (p.w) R::unpack(row_piece<T, true>(gcptr<S>(p.w), col, p.D), t);
 #pragma unroll
@@ -395,6 +394,20 @@ __global__ __launch_bounds__(256) void rms_back_long(hrt_rms_bwd_args p, int64_t
       row_put<T, true>(gptr<S>(p.dx) + row * p.D, col, p.D, R::pack(t));
     }
   }
+}
+
+// Without gy: the norm's share is zeros whatever the row, and h, rstd and w, which need not be finite, are not read.  A workgroup a row,
+// every 65536th from there on.
+template <typename T>
+__global__ __launch_bounds__(256) void rms_back_rest(hrt_rms_bwd_args p) {
+  using S = typename T::storage;
+  constexpr int V = RowVec<T>::V;
+  for (int64_t row = blockIdx.x; p.dx && row < p.rows; row += gridDim.x) {
+    const HK_G S* const gh = gcptr<S>(p.gh) + (p.gh ? row_at(row, p.n1, p.n2, p.ghs) : 0);
+    for (int64_t col = threadIdx.x * V; col < p.D; col += 256 * V)
+      row_put<T, true>(gptr<S>(p.dx) + row * p.D, col, p.D, p.gh ? row_piece<T, true>(gh, col, p.D) : u32x4{0, 0, 0, 0});
+  }
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; p.dw && i < p.D; i += (int64_t)gridDim.x * 256) gptr<S>(p.dw)[i] = 0;
 }
 
 // dw: the workgroups' sums of 32 columns, a thread every 32nd of one column in order (16 loads in flight: one round for 512), then the
@@ -562,6 +575,10 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
       (a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
       (a.dw && !ctx.check(a.dw, a.D * E, "dw")))
     return false;
+  if (!a.gy) {
+    hipLaunchKernelGGL(rms_back_rest<T>, dim3(a.rows < 65536 ? (uint32_t)a.rows : 65536u), dim3(256), 0, ctx.stream, a);
+    return hrt::launch_ok(hipGetLastError(), ctx, "rms_bwd");
+  }
   const Share s = share_of(a.rows, a.D, V);
   const bool sums = a.dw && !strips(a, s);
   if (sums && !ctx.check(a.ws, (uint64_t)(blocks * a.D) * 4, "ws")) return false;
@@ -600,7 +617,7 @@ HK_ROWS("f16", F16);
 
 extern "C" int64_t hrt_rms_workspace(const hrt_rms_bwd_args* a, int32_t dtype) {
   using namespace hk;
-  if (!a || a->rows <= 0 || a->D <= 0 || !a->dw) return 0;
+  if (!a || a->rows <= 0 || a->D <= 0 || !a->dw || !a->gy) return 0;
   if (strips(*a, share_of(a->rows, a->D, dtype == HRT_F32 ? 4 : 8))) return 0;
   return (dtype == HRT_F32 ? back_blocks<F32>(*a) : back_blocks<BF16>(*a)) * a->D;
 }
