@@ -589,3 +589,13 @@ def test_tangents_and_gradients_are_not_dropped():
     with torch.no_grad():
         assert torch.equal(torch_vulkan.dequant_int8_rows(c, wants).cpu(), torch_vulkan.dequant_int8_rows(c, s).cpu())
     assert torch.equal(torch_vulkan.quantize_int8_rows(x.detach().requires_grad_())[0].cpu(), c.cpu())  # a weight at rest
+
+
+@pytest.mark.gpu
+def test_autocast_does_not_pass_over_a_named_type():
+    x, w, s, b = (t.to(vk) for t in operands(6, 64, 96, torch.float16, 2))
+    with torch.autocast("vk", dtype=torch.bfloat16):
+        for out in (torch.float16, torch.float32):
+            with pytest.raises(RuntimeError, match="out_dtype"):
+                torch_vulkan.int8_linear(x, w, s, b, out_dtype=out)
+        assert torch_vulkan.int8_linear(x, w, s, b, out_dtype=torch.bfloat16).dtype == torch.bfloat16

@@ -47,8 +47,8 @@ at::Tensor int8_linear_autocast(const at::Tensor& x, const at::Tensor& weight, c
                                 const std::optional<at::Tensor>& x_scale, std::optional<at::ScalarType> out_dtype) {
   if (!at::autocast::is_autocast_enabled(kDev)) return int8_linear_vk(x, weight, weight_scale, bias, x_scale, out_dtype);
   const c10::impl::ExcludeDispatchKeyGuard done(c10::DispatchKey::AutocastPrivateUse1);
-  // an int8 x has its output's type named, if any is
-  const at::ScalarType t = x.scalar_type() == at::kChar && out_dtype ? *out_dtype : at::autocast::get_autocast_dtype(kDev);
+  // an output's type that is named stays: int8_linear refuses one that is not x's, unless x is int8
+  const at::ScalarType t = out_dtype.value_or(at::autocast::get_autocast_dtype(kDev));
   return int8_linear_vk(low(x), weight, weight_scale, present(bias) ? std::optional<at::Tensor>(at::autocast::cached_cast(t, *bias, kDev)) : std::nullopt,
                         x_scale, t);
 }

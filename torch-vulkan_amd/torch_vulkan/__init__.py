@@ -405,7 +405,7 @@ def int8_linear(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None
 
     Differentiable in a 16-bit x and in bias, any number of times (create_graph), in reverse mode.  The gradient of x goes straight
     through its rounding: grad @ dequant_int8_rows(weight, weight_scale, grad.dtype).  Autocast casts x and bias, as it does
-    for linear."""
+    for linear; an out_dtype that is named stays, and has to be the type that a 16-bit x was cast to."""
     if x.device.type != "vk":
         raise RuntimeError("int8_linear: x must be a vk tensor")
     return _C.int8_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
