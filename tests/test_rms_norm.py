@@ -440,3 +440,13 @@ def test_the_residuals_way_is_its_own(shape, dtype):
     torch_vulkan.rms_norm(X, None, residual=R, eps=0.0)[1].backward(gh.to(vk))
     X.grad.add_(1)  # two gradients, not one tensor
     assert torch.equal(R.grad.cpu(), gh)
+
+
+@pytest.mark.gpu
+def test_an_eps_that_fp32_does_not_hold():
+    """Taken as 0 it would make NaN of rows of zeros, where the formula has 0."""
+    x = torch.zeros(3, 40).to(vk)
+    for f in (torch_vulkan.rms_norm, torch_vulkan.rms_norm_int8):
+        with pytest.raises(RuntimeError, match="eps"):
+            f(x, eps=1e-46)
+        assert (f(x, eps=2e-45)[0].cpu() == 0).all()

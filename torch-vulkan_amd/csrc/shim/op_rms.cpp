@@ -159,6 +159,7 @@ void check(const at::Tensor& x, const std::optional<at::Tensor>& w, const std::o
   if (present(r))
     TORCH_CHECK(on_vk(*r) && r->scalar_type() == x.scalar_type() && r->sizes() == x.sizes(), who, ": residual must be a vk tensor of x's shape and dtype");
   TORCH_CHECK(eps >= 0 && eps <= 1e30, who, ": eps must be 0 or more, got ", eps);
+  TORCH_CHECK(eps == 0 || static_cast<float>(eps) > 0, who, ": eps ", eps, " is 0 in float32: rows of zeros would be 0 / 0");
   constexpr int64_t lim = int64_t(1) << 31;
   TORCH_CHECK(x.size(-1) < lim && x.numel() / x.size(-1) < lim, who, ": too many rows or columns");
   no_tangent(x, who);
