@@ -442,6 +442,10 @@ static inline int hrt_i8_mm_quantises(int64_t M, int64_t K) {
   const int64_t waves = K <= 1024 ? 4 : 8, slots = hrt_i8_mm_row_slots(M);
   return K % 16 == 0 && M <= 8 && slots <= waves && slots * K <= 2048 * waves;
 }
+/* The kernel of a product, by M, N, K and whether x_scale is 0 alone: 0 .. HRT_I8_MM_TILES - 1 a tile's, -1 the one for few rows.
+ * *rounds (if not null): how often a tile's unguarded loop runs; the steps after it are guarded. */
+#define HRT_I8_MM_TILES 5
+int32_t hrt_i8_mm_plan(const hrt_i8_mm_args* args, int64_t* rounds);
 
 /* Root-mean-square norm of rows (no reference counterpart).  Row i of a tensor is found through up to three outer dimensions,
  * i = (i0 * n1 + i1) * n2 + i2, at element i0 * s[0] + i1 * s[1] + i2 * s[2]; D values with unit stride.

@@ -230,6 +230,7 @@ def check_back(got, g, w, s, dtype):
 
 
 # every tile and both sides of its borders, rows, odd widths, ends of K inside a line and inside a piece of 16
+# (the tile of 128 x 128, and the loops of all tiles: LONG_PRODUCTS)
 PRODUCTS = [(1, 16, 16), (1, 1, 1), (2, 8, 144), (16, 48, 2064), (16, 100, 128), (17, 64, 1024), (32, 40, 1040), (33, 136, 320), (64, 64, 512), (77, 130, 272),
             (130, 256, 400), (129, 129, 128), (257, 264, 1000), (300, 512, 77), (5, 33, 50), (200, 2056, 656), (1, 4096, 4096), (20, 512, 9000), (308, 72, 4112),
             (3, 40, 2720), (3, 24, 4096), (4, 24, 4112), (8, 24, 2048), (7, 24, 1040), (5, 24, 1024), (3, 24, 1008), (4, 8, 512), (8, 24, 2064), (1, 24, 16384), (1, 8, 16400), (2, 8, 8192), (700, 2048, 512), (1500, 4096, 256), (4100, 2048, 144)]
@@ -599,3 +600,36 @@ def test_autocast_does_not_pass_over_a_named_type():
             with pytest.raises(RuntimeError, match="out_dtype"):
                 torch_vulkan.int8_linear(x, w, s, b, out_dtype=out)
         assert torch_vulkan.int8_linear(x, w, s, b, out_dtype=torch.bfloat16).dtype == torch.bfloat16
+
+
+# Each tile at lengths of K that its loop takes in one round and in several, with as few and as many steps left behind it, whole lines
+# of y and odd ends.
+LONG_PRODUCTS = [(4100, 2056, 1024), (4090, 4095, 1616), (4100, 2056, 2064), (4090, 4095, 2200), (1500, 4104, 640), (2000, 2055, 880), (1500, 4104, 2064), (2000, 2055, 2050),
+                 (1030, 2056, 1024), (700, 4101, 1616), (700, 4104, 2064), (1030, 2050, 2200), (500, 4101, 272), (520, 2056, 880), (700, 2050, 640), (1024, 2048, 2064),
+                 (600, 2050, 2050), (130, 1032, 2048), (300, 1030, 3216), (130, 1032, 4112), (300, 1030, 4100)]
+
+
+def test_products_reach_every_tile_and_its_loop():
+    """By the plan itself: a change of its rule that leaves a tile, its unguarded loop or the steps behind it to no test fails here."""
+    import ctypes
+
+    plan = ctypes.CDLL(abi._LIB_PATH).hrt_i8_mm_plan
+    plan.argtypes, plan.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int32
+    seen = set()
+    for M, N, K in PRODUCTS + LONG_PRODUCTS:
+        rounds = ctypes.c_int64()
+        args = abi.I8MmArgs(x_scale=4, M=M, N=N, K=(K + 15) // 16 * 16)  # rows are filled up to 16
+        seen.add((plan(ctypes.byref(args), ctypes.byref(rounds)), N % 8 == 0, min(rounds.value, 2)))
+    for tile in range(abi.I8_MM_TILES):
+        for lines in (True, False):
+            assert (tile, lines, 2) in seen
+        for rounds in (0, 1):
+            assert (tile, True, rounds) in seen or (tile, False, rounds) in seen
+    assert {t for t, _, _ in seen} == {-1, *range(abi.I8_MM_TILES)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,N,K", LONG_PRODUCTS)
+def test_long_products(M, N, K, dtype):
+    test_linear(M, N, K, dtype)

@@ -447,11 +447,15 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
 // 25, 15.5, 11.4, 13.5, 15; 308 x 2048 x 2048 25, 14.5, 10, 7.7, 6.2 (before: 128 x 128 in two groups along K and 64 x 64 in four, one to a
 // CU, 11.6 and 7.5).  Over 44 sizes the choice is 2% behind the best.
 struct Tile {
-  int bm, bn;
+  int bm, bn, wm, wn, kg, xr, wr, sp;  // as i8_tile has them
   float once, per256, per128;
 };
-constexpr Tile kTiles[] = {{256, 256, 0.f, 11.f, 1.48f}, {128, 256, 0.f, 9.f, 0.82f}, {128, 128, 6.5f, 1.2f, 0.49f}, {128, 64, 4.f, 1.35f, 0.29f}, {64, 64, 3.2f, 0.97f, 0.183f}};
-constexpr int kNumTiles = 5;
+constexpr int kNumTiles = HRT_I8_MM_TILES;
+constexpr Tile kTiles[kNumTiles] = {{256, 256, 128, 64, 1, 3, 2, 3, 0.f, 11.f, 1.48f},
+                                    {128, 256, 64, 64, 1, 3, 3, 3, 0.f, 9.f, 0.82f},
+                                    {128, 128, 32, 64, 1, 3, 2, 0, 6.5f, 1.2f, 0.49f},
+                                    {128, 64, 32, 32, 1, 3, 3, 0, 4.f, 1.35f, 0.29f},
+                                    {64, 64, 32, 32, 2, 3, 2, 0, 3.2f, 0.97f, 0.183f}};
 
 int64_t tiles_of(const hrt_i8_mm_args& a, int t) { return cdiv(a.M, kTiles[t].bm) * cdiv(a.N, kTiles[t].bn); }
 // Index of the tile, -1: i8_rows (up to 16 rows, or 32 where K is short).  us of i8_rows and of the tile chosen otherwise, at 16, 17 and 32
@@ -470,22 +474,30 @@ int plan_of(const hrt_i8_mm_args& a) {
   return best;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int KG, int XR, int WR, int SP>
+// Steps of a product, and how many rounds of them i8_tile takes without a guard.
+int64_t steps_of(const hrt_i8_mm_args& a, const Tile& t) { return cdiv(a.K, kLine * t.kg); }
+int64_t whole_rounds(const hrt_i8_mm_args& a, const Tile& t) {
+  const int64_t left = steps_of(a, t) - (t.xr - 1);
+  return left > 0 ? left / (t.xr == t.wr ? t.xr : t.xr * t.wr) : 0;
+}
+
+template <typename T, int I>
 void queue_tile(const hrt_i8_mm_args& a, hipStream_t s, bool lines) {
-  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), nk = cdiv(a.K, kLine * KG);
-  hipLaunchKernelGGL((i8_tile<T, BM, BN, WM, WN, KG, XR, WR, SP>), dim3((uint32_t)(tm * tn)), dim3(64 * TileShape<BM, BN, WM, WN, KG, XR, WR>::NW), 0, s, a, (int)tn,
-                     (int)nk, lines);
+  constexpr Tile t = kTiles[I];
+  const int64_t tm = cdiv(a.M, t.bm), tn = cdiv(a.N, t.bn);
+  hipLaunchKernelGGL((i8_tile<T, t.bm, t.bn, t.wm, t.wn, t.kg, t.xr, t.wr, t.sp>), dim3((uint32_t)(tm * tn)),
+                     dim3(64 * TileShape<t.bm, t.bn, t.wm, t.wn, t.kg, t.xr, t.wr>::NW), 0, s, a, (int)tn, (int)steps_of(a, t), lines);
 }
 
 template <typename T>
 void queue_mm(const hrt_i8_mm_args& a, int tile, hipStream_t s) {
   const bool vec = a.N % 4 == 0 && a.y % 8 == 0 && a.bias % 8 == 0 && a.w_scale % 16 == 0, lines = vec && a.N % 8 == 0 && a.y % 16 == 0;
   switch (tile) {
-    case 0: return queue_tile<T, 256, 256, 128, 64, 1, 3, 2, 3>(a, s, lines);
-    case 1: return queue_tile<T, 128, 256, 64, 64, 1, 3, 3, 3>(a, s, lines);
-    case 2: return queue_tile<T, 128, 128, 32, 64, 1, 3, 2, 0>(a, s, lines);
-    case 3: return queue_tile<T, 128, 64, 32, 32, 1, 3, 3, 0>(a, s, lines);
-    case 4: return queue_tile<T, 64, 64, 32, 32, 2, 3, 2, 0>(a, s, lines);
+    case 0: return queue_tile<T, 0>(a, s, lines);
+    case 1: return queue_tile<T, 1>(a, s, lines);
+    case 2: return queue_tile<T, 2>(a, s, lines);
+    case 3: return queue_tile<T, 3>(a, s, lines);
+    case 4: return queue_tile<T, 4>(a, s, lines);
   }
   // wavefronts and batches that cover K once where they can
   const dim3 grid((uint32_t)cdiv(a.N, 16));
@@ -530,3 +542,10 @@ HRT_REGISTER("i8_mm_f16", hrt_i8_mm_args, launch_i8_mm<F16>);
 
 }  // namespace
 }  // namespace hk
+
+extern "C" int32_t hrt_i8_mm_plan(const hrt_i8_mm_args* a, int64_t* rounds) {
+  using namespace hk;
+  const int tile = a->M > 0 && a->N > 0 && a->K > 0 ? plan_of(*a) : -1;
+  if (rounds) *rounds = tile < 0 ? 0 : whole_rounds(*a, kTiles[tile]);
+  return tile;
+}

@@ -59,6 +59,9 @@ class I8MmArgs(ctypes.Structure):
                 ("M", i64), ("N", i64), ("K", i64), ("x_sm", i64), ("w_sn", i64)]
 
 
+I8_MM_TILES = 5  # HRT_I8_MM_TILES (include/hrt_ops.h)
+
+
 class I8LinearBackArgs(ctypes.Structure):
     _fields_ = [("w", u64), ("w_scale", u64), ("v", u64), ("g", u64), ("db", u64), ("M", i64), ("N", i64), ("K", i64),
                 ("w_sn", i64), ("g_sm", i64)]
@@ -271,6 +274,7 @@ class Runtime:
             "hrt_graph_destroy": (ctypes.c_int, [i64]),
             "hrt_reduce_workspace": (i64, [vp]),
             "hrt_rms_workspace": (i64, [vp, i32]),
+            "hrt_i8_mm_plan": (i32, [vp, vp]),
             "hrt_ln_bwd_noalloc": (ctypes.c_int, [vp, i32]),
         }
         for name, (res, args) in sig.items():
