@@ -450,3 +450,39 @@ def test_an_eps_that_fp32_does_not_hold():
         with pytest.raises(RuntimeError, match="eps"):
             f(x, eps=1e-46)
         assert (f(x, eps=2e-45)[0].cpu() == 0).all()
+
+
+# sums of the weight's gradient over more rows than the strips take: every sharing with a workspace, several rows to a workgroup of the
+# passes too
+MANY_ROWS = [(1100, 2052), (1100, 2056), (1100, 4096), (1100, 4100), (1030, 8200), (1030, 8201), (600, 16400), (1200, 16401)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", MANY_ROWS)
+def test_many_wide_rows_against_the_formula(shape, dtype):
+    test_against_the_formula(shape, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1500, 264), (1500, 520), (600, 16400)])
+def test_two_threads_with_workspaces(shape):
+    """Gradients whose sums go through a workspace, from two threads at once: one thread's bits."""
+    x, w, r, gy, _ = (t.to(vk) for t in data(shape, torch.float16, 2))
+
+    def gradients_of():
+        X, W = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y, _ = torch_vulkan.rms_norm(X, W, residual=r)
+        return torch.autograd.grad(y, (X, W), gy)
+
+    want, bad = [t.cpu() for t in gradients_of()], []
+
+    def work():
+        for _ in range(10):
+            if not all(torch.equal(a.cpu(), b) for a, b in zip(gradients_of(), want)):
+                bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
