@@ -633,3 +633,36 @@ def test_products_reach_every_tile_and_its_loop():
 @pytest.mark.parametrize("M,N,K", LONG_PRODUCTS)
 def test_long_products(M, N, K, dtype):
     test_linear(M, N, K, dtype)
+
+
+def f16_quotients():
+    """Rows under every f16 mantissa as the largest value, with every mantissa not above it in its own binade, where quotients come
+    closest to a border (a 2^19th of their size), and the closest of the binades below."""
+    man = 1 + torch.arange(1024) / 1024
+    top = man.unsqueeze(-1)
+    x = (man * torch.exp2(-torch.arange(9.0)).unsqueeze(-1)).flatten().expand(1024, -1)
+    x = torch.cat([top, torch.where(x <= top, x, torch.zeros(()))], -1)
+    return torch.cat([x, -x]).half()
+
+
+def test_how_close_quotients_come_to_a_border():
+    """254 a and k b of 11-bit a <= b, k odd, differ by 1 at least, of at most 254 x 2047: 2^-19, and 2^-32 for 24 bits."""
+    a = torch.arange(1024, 2048, dtype=torch.int64)
+    gap = 1.0
+    for b in a.tolist():
+        n = 254 * a[a <= b]
+        k = n // b
+        near = torch.minimum((n - (k - 1 + k % 2) * b).abs(), (n - (k + 1 + k % 2) * b).abs())
+        gap = min(gap, float((near[near > 0] / n[near > 0]).min()))
+    assert 2.0**-19 < gap < 2.0**-18
+
+
+def test_every_f16_quotient_on_the_cpu():
+    x = f16_quotients()[::7]
+    same(torch_vulkan.quantize_int8_rows(x), packed(x))
+
+
+@pytest.mark.gpu
+def test_every_f16_quotient():
+    x = f16_quotients()
+    same(torch_vulkan.quantize_int8_rows(x.to(vk)), packed(x))

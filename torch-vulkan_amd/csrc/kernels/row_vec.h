@@ -159,9 +159,11 @@ constexpr float kRound32 = 12582912.f;
 constexpr double kRound64 = 6755399441055744.0;  // 1.5 2^52
 // Codes of fp32 values that are roundings themselves: the quotient as it comes out.
 __device__ __forceinline__ uint32_t code_of(float v, const RowCode& r) { return __float_as_uint(v * r.mul * r.per + kRound32); }
-// The nearest code exactly.  Relative to its size, a quotient that is no tie is at least 2^-18 away from one (127 times an 11-bit
-// number against an odd multiple of an 11-bit one; 2^-31 for 24-bit ones), and comes out within 2^-22 (2^-51 in fp64).  Rounded to
-// 20 bits (45), ties, which have 8, are ties again, and nothing else becomes one.
+// The nearest code exactly.  With v and top of p bits, 254 v against an odd multiple k top of a border are whole numbers (times a power
+// of two) that differ by 1 at least where v and top share a binade, by 2 below: relative to its size a quotient that is no tie is at
+// least 1 / (254 (2^p - 1)) > 2^-19 away from one (p = 11; 2^-32 for 24 bits).  It comes out within 2^-22 (2^-51 in fp64), and is
+// rounded to 20 bits (45), which moves it by at most 2^-20 (2^-45): ties, which have 8 bits, are ties again, and nothing else
+// reaches one.
 template <typename T>
 __device__ __forceinline__ uint32_t nearest_code(float v, const RowCode& r) {
   if constexpr (std::is_same<T, F32>::value) {
