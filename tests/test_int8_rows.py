@@ -626,6 +626,8 @@ def test_products_reach_every_tile_and_its_loop():
         for rounds in (0, 1):
             assert (tile, True, rounds) in seen or (tile, False, rounds) in seen
     assert {t for t, _, _ in seen} == {-1, *range(abi.I8_MM_TILES)}
+    none = ctypes.c_int64(7)
+    assert plan(None, None) == -1 and plan(ctypes.byref(abi.I8MmArgs()), ctypes.byref(none)) == -1 and none.value == 0
 
 
 @pytest.mark.gpu

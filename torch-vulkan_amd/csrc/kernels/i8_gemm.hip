@@ -545,7 +545,7 @@ HRT_REGISTER("i8_mm_f16", hrt_i8_mm_args, launch_i8_mm<F16>);
 
 extern "C" int32_t hrt_i8_mm_plan(const hrt_i8_mm_args* a, int64_t* rounds) {
   using namespace hk;
-  const int tile = a->M > 0 && a->N > 0 && a->K > 0 ? plan_of(*a) : -1;
+  const int tile = a && a->M > 0 && a->N > 0 && a->K > 0 ? plan_of(*a) : -1;
   if (rounds) *rounds = tile < 0 ? 0 : whole_rounds(*a, kTiles[tile]);
   return tile;
 }
