@@ -7,6 +7,7 @@ Backward: n = h rstd from the kept h, which with a residual was rounded to its t
 the mean of |d n|; three more roundings and the output's.  dw: each term e + 10 u, the sum over the rows at most rows + 80
 roundings."""
 
+import ctypes
 import threading
 
 import numpy as np
@@ -486,3 +487,21 @@ def test_two_threads_with_workspaces(shape):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_backward_block_without_gy(dtype):
+    """dx = gh and dw = 0, with nothing else given, and zeros where there is no gh either; no workspace is asked for."""
+    rt, (rows, D) = abi.Runtime(), (1100, 70)
+    suffix, code = {torch.float32: ("f32", 0), torch.bfloat16: ("bf16", 1), torch.float16: ("f16", 2)}[dtype]
+    gh = data((rows, D), dtype, 4)[4].to(vk)
+    for g in (gh, None):
+        dx, dw = torch.ones(rows, D, dtype=dtype, device=vk), torch.ones(D, dtype=dtype, device=vk)
+        a = abi.RmsBwdArgs(gh=g.data_ptr() if g is not None else 0, dx=dx.data_ptr(), dw=dw.data_ptr(), rows=rows, D=D, n1=1, n2=1, ghs=(abi.i64 * 3)(D, 0, 0))
+        assert rt.lib.hrt_rms_workspace(ctypes.byref(a), code) == 0
+        rt.dispatch("rms_bwd_" + suffix, a)
+        assert torch.equal(dx.cpu(), gh.cpu() if g is not None else torch.zeros(rows, D, dtype=dtype)) and (dw.cpu() == 0).all()
+    with pytest.raises(RuntimeError, match="h"):
+        a.gy = gh.data_ptr()
+        rt.dispatch("rms_bwd_" + suffix, a)

@@ -571,8 +571,8 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   const int64_t blocks = back_blocks<T>(a);
   if ((a.gy && !ctx.check(a.gy, rows_span(a.rows, a.n1, a.n2, a.D, a.gys, E), "gy")) ||
       (a.gh && !ctx.check(a.gh, rows_span(a.rows, a.n1, a.n2, a.D, a.ghs, E), "gh")) ||
-      !ctx.check(a.h, rows_span(a.rows, a.n1, a.n2, a.D, a.hs, E), "h") || !ctx.check(a.rstd, a.rows * 4, "rstd") ||
-      (a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
+      (a.gy && (!ctx.check(a.h, rows_span(a.rows, a.n1, a.n2, a.D, a.hs, E), "h") || !ctx.check(a.rstd, a.rows * 4, "rstd"))) ||
+      (a.gy && a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
       (a.dw && !ctx.check(a.dw, a.D * E, "dw")))
     return false;
   if (!a.gy) {
