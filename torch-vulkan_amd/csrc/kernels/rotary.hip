@@ -3,7 +3,7 @@
 // Bound by memory: every value is read once and written once.  The sines and cosines depend on the token and the pair alone, so a
 // workgroup takes all heads of a few tokens, computes each of them once into LDS and its lanes keep theirs in registers over
 // the heads.  Far positions: the angle is reduced to an eighth of a turn in fp64 (position times frequency in 53 bits) before its
-// sine and cosine are taken in fp32, which leaves them within 2^-23.  Measured, bf16, 16 + 16 heads of 128: 2 x 4096 tokens 24.9 us
+// sine and cosine are taken in fp32, which leaves them within 2^-22 + |angle| 2^-51: up to 2^29 radians the fp32 steps are the larger part.  Measured, bf16, 16 + 16 heads of 128: 2 x 4096 tokens 24.9 us
 // by the kernel trace (5.4 TB/s, part of it from the last cache; 26.6 with four tokens to a workgroup), 22.5 replayed on the same operands; 8 tokens 3.7 us.
 #include "../hrt/registry.h"
 #include "row_vec.h"

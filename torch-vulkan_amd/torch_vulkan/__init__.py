@@ -451,7 +451,7 @@ def rotary_embedding(q, k, positions, freqs, sections, interleaved=False):
     belong to each axis (1..4 of them), P in all; pair j is the values (j, j + P) of a head, or (2 j, 2 j + 1) where interleaved,
     and the values behind 2 P stay as they are.  positions [S, axes] or [B, S, axes]: int32, int64 or float32.  freqs [P]: float64,
     in radians per position (rotary_frequencies gives the usual ones).  Angles are taken in float64, so that far positions keep
-    theirs.
+    theirs: sines and cosines are within 2**-22 + |angle| * 2**-51.
 
     Returns (q, k), or q alone where k is None, in token-major memory, as the fused attention reads them; differentiable in q and k,
     any number of times, in reverse mode."""
