@@ -451,9 +451,11 @@ int32_t hrt_i8_mm_plan(const hrt_i8_mm_args* args, int64_t* rounds);
  * i = (i0 * n1 + i1) * n2 + i2, at element i0 * s[0] + i1 * s[1] + i2 * s[2]; D values with unit stride.
  * "rms_fwd_{f32,bf16,f16}" — h = x + r (r 0: h = x), y = h * rstd * w with rstd = 1 / sqrt(mean(h^2) + eps) in fp32 from the
  *   unrounded h (w 0: none).  y and, where h_out is not 0, the rounded h are [rows, D] contiguous; rstd [rows] if not 0.
+ *   h_rest (16-bit kernels with r and h_out, if not 0): int8 [rows, D rounded up to 8], 8-byte aligned: what rounding took
+ *   from h, in 256ths of its type's last place, for rms_bwd.
  *   q not 0: in place of y its rows in 8 bits, q [rows, D] and scale [rows] as "i8_rows_quant_*" makes them from the
  *   unrounded y (up to the rounding of 127 y / top in fp32).
- * "rms_bwd_{dt}" — from gy, gh (gradients of y and h, either 0), h (strides hs) and rstd:
+ * "rms_bwd_{dt}" — from gy, gh (gradients of y and h, either 0), h (strides hs), h_rest (if not 0, 16-bit kernels: added back to h) and rstd:
  *   dx = rstd * (gy w - n * mean(gy w n)) + gh with n = h rstd; dw (if not 0) = the sum of gy n over the rows; without gy dx = gh
  *   and dw = 0, and h, rstd and w are not read.  dx (if not 0) [rows, D] contiguous.  dw needs ws, hrt_rms_workspace(&args, dtype) floats (none for few rows): sums of runs of rows, added in
  *   order. */
@@ -463,11 +465,13 @@ typedef struct hrt_rms_args {
   int64_t xs[3], rs[3];
   float eps;
   uint32_t pad;
+  uint64_t h_rest;
 } hrt_rms_args;
 typedef struct hrt_rms_bwd_args {
   uint64_t gy, gh, h, rstd, w, dx, dw, ws;
   int64_t rows, D, n1, n2;
   int64_t gys[3], ghs[3], hs[3];
+  uint64_t h_rest;
 } hrt_rms_bwd_args;
 int64_t hrt_rms_workspace(const hrt_rms_bwd_args* args, int32_t dtype);
 

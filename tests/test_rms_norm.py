@@ -505,3 +505,68 @@ def test_the_backward_block_without_gy(dtype):
     with pytest.raises(RuntimeError, match="h"):
         a.gy = gh.data_ptr()
         rt.dispatch("rms_bwd_" + suffix, a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(64, 96), (64, 97), (64, 5), (700, 264), (1030, 130), (1100, 2048), (1100, 4100), (64, 8201), (600, 16400), (520, 16403)])
+def test_the_weights_gradient_of_an_unrounded_sum(shape, dtype):
+    """Rows in pairs of equal gradients of opposite sign and of sums that round alike: the weight's gradient is what rounding takes
+    from the sums.  It is left within a 512th of half the type's last place (2^-16, 2^-19 of the value; a subnormal sum within half
+    its last place, 2^-25 in f16), for which the header's tolerance has e, and is tested against the formula with that bound."""
+    rows, D = shape
+    g = torch.Generator().manual_seed(rows + D)
+    e = torch.finfo(dtype).eps
+    h = (torch.randint(-512, 513, (rows // 2, D), generator=g).float() / 256 + torch.randint(0, 2, (rows // 2, D), generator=g).float() * 4).to(dtype)
+    rest = (h.double().abs() * (torch.rand(rows // 2, D, generator=g).double() - 0.5) * 0.9 * e / 2).to(dtype)  # below half of any last place
+    x, r = torch.stack((h, h), 1).view(rows, D), torch.stack((rest, torch.zeros_like(rest)), 1).view(rows, D)
+    gy = torch.randn(rows // 2, D, generator=g).to(dtype)
+    gy = torch.stack((gy, -gy), 1).view(rows, D)
+    w = (1 + 0.2 * torch.randn(D, generator=g)).to(dtype)
+    X, W, R = (t.to(vk).requires_grad_() for t in (x, w, r))
+    y, hh = torch_vulkan.rms_norm(X, W, residual=R)
+    if dtype != torch.float32:
+        assert torch.equal(hh.detach().cpu(), x)
+    dx, dw = torch.autograd.grad(y, (X, W), gy.to(vk))
+    want, _, dw64, _ = gradients(x, w, r, gy, None, 1e-6)
+    n, _, size = norm(x, None, r, 1e-6)
+    left = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-16, torch.float16: 2.0**-19}[dtype]
+    terms = np.abs(f64(gy)) * (np.abs(n) * (left + (steps(D) + 8 + 10 + rows + 80) * U) + (2.0**-25 / size if dtype == torch.float16 else 0.0))
+    within(dw, dw64, terms.sum(0), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("D", [5, 64, 97, 1000, 4100, 16403])
+def test_what_rounding_takes_from_a_sum(D, dtype):
+    """h and its rests give the fp32 sum within half a 256th of the type's last place (a whole one where that is half the last place up),
+    at both ends of the exponent range, beside rows that are not finite; refused where there is nothing to round."""
+    rt, rows = abi.Runtime(), 9
+    suffix, bits = ("bf16", 16) if dtype == torch.bfloat16 else ("f16", 13)  # fp32 patterns in a last place
+    g = torch.Generator().manual_seed(D)
+    big = torch.finfo(dtype).max
+    size = torch.tensor([1.0, 2.0**-10, 2.0**-13, 300.0, big / 8, 1.0, 1.0, 1.0, 2.0**-30 if dtype == torch.bfloat16 else 2.0**-5]).unsqueeze(1)
+    x, r = (torch.randn(rows, D, generator=g) * size).to(dtype), (torch.randn(rows, D, generator=g) * size / 64).to(dtype)
+    x[5, 3], x[6, 1], x[7], r[7] = float("inf"), float("nan"), big, big * 2.0**-10  # the last: a sum that rounds to an infinity, or to the largest
+    x[8, :2], r[8, :2] = 0, 0
+    pitch = (D + 7) // 8 * 8
+    X, R, Y, H = x.to(vk), r.to(vk), torch.zeros(rows, D, dtype=dtype, device=vk), torch.zeros(rows, D, dtype=dtype, device=vk)
+    rest = torch.full((rows, pitch), 7, dtype=torch.int8, device=vk)
+    xs = (abi.i64 * 3)(D, 0, 0)
+    args = dict(x=X.data_ptr(), y=Y.data_ptr(), rows=rows, D=D, n1=1, n2=1, xs=xs, rs=xs, eps=1e-6)
+    rt.dispatch("rms_fwd_" + suffix, abi.RmsArgs(r=R.data_ptr(), h_out=H.data_ptr(), h_rest=rest.data_ptr(), **args))
+    s, h = x.float() + r.float(), H.cpu()
+    assert torch.equal(torch.nan_to_num(h.float()), torch.nan_to_num(s.to(dtype).float())) and (rest.cpu()[:, D:] == 0).all()
+    back = (h.float().view(torch.int32) + (rest.cpu()[:, :D].int() << (bits - 8))).view(torch.float32)
+    fine = h.isfinite()
+    normal = fine & (h.float().abs() >= 2.0**-14)
+    assert torch.equal(back[~fine].isnan(), s[~fine].isnan()) and not back[~fine].isfinite().any()
+    off = (back.double() - s.double()).abs()
+    assert (off[normal] <= s.double().abs()[normal] * 2.0 ** (bits - 8 - 23)).all()
+    assert (off[fine] <= (h.double() - s.double()).abs()[fine] + s.double().abs()[fine] * 2.0 ** (bits - 8 - 23)).all()
+    for bad in (dict(r=R.data_ptr(), h_rest=rest.data_ptr()), dict(h_out=H.data_ptr(), h_rest=rest.data_ptr()),
+                dict(r=R.data_ptr(), h_out=H.data_ptr(), h_rest=rest.data_ptr() + 4)):
+        with pytest.raises(RuntimeError, match="h_rest"):
+            rt.dispatch("rms_fwd_" + suffix, abi.RmsArgs(**bad, **args))
+    with pytest.raises(RuntimeError, match="h_rest"):
+        rt.dispatch("rms_bwd_f32", abi.RmsBwdArgs(gy=X.data_ptr(), h=X.data_ptr(), rstd=Y.data_ptr(), dx=Y.data_ptr(), h_rest=rest.data_ptr(), rows=1, D=2, n1=1, n2=1))

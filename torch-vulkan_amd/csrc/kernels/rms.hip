@@ -24,6 +24,43 @@ constexpr int threads_of(int lpr) { return lpr > 256 ? lpr : 256; }
 
 enum Mode { kNorm, kNorm8, kQuant };
 
+// What rounding a sum to 16 bits took from it, in whole 256ths of the type's last place, for the backward pass, whose gradients would else be
+// those of the rounded sum (the weight's of 4020 x 2048 0.0027 of its norm off for 0.0018 of its own rounding).  Neighbouring fp32
+// numbers have neighbouring bit patterns across binades too, so it is the patterns' difference, 2^8 of them a unit for bf16 and 2^5 for
+// f16; sums that f16 holds as subnormals, whose rests are larger than a byte, keep what fits.  Half the bytes of a second 16-bit
+// tensor, and within 2^-16 (2^-19) of the sum.
+template <typename T>
+struct Rest {
+  static constexpr int SH = std::is_same<T, BF16>::value ? 8 : 5;
+  __device__ __forceinline__ static int of(float sum, float h) {
+    const uint32_t b = __float_as_uint(h);
+    const int units = ((int)(__float_as_uint(sum) - b) + (1 << (SH - 1))) >> SH;
+    return (b & 0x7f800000u) == 0x7f800000u ? 0 : units > 127 ? 127 : units < -128 ? -128 : units;
+  }
+  __device__ __forceinline__ static float sum(float h, int rest) { return __uint_as_float(__float_as_uint(h) + ((uint32_t)rest << SH)); }
+  // Rows are filled up to whole pieces of eight.
+  __device__ __forceinline__ static int64_t pitch(int64_t D) { return (D + 7) & ~(int64_t)7; }
+  // Piece `col` of a row; one past its end: any, for `add` to drop.
+  __device__ __forceinline__ static u32x2 load(uint64_t rests, int64_t row, int64_t col, int64_t D) {
+    return *reinterpret_cast<const HK_G u32x2*>(gcptr<uint8_t>(rests) + row * pitch(D) + (col < D ? col : 0));
+  }
+  __device__ __forceinline__ static void add(u32x2 w, bool in, float* h) {
+    if (!in) w = u32x2{0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = sum(h[e], (int8_t)(w[e >> 2] >> (8 * (e & 3))));
+  }
+  __device__ __forceinline__ static void put(uint64_t rests, int64_t row, int64_t col, int64_t D, const float* v, u32x4 packed) {
+    float h[8];
+    uint32_t q[8];
+    RowVec<T>::unpack(packed, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = (uint32_t)of(v[e], h[e]);
+    if (col < D) *reinterpret_cast<HK_G u32x2*>(gptr<uint8_t>(rests) + row * pitch(D) + col) = u32x2{pack_codes4(q), pack_codes4(q + 4)};
+  }
+};
+template <typename T>
+constexpr bool kRests = sizeof(typename T::storage) == 2;
+
 // kQuant reads rows x (stride xs[0]) and writes codes (pitch q_sr) and scales; its arguments come in the same block, so that one
 // kernel serves all three.
 template <typename T, int MODE, int LPR, int NV, bool TAIL>
@@ -63,7 +100,12 @@ __global__ __launch_bounds__(threads_of(LPR)) void rms_rows(hrt_rms_args p, int6
 #pragma unroll
       for (int e = 0; e < V; ++e) v[c][e] += t[e];
     }
-    if (MODE != kQuant && p.h_out && live) row_put<T, TAIL>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v[c]));
+    if (MODE != kQuant && p.h_out && live) {
+      const u32x4 h = R::pack(v[c]);
+      row_put<T, TAIL>(gptr<S>(p.h_out) + row * p.D, col, p.D, h);
+      if constexpr (MODE == kNorm && kRests<T>)
+        if (p.h_rest) Rest<T>::put(p.h_rest, row, col, p.D, v[c], h);
+    }
     if (!TAIL && col >= p.D) {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[c][e] = 0.f;
@@ -159,6 +201,8 @@ __global__ __launch_bounds__(256) void rms_long(hrt_rms_args p, int64_t q_sr) {
 #pragma unroll
       for (int e = 0; e < V; ++e) ss = fmaf(v[e], v[e], ss);
       if (p.h_out) row_put<T, true>(gptr<S>(p.h_out) + row * p.D, col, p.D, R::pack(v));
+      if constexpr (MODE == kNorm && kRests<T>)
+        if (p.h_rest) Rest<T>::put(p.h_rest, row, col, p.D, v, R::pack(v));
     }
     rstd = 1.f / sqrtf(lanes_sum<256>(ss, red) / (float)p.D + p.eps);
     if (p.rstd && threadIdx.x == 0) gptr<float>(p.rstd)[row] = rstd;
@@ -204,7 +248,7 @@ __global__ __launch_bounds__(256) void rms_long(hrt_rms_args p, int64_t q_sr) {
 // ---- backward -------------------------------------------------------------------------------------------------------------
 // dw where there are few rows: the workgroups behind those that take rows have strips of 128 bytes of columns each, of all rows
 // (which the others read too: from L2).
-template <typename T, bool TAIL, int TPB>
+template <typename T, bool TAIL, bool REST, int TPB>
 __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) {
   using R = RowVec<T>;
   using S = typename T::storage;
@@ -217,6 +261,7 @@ __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) 
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
   for (int64_t r0 = group; r0 < p.rows; r0 += 4 * G) {
     u32x4 a[4], b[4];
+    u32x2 rest[4];
     float rstd[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {  // four rows' loads in flight; a row past the end repeats the last one
@@ -224,12 +269,14 @@ __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) 
       a[u] = row_load<T, TAIL>(gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys), col, p.D);
       b[u] = row_load<T, TAIL>(gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs), col, p.D);
       rstd[u] = gcptr<float>(p.rstd)[row];
+      if constexpr (REST) rest[u] = Rest<T>::load(p.h_rest, row, col, p.D);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float d[V], n[V];
       R::unpack(row_fix<T, TAIL>(a[u], col, p.D), d);
       R::unpack(row_fix<T, TAIL>(b[u], col, p.D), n);
+      if constexpr (REST) Rest<T>::add(rest[u], col < p.D, n);
       if (r0 + u * G < p.rows) {
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] += d[e] * (n[e] * rstd[u]);
@@ -249,13 +296,14 @@ __device__ __forceinline__ void rms_strip(const hrt_rms_bwd_args& p, int strip) 
 
 // A workgroup takes `per` consecutive rows, one for every LPR threads at a time.  DW: a lane adds gy n of its columns up over its rows, the
 // workgroup's lanes of a column are added in order through LDS, and the sums of all workgroups by rms_dw_sum.
-template <typename T, int LPR, int NV, bool TAIL, bool DW>
+// REST: what rounding took from h is there (kernels of their own: without it 800 x 800 would take 8.1 us, so 7.6).
+template <typename T, int LPR, int NV, bool TAIL, bool DW, bool REST>
 __global__ __launch_bounds__(threads_of(LPR)) void rms_back(hrt_rms_bwd_args p, int64_t per, int blocks) {
   using R = RowVec<T>;
   using S = typename T::storage;
   constexpr int V = R::V, RPB = threads_of(LPR) / LPR;
   if constexpr (!DW) {
-    if ((int)blockIdx.x >= blocks) return rms_strip<T, TAIL, threads_of(LPR)>(p, (int)blockIdx.x - blocks);
+    if ((int)blockIdx.x >= blocks) return rms_strip<T, TAIL, REST, threads_of(LPR)>(p, (int)blockIdx.x - blocks);
   }
   __shared__ float red[2][threads_of(LPR) / 64];
   __shared__ __attribute__((aligned(16))) float part[DW && RPB > 1 ? RPB * LPR * NV * V : 4];
@@ -277,6 +325,7 @@ __global__ __launch_bounds__(threads_of(LPR)) void rms_back(hrt_rms_bwd_args p, 
     const HK_G S* const gy = gcptr<S>(p.gy) + row_at(row, p.n1, p.n2, p.gys);
     const HK_G S* const h = gcptr<S>(p.h) + row_at(row, p.n1, p.n2, p.hs);
     u32x4 a[NV], b[NV], g[NV];
+    u32x2 rest[NV];
     const float rstd = gcptr<float>(p.rstd)[row];
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
@@ -284,6 +333,7 @@ __global__ __launch_bounds__(threads_of(LPR)) void rms_back(hrt_rms_bwd_args p, 
       g[c] = u32x4{0, 0, 0, 0};
       b[c] = row_load<T, TAIL>(h, col, p.D);
       a[c] = row_load<T, TAIL>(gy, col, p.D);
+      if constexpr (REST) rest[c] = Rest<T>::load(p.h_rest, row, col, p.D);
     }
     if (p.gh) {
       const HK_G S* const gh = gcptr<S>(p.gh) + row_at(row, p.n1, p.n2, p.ghs);
@@ -300,6 +350,7 @@ __global__ __launch_bounds__(threads_of(LPR)) void rms_back(hrt_rms_bwd_args p, 
       float t[V];
       R::unpack(a[c], d[c]);
       R::unpack(b[c], n[c]);
+      if constexpr (REST) Rest<T>::add(rest[c], live && col < p.D, n[c]);
       if (p.w) R::unpack(w[c], t);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -366,6 +417,8 @@ __global__ __launch_bounds__(256) void rms_back_long(hrt_rms_bwd_args p, int64_t
       for (int e = 0; e < V; ++e) t[e] = 1.f;
       R::unpack(row_piece<T, true>(gy, col, p.D), d);
       R::unpack(row_piece<T, true>(h, col, p.D), n);
+      if constexpr (kRests<T>)
+        if (p.h_rest) Rest<T>::add(Rest<T>::load(p.h_rest, row, col, p.D), true, n);
       if (p.w) R::unpack(row_piece<T, true>(gcptr<S>(p.w), col, p.D), t);
 #pragma unroll
       for (int e = 0; e < V; ++e) n[e] *= rstd, gyn[e] = d[e] * n[e], d[e] *= t[e];
@@ -515,11 +568,13 @@ bool launch_rms_fwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   constexpr uint64_t E = sizeof(S);
   if (!rows_ok(a.rows, a.D, a.n1, a.n2, {a.xs, a.rs}, E, {a.x, a.r, a.w, a.y, a.h_out}, ctx)) return false;
   if (a.scale % 4 != 0 || a.rstd % 4 != 0) return ctx.fail("scale and rstd must be 4-byte aligned");
+  if (a.h_rest && (E != 2 || !a.r || !a.y || !a.h_out || a.h_rest % 8 != 0)) return ctx.fail("h_rest: beside a 16-bit h and y of a sum, 8-byte aligned");
   if ((a.q != 0) != (a.scale != 0) || (a.q != 0) == (a.y != 0)) return ctx.fail("either y, or q and scale");
   const uint64_t n = (uint64_t)a.rows * a.D;
   if (!ctx.check(a.x, rows_span(a.rows, a.n1, a.n2, a.D, a.xs, E), "x") ||
       (a.r && !ctx.check(a.r, rows_span(a.rows, a.n1, a.n2, a.D, a.rs, E), "r")) || (a.w && !ctx.check(a.w, a.D * E, "w")) ||
       (a.y && !ctx.check(a.y, n * E, "y")) || (a.h_out && !ctx.check(a.h_out, n * E, "h_out")) || (a.q && !ctx.check(a.q, n, "q")) ||
+      (a.h_rest && !ctx.check(a.h_rest, a.rows * (cdiv(a.D, 8) * 8), "h_rest")) ||
       (a.scale && !ctx.check(a.scale, a.rows * 4, "scale")) || (a.rstd && !ctx.check(a.rstd, a.rows * 4, "rstd")))
     return false;
   if (!(a.q ? queue_rows<T, kNorm8>(a, a.D, ctx) : queue_rows<T, kNorm>(a, a.D, ctx))) return false;
@@ -566,13 +621,14 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   constexpr int V = RowVec<T>::V;
   if (!rows_ok(a.rows, a.D, a.n1, a.n2, {a.gys, a.ghs, a.hs}, E, {a.gy, a.gh, a.h, a.w, a.dx, a.dw}, ctx)) return false;
   if (a.rstd % 4 != 0 || a.ws % 4 != 0) return ctx.fail("rstd and ws must be 4-byte aligned");
+  if (a.h_rest && (E != 2 || a.h_rest % 8 != 0)) return ctx.fail("h_rest: of 16-bit values, 8-byte aligned");
   if (!a.dx && !a.dw) return true;
   const uint64_t n = (uint64_t)a.rows * a.D;
   const int64_t blocks = back_blocks<T>(a);
   if ((a.gy && !ctx.check(a.gy, rows_span(a.rows, a.n1, a.n2, a.D, a.gys, E), "gy")) ||
       (a.gh && !ctx.check(a.gh, rows_span(a.rows, a.n1, a.n2, a.D, a.ghs, E), "gh")) ||
       (a.gy && (!ctx.check(a.h, rows_span(a.rows, a.n1, a.n2, a.D, a.hs, E), "h") || !ctx.check(a.rstd, a.rows * 4, "rstd"))) ||
-      (a.gy && a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
+      (a.gy && a.h_rest && !ctx.check(a.h_rest, a.rows * (cdiv(a.D, 8) * 8), "h_rest")) || (a.gy && a.w && !ctx.check(a.w, a.D * E, "w")) || (a.dx && !ctx.check(a.dx, n * E, "dx")) ||
       (a.dw && !ctx.check(a.dw, a.D * E, "dw")))
     return false;
   if (!a.gy) {
@@ -590,13 +646,18 @@ bool launch_rms_bwd(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
   } else {
     with_share(s, [&](auto lc, auto nc) {
       constexpr int L = decltype(lc)::value, N = decltype(nc)::value;
-      const auto go = [&](auto tail, auto dw) {
-        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value>), grid, dim3(threads_of(L)), 0, ctx.stream, a, per, (int)blocks);
+      const auto go = [&](auto tail, auto dw, auto rest) {
+        hipLaunchKernelGGL((rms_back<T, L, N, decltype(tail)::value, decltype(dw)::value, decltype(rest)::value>), grid, dim3(threads_of(L)), 0, ctx.stream, a,
+                           per, (int)blocks);
       };
       using Y = std::true_type;
       using No = std::false_type;
-      if (a.D % V == 0) sums ? go(No(), Y()) : go(No(), No());
-      else sums ? go(Y(), Y()) : go(Y(), No());
+      const auto both = [&](auto rest) {
+        if (a.D % V == 0) sums ? go(No(), Y(), rest) : go(No(), No(), rest);
+        else sums ? go(Y(), Y(), rest) : go(Y(), No(), rest);
+      };
+      if constexpr (kRests<T>) a.h_rest ? both(Y()) : both(No());
+      else both(No());
     });
   }
   if (sums)

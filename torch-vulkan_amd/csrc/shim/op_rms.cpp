@@ -71,10 +71,10 @@ struct Rows {
 };
 
 struct Out {
-  at::Tensor y, h, rstd, q, scale;
+  at::Tensor y, h, rstd, rest, q, scale;
 };
 
-// keep: also rstd, for the backward pass.  coded: 8-bit rows in place of y.
+// keep: also rstd, and what rounding took from h, for the backward pass.  coded: 8-bit rows in place of y.
 Out forward_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& r, double eps, bool keep, bool coded) {
   Out o;
   const auto f32 = x.options().dtype(at::kFloat);
@@ -83,6 +83,7 @@ Out forward_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& r, 
   else o.y = at::empty(x.sizes(), x.options());
   if (r.defined()) o.h = at::empty(x.sizes(), x.options());
   if (keep) o.rstd = at::empty({x.numel() / x.size(-1)}, f32);
+  if (keep && r.defined() && x.scalar_type() != at::kFloat) o.rest = at::empty({x.numel() / x.size(-1), (x.size(-1) + 7) / 8 * 8}, x.options().dtype(at::kChar));
   if (x.numel() == 0) return o;
   const Rows in({x, r});
   const at::Tensor wd = w.defined() ? dense(w) : w;
@@ -93,19 +94,19 @@ Out forward_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& r, 
   else A.y = dptr(o.y);
   if (o.h.defined()) A.h_out = dptr(o.h);
   if (keep) A.rstd = dptr(o.rstd);
+  if (o.rest.defined()) A.h_rest = dptr(o.rest);
   A.rows = in.rows, A.D = in.D, A.n1 = in.n1, A.n2 = in.n2, A.eps = static_cast<float>(eps);
   queue(typed("rms_fwd", x.scalar_type()), A);
   return o;
 }
 
-// With a residual the backward pass reads h as it was rounded: n is then off by half a step of its type in each value, as is a norm's
-// of a stored stream, instead of both of its terms being kept (a tensor of x's size more, read again).
+// With a residual the backward pass reads h, and in 16 bits a byte a value that rounding h left, instead of both of its terms.
 struct Norm : torch::autograd::Function<Norm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& w,
                                                 const std::optional<at::Tensor>& r, double eps) {
     const at::Tensor wd = w.value_or(at::Tensor()), rd = r.value_or(at::Tensor());
     const Out o = forward_rows(x, wd, rd, eps, true, false);
-    ctx->save_for_backward({rd.defined() ? o.h : x, o.rstd, wd});
+    ctx->save_for_backward({rd.defined() ? o.h : x, o.rstd, wd, o.rest});
     ctx->set_materialize_grads(false);  // the gradient of an output that nothing uses is not read
     return rd.defined() ? torch::autograd::variable_list{o.y, o.h} : torch::autograd::variable_list{o.y};
   }
@@ -113,7 +114,7 @@ struct Norm : torch::autograd::Function<Norm> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm: its gradient is not differentiable (create_graph)");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &h = saved[0], &rstd = saved[1], &w = saved[2];
+    const at::Tensor &h = saved[0], &rstd = saved[1], &w = saved[2], &rest = saved[3];
     const at::Tensor gy = grads[0], gh = grads.size() > 1 ? grads[1] : at::Tensor();
     for (const at::Tensor* g : {&gy, &gh})
       if (g->defined()) no_tangent(*g, "rms_norm");
@@ -136,6 +137,7 @@ struct Norm : torch::autograd::Function<Norm> {
       in.put(0, &A.gy, A.gys), in.put(1, &A.gh, A.ghs), in.put(2, &A.h, A.hs);
       A.rstd = dptr(rstd), A.rows = in.rows, A.D = in.D, A.n1 = in.n1, A.n2 = in.n2;
       if (wd.defined()) A.w = dptr(wd);
+      if (rest.defined()) A.h_rest = dptr(rest);
       if (dx.defined()) A.dx = dptr(dx);
       if (wants_w) {
         A.dw = dptr(dw);

@@ -417,7 +417,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     x [..., D] on vk (float32, bfloat16 or float16, any strides), weight [D] and residual [..., D] of the same dtype.  Returns y, or
     (y, h) where residual is given: h, the sum rounded to x's dtype, is the next residual; y is taken from the unrounded sum.
     Differentiable once, in reverse mode, in x, weight and residual.  The backward pass reads h (or x): one changed in place is refused
-    there.  Squares are summed in float32, so magnitudes beyond 1e19 overflow.  Autocast runs it in float32, as it does
+    there.  Its gradients are those of the unrounded sum, for which 16-bit types keep a byte a value beside h.  Squares are summed in float32, so magnitudes beyond 1e19 overflow.  Autocast runs it in float32, as it does
     layer_norm."""
     if x.device.type != "vk":
         raise RuntimeError("rms_norm: x must be a vk tensor")

@@ -69,12 +69,12 @@ class I8LinearBackArgs(ctypes.Structure):
 
 class RmsArgs(ctypes.Structure):
     _fields_ = [("x", u64), ("r", u64), ("w", u64), ("y", u64), ("h_out", u64), ("q", u64), ("scale", u64), ("rstd", u64),
-                ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("xs", i64 * 3), ("rs", i64 * 3), ("eps", f32), ("pad", u32)]
+                ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("xs", i64 * 3), ("rs", i64 * 3), ("eps", f32), ("pad", u32), ("h_rest", u64)]
 
 
 class RmsBwdArgs(ctypes.Structure):
     _fields_ = [("gy", u64), ("gh", u64), ("h", u64), ("rstd", u64), ("w", u64), ("dx", u64), ("dw", u64), ("ws", u64),
-                ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("gys", i64 * 3), ("ghs", i64 * 3), ("hs", i64 * 3)]
+                ("rows", i64), ("D", i64), ("n1", i64), ("n2", i64), ("gys", i64 * 3), ("ghs", i64 * 3), ("hs", i64 * 3), ("h_rest", u64)]
 
 
 class RotaryArgs(ctypes.Structure):
