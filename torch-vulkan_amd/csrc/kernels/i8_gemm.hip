@@ -8,9 +8,10 @@
 // Lane layout of the 8-bit products (checked on the device), l = lane: 32x32x32: operand row l % 32, bytes 16 (l / 32) .. + 15 of K;
 // 16x16x64: row l % 16, bytes 16 (l / 16) .. + 15; accumulators as for the 16-bit products of the same shape.
 // W is the first operand, so an accumulator holds four consecutive columns n of one row m of y.
-// Measured, M x N x K: 1 x 8192 x 2048 4.6 us, 16 x 8192 x 2048 5.7, 308 x 2048 x 2048 6.4, 1024 x 2048 x 8192 27, 4096 x 8192 x 2048 71 us
-// (1.93 POP/s), 4096 x 2048 x 8192 65 (2.1), 8192 cubed 422 to 445 us by box, 2.5 to 2.6 POP/s (a library's 8-bit
-// product of that size: 526).
+// Measured, M x N x K, us, replayed on the same operands (in brackets on operands from HBM, rotated through 600 MB): 1 x 8192 x 2048 5.8 (5.5),
+// 16 x 8192 x 2048 7.1 (7.4), 308 x 2048 x 2048 6.2 (9.9), 308 x 8192 x 2048 11.6 (17.9), 2048 cubed 15 (18.6), 1024 x 2048 x 8192 26 (34),
+// 4096 x 8192 x 2048 69 to 72 by box (74 to 78; 1.9 to 2.0 POP/s), 4096 x 2048 x 8192 63 to 66 (73; 2.1 to 2.2), 8192 cubed 422 to 452 (2.4 to
+// 2.6 POP/s; a library's 8-bit product of that size: 526).
 // The largest tiles' step has 2048 cycles of products, 2048 of LDS (192 KiB of fragments, 64 KiB of copies) and 2200 of L2 -> LDS; it takes
 // 2900 on half of the CUs and 4000 on all of them (matrix cores busy 55%).
 #include <utility>
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN) * KG) void i8_tile(hrt_i
 // barriers.  A grid that leaves CUs idle runs up to a fifth faster.  Measured, us (tiles in this order): 4096 x 8192 x 2048 71, 84, 79, 99,
 // 130; 4096 x 2048 x 8192 79, 65, 72, 86, 104; 2048 cubed 27, 17, 15.6, 15.8, 19; 1024 x 2048 x 8192 73, 41, 34, 26, 29; 308 x 8192 x 2048
 // 25, 15.5, 11.4, 13.5, 15; 308 x 2048 x 2048 25, 14.5, 10, 7.7, 6.2 (before: 128 x 128 in two groups along K and 64 x 64 in four, one to a
-// CU, 11.6 and 7.5).  Over 44 sizes the choice is 2% behind the best.
+// CU, 11.6 and 7.5).
 struct Tile {
   int bm, bn, wm, wn, kg, xr, wr, sp;  // as i8_tile has them
   float once, per256, per128;

@@ -2,9 +2,11 @@
 //
 // Bound by memory: a row is read once, held in registers as fp32 and written once.  16, 64, 256 or 1024 lanes share a row (heads,
 // model widths, wide rows or few of them), which DPP steps and lane swaps add up without LDS, or through a few floats of it.
-// Rows longer than a workgroup's registers take several passes.  Measured, GPU us (bf16, forward with a residual, backward with dw, without):
-// 1 x 2048 3.1, 3.3, 3.0; 4020 x 2048 12.3, 15.7, 10.4 (66 and 82 MB: 5.4 and 5.2 TB/s); 65536 x 128 14.0, 15.6, 10.3; 16384 x 2048 43, 38,
-// 32.  Into 8 bits without the norm: 4020 x 2048 5.6, 8192 x 2048 9.5.
+// Rows longer than a workgroup's registers take several passes.  Measured, GPU us, bf16 with a residual, replayed on the same operands and, in
+// brackets, on operands from HBM (rotated through 600 MB): forward; forward in training, which keeps the sums' rests; dx and dw; dx alone:
+// 1 x 2048 3.1 (2.3), 3.3 (2.5), 3.3 (2.6), 3.1 (2.2); 4020 x 2048 11.8 (15.7: 66 MB, 4.2 TB/s), 13.5 (19.2: 74 MB), 18.8 (22.4: 74 MB and
+// twice 4 MB of sums), 14.1 (17.9); 65536 x 128 12.7 (15.8), 15.1 (18.9), 17.4 (21.4), 13.5 (17.2); 16384 x 2048 40 (49: 268 MB, 5.5 TB/s),
+// 52 (58), 54 (69), 48 (57).  Into 8 bits without the norm: 4020 x 2048 5.6 (7.9), 8192 x 2048 10.1 (12.6).
 #include <initializer_list>
 
 #include "../hrt/registry.h"

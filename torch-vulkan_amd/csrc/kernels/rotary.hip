@@ -3,8 +3,10 @@
 // Bound by memory: every value is read once and written once.  The sines and cosines depend on the token and the pair alone, so a
 // workgroup takes all heads of a few tokens, computes each of them once into LDS and its lanes keep theirs in registers over
 // the heads.  Far positions: the angle is reduced to an eighth of a turn in fp64 (position times frequency in 53 bits) before its
-// sine and cosine are taken in fp32, which leaves them within 2^-22 + |angle| 2^-51: up to 2^29 radians the fp32 steps are the larger part.  Measured, bf16, 16 + 16 heads of 128: 2 x 4096 tokens 24.9 us
-// by the kernel trace (5.4 TB/s, part of it from the last cache; 26.6 with four tokens to a workgroup), 22.5 replayed on the same operands; 8 tokens 3.7 us.
+// sine and cosine are taken in fp32, which leaves them within 2^-22 + |angle| 2^-51: up to 2^29 radians the fp32 steps are the larger part.  Measured, bf16, 16 + 16 heads of 128: 2 x 4096 tokens 25 us
+// by the kernel trace (26.6 with four tokens to a workgroup), 22.4 replayed on the same operands, 26.5 on operands from HBM (134 MB, 5.1 TB/s); 8 tokens
+// 3.7 us.  Few heads leave threads idle: 16384 tokens of 4 + 4 heads of 64, 32 threads of 256, 15.6 us (18.3 from HBM, 1.8 TB/s), of 8 + 4 heads
+// of 128 21.9 (27.8, 3.6 TB/s).
 #include "../hrt/registry.h"
 #include "row_vec.h"
 
@@ -154,7 +156,7 @@ bool launch_rotary(const void* pp, const uint32_t*, hrt::LaunchCtx& ctx) {
       !ctx.check(a.k, hrt::span_bytes(4, kz, kt, E), "k") || !ctx.check(a.k_out, row * a.Hk, "k_out") ||
       !ctx.check(a.pos, hrt::span_bytes(3, pz, pt, pe), "pos") || !ctx.check(a.freqs, (uint64_t)a.P * 8, "freqs"))
     return false;
-  // A workgroup for every token until the chip is full, then one for two.  bf16, 16 + 16 heads of 128, replayed on the same operands, us
+  // A workgroup for every token until the chip is full, then one for two; other shapes of heads were not measured for it.  bf16, 16 + 16 heads of 128, replayed on the same operands, us
   // with 1, 2, 4 tokens each: 2048 tokens 7.6, 7.7, 8.4; 4096 13.5, 12.8, 13.6; 8192 23.7, 22.5, 23.6; 16384 46.5, 44.0, 46.6.
   const int64_t all = a.B * a.S;
   const int tokens = all >= 4096 ? 2 : 1;
