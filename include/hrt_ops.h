@@ -455,9 +455,10 @@ int32_t hrt_i8_mm_plan(const hrt_i8_mm_args* args, int64_t* rounds);
  *   from h, in 256ths of its type's last place, for rms_bwd.
  *   q not 0: in place of y its rows in 8 bits, q [rows, D] and scale [rows] as "i8_rows_quant_*" makes them from the
  *   unrounded y (up to the rounding of 127 y / top in fp32).
- * "rms_bwd_{dt}" — from gy, gh (gradients of y and h, either 0), h (strides hs), h_rest (if not 0, 16-bit kernels: added back to h) and rstd:
+ * "rms_bwd_{dt}" — from gy, gh (gradients of y and h, either 0), h (strides hs), h_rest (16-bit kernels, if not 0: added back to h) and rstd:
  *   dx = rstd * (gy w - n * mean(gy w n)) + gh with n = h rstd; dw (if not 0) = the sum of gy n over the rows; without gy dx = gh
- *   and dw = 0, and h, rstd and w are not read.  dx (if not 0) [rows, D] contiguous.  dw needs ws, hrt_rms_workspace(&args, dtype) floats (none for few rows): sums of runs of rows, added in
+ *   and dw = 0, and h, rstd and w are not read.  dx (if not 0) [rows, D] contiguous.  dw needs ws, hrt_rms_workspace(&args, dtype)
+ *   floats (none for few rows or without gy): sums of runs of rows, added in
  *   order. */
 typedef struct hrt_rms_args {
   uint64_t x, r, w, y, h_out, q, scale, rstd;
